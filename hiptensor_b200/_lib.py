@@ -9,6 +9,7 @@ _lib = None
 
 _vp, _i32p, _i64p = ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int64)
 _u32, _u64, _int = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int
+_u32p = ctypes.POINTER(ctypes.c_uint32)
 
 # name -> (restype, argtypes); the same list is what tests check against the header
 SIGNATURES = {
@@ -45,6 +46,16 @@ SIGNATURES = {
     "htInjectDeviceStatus": (_int, [_vp, ctypes.c_int32]),
     "htKernelLaunchCount": (_u64, []),
     "htReloadSwitches": (None, []),
+    "htBlockQuantize": (_int, [_vp, _vp, _vp, _i32p, _u32p, _vp, _vp, _i32p, _vp, _vp, _vp]),
+    "htCreateScaledContractionPlan": (_int, [_vp, ctypes.POINTER(_vp), _vp, _i32p, _vp, _u32p, _vp, _i32p, _vp, _u32p, _vp,
+                                             _vp, _i32p, _int]),
+    "htDestroyScaledContractionPlan": (_int, [_vp]),
+    "htScaledContraction": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "htCreateCrossEntropyPlan": (_int, [_vp, ctypes.POINTER(_vp), _vp, _i32p, _vp, _i32p, ctypes.c_int64, _int]),
+    "htDestroyCrossEntropyPlan": (_int, [_vp]),
+    "htCrossEntropyGetWorkspaceSize": (_int, [_vp, _vp, _int, _int, ctypes.POINTER(_u64)]),
+    "htCrossEntropy": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
+    "htCrossEntropyGradient": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
     "htReductionFinish": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp]),
 }
 
@@ -75,3 +86,9 @@ def i32(v):
     if v is None:
         return None
     return (ctypes.c_int32 * len(v))(*[int(x) for x in v])
+
+
+def u32(v):
+    if v is None:
+        return None
+    return (ctypes.c_uint32 * len(v))(*[int(x) for x in v])

@@ -12,7 +12,7 @@ from . import _lib
 
 __all__ = [
     "HiptensorError", "Handle", "TensorDescriptor",
-    "R_32F", "R_64F", "R_16F", "R_16BF", "C_32F", "C_64F",
+    "R_32F", "R_64F", "R_16F", "R_16BF", "C_32F", "C_64F", "R_8F_E4M3", "R_8F_E5M2",
     "COMPUTE_16F", "COMPUTE_32F", "COMPUTE_64F", "COMPUTE_16BF", "COMPUTE_C32F", "COMPUTE_C64F",
     "OP_IDENTITY", "OP_SQRT", "OP_ADD", "OP_MUL", "OP_MAX", "OP_MIN",
     "ALGO_DEFAULT", "ALGO_DEFAULT_PATIENT", "ALGO_ACTOR_CRITIC",
@@ -27,6 +27,8 @@ __all__ = [
 # hipDataType (hiptensor_types.hpp uses hipDataType; values equal cudaDataType)
 R_32F, R_64F, R_16F, R_16BF = 0, 1, 2, 14
 C_32F, C_64F = 4, 5
+# the 8-bit types of block_quantize and scaled_contraction (cudaDataType)
+R_8F_E4M3, R_8F_E5M2 = 28, 29
 # hiptensorComputeType_t (hiptensor_types.hpp:74-99)
 COMPUTE_16F, COMPUTE_32F, COMPUTE_64F, COMPUTE_16BF = 1, 4, 16, 1024
 COMPUTE_C32F, COMPUTE_C64F = 2048, 4096
@@ -41,7 +43,7 @@ STATUS_SUCCESS, STATUS_NOT_INITIALIZED, STATUS_INVALID_VALUE, STATUS_ARCH_MISMAT
 STATUS_INTERNAL_ERROR, STATUS_NOT_SUPPORTED, STATUS_HIP_ERROR, STATUS_INSUFFICIENT_WORKSPACE = 14, 15, 18, 19
 STATUS_EXECUTION_FAILED = 13
 
-_DTYPE_SIZE = {R_32F: 4, R_64F: 8, R_16F: 2, R_16BF: 2, C_32F: 8, C_64F: 16}
+_DTYPE_SIZE = {R_32F: 4, R_64F: 8, R_16F: 2, R_16BF: 2, C_32F: 8, C_64F: 16, R_8F_E4M3: 1, R_8F_E5M2: 1}
 
 
 def dtype_size(dt):
@@ -262,6 +264,69 @@ class Handle:
         b = _scalar_for_compute(beta, plan.type_compute)
         _check(self._L.htContraction(self._h, plan._p, a, _ptr(A), _ptr(B), b, _ptr(C), _ptr(D), _ptr(workspace),
                                      int(workspace_size), _stream_ptr(stream)), "hiptensorContraction")
+
+
+    # ---- 8-bit tensors with a scale for each block of 128 (include/hiptensor_b200.h has the definitions) ----
+
+    def block_quantize(self, A, descA, modeA, blockA, Q, descQ, modeQ, S, descS, stream=None):
+        """htBlockQuantize: Q[modeQ] (e4m3 / e5m2) and the f32 scales S of A[modeA]; blockA: 1 or 128 for each mode of A. S
+        has A's modes with extents ceil(extent / block)."""
+        self._same_rank("htBlockQuantize", (descA, modeA, blockA), (descQ, modeQ), (descS, modeA))
+        _check(self._L.htBlockQuantize(self._h, _ptr(A), descA._p, _lib.i32(modeA), _lib.u32(blockA), _ptr(Q), descQ._p,
+                                       _lib.i32(modeQ), _ptr(S), descS._p, _stream_ptr(stream)), "htBlockQuantize")
+
+    def scaled_contraction_plan(self, descA, modeA, descScaleA, blockA, descB, modeB, descScaleB, blockB, descC, descD, modeD,
+                                type_compute=COMPUTE_32F):
+        """htCreateScaledContractionPlan; descC=None: no C, else it is described as D is."""
+        self._same_rank("htCreateScaledContractionPlan", (descA, modeA, blockA), (descScaleA, modeA), (descB, modeB, blockB),
+                        (descScaleB, modeB), (descD, modeD))
+        p = ctypes.c_void_p(0)
+        _check(self._L.htCreateScaledContractionPlan(
+            self._h, ctypes.byref(p), descA._p, _lib.i32(modeA), descScaleA._p, _lib.u32(blockA), descB._p, _lib.i32(modeB),
+            descScaleB._p, _lib.u32(blockB), descC._p if descC is not None else None, descD._p, _lib.i32(modeD),
+            int(type_compute)), "htCreateScaledContractionPlan")
+        return _Owned(p, "htDestroyScaledContractionPlan")
+
+    def scaled_contraction(self, plan, alpha, A, scaleA, B, scaleB, beta, C, D, stream=None):
+        """htScaledContraction: D = alpha * (A scaleA) (B scaleB) + beta * C."""
+        _check(self._L.htScaledContraction(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _ptr(A), _ptr(scaleA), _ptr(B),
+                                           _ptr(scaleB), ctypes.byref(ctypes.c_float(beta)), _ptr(C), _ptr(D),
+                                           _stream_ptr(stream)), "htScaledContraction")
+
+    # ---- softmax cross entropy of a linear head, logits not kept ----
+
+    def cross_entropy_plan(self, descH, modeH, descW, modeW, ignore_index=-100, type_compute=COMPUTE_32F):
+        """htCreateCrossEntropyPlan: modes shared by H and W are contracted, H's others are tokens, W's others classes."""
+        self._same_rank("htCreateCrossEntropyPlan", (descH, modeH), (descW, modeW))
+        p = ctypes.c_void_p(0)
+        _check(self._L.htCreateCrossEntropyPlan(self._h, ctypes.byref(p), descH._p, _lib.i32(modeH), descW._p, _lib.i32(modeW),
+                                                int(ignore_index), int(type_compute)), "htCreateCrossEntropyPlan")
+        return _Owned(p, "htDestroyCrossEntropyPlan")
+
+    def cross_entropy_workspace_size(self, plan, gradient=False, pref=WORKSPACE_RECOMMENDED):
+        out = ctypes.c_uint64(0)
+        _check(self._L.htCrossEntropyGetWorkspaceSize(self._h, plan._p, 1 if gradient else 0, int(pref), ctypes.byref(out)),
+               "htCrossEntropyGetWorkspaceSize")
+        return out.value
+
+    def cross_entropy(self, plan, alpha, H, W, targets, loss, lse, workspace, workspace_size, stream=None):
+        """htCrossEntropy: loss (0 for ignored tokens) and lse, f32, one for each token; targets int64."""
+        _check(self._L.htCrossEntropy(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _ptr(H), _ptr(W), _ptr(targets),
+                                      _ptr(loss), _ptr(lse), _ptr(workspace), int(workspace_size), _stream_ptr(stream)),
+               "htCrossEntropy")
+
+    def cross_entropy_gradient(self, plan, alpha, H, W, targets, lse, grad_loss, dH, dW, workspace, workspace_size, stream=None):
+        """htCrossEntropyGradient: dH (like H) and dW (like W), either may be None; lse from cross_entropy."""
+        _check(self._L.htCrossEntropyGradient(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _ptr(H), _ptr(W),
+                                              _ptr(targets), _ptr(lse), _ptr(grad_loss), _ptr(dH), _ptr(dW), _ptr(workspace),
+                                              int(workspace_size), _stream_ptr(stream)), "htCrossEntropyGradient")
+
+    @staticmethod
+    def _same_rank(where, *groups):
+        # the library reads one mode (and one block) for each mode of the descriptor
+        for desc, *lists in groups:
+            if any(len(x) != len(desc.lens) for x in lists):
+                raise HiptensorError(STATUS_INVALID_VALUE, where)
 
 
 def last_kernel_name():

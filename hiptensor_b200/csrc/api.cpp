@@ -21,13 +21,8 @@
 
 using namespace htb;
 
-namespace
+namespace htb
 {
-    HandleState* mutableState(hiptensorHandle_t* h)
-    {
-        return reinterpret_cast<HandleState*>(h->fields);
-    }
-
     // ARCH_MISMATCH unless the current device is the one the handle was made on
     // (hiptensor_contraction.cpp:263-277).
     hiptensorStatus_t checkDevice(const char* func, const HandleState* st)
@@ -42,17 +37,34 @@ namespace
             return HIPTENSOR_STATUS_ARCH_MISMATCH;
         }
         // A kernel of an earlier call gave up a bounded wait (it skipped its remaining work, so that call's
-        // output is incomplete): reported once, on the next call, then cleared. The kernels exit cleanly, the
-        // handle stays usable.
+        // output is incomplete) or met a target that is no class: reported once, on the next call, then cleared. The
+        // kernels exit cleanly, the handle stays usable.
         if(st->hostStatus && *st->hostStatus != 0)
         {
             const int code = *st->hostStatus;
             *st->hostStatus = 0;
-            HTB_LOG_ERROR(func, "an earlier kernel on this handle timed out in a device-side wait (code %d) (%s)", code,
+            HTB_LOG_ERROR(func, "an earlier kernel on this handle %s (code %d) (%s)",
+                          code == kStatusBadTarget ? "met a target outside the vocabulary" : "timed out in a device-side wait", code,
                           hiptensorGetErrorString(HIPTENSOR_STATUS_EXECUTION_FAILED));
             return HIPTENSOR_STATUS_EXECUTION_FAILED;
         }
         return HIPTENSOR_STATUS_SUCCESS;
+    }
+
+    int launchResult(const char* func, cudaError_t e)
+    {
+        if(e == cudaSuccess)
+            return HIPTENSOR_STATUS_SUCCESS;
+        HTB_LOG_ERROR(func, "kernel launch failed: %s (%s)", cudaGetErrorString(e), hiptensorGetErrorString(HIPTENSOR_STATUS_HIP_ERROR));
+        return HIPTENSOR_STATUS_HIP_ERROR;
+    }
+} // namespace htb
+
+namespace
+{
+    HandleState* mutableState(hiptensorHandle_t* h)
+    {
+        return reinterpret_cast<HandleState*>(h->fields);
     }
 
     std::vector<int64_t> toI64(const std::vector<std::size_t>& v)
@@ -285,7 +297,8 @@ hiptensorStatus_t hiptensorInitTensorDescriptor(const hiptensorHandle_t* handle,
         return HIPTENSOR_STATUS_NOT_INITIALIZED;
     }
     const bool typeOk = dataType == HIP_R_16F || dataType == HIP_R_16BF || dataType == HIP_R_32F
-                        || dataType == HIP_R_64F || dataType == HIP_C_32F || dataType == HIP_C_64F;
+                        || dataType == HIP_R_64F || dataType == HIP_C_32F || dataType == HIP_C_64F
+                        || dataType == CUDA_R_8F_E4M3 || dataType == CUDA_R_8F_E5M2; // the last two: see hiptensor_b200.h
     const bool opOk = unaryOp == HIPTENSOR_OP_IDENTITY || unaryOp == HIPTENSOR_OP_SQRT;
     if((lens == nullptr && strides != nullptr) || !typeOk || !opOk || (lens == nullptr && numModes > 0))
     {

@@ -9,7 +9,9 @@
 #include <hiptensor/hiptensor.hpp>
 #include <hiptensor_b200.h>
 
+#include "cross_entropy.hpp"
 #include "kernels.hpp"
+#include "scaled.hpp"
 
 struct htHandle
 {
@@ -30,6 +32,14 @@ struct htContractionFind
 struct htContractionPlan
 {
     hiptensorContractionPlan_t p;
+};
+struct htScaledContractionPlan
+{
+    htb::ScaledPlan p;
+};
+struct htCrossEntropyPlan
+{
+    htb::CrossEntropyPlan p;
 };
 
 namespace
@@ -313,6 +323,104 @@ int htReductionFinish(const htHandle* handle, const void* alpha, const void* par
                       void* D, const htTensorDescriptor* descD, int typeCompute, void* stream)
 {
     return htb::reductionFinish(H(handle), alpha, partial, beta, C, D, TD(descD), typeCompute, stream);
+}
+
+int htBlockQuantize(const htHandle* handle, const void* A, const htTensorDescriptor* descA, const int32_t* modeA,
+                    const uint32_t* blockA, void* Q, const htTensorDescriptor* descQ, const int32_t* modeQ, float* S,
+                    const htTensorDescriptor* descS, void* stream)
+{
+    return htb::blockQuantize(H(handle), A, TD(descA), modeA, blockA, Q, TD(descQ), modeQ, S, TD(descS), stream);
+}
+
+int htCreateScaledContractionPlan(const htHandle* handle, htScaledContractionPlan** plan, const htTensorDescriptor* descA,
+                                  const int32_t* modeA, const htTensorDescriptor* descScaleA, const uint32_t* blockA,
+                                  const htTensorDescriptor* descB, const int32_t* modeB, const htTensorDescriptor* descScaleB,
+                                  const uint32_t* blockB, const htTensorDescriptor* descC, const htTensorDescriptor* descD,
+                                  const int32_t* modeD, int typeCompute)
+{
+    if(!plan)
+        return HIPTENSOR_STATUS_NOT_INITIALIZED;
+    *plan = nullptr;
+    if(!handle || !descA || !modeA || !descScaleA || !blockA || !descB || !modeB || !descScaleB || !blockB || !descD || !modeD)
+        return HIPTENSOR_STATUS_NOT_INITIALIZED;
+    htb::ScaledPlan p;
+    const int rc = htb::planScaled(descA->d, modeA, descScaleA->d, blockA, descB->d, modeB, descScaleB->d, blockB, TD(descC), descD->d,
+                                   modeD, typeCompute, &p);
+    if(rc != HIPTENSOR_STATUS_SUCCESS)
+    {
+        HTB_LOG_ERROR("htCreateScaledContractionPlan", "these tensors cannot be contracted in blocks (%s)",
+                      hiptensorGetErrorString(hiptensorStatus_t(rc)));
+        return rc;
+    }
+    auto* out = new(std::nothrow) htScaledContractionPlan;
+    if(!out)
+        return HIPTENSOR_STATUS_ALLOC_FAILED;
+    out->p = p;
+    *plan  = out;
+    return HIPTENSOR_STATUS_SUCCESS;
+}
+int htDestroyScaledContractionPlan(htScaledContractionPlan* plan)
+{
+    delete plan;
+    return HIPTENSOR_STATUS_SUCCESS;
+}
+int htScaledContraction(const htHandle* handle, const htScaledContractionPlan* plan, const void* alpha, const void* A,
+                        const float* scaleA, const void* B, const float* scaleB, const void* beta, const void* C, void* D,
+                        void* stream)
+{
+    return htb::scaledContraction(H(handle), plan ? &plan->p : nullptr, alpha, A, scaleA, B, scaleB, beta, C, D, stream);
+}
+
+int htCreateCrossEntropyPlan(const htHandle* handle, htCrossEntropyPlan** plan, const htTensorDescriptor* descH,
+                             const int32_t* modeH, const htTensorDescriptor* descW, const int32_t* modeW, int64_t ignoreIndex,
+                             int typeCompute)
+{
+    if(!plan)
+        return HIPTENSOR_STATUS_NOT_INITIALIZED;
+    *plan = nullptr;
+    if(!handle || !descH || !modeH || !descW || !modeW)
+        return HIPTENSOR_STATUS_NOT_INITIALIZED;
+    htb::CrossEntropyPlan p;
+    const int rc = htb::planCrossEntropy(descH->d, modeH, descW->d, modeW, ignoreIndex, typeCompute, &p);
+    if(rc != HIPTENSOR_STATUS_SUCCESS)
+    {
+        HTB_LOG_ERROR("htCreateCrossEntropyPlan", "no cross entropy over these tensors (%s)", hiptensorGetErrorString(hiptensorStatus_t(rc)));
+        return rc;
+    }
+    auto* out = new(std::nothrow) htCrossEntropyPlan;
+    if(!out)
+        return HIPTENSOR_STATUS_ALLOC_FAILED;
+    out->p = p;
+    *plan  = out;
+    return HIPTENSOR_STATUS_SUCCESS;
+}
+int htDestroyCrossEntropyPlan(htCrossEntropyPlan* plan)
+{
+    delete plan;
+    return HIPTENSOR_STATUS_SUCCESS;
+}
+int htCrossEntropyGetWorkspaceSize(const htHandle* handle, const htCrossEntropyPlan* plan, int gradient, int pref,
+                                   uint64_t* workspaceSize)
+{
+    if(!handle || !plan)
+        return HIPTENSOR_STATUS_NOT_INITIALIZED;
+    if(!workspaceSize || (pref != HIPTENSOR_WORKSPACE_MIN && pref != HIPTENSOR_WORKSPACE_RECOMMENDED && pref != HIPTENSOR_WORKSPACE_MAX))
+        return HIPTENSOR_STATUS_INVALID_VALUE;
+    *workspaceSize = htb::crossEntropyWorkspace(plan->p, gradient != 0, pref);
+    return HIPTENSOR_STATUS_SUCCESS;
+}
+int htCrossEntropy(const htHandle* handle, const htCrossEntropyPlan* plan, const void* alpha, const void* hidden, const void* W,
+                   const int64_t* targets, float* loss, float* lse, void* workspace, uint64_t workspaceSize, void* stream)
+{
+    return htb::crossEntropy(H(handle), plan ? &plan->p : nullptr, alpha, hidden, W, targets, loss, lse, workspace, workspaceSize,
+                             stream);
+}
+int htCrossEntropyGradient(const htHandle* handle, const htCrossEntropyPlan* plan, const void* alpha, const void* hidden,
+                           const void* W, const int64_t* targets, const float* lse, const float* gradLoss, void* dH, void* dW,
+                           void* workspace, uint64_t workspaceSize, void* stream)
+{
+    return htb::crossEntropyGradient(H(handle), plan ? &plan->p : nullptr, alpha, hidden, W, targets, lse, gradLoss, dH, dW,
+                                     workspace, workspaceSize, stream);
 }
 
 void htReloadSwitches(void)

@@ -26,6 +26,8 @@ namespace htb
         case CUDA_R_64F: return 8;
         case CUDA_R_16F: return 2;
         case CUDA_R_16BF: return 2;
+        case CUDA_R_8F_E4M3: return 1;
+        case CUDA_R_8F_E5M2: return 1;
         case CUDA_C_32F: return 8;
         case CUDA_C_64F: return 16;
         default: return 0;
@@ -40,6 +42,8 @@ namespace htb
         case CUDA_R_64F: return "f64";
         case CUDA_R_16F: return "f16";
         case CUDA_R_16BF: return "bf16";
+        case CUDA_R_8F_E4M3: return "e4m3";
+        case CUDA_R_8F_E5M2: return "e5m2";
         case CUDA_C_32F: return "cf32";
         case CUDA_C_64F: return "cf64";
         default: return "none";
@@ -75,6 +79,16 @@ namespace htb
         volatile int* hostStatus; // the same word as the host sees it (pinned, mapped memory)
     };
     constexpr uint64_t kHandleMagic = 0x4854423230300001ull;
+
+    // Codes of the device status word (1 to 4: see htGetDeviceStatus in include/hiptensor_b200.h)
+    constexpr int kStatusScaled    = 5; // a wait of the block-scaled kernel ran out
+    constexpr int kStatusSoftmax   = 6; // a wait of the cross-entropy kernel ran out
+    constexpr int kStatusBadTarget = 7; // a target of a cross entropy is neither a class nor the ignored index
+
+    // ARCH_MISMATCH unless the current device is the handle's; EXECUTION_FAILED once after a kernel raised the status word.
+    hiptensorStatus_t checkDevice(const char* func, const HandleState* st);
+    // HIP_ERROR, logged, for a launch that failed
+    int launchResult(const char* func, cudaError_t e);
 
     inline const HandleState* stateOf(const hiptensorHandle_t* h)
     {

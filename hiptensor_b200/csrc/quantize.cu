@@ -1,0 +1,316 @@
+// Block quantisation: f16 / bf16 / f32 -> e4m3 / e5m2 with one f32 scale for each block of 128 elements of a mode, or of
+// 128 x 128 elements of two modes, in any order of the result's modes (a permutation in the same pass).
+//
+//   a = max(max |A| over the block, 2^-100)   S = q / q' with q = a, q' = 448 (e4m3) or 57344 (e5m2), rounded to f32
+//   R = q' / a rounded to f32                 Q = the 8-bit number nearest to A * R, ties to even
+//
+// The floor keeps R finite: a block of zeros gets the scale of the floor and quantises to zeros. A block that holds a NaN
+// gets the scale NaN; one that holds an infinity the scale infinity: either way all of it is NaN once multiplied out.
+//
+// ONE rounding. A * R rounded to f32 and then to 8 bits would round twice: an f32 product can land exactly on the border
+// between two 8-bit numbers although the product itself lies beside it. The product is therefore rounded to f32 "to odd":
+// truncated, and its last bit set when the truncation was not exact (the fused multiply-add gives the exact remainder).
+// A number rounded to odd at 24 bits rounds to 4 bits or fewer as the number itself does.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "kernels.hpp"
+#include "scaled.hpp"
+
+namespace htb
+{
+    namespace
+    {
+        constexpr int   kTile    = 128; // columns of a tile; rows too unless the blocks are rows and the order is kept
+        constexpr int   kThreads = 256; // 16 threads along a row of the tile, eight columns each, times 16 groups of rows
+        constexpr float kFloor   = 7.88860905221011805411728565282787e-31f; // 2^-100
+
+        __device__ __forceinline__ float maxNan(float a, float b)
+        {
+            float r;
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+            return r;
+        }
+        __device__ __forceinline__ float widen(float v)
+        {
+            return v;
+        }
+        __device__ __forceinline__ float widen(__half v)
+        {
+            return __half2float(v);
+        }
+        __device__ __forceinline__ float widen(__nv_bfloat16 v)
+        {
+            return __bfloat162float(v);
+        }
+        // a * r rounded to odd
+        __device__ __forceinline__ float mulOdd(float a, float r)
+        {
+            const float p = __fmul_rz(a, r);
+            const float e = __fmaf_rn(a, r, -p);
+            return e != 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+        }
+        template <bool E5M2>
+        __device__ __forceinline__ uint32_t pair8(float lo, float hi)
+        {
+            return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
+        }
+
+        struct QuantArgs
+        {
+            QuantPlan p;
+            int64_t   tilesR, tilesC, tiles;
+            int       vecStore; // the result's runs are aligned: 8- and 16-byte stores
+        };
+
+        enum BlockForm : int
+        {
+            BLOCK_ROW  = 0, // 1 x 128
+            BLOCK_COL  = 1, // 128 x 1
+            BLOCK_BOTH = 2 // 128 x 128
+        };
+
+        // One tile of P * 16 rows and 128 columns at a time. Thread (tx, ty) holds columns tx * 8 .. + 7 of rows
+        // ty * P .. + P - 1 in registers, so A is read once; a row's maximum is a shuffle over 16 lanes, a column's goes
+        // through shared memory. VEC: rows of A are read as 16-byte words. TRANS: the result is contiguous along A's
+        // rows' mode: the bytes pass through shared memory, 8 rows at a time, in units of 8 bytes whose place in a column
+        // is XORed with the thread's tx so that the 16 threads of a row write to 16 different pairs of banks.
+        template <typename T, int FORM, bool TRANS, bool VEC, bool E5M2>
+        __global__ void __launch_bounds__(kThreads) block_quantize_kernel(const T* __restrict__ A, unsigned char* __restrict__ Q,
+                                                                          float* __restrict__ S, const __grid_constant__ QuantArgs a)
+        {
+            constexpr int   P    = (FORM == BLOCK_ROW && !TRANS) ? 2 : 8;
+            constexpr float kMax = E5M2 ? 57344.f : 448.f;
+            const QuantPlan& p   = a.p;
+            const int        tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+            __shared__ float part[FORM == BLOCK_ROW ? 1 : (FORM == BLOCK_COL ? 16 * kTile : 16)];
+            __shared__ __align__(16) unsigned char turn[TRANS ? kTile * kTile : 16];
+
+            for(int64_t t = blockIdx.x; t < a.tiles; t += gridDim.x)
+            {
+                const int64_t tc = t % a.tilesC, rest = t / a.tilesC;
+                const int64_t tr = rest % a.tilesR, b = rest / a.tilesR;
+                const int64_t r0 = tr * (16 * P) + ty * P, c0 = tc * kTile + tx * 8;
+                const int     nr = int(min(int64_t(P), p.rows - r0)), nc = int(min(int64_t(8), p.cols - c0)); // may be negative
+                const T*      src = A + b * p.aB + r0 * p.aR + c0 * p.aC;
+                float         v[P][8];
+#pragma unroll
+                for(int i = 0; i < P; i++)
+                {
+                    if(VEC && i < nr && nc == 8)
+                    {
+                        constexpr int kWords = int(sizeof(T)) / 2; // 16-byte words of eight elements
+                        T             e[8];
+#pragma unroll
+                        for(int w = 0; w < kWords; w++)
+                            reinterpret_cast<uint4*>(e)[w] = __ldg(reinterpret_cast<const uint4*>(src + i * p.aR) + w);
+#pragma unroll
+                        for(int j = 0; j < 8; j++)
+                            v[i][j] = widen(e[j]);
+                    }
+                    else
+                    {
+#pragma unroll
+                        for(int j = 0; j < 8; j++)
+                            v[i][j] = (i < nr && j < nc) ? widen(src[i * p.aR + j * p.aC]) : 0.f;
+                    }
+                }
+
+                // factors of the thread's elements: one per row, one per column, or one
+                float scale[FORM == BLOCK_ROW ? P : (FORM == BLOCK_COL ? 8 : 1)];
+                if constexpr(FORM == BLOCK_ROW)
+                {
+#pragma unroll
+                    for(int i = 0; i < P; i++)
+                    {
+                        float m = kFloor;
+#pragma unroll
+                        for(int j = 0; j < 8; j++)
+                            m = maxNan(m, fabsf(v[i][j]));
+#pragma unroll
+                        for(int s = 8; s >= 1; s >>= 1)
+                            m = maxNan(m, __shfl_xor_sync(0xffffffffu, m, s));
+                        scale[i] = __fdiv_rn(kMax, m);
+                        if(tx == 0 && i < nr)
+                            S[b * p.sB + (r0 + i) * p.sR + tc * p.sC] = __fdiv_rn(m, kMax);
+                    }
+                }
+                else if constexpr(FORM == BLOCK_COL)
+                {
+                    float m[8];
+#pragma unroll
+                    for(int j = 0; j < 8; j++)
+                    {
+                        m[j] = kFloor;
+#pragma unroll
+                        for(int i = 0; i < P; i++)
+                            m[j] = maxNan(m[j], fabsf(v[i][j]));
+                    }
+                    __syncthreads(); // the maxima of the tile before have been read
+#pragma unroll
+                    for(int j = 0; j < 8; j += 4)
+                        *reinterpret_cast<float4*>(&part[ty * kTile + tx * 8 + j]) = make_float4(m[j], m[j + 1], m[j + 2], m[j + 3]);
+                    __syncthreads();
+                    if(threadIdx.x < kTile)
+                    {
+                        float top = part[threadIdx.x];
+#pragma unroll
+                        for(int g = 1; g < 16; g++)
+                            top = maxNan(top, part[g * kTile + threadIdx.x]);
+                        const int64_t c = tc * kTile + threadIdx.x;
+                        if(c < p.cols)
+                            S[b * p.sB + tr * p.sR + c * p.sC] = __fdiv_rn(top, kMax);
+                        part[threadIdx.x] = __fdiv_rn(kMax, top);
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for(int j = 0; j < 8; j++)
+                        scale[j] = part[tx * 8 + j];
+                }
+                else
+                {
+                    float m = kFloor;
+#pragma unroll
+                    for(int i = 0; i < P; i++)
+#pragma unroll
+                        for(int j = 0; j < 8; j++)
+                            m = maxNan(m, fabsf(v[i][j]));
+#pragma unroll
+                    for(int s = 16; s >= 1; s >>= 1)
+                        m = maxNan(m, __shfl_xor_sync(0xffffffffu, m, s));
+                    __syncthreads();
+                    if((threadIdx.x & 31) == 0)
+                        part[threadIdx.x >> 5] = m;
+                    __syncthreads();
+#pragma unroll
+                    for(int g = 0; g < kThreads / 32; g++)
+                        m = maxNan(m, part[g]);
+                    scale[0] = __fdiv_rn(kMax, m);
+                    if(threadIdx.x == 0)
+                        S[b * p.sB + tr * p.sR + tc * p.sC] = __fdiv_rn(m, kMax);
+                }
+                auto factor = [&](int i, int j) { return scale[FORM == BLOCK_ROW ? i : (FORM == BLOCK_COL ? j : 0)]; };
+
+                if constexpr(!TRANS)
+                {
+                    unsigned char* dst = Q + b * p.qB + r0 * p.qR + c0 * p.qC;
+#pragma unroll
+                    for(int i = 0; i < P; i++)
+                    {
+                        if(i >= nr || nc <= 0)
+                            continue;
+                        uint32_t w[4];
+#pragma unroll
+                        for(int j = 0; j < 4; j++)
+                            w[j] = pair8<E5M2>(mulOdd(v[i][2 * j], factor(i, 2 * j)), mulOdd(v[i][2 * j + 1], factor(i, 2 * j + 1)));
+                        if(a.vecStore && nc == 8)
+                            *reinterpret_cast<uint2*>(dst + i * p.qR) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+                        else
+                        {
+#pragma unroll
+                            for(int j = 0; j < 8; j++)
+                                if(j < nc)
+                                    dst[i * p.qR + j * p.qC] = (unsigned char)(w[j >> 1] >> (8 * (j & 1)));
+                        }
+                    }
+                }
+                else
+                {
+                    __syncthreads(); // the tile before has been written out
+#pragma unroll
+                    for(int j = 0; j < 8; j++)
+                    {
+                        uint32_t w[4];
+#pragma unroll
+                        for(int i = 0; i < 4; i++)
+                            w[i] = pair8<E5M2>(mulOdd(v[2 * i][j], factor(2 * i, j)), mulOdd(v[2 * i + 1][j], factor(2 * i + 1, j)));
+                        *reinterpret_cast<uint2*>(&turn[(tx * 8 + j) * kTile + ((ty ^ tx) << 3)])
+                            = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+                    }
+                    __syncthreads();
+                    // eight threads write the 128 rows of a column, 16 bytes each
+                    const int     unit = int(threadIdx.x & 7) * 2;
+                    const int64_t row  = tr * kTile + unit * 8;
+                    const int     left = int(min(int64_t(16), p.rows - row));
+#pragma unroll
+                    for(int k = 0; k < kTile / 32; k++)
+                    {
+                        const int     col = k * 32 + int(threadIdx.x >> 3);
+                        const int64_t c   = tc * kTile + col;
+                        if(c >= p.cols || left <= 0)
+                            continue;
+                        const int x = col >> 3;
+                        uint4     w = *reinterpret_cast<const uint4*>(&turn[col * kTile + (((unit ^ x) & ~1) << 3)]);
+                        if(x & 1)
+                            w = make_uint4(w.z, w.w, w.x, w.y);
+                        unsigned char* dst = Q + b * p.qB + c * p.qC + row * p.qR;
+                        if(a.vecStore && left == 16)
+                            *reinterpret_cast<uint4*>(dst) = w;
+                        else
+                        {
+                            const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for(int i = 0; i < 16; i++)
+                                if(i < left)
+                                    dst[i * p.qR] = (unsigned char)(e[i >> 2] >> (8 * (i & 3)));
+                        }
+                    }
+                }
+            }
+        }
+
+        template <typename T, int FORM, bool TRANS>
+        cudaError_t launchForm(const QuantArgs& a, bool vec, int grid, const void* A, void* Q, float* S, cudaStream_t stream)
+        {
+            const bool e5m2 = a.p.typeQ == CUDA_R_8F_E5M2;
+            auto       kernel = vec ? (e5m2 ? block_quantize_kernel<T, FORM, TRANS, true, true> : block_quantize_kernel<T, FORM, TRANS, true, false>)
+                                    : (e5m2 ? block_quantize_kernel<T, FORM, TRANS, false, true>
+                                            : block_quantize_kernel<T, FORM, TRANS, false, false>);
+            kernel<<<grid, kThreads, 0, stream>>>((const T*)A, (unsigned char*)Q, S, a);
+            const cudaError_t e = cudaGetLastError();
+            if(e == cudaSuccess)
+                noteLaunch("block_quantize");
+            return e;
+        }
+
+        template <typename T>
+        cudaError_t launchTyped(const QuantPlan& p, const void* A, void* Q, float* S, int smCount, cudaStream_t stream)
+        {
+            const int  form  = p.blockR > 1 ? (p.blockC > 1 ? BLOCK_BOTH : BLOCK_COL) : BLOCK_ROW;
+            const bool trans = p.qR == 1 && p.qC != 1; // else along the columns, or along neither
+            // 16-byte loads: rows contiguous, and every row starts at a multiple of 16 bytes
+            const int64_t words = 16 / int64_t(sizeof(T));
+            const bool    vec   = p.aC == 1 && p.aR % words == 0 && p.aB % words == 0 && (uintptr_t(A) & 15) == 0;
+            const int64_t unit  = trans ? 16 : 8;
+            QuantArgs     a;
+            a.p        = p;
+            a.tilesR   = (p.rows + (form == BLOCK_ROW && !trans ? 31 : 127)) / (form == BLOCK_ROW && !trans ? 32 : 128);
+            a.tilesC   = (p.cols + kTile - 1) / kTile;
+            a.tiles    = a.tilesR * a.tilesC * p.batch;
+            a.vecStore = (trans ? p.qR : p.qC) == 1 && (trans ? p.qC : p.qR) % unit == 0 && p.qB % unit == 0 && uintptr_t(Q) % unit == 0;
+            const int grid = int(std::min<int64_t>(a.tiles, int64_t(smCount > 0 ? smCount : 148) * 4096));
+            if(form == BLOCK_ROW)
+                return trans ? launchForm<T, BLOCK_ROW, true>(a, vec, grid, A, Q, S, stream)
+                             : launchForm<T, BLOCK_ROW, false>(a, vec, grid, A, Q, S, stream);
+            if(form == BLOCK_COL)
+                return trans ? launchForm<T, BLOCK_COL, true>(a, vec, grid, A, Q, S, stream)
+                             : launchForm<T, BLOCK_COL, false>(a, vec, grid, A, Q, S, stream);
+            return trans ? launchForm<T, BLOCK_BOTH, true>(a, vec, grid, A, Q, S, stream)
+                         : launchForm<T, BLOCK_BOTH, false>(a, vec, grid, A, Q, S, stream);
+        }
+    } // namespace
+
+    cudaError_t launchQuantize(const QuantPlan& p, const void* A, void* Q, float* S, int smCount, cudaStream_t stream)
+    {
+        switch(p.typeA)
+        {
+        case CUDA_R_32F: return launchTyped<float>(p, A, Q, S, smCount, stream);
+        case CUDA_R_16F: return launchTyped<__half>(p, A, Q, S, smCount, stream);
+        case CUDA_R_16BF: return launchTyped<__nv_bfloat16>(p, A, Q, S, smCount, stream);
+        }
+        return cudaErrorNotSupported;
+    }
+} // namespace htb

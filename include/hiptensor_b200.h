@@ -27,6 +27,8 @@ typedef struct htTensorDescriptor htTensorDescriptor; /* hiptensorTensorDescript
 typedef struct htContractionDesc  htContractionDesc;  /* hiptensorContractionDescriptor_t */
 typedef struct htContractionFind  htContractionFind;  /* hiptensorContractionFind_t */
 typedef struct htContractionPlan  htContractionPlan;  /* hiptensorContractionPlan_t */
+typedef struct htScaledContractionPlan htScaledContractionPlan; /* no counterpart in the reference */
+typedef struct htCrossEntropyPlan      htCrossEntropyPlan;      /* no counterpart in the reference */
 
 /* library/include/hiptensor/hiptensor.hpp:41,46 (library/src/hiptensor.cpp:35-104) */
 int htCreate(htHandle** handle);
@@ -36,7 +38,8 @@ int htDestroy(htHandle* handle);
 const char* htGetErrorString(int status);
 
 /* hiptensor.hpp:60-66 (hiptensor.cpp:106-214). strides == NULL: packed, LAST mode fastest.
- * dataType: 0 f32, 1 f64, 2 f16, 14 bf16. unaryOp: 1 identity, 2 "sqrt" (= square). */
+ * dataType: 0 f32, 1 f64, 2 f16, 14 bf16, 4 cf32, 5 cf64, and for the block-scaled operations 28 e4m3, 29 e5m2.
+ * unaryOp: 1 identity, 2 "sqrt" (= square). */
 int htCreateTensorDescriptor(const htHandle* handle, htTensorDescriptor** desc, uint32_t numModes,
                              const int64_t* lens, const int64_t* strides, int dataType, int unaryOp);
 int htDestroyTensorDescriptor(htTensorDescriptor* desc);
@@ -125,6 +128,70 @@ int htReductionNoAlloc(const htHandle* handle, const void* alpha, const void* A,
 int htReductionFinish(const htHandle* handle, const void* alpha, const void* partial, const void* beta, const void* C,
                       void* D, const htTensorDescriptor* descD, int typeCompute, void* stream);
 
+/* ---- 8-bit tensors with a scale for each block of 128 (no counterpart in the reference) ----
+ *
+ * htBlockQuantize writes A[modeA] (f32, f16, bf16) as Q[modeQ] (e4m3 or e5m2; the modes of A in any order) and f32
+ * scales S, so that Q * S is A again up to the 8-bit rounding. blockA gives 1 or 128 for each mode of A; one or two modes
+ * of extent above 1 may have 128. S has A's modes in A's order with extents ceil(extent / block). For every block
+ *     a = max(max |A|, 2^-100),  S = a / q,  Q = A * (q / a) rounded once to the nearest 8-bit number, ties to even,
+ * with q = 448 (e4m3) or 57344 (e5m2); S and q / a are f32 numbers. A block with a NaN gets the scale NaN, one with an
+ * infinity the scale infinity: multiplied out, all of either is NaN. Strides of A, Q and S are the caller's (an output
+ * needs a place for every element); the modes of block 1 must fold into one (two blocked modes) or two modes. What lies
+ * between the rows of Q and S (padding) stays as it was. A contiguous mode and rows at multiples of 16 bytes run fastest.
+ *
+ * Returns 15 for types, operators and mode groups outside this, 7 for extents that do not fit together. */
+int htBlockQuantize(const htHandle* handle, const void* A, const htTensorDescriptor* descA, const int32_t* modeA,
+                    const uint32_t* blockA, void* Q, const htTensorDescriptor* descQ, const int32_t* modeQ, float* S,
+                    const htTensorDescriptor* descS, void* stream);
+
+/* D[modeD] = alpha * sum over the contracted mode of (A * scaleA) (B * scaleB), + beta * C. A and B are e4m3 or e5m2 (each
+ * its own), D is f32, f16 or bf16, C (descC == NULL: none) is described as D is. descScaleA / blockA and descScaleB /
+ * blockB are those of htBlockQuantize for A's and B's modes. One mode is contracted, with block 128 in both operands; the
+ * free modes of an operand fold into one mode, of block 1 or 128. Each block's products are summed in f32, multiplied by the two
+ * scales (one after the other, so that only the result has to be in f32's range), and summed in f32 over the blocks.
+ * typeCompute: 4 (f32); alpha and beta point to floats. A mode in A, B and D is not supported (15), as in htContraction. No
+ * workspace is needed, and a plan may be used by several calls and streams at once. Operands that are contiguous along the
+ * contracted mode, with rows at multiples of 16 bytes, run on the tensor cores; any other strides on FMA. */
+int htCreateScaledContractionPlan(const htHandle* handle, htScaledContractionPlan** plan, const htTensorDescriptor* descA,
+                                  const int32_t* modeA, const htTensorDescriptor* descScaleA, const uint32_t* blockA,
+                                  const htTensorDescriptor* descB, const int32_t* modeB, const htTensorDescriptor* descScaleB,
+                                  const uint32_t* blockB, const htTensorDescriptor* descC, const htTensorDescriptor* descD,
+                                  const int32_t* modeD, int typeCompute);
+int htDestroyScaledContractionPlan(htScaledContractionPlan* plan);
+int htScaledContraction(const htHandle* handle, const htScaledContractionPlan* plan, const void* alpha, const void* A,
+                        const float* scaleA, const void* B, const float* scaleB, const void* beta, const void* C, void* D,
+                        void* stream);
+
+/* ---- softmax cross entropy of a linear head (no counterpart in the reference) ----
+ *
+ * Logits z = alpha * (H contracted with W) are never kept: they are made, used and dropped piece by piece of the
+ * vocabulary. The modes that H and W share are contracted, H's other modes are the tokens (numbered in modeH's order, the
+ * last one fastest), W's other modes the classes (numbered likewise). H and W are f16, bf16 or f32, both the same, and start at
+ * multiples of 16 bytes; targets are int64, loss, lse and gradLoss f32, one packed value for each token.
+ *     lse = log sum over classes of exp z,   loss = lse - z[target];   loss = 0 where target == ignoreIndex
+ *     P = (exp(z - lse) - [class == target]) * gradLoss * alpha, 0 where target == ignoreIndex
+ *     dH = P contracted with W (laid out like H),   dW = P contracted with H (laid out like W)
+ * htCrossEntropyGradient takes lse as htCrossEntropy wrote it; dH or dW may be NULL (not wanted). Rows of H whose target is
+ * ignored take no part in the gradient, whatever they hold. A target that is neither a class nor ignoreIndex reads
+ * nothing out of range: its loss is NaN, its row of P zero, and the next call on the handle returns 13
+ * (EXECUTION_FAILED) once. P is rounded to the type of H (f16: scaled by a power of two for max |gradLoss * alpha|), sums are f32.
+ *
+ * The workspace holds the pieces: any size from htCrossEntropyGetWorkspaceSize's MIN on (19 below it); with more, pieces
+ * are larger and fewer. gradient: 0 for htCrossEntropy, 1 for htCrossEntropyGradient. Two calls that run at the same time (two
+ * streams, two captured graphs) need a workspace each. Results do not depend on other calls and are the same every time
+ * for the same workspace size. */
+int htCreateCrossEntropyPlan(const htHandle* handle, htCrossEntropyPlan** plan, const htTensorDescriptor* descH,
+                             const int32_t* modeH, const htTensorDescriptor* descW, const int32_t* modeW, int64_t ignoreIndex,
+                             int typeCompute);
+int htDestroyCrossEntropyPlan(htCrossEntropyPlan* plan);
+int htCrossEntropyGetWorkspaceSize(const htHandle* handle, const htCrossEntropyPlan* plan, int gradient, int pref,
+                                   uint64_t* workspaceSize);
+int htCrossEntropy(const htHandle* handle, const htCrossEntropyPlan* plan, const void* alpha, const void* H, const void* W,
+                   const int64_t* targets, float* loss, float* lse, void* workspace, uint64_t workspaceSize, void* stream);
+int htCrossEntropyGradient(const htHandle* handle, const htCrossEntropyPlan* plan, const void* alpha, const void* H,
+                           const void* W, const int64_t* targets, const float* lse, const float* gradLoss, void* dH, void* dW,
+                           void* workspace, uint64_t workspaceSize, void* stream);
+
 /* hiptensor.hpp:308-338 (library/src/logger.cpp). mask: OR of 1 error, 2 perf, 4 hint, 8 heuristics, 16 api. */
 int htLoggerSetMask(int32_t mask);
 int htLoggerOpenFile(const char* logFile);
@@ -150,7 +217,8 @@ int htDescribeContractionPlan(uint32_t numModesA, const int64_t* lensA, const in
  * For tests and the bench, to show which CUDA path ran. */
 const char* htLastKernelName(void);
 /* Device status word of the handle: 0, or the code a kernel left when one of its bounded device-side waits ran
- * out (1 permutation, 2 single-CTA f16 kernel, 3 CTA-pair f16 kernel, 4 fp32 tensor-core kernel). Reading does not
+ * out (1 permutation, 2 single-CTA f16 kernel, 3 CTA-pair f16 kernel, 4 fp32 tensor-core kernel, 5 block-scaled 8-bit
+ * kernel, 6 cross-entropy kernel), or 7 when a cross entropy met a target outside the vocabulary. Reading does not
  * clear it; the next operation on the handle reports HIPTENSOR_STATUS_EXECUTION_FAILED once and clears it. No
  * reference counterpart: the reference's kernels have no device-side waits. */
 int htGetDeviceStatus(const htHandle* handle, int32_t* status);

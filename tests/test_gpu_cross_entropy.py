@@ -1,0 +1,340 @@
+"""Linear cross entropy and its gradient on the GPU against their definitions in 64 bits."""
+import pytest
+import torch
+
+import hiptensor_b200 as ht
+import training_helpers as ref
+
+pytestmark = pytest.mark.gpu
+KIND = {v: k for k, v in ref.TYPES.items()}
+IGNORE = -100
+
+
+@pytest.fixture(scope="module")
+def h():
+    return ht.Handle()
+
+
+def desc(h, x):
+    return h.tensor_descriptor(x.shape, x.stride(), KIND[x.dtype])
+
+
+def inputs(t, v, d, kind, seed=5, ignored=0.2, ldpad=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    H = torch.randn(t, d + ldpad, generator=g, device="cuda").to(kind)[:, :d]
+    W = (torch.randn(v, d + ldpad, generator=g, device="cuda") * 2 / d ** 0.5).to(kind)[:, :d]
+    y = torch.randint(0, v, (t,), generator=g, device="cuda")
+    y[torch.rand(t, generator=g, device="cuda") < ignored] = IGNORE
+    gl = torch.rand(t, generator=g, device="cuda") * (100.0 if kind == torch.float16 else 1.0) / t
+    return H, W, y, gl
+
+
+class Call:
+    """One plan with its buffers, forward and backward."""
+
+    def __init__(self, h, H, W, y, gl, modes=((0, 2), (1, 2)), alpha=1.0, ignore=IGNORE, pref=ht.WORKSPACE_RECOMMENDED):
+        self.h, self.H, self.W, self.y, self.gl, self.alpha, self.ignore = h, H, W, y, gl, alpha, ignore
+        self.plan = h.cross_entropy_plan(desc(h, H), modes[0], desc(h, W), modes[1], ignore)
+        sizes = [h.cross_entropy_workspace_size(self.plan, g, pref) for g in (False, True)]
+        self.ws = [torch.full((n,), 0xFF, device="cuda", dtype=torch.uint8) for n in sizes]  # NaN in every type
+        t = y.numel()
+        self.loss, self.lse = torch.full((t,), 9.0, device="cuda"), torch.full((t,), 9.0, device="cuda")
+        self.dH, self.dW = torch.empty_strided(H.shape, H.stride(), dtype=H.dtype, device="cuda"), torch.empty_strided(
+            W.shape, W.stride(), dtype=W.dtype, device="cuda")
+
+    def forward(self, stream=None):
+        self.h.cross_entropy(self.plan, self.alpha, self.H, self.W, self.y, self.loss, self.lse, self.ws[0], self.ws[0].numel(), stream)
+
+    def backward(self, stream=None, want=(True, True)):
+        self.h.cross_entropy_gradient(self.plan, self.alpha, self.H, self.W, self.y, self.lse, self.gl, self.dH if want[0] else None,
+                                      self.dW if want[1] else None, self.ws[1], self.ws[1].numel(), stream)
+
+    def check(self, H2=None, W2=None):
+        """Against 64 bits; H2 / W2: H and W as matrices where they are not."""
+        H, W = self.H if H2 is None else H2, self.W if W2 is None else W2
+        within(*ref.loss(H, W, self.y, self.alpha, self.ignore), self.loss, self.lse)
+
+    def check_gradient(self, dH=None, dW=None, H2=None, W2=None):
+        H, W = self.H if H2 is None else H2, self.W if W2 is None else W2
+        a, b, ea, eb = ref.gradient(H, W, self.y, self.lse, self.gl, self.alpha, self.ignore)
+        within(a, b, ea, eb, self.dH if dH is None else dH, self.dW if dW is None else dW)
+
+
+def within(a, b, ea, eb, x, y):
+    for want, bound, got in ((a, ea, x), (b, eb, y)):
+        off = (got.double() - want).abs()
+        assert bool((off <= bound).all()), float((off - bound).nan_to_num(nan=9e9).max())
+
+
+ALL = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.mark.parametrize("pref", [ht.WORKSPACE_MIN, ht.WORKSPACE_MAX])
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t,v,d", [(1, 1, 1), (1, 1000, 64), (2, 257, 8), (17, 1031, 136), (130, 2000, 72), (300, 777, 260),
+                                   (513, 513, 64), (700, 4100, 520)])
+def test_sizes(h, t, v, d, kind, pref):
+    c = Call(h, *inputs(t, v, d, kind), pref=pref)
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+    assert h.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t,v,d,ldpad", [(5, 300, 33, 0), (260, 700, 101, 0), (260, 700, 101, 3), (64, 1000, 64, 8)])
+def test_odd_widths_and_padded_rows(h, t, v, d, ldpad, kind):
+    c = Call(h, *inputs(t, v, d, kind, ldpad=ldpad))
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_tokens_in_several_modes_and_weights_the_other_way_round(h, kind):
+    """The hidden states without the last position of every sequence (modes that do not fold), W stored [d, v]."""
+    full, W, _, _ = inputs(7 * 21, 600, 64, kind)
+    H = full.view(7, 21, 64)[:, :-1]
+    y = torch.randint(0, 600, (140,), device="cuda")
+    gl = torch.rand(140, device="cuda") / 140
+    Wt = W.T.contiguous()
+    c = Call(h, H, Wt, y, gl, modes=((5, 0, 2), (2, 1)))
+    c.dH = torch.full_like(full, 3.0).view(7, 21, 64)[:, :-1]
+    c.forward()
+    c.check(H.reshape(140, 64), W)
+    c.backward()
+    c.check_gradient(c.dH.reshape(140, 64), c.dW.T, H.reshape(140, 64), W)
+    assert bool((c.dH._base.view(7, 21, 64)[:, -1] == 3).all())
+
+
+@pytest.mark.parametrize("kind", ALL)
+def test_what_ignored_tokens_hold_counts_for_nothing(h, kind):
+    H, W, y, gl = inputs(200, 900, 128, kind)
+    H[y == IGNORE] = float("nan")
+    H[torch.nonzero(y == IGNORE)[0]] = float("inf")
+    gl[y == IGNORE] = float("nan")
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    keep = y != IGNORE
+    assert bool((c.loss[~keep] == 0).all()) and bool(c.loss[keep].isfinite().all())
+    c.backward()
+    assert bool((c.dH[~keep] == 0).all())
+    gz = torch.where(keep, gl, torch.zeros_like(gl))
+    a, b, ea, eb = ref.gradient(H, W, y, c.lse, gz, 1.0, IGNORE)
+    within(a, b, ea, eb, c.dH, c.dW)
+
+
+@pytest.mark.parametrize("kind", ALL)
+def test_every_token_ignored(h, kind):
+    H, W, y, gl = inputs(70, 300, 64, kind)
+    y[:] = IGNORE
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    c.backward()
+    assert bool((c.loss == 0).all()) and bool((c.dH == 0).all()) and bool((c.dW == 0).all())
+
+
+def test_an_ignored_index_inside_the_vocabulary(h):
+    H, W, y, gl = inputs(100, 300, 64, torch.bfloat16, ignored=0)
+    y[::3] = 0
+    c = Call(h, H, W, y, gl, ignore=0)
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+
+
+def test_a_target_outside_the_vocabulary(h):
+    H, W, y, gl = inputs(100, 300, 64, torch.bfloat16, ignored=0)
+    y[3], y[50] = 300, -1
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    torch.cuda.synchronize()
+    assert h.device_status() == 7
+    assert torch.equal(c.loss.isnan(), (y < 0) | (y >= 300))
+    with pytest.raises(ht.HiptensorError) as e:
+        c.backward()
+    assert e.value.status == ht.STATUS_EXECUTION_FAILED
+    c.backward()
+    c.check_gradient()
+    assert bool((c.dH[3] == 0).all())
+    with pytest.raises(ht.HiptensorError):
+        c.forward()
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("alpha", [-0.5, 30.0])
+def test_alpha_and_large_logits(h, kind, alpha):
+    H, W, y, gl = inputs(150, 1300, 96, kind)
+    c = Call(h, H, W, y, gl, alpha=alpha)
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+
+
+def test_infinite_logits(h):
+    H, W, y, gl = inputs(40, 600, 64, torch.bfloat16, ignored=0)
+    H[:], y[:] = H.abs() + 0.1, 5
+    W[17], W[400] = -float("inf"), -float("inf")
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    keep = [i for i in range(600) if i not in (17, 400)]
+    lse = torch.logsumexp(H.double() @ W[keep].double().T, 1)
+    assert bool(((c.lse.double() - lse).abs() < 2.0 ** -12 * (1 + lse.abs())).all())
+    W[17] = float("inf")
+    c.forward()
+    assert bool((c.lse == float("inf")).all())
+    W[17] = float("nan")
+    c.forward()
+    assert bool(c.lse.isnan().all()) and bool(c.loss.isnan().all())
+
+
+@pytest.mark.parametrize("want", [(True, False), (False, True)])
+def test_one_gradient_alone(h, want):
+    H, W, y, gl = inputs(300, 900, 128, torch.bfloat16)
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    c.backward()
+    both = c.dH.clone(), c.dW.clone()
+    c.dH.fill_(7), c.dW.fill_(7)
+    c.backward(want=want)
+    for got, before, wanted in zip((c.dH, c.dW), both, want):
+        assert torch.equal(got, before) if wanted else bool((got == 7).all())
+
+
+@pytest.mark.parametrize("kind", ALL)
+def test_no_tokens(h, kind):
+    H, W, y, gl = inputs(0, 300, 64, kind)
+    c = Call(h, H, W, y, gl)
+    c.dW.fill_(5)
+    c.forward()
+    c.backward()
+    assert bool((c.dW == 0).all())
+
+
+def test_too_little_workspace(h):
+    H, W, y, gl = inputs(100, 3000, 64, torch.bfloat16)
+    c = Call(h, H, W, y, gl, pref=ht.WORKSPACE_MIN)
+    for k, call in enumerate((c.forward, c.backward)):
+        full = c.ws[k]
+        c.ws[k] = full[:-1]
+        with pytest.raises(ht.HiptensorError) as e:
+            call()
+        assert e.value.status == ht.STATUS_INSUFFICIENT_WORKSPACE
+        c.ws[k] = full
+        call()
+
+
+def test_unaligned_workspace_and_refused_pointers(h):
+    H, W, y, gl = inputs(100, 3000, 64, torch.bfloat16)
+    c = Call(h, H, W, y, gl, pref=ht.WORKSPACE_MIN)
+    c.ws = [torch.empty(w.numel() + 3, device="cuda", dtype=torch.uint8)[3:] for w in c.ws]
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+    c.H = torch.empty(100 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:]
+    for call in (c.forward, c.backward):
+        with pytest.raises(ht.HiptensorError) as e:
+            call()
+        assert e.value.status == ht.STATUS_INVALID_VALUE
+
+
+@pytest.mark.parametrize("kind", ALL)
+def test_the_gradient_is_the_loss_s_slope(h, kind):
+    """Differences of the loss along a direction, in f32 from the operator itself, against the gradient's product with it."""
+    H, W, y, gl = inputs(60, 500, 64, torch.float32)
+    H, W = H.to(kind).float(), W.to(kind).float()
+    c = Call(h, H.to(kind), W.to(kind), y, torch.ones_like(gl))
+    c.forward()
+    c.backward()
+    u, v = torch.randn_like(H), torch.randn_like(W) * 0.1
+    f = Call(h, H, W, y, torch.ones_like(gl))
+    e, ends = 2.0 ** -6, []
+    for s in (e, -e):
+        f.H, f.W = H + s * u, W + s * v
+        f.forward()
+        ends.append(f.loss.double().sum())
+    slope = float((ends[0] - ends[1]) / (2 * e))
+    exact = float((c.dH.double() * u).sum() + (c.dW.double() * v).sum())
+    # third derivatives times e^2 / 6 (logits move by about 2 a unit), and the gradient's own rounding over its terms
+    size = float((c.dH.double() * u).norm() + (c.dW.double() * v).norm())
+    assert abs(slope - exact) <= 60 * 8 * e * e / 6 + 8 * ref.half_step(kind) * size + 60 * 2.0 ** -16 / e
+
+
+def test_twice_the_same_and_two_captured_graphs(h):
+    H, W, y, gl = inputs(333, 5000, 256, torch.bfloat16)
+    one, two = Call(h, H, W, y, gl), Call(h, H.flip(0).contiguous(), W, y.flip(0).contiguous(), gl)
+    for c in (one, two):
+        c.forward()
+        c.backward()
+    first = [x.clone() for x in (one.loss, one.dH, one.dW, two.loss, two.dH, two.dW)]
+    graphs = []
+    for c in (one, two):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            c.forward(torch.cuda.current_stream())
+            c.backward(torch.cuda.current_stream())
+        graphs.append((g, side))
+    for c in (one, two):
+        for x in (c.loss, c.lse, c.dH, c.dW):
+            x.fill_(0)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, side in graphs:  # at the same time: each has its own workspace
+            with torch.cuda.stream(side):
+                g.replay()
+    torch.cuda.synchronize()
+    for x, want in zip((one.loss, one.dH, one.dW, two.loss, two.dH, two.dW), first):
+        assert torch.equal(x, want)
+
+
+def test_a_training_step_in_8_bits(h):
+    """Activations and weights quantised, a linear layer, the head's loss and gradient, and the layer's two gradient products."""
+    t, k, n, v = 300, 512, 384, 2000
+    E4, E5 = ht.R_8F_E4M3, ht.R_8F_E5M2
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(t, k, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randn(n, k, generator=g, device="cuda") / k ** 0.5
+    head = (torch.randn(v, n, generator=g, device="cuda") / n ** 0.5).to(torch.bfloat16)
+    y = torch.randint(0, v, (t,), generator=g, device="cuda")
+    kinds = {E4: torch.float8_e4m3fn, E5: torch.float8_e5m2}
+    kind_of = lambda z: {torch.bfloat16: ht.R_16BF, torch.float32: ht.R_32F, torch.float8_e4m3fn: E4, torch.float8_e5m2: E5}[z.dtype]  # noqa: E731
+    d = lambda z: h.tensor_descriptor(z.shape, z.stride(), kind_of(z))  # noqa: E731
+
+    def quant(z, block, to, turned=False):
+        ld = -(-(z.shape[0] if turned else z.shape[1]) // 16) * 16
+        q = torch.zeros(z.shape[1] if turned else z.shape[0], ld, device="cuda", dtype=kinds[to])
+        q = q[:, :z.shape[0]] if turned else q[:, :z.shape[1]]
+        s = torch.empty([-(-a // b) for a, b in zip(z.shape, block)], device="cuda")
+        h.block_quantize(z, d(z), (0, 1), block, q, d(q), (1, 0) if turned else (0, 1), s, d(s))
+        return (q, s.T, block[::-1]) if turned else (q, s, block)
+
+    def product(A, B, out, c=None):
+        (a, sa, ba), (b, sb, bb) = A, B
+        plan = h.scaled_contraction_plan(d(a), (0, 2), d(sa), ba, d(b), (1, 2), d(sb), bb, None if c is None else d(out), d(out), (0, 1))
+        h.scaled_contraction(plan, 1.0, a, sa, b, sb, 0.0 if c is None else 1.0, c, out)
+        want, bound = ref.scaled(a, sa, ba, b, sb, bb, 1.0, 1.0, c)
+        tail = 1.01 * 2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -23
+        return want, bound + tail * want.abs()
+
+    hidden = torch.empty(t, n, device="cuda", dtype=torch.bfloat16)
+    master = torch.randn(n, k, device="cuda") * 1e-3
+    before = master.clone()
+    want, bound = product(quant(x, (1, 128), E4), quant(w, (128, 128), E4), hidden)
+    assert bool(((hidden.double() - want).abs() <= bound).all())
+    c = Call(h, hidden, head, y, torch.full((t,), 1.0 / t, device="cuda"))
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+    dx = torch.empty_like(x)
+    want, bound = product(quant(c.dH, (1, 128), E5), quant(w, (128, 128), E4, turned=True), dx)
+    assert bool(((dx.double() - want).abs() <= bound).all())
+    want, bound = product(quant(c.dH, (128, 1), E5, turned=True), quant(x, (128, 1), E4, turned=True), master, before)
+    assert bool(((master.double() - want).abs() <= bound).all())
