@@ -1,0 +1,433 @@
+// Pipeline shared by the block-scaled 8-bit contraction and the cross-entropy kernels: tiles of X Y^T (two K-major matrices)
+// on the 5th-generation tensor cores whose sums are carried on in REGISTERS. The K range of a tile is cut into chunks; each
+// chunk is summed in tensor memory from zero and then added to the running sums of the epilogue threads:
+//   * 8-bit operands with scales per block of 128: a chunk is one block, its sums are multiplied by the block's scales on
+//     the way;
+//   * half-precision operands: the tensor cores truncate when they add a product sum to an accumulator (measured: sums over
+//     4096 elements are short by 3.6e-6 of their value), so a long sum is made of chunks of 1024 whose sums are added with
+//     rounding.
+//
+// Roles: warp 0 loads by TMA, one thread of warp 1 issues the MMAs, warps 4 .. 11 are the epilogue. Tensor memory holds two
+// chunks: while one is read, the next is summed. Epilogue warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and half
+// (w - 4) / 4 of the columns, so a thread owns one row and TN / 2 neighbouring columns of the tile.
+//
+// PAIR: two CTAs work on a 256 x 256 tile (cta_group::2), each with 128 rows of X and half of the 256 rows of Y in shared
+// memory; halves what a CTA loads for Y. Otherwise a CTA has a 128 x TN tile, and a cluster of `ksplit` CTAs may cut a
+// tile's K range.
+#pragma once
+
+#include "tcgen05_util.cuh"
+
+namespace htb
+{
+    namespace
+    {
+        constexpr int kAccThreads = 384; // three warpgroups: loads and MMAs, two of the epilogue
+        constexpr int kAccEpi     = 256; // epilogue threads
+        // Registers a thread: 168 at launch (384 x 168 = 64512 of the SM's 65536). Wide tiles need more for the running sums:
+        // the first warpgroup gives some back, the epilogue takes them: 128 x 56 + 256 x 224 = 64512.
+        constexpr int kAccRegs = 168, kAccRegsLoad = 56, kAccRegsEpi = 224;
+        static_assert(128 * kAccRegsLoad + 256 * kAccRegsEpi <= kAccThreads * kAccRegs, "the shares exceed what the launch has");
+        constexpr int kAccMaxStages = 12;
+
+        struct AccArgs
+        {
+            int      tilesM, tilesN; // tiles of (PAIR ? 256 : 128) rows and TN columns
+            int      groupM; // tiles of M that are walked together, for the sake of L2
+            int      kBlocks; // 128-byte blocks along K
+            int      chunk; // K blocks per chunk
+            int      kElems; // elements of a 128-byte block: 128 (8 bit) or 64
+            int      ksplit; // CTAs of a cluster that share a tile (not PAIR)
+            int      stages;
+            uint32_t idesc;
+            int*     status;
+            int      statusCode;
+        };
+
+        __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi)
+        {
+            uint64_t r;
+            asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+            return r;
+        }
+        __device__ __forceinline__ uint64_t pack2(float lo, float hi)
+        {
+            return pack2(__float_as_uint(lo), __float_as_uint(hi));
+        }
+        __device__ __forceinline__ float2 unpack2(uint64_t v)
+        {
+            uint32_t lo, hi;
+            asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+            return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+        }
+        __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+        {
+            uint64_t r;
+            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+            return r;
+        }
+        __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+        {
+            uint64_t r;
+            asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+            return r;
+        }
+        __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+        {
+            uint64_t r;
+            asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+            return r;
+        }
+
+        // N columns of this warp's 32 lanes, one row a thread; the values are there after tmemWait()
+        template <int N>
+        __device__ __forceinline__ void tmemLoad(uint32_t addr, uint32_t (&v)[N])
+        {
+            if constexpr(N == 32)
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                             "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                             "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                             : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                               "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                               "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+                               "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+                               "=r"(v[30]), "=r"(v[31])
+                             : "r"(addr)
+                             : "memory");
+            else
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                             "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                             : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                               "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                             : "r"(addr)
+                             : "memory");
+        }
+        __device__ __forceinline__ void tmemWait()
+        {
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        }
+
+        __device__ __forceinline__ void tmaLoadPair2(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1)
+        {
+            asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+                         "[%2];" ::"r"(dst),
+                         "l"(map), "r"(bar), "r"(c0), "r"(c1)
+                         : "memory");
+        }
+
+        template <bool PAIR, bool F8>
+        __device__ __forceinline__ void issueMma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+        {
+            if constexpr(PAIR && F8)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                             "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                             "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                             : "memory");
+            else if constexpr(PAIR)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                             "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                             "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                             : "memory");
+            else if constexpr(F8)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                             "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                             "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                             : "memory");
+            else
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                             "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                             "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                             : "memory");
+        }
+        template <bool PAIR>
+        __device__ __forceinline__ void commitTo(uint32_t bar)
+        {
+            if constexpr(PAIR)
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                             "h"((unsigned short)3)
+                             : "memory");
+            else
+                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+        }
+
+        // tile u of the walk: groups of groupM tiles of M, inside a group M fastest
+        __device__ __forceinline__ void tileOf(const AccArgs& a, int u, int& tm, int& tn)
+        {
+            const int per = a.groupM * a.tilesN, g = u / per, in = u - g * per;
+            const int gm  = min(a.groupM, a.tilesM - g * a.groupM);
+            tn            = in / gm;
+            tm            = g * a.groupM + in - tn * gm;
+        }
+
+        // Epi: the epilogue, one object per epilogue thread:
+        //   Epi(args, warp 0 .. 7, lane, shared memory of this warp)
+        //   begin(row, col, kb0)      the thread's row and first column in the product; K blocks from kb0 on
+        //   add(chunk, taddr, first)  reads the chunk's sums from tensor memory and adds them
+        //   end(...)                  the tile's sums are complete
+        // Registers that a kernel with wide tiles was built with must be what the shares above add up to: a smaller
+        // launch would make the epilogue wait for registers that are not there.
+        inline cudaError_t accCheckRegs(const void* kernel, int tn)
+        {
+            if(tn < 128)
+                return cudaSuccess;
+            cudaFuncAttributes  at;
+            const cudaError_t e = cudaFuncGetAttributes(&at, kernel);
+            if(e != cudaSuccess)
+                return e;
+            return at.numRegs >= kAccRegs ? cudaSuccess : cudaErrorInvalidKernelImage;
+        }
+
+        template <class Epi, bool PAIR, int TN, bool F8>
+        __global__ void __launch_bounds__(kAccThreads, 1)
+            accumulate_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapY, const __grid_constant__ AccArgs a,
+                              const __grid_constant__ typename Epi::Args ea)
+        {
+            constexpr int      ROWS   = PAIR ? 256 : 128;
+            constexpr uint32_t kStage = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u; // 128 rows of X, this CTA's rows of Y
+            constexpr uint32_t kCols  = 2 * TN < 32 ? 32 : 2 * TN;
+            extern __shared__ unsigned char smemRaw[];
+            unsigned char* tiles = (unsigned char*)((uintptr_t(smemRaw) + 1023) & ~uintptr_t(1023));
+            __shared__ __align__(8) unsigned long long fullBar[kAccMaxStages], emptyBar[kAccMaxStages];
+            __shared__ __align__(8) unsigned long long tmemFullBar[2], tmemEmptyBar[2];
+            __shared__ uint32_t tmemBase;
+            __shared__ int      abortFlag;
+
+            const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+            const uint32_t rank = (PAIR || a.ksplit > 1) ? clusterRank() : 0u;
+            const bool     leader = !PAIR || rank == 0;
+            const int      csize = PAIR ? 2 : a.ksplit;
+            const int      clusterId = int(blockIdx.x) / csize, numClusters = int(gridDim.x) / csize;
+            const bool     clustered = csize > 1;
+
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            if(threadIdx.x == 32)
+            {
+                prefetchTensorMap(&mapX);
+                prefetchTensorMap(&mapY);
+            }
+            if(threadIdx.x == 0)
+            {
+                abortFlag = 0;
+                for(int s = 0; s < a.stages; s++)
+                {
+                    mbarInit(smemAddr(&fullBar[s]), 1);
+                    mbarInit(smemAddr(&emptyBar[s]), 1);
+                }
+                for(int i = 0; i < 2; i++)
+                {
+                    mbarInit(smemAddr(&tmemFullBar[i]), 1);
+                    mbarInit(smemAddr(&tmemEmptyBar[i]), (PAIR ? 2 : 1) * (kAccEpi / 32));
+                }
+                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            }
+            if(warp == 1)
+            {
+                if constexpr(PAIR)
+                {
+                    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&tmemBase)), "r"(kCols)
+                                 : "memory");
+                    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+                }
+                else
+                {
+                    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&tmemBase)), "r"(kCols)
+                                 : "memory");
+                    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncthreads();
+            if(clustered)
+                clusterSync(); // the peers' barriers exist before anything signals them
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t tmem   = tmemBase;
+            volatile int*  abortP = &abortFlag;
+            const uint32_t tilesAddr = smemAddr(tiles), fullAddr = smemAddr(&fullBar[0]), emptyAddr = smemAddr(&emptyBar[0]);
+            const int      units = a.tilesM * a.tilesN;
+            // K blocks of this CTA: all, or its part of a split tile
+            const int kbBegin = PAIR ? 0 : int((long long)a.kBlocks * int(rank) / a.ksplit);
+            const int kbEnd   = PAIR ? a.kBlocks : int((long long)a.kBlocks * (int(rank) + 1) / a.ksplit);
+            // global memory is read and written from here on: the grid ahead of this one must be complete
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+
+            constexpr bool kMoreRegs = TN >= 128;
+            if(warp < 4)
+            {
+                if constexpr(kMoreRegs)
+                    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAccRegsLoad));
+            if(warp == 0)
+            {
+                if(lane == 0)
+                {
+                    const uint32_t leaderFull = PAIR ? mapToRank(fullAddr, 0) : fullAddr;
+                    uint32_t       stage = 0, phase = 0;
+                    bool           ok = true;
+                    for(int u = clusterId; ok && u < units; u += numClusters)
+                    {
+                        int tm, tn;
+                        tileOf(a, u, tm, tn);
+                        const int x0 = tm * ROWS + (PAIR ? int(rank) * 128 : 0), y0 = tn * TN + (PAIR ? int(rank) * 128 : 0);
+                        for(int kb = kbBegin; kb < kbEnd; kb++)
+                        {
+                            ok = mbarWaitTight(emptyAddr + 8 * stage, phase ^ 1, abortP);
+                            if(!ok)
+                                break;
+                            const uint32_t dst = tilesAddr + stage * kStage, bar = leaderFull + 8 * stage;
+                            if(leader)
+                                mbarArriveExpectTx(fullAddr + 8 * stage, (PAIR ? 2 : 1) * kStage);
+                            const int k0 = kb * a.kElems;
+                            if constexpr(PAIR)
+                            {
+                                tmaLoadPair2(dst, &mapX, bar, k0, x0);
+                                tmaLoadPair2(dst + 16384, &mapY, bar, k0, y0);
+                            }
+                            else
+                            {
+                                const int cx[2] = {k0, x0}, cy[2] = {k0, y0};
+                                tmaLoad<2>(dst, &mapX, bar, cx);
+                                tmaLoad<2>(dst + 16384, &mapY, bar, cy);
+                            }
+                            if(++stage == uint32_t(a.stages))
+                            {
+                                stage = 0;
+                                phase ^= 1;
+                            }
+                        }
+                    }
+                }
+                if(!PAIR && clustered)
+                {
+                    __syncwarp();
+                    clusterSync(); // the two meeting points of the exchange (see the epilogue)
+                    clusterSync();
+                }
+            }
+            else if(warp == 1)
+            {
+                if(lane == 0 && leader)
+                {
+                    const uint64_t descX = smemDesc(tilesAddr), descY = smemDesc(tilesAddr + 16384);
+                    uint32_t       stage = 0, phase = 0, buf = 0, bufPhase = 0;
+                    bool           ok = true;
+                    for(int u = clusterId; ok && u < units; u += numClusters)
+                        for(int kb = kbBegin; ok && kb < kbEnd; kb += a.chunk)
+                        {
+                            ok = mbarWaitTight(smemAddr(&tmemEmptyBar[buf]), bufPhase ^ 1, abortP);
+                            if(!ok)
+                                break;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            const uint32_t d   = tmem + buf * TN;
+                            const int      end = min(kb + a.chunk, kbEnd);
+                            for(int k = kb; k < end; k++)
+                            {
+                                ok = mbarWaitTight(fullAddr + 8 * stage, phase, abortP);
+                                if(!ok)
+                                    break;
+                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                                const uint64_t off = uint64_t((stage * kStage) >> 4);
+#pragma unroll
+                                for(int s = 0; s < 4; s++) // 32 bytes of K each
+                                    issueMma<PAIR, F8>(d, descX + off + 2 * s, descY + off + 2 * s, a.idesc, (k != kb || s != 0) ? 1u : 0u);
+                                commitTo<PAIR>(emptyAddr + 8 * stage); // frees the stage once these MMAs have read it
+                                if(++stage == uint32_t(a.stages))
+                                {
+                                    stage = 0;
+                                    phase ^= 1;
+                                }
+                            }
+                            if(ok)
+                                commitTo<PAIR>(smemAddr(&tmemFullBar[buf]));
+                            buf ^= 1;
+                            bufPhase ^= buf == 0;
+                        }
+                }
+                if(!PAIR && clustered)
+                {
+                    __syncwarp();
+                    clusterSync();
+                    clusterSync();
+                }
+            }
+            else if(!PAIR && clustered)
+            {
+                clusterSync();
+                clusterSync();
+            }
+            }
+            else
+            {
+                if constexpr(kMoreRegs)
+                    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAccRegsEpi));
+                const int quad = warp & 3, half = (warp - 4) >> 2;
+                Epi       epi(ea, warp - 4, lane, tiles + size_t(a.stages) * kStage);
+                uint32_t  buf = 0, bufPhase = 0;
+                bool      ok = true;
+                int       syncs = 0;
+                const uint32_t emptyLeader = PAIR ? mapToRank(smemAddr(&tmemEmptyBar[0]), 0) : smemAddr(&tmemEmptyBar[0]);
+                for(int u = clusterId; ok && u < units; u += numClusters)
+                {
+                    int tm, tn;
+                    tileOf(a, u, tm, tn);
+                    const int     row = quad * 32 + lane;
+                    const int64_t r = int64_t(tm) * ROWS + (PAIR ? int(rank) * 128 : 0) + row, c = int64_t(tn) * TN + half * (TN / 2);
+                    epi.begin(r, c, kbBegin, kbEnd);
+                    for(int kb = kbBegin; kb < kbEnd; kb += a.chunk)
+                    {
+                        ok = __all_sync(0xffffffffu, mbarWait(smemAddr(&tmemFullBar[buf]), bufPhase, abortP));
+                        if(!ok)
+                            break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        epi.add(kb, tmem + (uint32_t(quad * 32) << 16) + buf * TN + uint32_t(half * (TN / 2)), kb == kbBegin);
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if(lane == 0)
+                        {
+                            if constexpr(PAIR)
+                                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(emptyLeader + 8 * buf)
+                                             : "memory");
+                            else
+                                mbarArrive(emptyLeader + 8 * buf);
+                        }
+                        buf ^= 1;
+                        bufPhase ^= buf == 0;
+                    }
+                    if(!ok)
+                        break;
+                    if constexpr(!PAIR)
+                    {
+                        if(clustered)
+                        {
+                            // K split: CTA r of the cluster finishes columns r TN / ksplit .. of the tile. Every CTA sends
+                            // the others their columns of its sums, into the (by then idle) stages, and adds what it
+                            // gets in the order of the ranks.
+                            clusterSync(); // every CTA of the cluster has its sums: all stages are idle
+                            epi.send(tilesAddr, rank, a.ksplit, row, half);
+                            clusterSync(); // the others' sums have arrived
+                            syncs = 2;
+                            epi.endSplit(tilesAddr, rank, a.ksplit, row, half, r, int64_t(tn) * TN);
+                            continue;
+                        }
+                    }
+                    epi.end(r, c);
+                }
+                for(; !PAIR && clustered && syncs < 2; syncs++)
+                    clusterSync(); // a CTA whose wait ran out still meets the others
+            }
+
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncthreads();
+            if(clustered)
+                clusterSync(); // all CTAs are done with tensor memory and with each other's barriers and shared memory
+            if(threadIdx.x == 0 && abortFlag && a.status)
+                atomicExch_system(a.status, a.statusCode);
+            if(warp == 1)
+            {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if constexpr(PAIR)
+                    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+                else
+                    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+            }
+        }
+    } // namespace
+} // namespace htb

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 
+#include "accumulate.cuh"
 #include "kernels.hpp"
 #include "scaled.hpp"
 
@@ -56,9 +57,11 @@ namespace htb
         {
             constexpr int    kStep = 32;
             __shared__ float a[kStep][65], b[kStep][65];
-            const int64_t    m0 = int64_t(blockIdx.x) * 64, n0 = int64_t(blockIdx.y) * 64;
             const int        tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
             const bool       aWide = p.typeA == CUDA_R_8F_E5M2, bWide = p.typeB == CUDA_R_8F_E5M2;
+            const int64_t    m0 = int64_t(blockIdx.x) * 64;
+            for(int64_t n0 = int64_t(blockIdx.y) * 64; n0 < p.N; n0 += int64_t(gridDim.y) * 64)
+            {
             float            sum[4][4] = {};
             for(int64_t k0 = 0; k0 < p.K; k0 += kScaleBlock)
             {
@@ -120,14 +123,401 @@ namespace htb
                     const float   v  = alpha * sum[i][j];
                     D[at]            = narrow<TD>(C ? fmaf(beta, widen(C[at]), v) : v);
                 }
+            }
+        }
+
+        // ------------------------------------------------------------------ tensor-core path
+        struct ScaledArgs
+        {
+            const float *sX, *sY; // scales of the operand on the rows' / columns' side of the tiles
+            int64_t      sxRow, sxK, syRow, syK;
+            int          blockX, blockY;
+            int64_t      rows, cols; // of the product
+            const void*  C;
+            void*        D;
+            int64_t      dRow, dCol;
+            float        alpha, beta;
+            int          vec; // columns contiguous, groups of four aligned
+        };
+
+        // Epilogue of accumulate_kernel: a chunk is one block of 128 along k. A thread multiplies the block's sums of its row by
+        // scaleX (one per thread and block) and scaleY (VECY: one per column, through shared memory; else one per block)
+        // and adds them to its running sums, two columns per instruction. Scales are fetched two blocks ahead.
+        template <typename TD, int TN, bool VECY>
+        struct ScaledEpi
+        {
+            using Args                = ScaledArgs;
+            static constexpr int COLS = TN / 2;
+            static constexpr int CH   = COLS < 32 ? COLS : 32; // columns per round of stores
+            static constexpr int CL   = (VECY && COLS == 128) ? 16 : CH; // columns per load from tensor memory (as registers allow)
+            static constexpr int PER  = VECY ? (COLS + 31) / 32 : 1; // column scales that a lane fetches
+
+            const Args&    a;
+            const int      warp, lane;
+            float*         slot; // of this warp: 4 KiB
+            uint64_t       acc[COLS / 2];
+            const float *  px, *py[PER];
+            float          x0, x1, y0[PER], y1[PER];
+            int            kbEnd;
+
+            __device__ ScaledEpi(const Args& args, int w, int l, unsigned char* smem)
+                : a(args)
+                , warp(w)
+                , lane(l)
+                , slot(reinterpret_cast<float*>(smem + w * 4096))
+            {
+            }
+            __device__ __forceinline__ void fetch(int kb, float& x, float (&y)[PER])
+            {
+                const bool in = kb < kbEnd;
+                x             = (px && in) ? __ldg(px + kb * a.sxK) : 0.f;
+#pragma unroll
+                for(int i = 0; i < PER; i++)
+                    y[i] = (py[i] && in) ? __ldg(py[i] + kb * a.syK) : 0.f;
+            }
+            __device__ __forceinline__ void begin(int64_t row, int64_t col, int kb0, int kb1)
+            {
+                kbEnd = kb1;
+                px    = row < a.rows ? a.sX + (a.blockX > 1 ? row / kScaleBlock : row) * a.sxRow : nullptr;
+#pragma unroll
+                for(int i = 0; i < PER; i++)
+                {
+                    const int64_t c = VECY ? col + i * 32 + lane : col;
+                    py[i] = (c < a.cols && (!VECY || i * 32 + lane < COLS)) ? a.sY + (VECY ? c : c / kScaleBlock) * a.syRow : nullptr;
+                }
+                fetch(kb0, x0, y0);
+                fetch(kb0 + 1, x1, y1);
+#pragma unroll
+                for(int j = 0; j < COLS / 2; j++)
+                    acc[j] = 0;
+            }
+            __device__ __forceinline__ void add(int kb, uint32_t taddr, bool)
+            {
+                const float x = x0;
+                float       y[PER];
+                x0 = x1;
+#pragma unroll
+                for(int i = 0; i < PER; i++)
+                {
+                    y[i]  = y0[i];
+                    y0[i] = y1[i];
+                }
+                fetch(kb + 2, x1, y1);
+                const float* ys = slot + (kb & 1) * COLS;
+                if constexpr(VECY)
+                {
+                    // two slots in turn: the warp barrier of the next block keeps a slot until every lane has read it
+#pragma unroll
+                    for(int i = 0; i < PER; i++)
+                        if(i * 32 + lane < COLS)
+                            slot[(kb & 1) * COLS + i * 32 + lane] = y[i];
+                    __syncwarp();
+                }
+                const uint64_t s = VECY ? pack2(x, x) : pack2(x * y[0], x * y[0]);
+                uint32_t buf[2][CL]; // the next columns are on their way while these are added
+                tmemLoad<CL>(taddr, buf[0]);
+#pragma unroll
+                for(int c = 0; c < COLS; c += CL)
+                {
+                    uint32_t(&v)[CL] = buf[(c / CL) & 1];
+                    tmemWait();
+                    if(c + CL < COLS)
+                        tmemLoad<CL>(taddr + c + CL, buf[(c / CL + 1) & 1]);
+#pragma unroll
+                    for(int j = 0; j < CL; j += 4)
+                    {
+                        uint64_t s0 = s, s1 = s;
+                        if constexpr(VECY)
+                        {
+                            const float4 q = *reinterpret_cast<const float4*>(ys + c + j);
+                            s0             = mul2(s, pack2(q.x, q.y));
+                            s1             = mul2(s, pack2(q.z, q.w));
+                        }
+                        acc[(c + j) / 2]     = fma2(pack2(v[j], v[j + 1]), s0, acc[(c + j) / 2]);
+                        acc[(c + j) / 2 + 1] = fma2(pack2(v[j + 2], v[j + 3]), s1, acc[(c + j) / 2 + 1]);
+                    }
+                }
+            }
+            __device__ __forceinline__ float sum(int j) const
+            {
+                const float2 f = unpack2(acc[j / 2]);
+                return (j & 1) ? f.y : f.x;
+            }
+            __device__ __forceinline__ TD finish(float v, int64_t at) const
+            {
+                v *= a.alpha;
+                return narrow<TD>(a.C ? fmaf(a.beta, widen(static_cast<const TD*>(a.C)[at]), v) : v);
+            }
+            // columns j0 .. j0 + W - 1 of this thread's sums (in w) to row, col0 + ..: through shared memory when the columns
+            // are contiguous, so that lanes that follow each other write (and read C) along a row; else as they are
+            template <int W>
+            __device__ __forceinline__ void store(const float (&w)[W], int64_t row, int64_t col0)
+            {
+                TD* D = static_cast<TD*>(a.D);
+                if(!a.vec)
+                {
+                    if(row < a.rows)
+                    {
+#pragma unroll
+                        for(int j = 0; j < W; j++)
+                            if(col0 + j < a.cols)
+                            {
+                                const int64_t at = row * a.dRow + (col0 + j) * a.dCol;
+                                D[at]            = finish(w[j], at);
+                            }
+                    }
+                    return;
+                }
+                constexpr int U = W / 4; // 16-byte units of a row, XORed with the row against bank conflicts
+                __syncwarp(); // the scales or the round before have been read
+#pragma unroll
+                for(int u = 0; u < U; u++)
+                    *reinterpret_cast<float4*>(slot + lane * W + ((u ^ (lane & (U - 1))) << 2))
+                        = make_float4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+                __syncwarp();
+                const int64_t row0 = row - lane;
+                const int     u = lane % U;
+                const int64_t c = col0 + 4 * u;
+#pragma unroll
+                for(int i = 0; i < U; i++)
+                {
+                    const int     rr = i * (32 / U) + lane / U;
+                    const float4  q  = *reinterpret_cast<const float4*>(slot + rr * W + ((u ^ (rr & (U - 1))) << 2));
+                    const int64_t at = (row0 + rr) * a.dRow + c;
+                    if(row0 + rr >= a.rows || c >= a.cols)
+                        continue;
+                    const float f[4] = {q.x, q.y, q.z, q.w};
+                    if(c + 4 <= a.cols)
+                    {
+                        struct alignas(4 * sizeof(TD)) Four
+                        {
+                            TD e[4];
+                        };
+                        Four o, in;
+                        if(a.C)
+                            in = *reinterpret_cast<const Four*>(static_cast<const TD*>(a.C) + at);
+#pragma unroll
+                        for(int j = 0; j < 4; j++)
+                        {
+                            const float v = f[j] * a.alpha;
+                            o.e[j]        = narrow<TD>(a.C ? fmaf(a.beta, widen(in.e[j]), v) : v);
+                        }
+                        *reinterpret_cast<Four*>(D + at) = o;
+                    }
+                    else
+                    {
+#pragma unroll
+                        for(int j = 0; j < 4; j++)
+                            if(c + j < a.cols)
+                                D[at + j] = finish(f[j], at + j);
+                    }
+                }
+            }
+            __device__ __forceinline__ void end(int64_t row, int64_t col)
+            {
+#pragma unroll
+                for(int c = 0; c < COLS; c += CH)
+                {
+                    float w[CH];
+#pragma unroll
+                    for(int j = 0; j < CH; j++)
+                        w[j] = sum(c + j);
+                    store<CH>(w, row, col + c);
+                }
+                __syncwarp(); // the slot is free for the next tile's scales
+            }
+            // exchange zone in the stages of CTA q: [sending rank][column of q's slice][128 rows]
+            __device__ __forceinline__ void send(uint32_t zone, uint32_t rank, int ksplit, int row, int half)
+            {
+                const int wide = TN / ksplit;
+#pragma unroll
+                for(int j = 0; j < COLS; j++)
+                {
+                    const int      col = half * COLS + j;
+                    const uint32_t q   = uint32_t(col / wide);
+                    if(q != rank)
+                    {
+                        const uint32_t dst = mapToRank(zone + uint32_t(((int(rank) * wide + col - int(q) * wide) * 128 + row) * 4), q);
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(sum(j)) : "memory");
+                    }
+                }
+            }
+            __device__ __forceinline__ void endSplit(uint32_t zone, uint32_t rank, int ksplit, int row, int half, int64_t r, int64_t col0)
+            {
+                const int wide = TN / ksplit, first = int(rank) * wide; // this CTA's columns of the tile
+#pragma unroll
+                for(int c = 0; c < COLS; c += 8)
+                {
+                    const int at = half * COLS + c - first; // a slice is a multiple of eight columns
+                    if(at < 0 || at >= wide)
+                        continue;
+                    float w[8];
+#pragma unroll
+                    for(int j = 0; j < 8; j++)
+                        w[j] = 0.f;
+                    for(int q = 0; q < ksplit; q++)
+#pragma unroll
+                        for(int j = 0; j < 8; j++)
+                        {
+                            float v = sum(c + j);
+                            if(q != int(rank))
+                                asm volatile("ld.shared.f32 %0, [%1];"
+                                             : "=f"(v)
+                                             : "r"(zone + uint32_t(((q * wide + at + j) * 128 + row) * 4))
+                                             : "memory");
+                            w[j] += v;
+                        }
+                    store<8>(w, r, col0 + half * COLS + c);
+                }
+            }
+        };
+
+        bool encodeRows(PFN_encodeTiled encode, CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64_t stride, int box)
+        {
+            cuuint64_t gdim[2] = {cuuint64_t(k), cuuint64_t(rows)}, gstr[1] = {rows > 1 ? cuuint64_t(stride) : cuuint64_t((k + 15) / 16 * 16)};
+            cuuint32_t bx[2] = {128, cuuint32_t(box)}, estr[2] = {1, 1};
+            return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstr, bx, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+                   == CUDA_SUCCESS;
+        }
+        // rows contiguous along k, starting at multiples of 16 bytes, no two of them in one place
+        bool rowsForTma(const void* base, int64_t k, int64_t rows, int64_t sK, int64_t sRow)
+        {
+            return (uintptr_t(base) & 15) == 0 && (sK == 1 || k == 1)
+                   && (rows == 1 || (sRow % 16 == 0 && sRow >= k && sRow < (int64_t(1) << 40)));
+        }
+
+        // which kernel a problem runs on
+        struct ScaledForm
+        {
+            bool swap; // B on the rows' side of the tiles
+            bool pair;
+            int  tn, ksplit;
+        };
+        ScaledForm formOf(const ScaledPlan& p, int sms)
+        {
+            ScaledForm    f{};
+            const int64_t kb = (p.K + 127) / 128, small = std::min(p.M, p.N), large = std::max(p.M, p.N);
+            // few rows on one side (a token, a few of them): that side becomes the columns of narrow tiles, the other
+            // one, the weights, fills the 128 rows
+            if(small <= 64)
+            {
+                f.swap = p.M < p.N;
+                f.tn   = small <= 32 ? 32 : 64;
+            }
+            else
+            {
+                f.swap = p.dN != 1 && p.dM == 1; // the result contiguous along the columns of the tiles
+                f.pair = ((p.M + 255) / 256) * ((p.N + 255) / 256) >= sms / 2 * 3 / 4;
+                f.tn   = f.pair ? 256 : 128;
+            }
+            f.ksplit            = 1;
+            const int64_t tiles = f.pair ? 0 : ((f.swap ? p.N : p.M) + 127) / 128 * (((f.swap ? p.M : p.N) + f.tn - 1) / f.tn);
+            while(!f.pair && f.ksplit < 4 && tiles * f.ksplit * 2 <= sms && kb >= f.ksplit * 4)
+                f.ksplit *= 2;
+            (void)large;
+            return f;
+        }
+
+        template <typename TD, bool PAIR, int TN, bool VECY>
+        cudaError_t launchTensor(const CUtensorMap& mapX, const CUtensorMap& mapY, AccArgs a, const ScaledArgs& ea, int smCount,
+                                 cudaStream_t stream)
+        {
+            using Epi               = ScaledEpi<TD, TN, VECY>;
+            auto           kernel   = accumulate_kernel<Epi, PAIR, TN, true>;
+            const uint32_t stage    = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
+            a.stages                = std::min<int>(kAccMaxStages, int(192 * 1024 / stage));
+            const size_t smem       = size_t(a.stages) * stage + 1024 + 32 * 1024;
+            static const cudaError_t regs = accCheckRegs((const void*)kernel, TN);
+            if(regs != cudaSuccess)
+                return regs;
+            if(cudaError_t e = ensureDynamicSmem((const void*)kernel, int(smem)))
+                return e;
+            const int           csize = PAIR ? 2 : a.ksplit;
+            cudaLaunchConfig_t  cfg{};
+            cudaLaunchAttribute attr[2];
+            attr[0].id                                         = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x                           = unsigned(csize);
+            attr[0].val.clusterDim.y                           = 1;
+            attr[0].val.clusterDim.z                           = 1;
+            attr[1].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[1].val.programmaticStreamSerializationAllowed = 1;
+            const int64_t units                                = int64_t(a.tilesM) * a.tilesN;
+            // a split tile is a cluster's only one; else the grid is resident and walks the tiles
+            cfg.gridDim          = dim3(unsigned(csize * (a.ksplit > 1 ? units : std::min<int64_t>(units, smCount / csize))));
+            cfg.blockDim         = dim3(kAccThreads);
+            cfg.dynamicSmemBytes = smem;
+            cfg.stream           = stream;
+            cfg.attrs            = attr;
+            cfg.numAttrs         = 2;
+            cudaError_t e        = cudaLaunchKernelEx(&cfg, kernel, mapX, mapY, a, ea);
+            if(e == cudaSuccess)
+                noteLaunch(PAIR ? "scaled_pair" : "scaled_tile");
+            return e;
+        }
+
+        template <typename TD, bool VECY>
+        cudaError_t launchForm(const ScaledForm& f, const CUtensorMap& mapX, const CUtensorMap& mapY, const AccArgs& a,
+                               const ScaledArgs& ea, int smCount, cudaStream_t stream)
+        {
+            if(f.pair)
+                return launchTensor<TD, true, 256, VECY>(mapX, mapY, a, ea, smCount, stream);
+            if(f.tn == 128)
+                return launchTensor<TD, false, 128, VECY>(mapX, mapY, a, ea, smCount, stream);
+            if(f.tn == 64)
+                return launchTensor<TD, false, 64, VECY>(mapX, mapY, a, ea, smCount, stream);
+            return launchTensor<TD, false, 32, VECY>(mapX, mapY, a, ea, smCount, stream);
         }
 
         template <typename TD>
         cudaError_t launchTyped(const ScaledPlan& p, float alpha, const void* A, const float* sA, const void* B, const float* sB,
-                                float beta, const void* C, void* D, cudaStream_t stream)
+                                float beta, const void* C, void* D, int smCount, int* status, cudaStream_t stream)
         {
-            const int64_t gx = (p.M + 63) / 64, gy = (p.N + 63) / 64;
-            if(gx > 0x7fffffffll || gy > 65535)
+            const int sms = smCount > 0 ? smCount : 148;
+            PFN_encodeTiled encode = tensorMapEncoder();
+            if(encode && p.K > 0 && rowsForTma(A, p.K, p.M, p.aK, p.aM) && rowsForTma(B, p.K, p.N, p.bK, p.bN))
+            {
+                const ScaledForm f = formOf(p, sms);
+                CUtensorMap      mapX, mapY;
+                const int        rowsX = 128, rowsY = f.pair ? 128 : f.tn;
+                const bool       ok = f.swap ? (encodeRows(encode, &mapX, B, p.K, p.N, p.bN, rowsX) && encodeRows(encode, &mapY, A, p.K, p.M, p.aM, rowsY))
+                                             : (encodeRows(encode, &mapX, A, p.K, p.M, p.aM, rowsX) && encodeRows(encode, &mapY, B, p.K, p.N, p.bN, rowsY));
+                const int64_t    rows = f.swap ? p.N : p.M, cols = f.swap ? p.M : p.N, tileRows = f.pair ? 256 : 128;
+                const int64_t    tilesM = (rows + tileRows - 1) / tileRows, tilesN = (cols + f.tn - 1) / f.tn;
+                if(ok && tilesM * tilesN < (int64_t(1) << 30))
+                {
+                    AccArgs a{};
+                    a.tilesM     = int(tilesM);
+                    a.tilesN     = int(tilesN);
+                    a.kBlocks    = int((p.K + 127) / 128);
+                    a.chunk      = 1;
+                    a.kElems     = 128;
+                    a.ksplit     = f.ksplit;
+                    a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(tilesM, (int64_t(32) << 20) / (tileRows * p.K))));
+                    a.status     = status;
+                    a.statusCode = kStatusScaled;
+                    // f32 sums; formats of X and Y (0 e4m3, 1 e5m2); N / 8; M / 16
+                    const int tX = f.swap ? p.typeB : p.typeA, tY = f.swap ? p.typeA : p.typeB;
+                    a.idesc = (1u << 4) | (tX == CUDA_R_8F_E5M2 ? 1u << 7 : 0u) | (tY == CUDA_R_8F_E5M2 ? 1u << 10 : 0u)
+                              | (uint32_t(f.tn >> 3) << 17) | (uint32_t(tileRows >> 4) << 24);
+                    ScaledArgs ea{};
+                    ea.sX = f.swap ? sB : sA, ea.sY = f.swap ? sA : sB;
+                    ea.sxRow = f.swap ? p.sbN : p.saM, ea.sxK = f.swap ? p.sbK : p.saK;
+                    ea.syRow = f.swap ? p.saM : p.sbN, ea.syK = f.swap ? p.saK : p.sbK;
+                    ea.blockX = f.swap ? p.blockN : p.blockM, ea.blockY = f.swap ? p.blockM : p.blockN;
+                    ea.rows = rows, ea.cols = cols;
+                    ea.C = C, ea.D = D;
+                    ea.dRow = f.swap ? p.dN : p.dM, ea.dCol = f.swap ? p.dM : p.dN;
+                    ea.alpha = alpha, ea.beta = beta;
+                    const uintptr_t four = 4 * sizeof(TD);
+                    ea.vec = (ea.dCol == 1 || cols == 1) && (rows == 1 || ea.dRow % 4 == 0) && uintptr_t(D) % four == 0 && uintptr_t(C) % four == 0;
+                    return ea.blockY > 1 ? launchForm<TD, false>(f, mapX, mapY, a, ea, sms, stream)
+                                         : launchForm<TD, true>(f, mapX, mapY, a, ea, sms, stream);
+                }
+            }
+            const int64_t gx = (p.M + 63) / 64, gy = std::min<int64_t>((p.N + 63) / 64, 65535);
+            if(gx > 0x7fffffffll)
                 return cudaErrorInvalidConfiguration;
             scaled_simt_kernel<TD><<<dim3(unsigned(gx), unsigned(gy)), 256, 0, stream>>>(
                 (const unsigned char*)A, sA, (const unsigned char*)B, sB, (const TD*)C, (TD*)D, alpha, beta, p);
@@ -142,13 +532,11 @@ namespace htb
                              const float* scaleB, float beta, const void* C, void* D, int smCount, int* deviceStatus,
                              cudaStream_t stream)
     {
-        (void)smCount;
-        (void)deviceStatus;
         switch(p.typeD)
         {
-        case CUDA_R_32F: return launchTyped<float>(p, alpha, A, scaleA, B, scaleB, beta, C, D, stream);
-        case CUDA_R_16F: return launchTyped<__half>(p, alpha, A, scaleA, B, scaleB, beta, C, D, stream);
-        case CUDA_R_16BF: return launchTyped<__nv_bfloat16>(p, alpha, A, scaleA, B, scaleB, beta, C, D, stream);
+        case CUDA_R_32F: return launchTyped<float>(p, alpha, A, scaleA, B, scaleB, beta, C, D, smCount, deviceStatus, stream);
+        case CUDA_R_16F: return launchTyped<__half>(p, alpha, A, scaleA, B, scaleB, beta, C, D, smCount, deviceStatus, stream);
+        case CUDA_R_16BF: return launchTyped<__nv_bfloat16>(p, alpha, A, scaleA, B, scaleB, beta, C, D, smCount, deviceStatus, stream);
         }
         return cudaErrorNotSupported;
     }
