@@ -373,7 +373,7 @@ namespace htb
                     epi.begin(r, c, kbBegin, kbEnd);
                     for(int kb = kbBegin; kb < kbEnd; kb += a.chunk)
                     {
-                        ok = __all_sync(0xffffffffu, mbarWait(smemAddr(&tmemFullBar[buf]), bufPhase, abortP));
+                        ok = __all_sync(0xffffffffu, mbarWaitTight(smemAddr(&tmemFullBar[buf]), bufPhase, abortP));
                         if(!ok)
                             break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -382,9 +382,11 @@ namespace htb
                         __syncwarp();
                         if(lane == 0)
                         {
+                            // At CTA scope even where the barrier is the other CTA's: nothing but the completed reads of
+                            // tensor memory is handed over, and a release at cluster scope is a fence that waits for the
+                            // scales on their way (4096^3: 162 us with it)
                             if constexpr(PAIR)
-                                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(emptyLeader + 8 * buf)
-                                             : "memory");
+                                asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(emptyLeader + 8 * buf) : "memory");
                             else
                                 mbarArrive(emptyLeader + 8 * buf);
                         }
