@@ -7,7 +7,7 @@
 //     4096 elements are short by 3.6e-6 of their value), so a long sum is made of chunks of 1024 whose sums are added with
 //     rounding.
 //
-// Roles: warp 0 loads by TMA, one thread of warp 1 issues the MMAs, warps 4 .. 11 are the epilogue. Tensor memory holds two
+// Roles: warp 0 loads by TMA, one thread each of warps 1 and 2 issues the MMAs, warps 4 .. 11 are the epilogue. Tensor memory holds two
 // chunks: while one is read, the next is summed. Epilogue warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and half
 // (w - 4) / 4 of the columns, so a thread owns one row and TN / 2 neighbouring columns of the tile.
 //
@@ -35,7 +35,7 @@ namespace htb
             int      tilesM, tilesN; // tiles of (PAIR ? 256 : 128) rows and TN columns
             int      groupM; // tiles of M that are walked together, for the sake of L2
             int      kBlocks; // 128-byte blocks along K
-            int      chunk; // K blocks per chunk
+            int      chunk; // K blocks per chunk (1 for 8-bit operands)
             int      kElems; // elements of a 128-byte block: 128 (8 bit) or 64
             int      ksplit; // CTAs of a cluster that share a tile (not PAIR)
             int      stages;
@@ -162,8 +162,9 @@ namespace htb
         // Epi: the epilogue, one object per epilogue thread:
         //   Epi(args, warp 0 .. 7, lane, shared memory of this warp)
         //   begin(row, col, kb0)      the thread's row and first column in the product; K blocks from kb0 on
-        //   add(chunk, taddr, first)  reads the chunk's sums from tensor memory and adds them
-        //   end(...)                  the tile's sums are complete
+        //   add(kb, taddr, first, release)  reads the chunk's sums from tensor memory, calls release, and adds them
+        //   end(row, col)                   the tile's sums are complete
+        //   leave()                         no tile follows
         // Registers that a kernel with wide tiles was built with must be what the shares above add up to: a smaller
         // launch would make the epilogue wait for registers that are not there.
         inline cudaError_t accCheckRegs(const void* kernel, int tn)
@@ -302,25 +303,43 @@ namespace htb
                     clusterSync();
                 }
             }
-            else if(warp == 1)
+            else if(warp <= 2)
             {
+                // Two issuers: warp 1 takes the even chunks (first accumulator), warp 2 the odd ones. An MMA is accepted only
+                // shortly before the one ahead of it is done, so what a thread does between its MMAs (the waits, the
+                // commits: 700 cycles around 512 of MMAs for a chunk of one block) would leave the tensor cores idle.
                 if(lane == 0 && leader)
                 {
                     const uint64_t descX = smemDesc(tilesAddr), descY = smemDesc(tilesAddr + 16384);
-                    uint32_t       stage = 0, phase = 0, buf = 0, bufPhase = 0;
+                    const uint32_t buf = uint32_t(warp) - 1, d = tmem + buf * TN;
+                    uint32_t       stage = 0, phase = 0, bufPhase = 0, seq = 0;
                     bool           ok = true;
                     for(int u = clusterId; ok && u < units; u += numClusters)
-                        for(int kb = kbBegin; ok && kb < kbEnd; kb += a.chunk)
+                        for(int kb = kbBegin; ok && kb < kbEnd; kb += a.chunk, seq++)
                         {
-                            ok = mbarWaitTight(smemAddr(&tmemEmptyBar[buf]), bufPhase ^ 1, abortP);
+                            const int end = min(kb + a.chunk, kbEnd);
+                            if((seq & 1) != buf)
+                            {
+                                // the other issuer's stages
+                                stage += uint32_t(end - kb);
+                                while(stage >= uint32_t(a.stages))
+                                {
+                                    stage -= uint32_t(a.stages);
+                                    phase ^= 1;
+                                }
+                                continue;
+                            }
+                            // the first stage before the accumulator: the latter is what comes late, and nothing should
+                            // stand between its release and the MMAs
+                            ok = mbarWaitTight(fullAddr + 8 * stage, phase, abortP)
+                                 && mbarWaitTight(smemAddr(&tmemEmptyBar[buf]), bufPhase ^ 1, abortP);
                             if(!ok)
                                 break;
+                            bufPhase ^= 1;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            const uint32_t d   = tmem + buf * TN;
-                            const int      end = min(kb + a.chunk, kbEnd);
                             for(int k = kb; k < end; k++)
                             {
-                                ok = mbarWaitTight(fullAddr + 8 * stage, phase, abortP);
+                                ok = k == kb || mbarWaitTight(fullAddr + 8 * stage, phase, abortP);
                                 if(!ok)
                                     break;
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -328,17 +347,17 @@ namespace htb
 #pragma unroll
                                 for(int s = 0; s < 4; s++) // 32 bytes of K each
                                     issueMma<PAIR, F8>(d, descX + off + 2 * s, descY + off + 2 * s, a.idesc, (k != kb || s != 0) ? 1u : 0u);
-                                commitTo<PAIR>(emptyAddr + 8 * stage); // frees the stage once these MMAs have read it
+                                // frees the stage once these MMAs have read it, which with one block a chunk (F8) also says
+                                // that the chunk is summed
+                                commitTo<PAIR>(emptyAddr + 8 * stage);
                                 if(++stage == uint32_t(a.stages))
                                 {
                                     stage = 0;
                                     phase ^= 1;
                                 }
                             }
-                            if(ok)
+                            if(!F8 && ok)
                                 commitTo<PAIR>(smemAddr(&tmemFullBar[buf]));
-                            buf ^= 1;
-                            bufPhase ^= buf == 0;
                         }
                 }
                 if(!PAIR && clustered)
@@ -360,7 +379,7 @@ namespace htb
                     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAccRegsEpi));
                 const int quad = warp & 3, half = (warp - 4) >> 2;
                 Epi       epi(ea, warp - 4, lane, tiles + size_t(a.stages) * kStage);
-                uint32_t  buf = 0, bufPhase = 0;
+                uint32_t  buf = 0, bufPhase = 0, stage = 0, phase = 0; // stage and phase: F8, a chunk is one stage
                 bool      ok = true;
                 int       syncs = 0;
                 const uint32_t emptyLeader = PAIR ? mapToRank(smemAddr(&tmemEmptyBar[0]), 0) : smemAddr(&tmemEmptyBar[0]);
@@ -373,25 +392,34 @@ namespace htb
                     epi.begin(r, c, kbBegin, kbEnd);
                     for(int kb = kbBegin; kb < kbEnd; kb += a.chunk)
                     {
-                        ok = __all_sync(0xffffffffu, mbarWaitTight(smemAddr(&tmemFullBar[buf]), bufPhase, abortP));
+                        ok = __all_sync(0xffffffffu, F8 ? mbarWaitTight(emptyAddr + 8 * stage, phase, abortP)
+                                                        : mbarWaitTight(smemAddr(&tmemFullBar[buf]), bufPhase, abortP));
                         if(!ok)
                             break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        epi.add(kb, tmem + (uint32_t(quad * 32) << 16) + buf * TN + uint32_t(half * (TN / 2)), kb == kbBegin);
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if(lane == 0)
-                        {
-                            // At CTA scope even where the barrier is the other CTA's: nothing but the completed reads of
-                            // tensor memory is handed over, and a release at cluster scope is a fence that waits for the
-                            // scales on their way (4096^3: 162 us with it)
-                            if constexpr(PAIR)
-                                asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(emptyLeader + 8 * buf) : "memory");
-                            else
-                                mbarArrive(emptyLeader + 8 * buf);
-                        }
+                        // called once the chunk is out of tensor memory: hands the accumulator back
+                        auto release = [&]() {
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if(lane == 0)
+                            {
+                                // At CTA scope even where the barrier is the other CTA's: nothing but the completed reads
+                                // of tensor memory is handed over, and a release at cluster scope is a fence that waits
+                                // for the scales on their way (4096^3: 162 us with it, 113 without)
+                                if constexpr(PAIR)
+                                    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(emptyLeader + 8 * buf) : "memory");
+                                else
+                                    mbarArrive(emptyLeader + 8 * buf);
+                            }
+                        };
+                        epi.add(kb, tmem + (uint32_t(quad * 32) << 16) + buf * TN + uint32_t(half * (TN / 2)), kb == kbBegin, release);
                         buf ^= 1;
                         bufPhase ^= buf == 0;
+                        if(++stage == uint32_t(a.stages))
+                        {
+                            stage = 0;
+                            phase ^= 1;
+                        }
                     }
                     if(!ok)
                         break;
@@ -412,6 +440,7 @@ namespace htb
                     }
                     epi.end(r, c);
                 }
+                epi.leave();
                 for(; !PAIR && clustered && syncs < 2; syncs++)
                     clusterSync(); // a CTA whose wait ran out still meets the others
             }

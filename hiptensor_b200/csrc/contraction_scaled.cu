@@ -138,6 +138,8 @@ namespace htb
             int64_t      dRow, dCol;
             float        alpha, beta;
             int          vec; // columns contiguous, groups of four aligned
+            int          tma; // the result goes out as bulk tensor stores (no C; rows at multiples of 16 bytes)
+            CUtensorMap  mapD;
         };
 
         // Epilogue of accumulate_kernel: a chunk is one block of 128 along k. A thread multiplies the block's sums of its row by
@@ -151,10 +153,17 @@ namespace htb
             static constexpr int CH   = COLS < 32 ? COLS : 32; // columns per round of stores
             static constexpr int CL   = (VECY && COLS == 128) ? 16 : CH; // columns per load from tensor memory (as registers allow)
             static constexpr int PER  = VECY ? (COLS + 31) / 32 : 1; // column scales that a lane fetches
+            // shared memory of a warp: slots of 4 KiB for the result (two where the scales leave room), then the scales of two
+            // blocks
+            static constexpr int SLOTS = VECY ? 1 : 2;
+            static constexpr int BYTES = SLOTS * 4096 + (VECY ? 2 * COLS * 4 : 0);
+            static constexpr int ROUND = 128 / int(sizeof(TD)); // columns of a slot: rows of 128 bytes
 
             const Args&    a;
             const int      warp, lane;
-            float*         slot; // of this warp: 4 KiB
+            float*         slot;
+            float*         scales;
+            int            stores; // bulk stores of this warp so far, they take the slots in turn
             uint64_t       acc[COLS / 2];
             const float *  px, *py[PER];
             float          x0, x1, y0[PER], y1[PER];
@@ -164,7 +173,9 @@ namespace htb
                 : a(args)
                 , warp(w)
                 , lane(l)
-                , slot(reinterpret_cast<float*>(smem + w * 4096))
+                , slot(reinterpret_cast<float*>(smem + w * (SLOTS * 4096)))
+                , scales(reinterpret_cast<float*>(smem + 8 * SLOTS * 4096 + w * (2 * COLS * 4)))
+                , stores(0)
             {
             }
             __device__ __forceinline__ void fetch(int kb, float& x, float (&y)[PER])
@@ -191,7 +202,8 @@ namespace htb
                 for(int j = 0; j < COLS / 2; j++)
                     acc[j] = 0;
             }
-            __device__ __forceinline__ void add(int kb, uint32_t taddr, bool)
+            template <class Release>
+            __device__ __forceinline__ void add(int kb, uint32_t taddr, bool, Release release)
             {
                 const float x = x0;
                 float       y[PER];
@@ -203,26 +215,18 @@ namespace htb
                     y0[i] = y1[i];
                 }
                 fetch(kb + 2, x1, y1);
-                const float* ys = slot + (kb & 1) * COLS;
+                const float* ys = scales + (kb & 1) * COLS;
                 if constexpr(VECY)
                 {
                     // two slots in turn: the warp barrier of the next block keeps a slot until every lane has read it
 #pragma unroll
                     for(int i = 0; i < PER; i++)
                         if(i * 32 + lane < COLS)
-                            slot[(kb & 1) * COLS + i * 32 + lane] = y[i];
+                            scales[(kb & 1) * COLS + i * 32 + lane] = y[i];
                     __syncwarp();
                 }
                 const uint64_t s = VECY ? pack2(x, x) : pack2(x * y[0], x * y[0]);
-                uint32_t buf[2][CL]; // the next columns are on their way while these are added
-                tmemLoad<CL>(taddr, buf[0]);
-#pragma unroll
-                for(int c = 0; c < COLS; c += CL)
-                {
-                    uint32_t(&v)[CL] = buf[(c / CL) & 1];
-                    tmemWait();
-                    if(c + CL < COLS)
-                        tmemLoad<CL>(taddr + c + CL, buf[(c / CL + 1) & 1]);
+                auto scaleAdd = [&](const uint32_t(&v)[CL], int c) {
 #pragma unroll
                     for(int j = 0; j < CL; j += 4)
                     {
@@ -236,6 +240,25 @@ namespace htb
                         acc[(c + j) / 2]     = fma2(pack2(v[j], v[j + 1]), s0, acc[(c + j) / 2]);
                         acc[(c + j) / 2 + 1] = fma2(pack2(v[j + 2], v[j + 3]), s1, acc[(c + j) / 2 + 1]);
                     }
+                };
+                // Two loads at a time (a wait is for all that are on their way), the next two behind the first additions
+                uint32_t v0[CL], v1[CL];
+                tmemLoad<CL>(taddr, v0);
+                if constexpr(CL < COLS)
+                    tmemLoad<CL>(taddr + CL, v1);
+#pragma unroll
+                for(int c = 0; c < COLS; c += 2 * CL)
+                {
+                    tmemWait();
+                    if(c + 2 * CL >= COLS)
+                        release();
+                    scaleAdd(v0, c);
+                    if(c + 2 * CL < COLS)
+                        tmemLoad<CL>(taddr + c + 2 * CL, v0);
+                    if(c + CL < COLS)
+                        scaleAdd(v1, c + CL);
+                    if(c + 3 * CL < COLS)
+                        tmemLoad<CL>(taddr + c + 3 * CL, v1);
                 }
             }
             __device__ __forceinline__ float sum(int j) const
@@ -243,15 +266,16 @@ namespace htb
                 const float2 f = unpack2(acc[j / 2]);
                 return (j & 1) ? f.y : f.x;
             }
-            __device__ __forceinline__ TD finish(float v, int64_t at) const
+            static __device__ __forceinline__ TD finish(const Args& a, float v, int64_t at)
             {
                 v *= a.alpha;
                 return narrow<TD>(a.C ? fmaf(a.beta, widen(static_cast<const TD*>(a.C)[at]), v) : v);
             }
-            // columns j0 .. j0 + W - 1 of this thread's sums (in w) to row, col0 + ..: through shared memory when the columns
-            // are contiguous, so that lanes that follow each other write (and read C) along a row; else as they are
+            // Columns col0 .. col0 + W - 1 of row `row` from w: through shared memory when the columns are contiguous, so that
+            // lanes that follow each other write (and read C) along a row; else as they are. Kept out of line where the
+            // columns' indexes allow it: unrolled over a tile it was 64 KiB of code, fetched anew for every tile.
             template <int W>
-            __device__ __forceinline__ void store(const float (&w)[W], int64_t row, int64_t col0)
+            static __device__ __noinline__ void store(const Args& a, float* slot, int lane, const float (&w)[W], int64_t row, int64_t col0)
             {
                 TD* D = static_cast<TD*>(a.D);
                 if(!a.vec)
@@ -263,13 +287,13 @@ namespace htb
                             if(col0 + j < a.cols)
                             {
                                 const int64_t at = row * a.dRow + (col0 + j) * a.dCol;
-                                D[at]            = finish(w[j], at);
+                                D[at]            = finish(a, w[j], at);
                             }
                     }
                     return;
                 }
                 constexpr int U = W / 4; // 16-byte units of a row, XORed with the row against bank conflicts
-                __syncwarp(); // the scales or the round before have been read
+                __syncwarp(); // the round before has been read
 #pragma unroll
                 for(int u = 0; u < U; u++)
                     *reinterpret_cast<float4*>(slot + lane * W + ((u ^ (lane & (U - 1))) << 2))
@@ -278,7 +302,7 @@ namespace htb
                 const int64_t row0 = row - lane;
                 const int     u = lane % U;
                 const int64_t c = col0 + 4 * u;
-#pragma unroll
+#pragma unroll 1
                 for(int i = 0; i < U; i++)
                 {
                     const int     rr = i * (32 / U) + lane / U;
@@ -309,12 +333,62 @@ namespace htb
 #pragma unroll
                         for(int j = 0; j < 4; j++)
                             if(c + j < a.cols)
-                                D[at + j] = finish(f[j], at + j);
+                                D[at + j] = finish(a, f[j], at + j);
                     }
+                }
+            }
+            // A slot of 32 rows x 128 bytes, 16-byte units permuted as the tensor map's 128-byte swizzle has them, and one
+            // bulk store of it: the tile leaves while the next one is summed.
+            __device__ __forceinline__ void bulkStore(int c, int64_t row, int64_t col)
+            {
+                const uint32_t at = smemAddr(slot) + uint32_t((stores % SLOTS) * 4096);
+                if(lane == 0)
+                    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(SLOTS - 1) : "memory"); // the slot's last store has read it
+                __syncwarp();
+                stores++;
+#pragma unroll
+                for(int u = 0; u < 8; u++)
+                {
+                    uint32_t q[4];
+#pragma unroll
+                    for(int j = 0; j < 4; j++)
+                    {
+                        if constexpr(sizeof(TD) == 4)
+                            q[j] = __float_as_uint(sum(c + 4 * u + j) * a.alpha);
+                        else
+                        {
+                            const TD lo = narrow<TD>(sum(c + 8 * u + 2 * j) * a.alpha), hi = narrow<TD>(sum(c + 8 * u + 2 * j + 1) * a.alpha);
+                            q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo)) | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
+                        }
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))),
+                                 "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                                 : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if(lane == 0)
+                {
+                    // a block that begins outside the result has nothing to store (one that ends outside is clipped)
+                    if(row < a.rows && col + c < a.cols)
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&a.mapD), "r"(at),
+                                     "r"(int(col + c)), "r"(int(row))
+                                     : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
             }
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
+                if constexpr(COLS >= ROUND)
+                {
+                    if(a.tma)
+                    {
+#pragma unroll
+                        for(int c = 0; c < COLS; c += ROUND)
+                            bulkStore(c, row, col);
+                        return;
+                    }
+                }
 #pragma unroll
                 for(int c = 0; c < COLS; c += CH)
                 {
@@ -322,9 +396,14 @@ namespace htb
 #pragma unroll
                     for(int j = 0; j < CH; j++)
                         w[j] = sum(c + j);
-                    store<CH>(w, row, col + c);
+                    store<CH>(a, slot, lane, w, row, col + c);
                 }
-                __syncwarp(); // the slot is free for the next tile's scales
+            }
+            // before the block ends: the bulk stores have read their slots
+            __device__ __forceinline__ void leave()
+            {
+                if(a.tma && lane == 0)
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             }
             // exchange zone in the stages of CTA q: [sending rank][column of q's slice][128 rows]
             __device__ __forceinline__ void send(uint32_t zone, uint32_t rank, int ksplit, int row, int half)
@@ -367,7 +446,7 @@ namespace htb
                                              : "memory");
                             w[j] += v;
                         }
-                    store<8>(w, r, col0 + half * COLS + c);
+                    store<8>(a, slot, lane, w, r, col0 + half * COLS + c);
                 }
             }
         };
@@ -378,6 +457,16 @@ namespace htb
             cuuint32_t bx[2] = {128, cuuint32_t(box)}, estr[2] = {1, 1};
             return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstr, bx, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+                   == CUDA_SUCCESS;
+        }
+        bool encodeResult(PFN_encodeTiled encode, CUtensorMap* map, int type, void* base, int64_t cols, int64_t rows, int64_t strideBytes)
+        {
+            const bool wide    = type == CUDA_R_32F;
+            cuuint64_t gdim[2] = {cuuint64_t(cols), cuuint64_t(rows)}, gstr[1] = {cuuint64_t(strideBytes)};
+            cuuint32_t bx[2] = {wide ? 32u : 64u, 32}, estr[2] = {1, 1};
+            return encode(map, wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, gdim, gstr, bx, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
                    == CUDA_SUCCESS;
         }
@@ -427,8 +516,8 @@ namespace htb
             using Epi               = ScaledEpi<TD, TN, VECY>;
             auto           kernel   = accumulate_kernel<Epi, PAIR, TN, true>;
             const uint32_t stage    = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
-            a.stages                = std::min<int>(kAccMaxStages, int(192 * 1024 / stage));
-            const size_t smem       = size_t(a.stages) * stage + 1024 + 32 * 1024;
+            a.stages                = std::min<int>(kAccMaxStages, int((225 * 1024 - 1024 - 8 * Epi::BYTES) / stage));
+            const size_t smem       = size_t(a.stages) * stage + 1024 + 8 * Epi::BYTES;
             static const cudaError_t regs = accCheckRegs((const void*)kernel, TN);
             if(regs != cudaSuccess)
                 return regs;
@@ -512,6 +601,12 @@ namespace htb
                     ea.alpha = alpha, ea.beta = beta;
                     const uintptr_t four = 4 * sizeof(TD);
                     ea.vec = (ea.dCol == 1 || cols == 1) && (rows == 1 || ea.dRow % 4 == 0) && uintptr_t(D) % four == 0 && uintptr_t(C) % four == 0;
+                    // bulk stores: the wide forms (a slot's row is 128 bytes of the result) without C and without a K split
+                    const int64_t size = int64_t(sizeof(TD)), ld = rows > 1 ? ea.dRow : (cols + 15) / 16 * 16;
+                    ea.tma = f.tn >= 128 && f.ksplit == 1 && !C && (ea.dCol == 1 || cols == 1) && ld * size % 16 == 0 && ld >= cols
+                             && ld < (int64_t(1) << 36) && (uintptr_t(D) & 15) == 0 && encodeResult(encode, &ea.mapD, p.typeD, D, cols, rows, ld * size);
+                    if(!ea.tma)
+                        ea.mapD = mapX; // a valid map, not used
                     return ea.blockY > 1 ? launchForm<TD, false>(f, mapX, mapY, a, ea, sms, stream)
                                          : launchForm<TD, true>(f, mapX, mapY, a, ea, sms, stream);
                 }
