@@ -25,10 +25,12 @@ namespace htb
         constexpr int kAccThreads = 384; // three warpgroups: loads and MMAs, two of the epilogue
         constexpr int kAccEpi     = 256; // epilogue threads
         // Registers a thread: 168 at launch (384 x 168 = 64512 of the SM's 65536). Wide tiles need more for the running sums:
-        // the first warpgroup gives some back, the epilogue takes them: 128 x 56 + 256 x 224 = 64512.
-        constexpr int kAccRegs = 168, kAccRegsLoad = 56, kAccRegsEpi = 224;
+        // the first warpgroup gives some back, the epilogue takes them: 128 x 72 + 256 x 216 = 64512.
+        constexpr int kAccRegs = 168, kAccRegsLoad = 72, kAccRegsEpi = 216;
         static_assert(128 * kAccRegsLoad + 256 * kAccRegsEpi <= kAccThreads * kAccRegs, "the shares exceed what the launch has");
         constexpr int kAccMaxStages = 12;
+        constexpr int kSideSlots    = 2; // groups of kSideGroup K blocks in the side ring
+        constexpr int kSideGroup    = 4;
 
         struct AccArgs
         {
@@ -160,11 +162,15 @@ namespace htb
         }
 
         // Epi: the epilogue, one object per epilogue thread:
-        //   Epi(args, warp 0 .. 7, lane, shared memory of this warp)
-        //   begin(row, col, kb0)      the thread's row and first column in the product; K blocks from kb0 on
-        //   add(kb, taddr, first, release)  reads the chunk's sums from tensor memory, calls release, and adds them
+        //   Epi(args, warp 0 .. 7, lane, shared memory behind the stages)
+        //   begin()                         a tile begins
+        //   side(values, row in the tile, half of the columns)  with kSide: this K block's side values
+        //   add(taddr, first, release)      reads the chunk's sums from tensor memory, calls release, and adds them
         //   end(row, col)                   the tile's sums are complete
         //   leave()                         no tile follows
+        // With Epi::kSide > 0, warp 3 fetches kSide floats for every K block (the scales), a group of kSideGroup blocks at a time,
+        // into a ring of kSideSlots groups, ahead of the epilogue and across tiles:
+        //   Side(args, lane), begin(first row of this CTA, first column), fetch(slot, first K block, past the last one)
         // Registers that a kernel with wide tiles was built with must be what the shares above add up to: a smaller
         // launch would make the epilogue wait for registers that are not there.
         inline cudaError_t accCheckRegs(const void* kernel, int tn)
@@ -192,6 +198,7 @@ namespace htb
             __shared__ __align__(8) unsigned long long tmemFullBar[2], tmemEmptyBar[2];
             __shared__ uint32_t tmemBase;
             __shared__ int      abortFlag;
+            __shared__ __align__(8) unsigned long long sideFullBar[kSideSlots], sideEmptyBar[kSideSlots];
 
             const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
             const uint32_t rank = (PAIR || a.ksplit > 1) ? clusterRank() : 0u;
@@ -218,6 +225,11 @@ namespace htb
                 {
                     mbarInit(smemAddr(&tmemFullBar[i]), 1);
                     mbarInit(smemAddr(&tmemEmptyBar[i]), (PAIR ? 2 : 1) * (kAccEpi / 32));
+                }
+                for(int i = 0; i < kSideSlots; i++)
+                {
+                    mbarInit(smemAddr(&sideFullBar[i]), 32);
+                    mbarInit(smemAddr(&sideEmptyBar[i]), kAccEpi / 32);
                 }
                 asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             }
@@ -367,10 +379,42 @@ namespace htb
                     clusterSync();
                 }
             }
-            else if(!PAIR && clustered)
+            else
             {
-                clusterSync();
-                clusterSync();
+                if constexpr(Epi::kSide > 0)
+                {
+                    float* const       ring = reinterpret_cast<float*>(tiles + size_t(a.stages) * kStage);
+                    typename Epi::Side side(ea, lane);
+                    uint32_t           slot = 0, phase = 0;
+                    bool               ok = true;
+                    for(int u = clusterId; ok && u < units; u += numClusters)
+                    {
+                        int tm, tn;
+                        tileOf(a, u, tm, tn);
+                        side.begin(int64_t(tm) * ROWS + (PAIR ? int(rank) * 128 : 0), int64_t(tn) * TN);
+                        for(int kb = kbBegin; kb < kbEnd;)
+                        {
+                            ok = __all_sync(0xffffffffu, mbarWaitTight(smemAddr(&sideEmptyBar[slot]), phase ^ 1, abortP));
+                            if(!ok)
+                                break;
+                            const int end = min((kb / kSideGroup + 1) * kSideGroup, kbEnd);
+                            side.fetch(ring + slot * (Epi::kSide * kSideGroup), kb, end);
+                            mbarArrive(smemAddr(&sideFullBar[slot]));
+                            kb = end;
+                            if(++slot == kSideSlots)
+                            {
+                                slot = 0;
+                                phase ^= 1;
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                if(!PAIR && clustered)
+                {
+                    clusterSync();
+                    clusterSync();
+                }
             }
             }
             else
@@ -380,6 +424,8 @@ namespace htb
                 const int quad = warp & 3, half = (warp - 4) >> 2;
                 Epi       epi(ea, warp - 4, lane, tiles + size_t(a.stages) * kStage);
                 uint32_t  buf = 0, bufPhase = 0, stage = 0, phase = 0; // stage and phase: F8, a chunk is one stage
+                uint32_t  slot = 0, slotPhase = 0;
+                const float* ring = reinterpret_cast<const float*>(tiles + size_t(a.stages) * kStage);
                 bool      ok = true;
                 int       syncs = 0;
                 const uint32_t emptyLeader = PAIR ? mapToRank(smemAddr(&tmemEmptyBar[0]), 0) : smemAddr(&tmemEmptyBar[0]);
@@ -389,9 +435,17 @@ namespace htb
                     tileOf(a, u, tm, tn);
                     const int     row = quad * 32 + lane;
                     const int64_t r = int64_t(tm) * ROWS + (PAIR ? int(rank) * 128 : 0) + row, c = int64_t(tn) * TN + half * (TN / 2);
-                    epi.begin(r, c, kbBegin, kbEnd);
+                    epi.begin();
                     for(int kb = kbBegin; kb < kbEnd; kb += a.chunk)
                     {
+                        if constexpr(Epi::kSide > 0)
+                        {
+                            if(kb == kbBegin || kb % kSideGroup == 0)
+                                ok = __all_sync(0xffffffffu, mbarWaitTight(smemAddr(&sideFullBar[slot]), slotPhase, abortP));
+                            if(!ok)
+                                break;
+                            epi.side(ring + (slot * kSideGroup + kb % kSideGroup) * Epi::kSide, row, half);
+                        }
                         ok = __all_sync(0xffffffffu, F8 ? mbarWaitTight(emptyAddr + 8 * stage, phase, abortP)
                                                         : mbarWaitTight(smemAddr(&tmemFullBar[buf]), bufPhase, abortP));
                         if(!ok)
@@ -412,7 +466,21 @@ namespace htb
                                     mbarArrive(emptyLeader + 8 * buf);
                             }
                         };
-                        epi.add(kb, tmem + (uint32_t(quad * 32) << 16) + buf * TN + uint32_t(half * (TN / 2)), kb == kbBegin, release);
+                        epi.add(tmem + (uint32_t(quad * 32) << 16) + buf * TN + uint32_t(half * (TN / 2)), kb == kbBegin, release);
+                        if constexpr(Epi::kSide > 0)
+                        {
+                            if(kb + 1 == kbEnd || (kb + 1) % kSideGroup == 0) // the group's last block
+                            {
+                                __syncwarp();
+                                if(lane == 0)
+                                    mbarArrive(smemAddr(&sideEmptyBar[slot]));
+                                if(++slot == kSideSlots)
+                                {
+                                    slot = 0;
+                                    slotPhase ^= 1;
+                                }
+                            }
+                        }
                         buf ^= 1;
                         bufPhase ^= buf == 0;
                         if(++stage == uint32_t(a.stages))

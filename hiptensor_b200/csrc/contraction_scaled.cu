@@ -132,6 +132,7 @@ namespace htb
             const float *sX, *sY; // scales of the operand on the rows' / columns' side of the tiles
             int64_t      sxRow, sxK, syRow, syK;
             int          blockX, blockY;
+            int          quadX, quadY; // scales of four blocks in one aligned 16-byte word
             int64_t      rows, cols; // of the product
             const void*  C;
             void*        D;
@@ -143,89 +144,126 @@ namespace htb
         };
 
         // Epilogue of accumulate_kernel: a chunk is one block of 128 along k. A thread multiplies the block's sums of its row by
-        // scaleX (one per thread and block) and scaleY (VECY: one per column, through shared memory; else one per block)
-        // and adds them to its running sums, two columns per instruction. Scales are fetched two blocks ahead.
-        template <typename TD, int TN, bool VECY>
+        // scaleX (one per row and block) and scaleY (VECY: one per column and block; else one for 128 columns) and adds
+        // them to its running sums, two columns per instruction. Both come through the side ring: 128 rows, then TN
+        // columns (VECY) or the two halves of the columns.
+        // BULK: the result goes out as bulk tensor stores.
+        template <typename TD, int TN, bool VECY, bool BULK>
         struct ScaledEpi
         {
-            using Args                = ScaledArgs;
-            static constexpr int COLS = TN / 2;
-            static constexpr int CH   = COLS < 32 ? COLS : 32; // columns per round of stores
-            static constexpr int CL   = (VECY && COLS == 128) ? 16 : CH; // columns per load from tensor memory (as registers allow)
-            static constexpr int PER  = VECY ? (COLS + 31) / 32 : 1; // column scales that a lane fetches
-            // shared memory of a warp: slots of 4 KiB for the result (two where the scales leave room), then the scales of two
-            // blocks
-            static constexpr int SLOTS = VECY ? 1 : 2;
-            static constexpr int BYTES = SLOTS * 4096 + (VECY ? 2 * COLS * 4 : 0);
+            using Args                 = ScaledArgs;
+            static constexpr int COLS  = TN / 2;
+            static constexpr int CH    = COLS < 32 ? COLS : 32; // columns per round of stores
+            static constexpr int CL    = CH; // columns per load from tensor memory
+            static constexpr int kSide = 128 + (VECY ? TN : 4);
+            static constexpr int SLOTS = 2; // of 4 KiB, per warp, for the result
+            static constexpr int BYTES = kSideSlots * kSideGroup * kSide * 4; // of the ring, in front of them
             static constexpr int ROUND = 128 / int(sizeof(TD)); // columns of a slot: rows of 128 bytes
 
-            const Args&    a;
-            const int      warp, lane;
-            float*         slot;
-            float*         scales;
-            int            stores; // bulk stores of this warp so far, they take the slots in turn
-            uint64_t       acc[COLS / 2];
-            const float *  px, *py[PER];
-            float          x0, x1, y0[PER], y1[PER];
-            int            kbEnd;
+            // Scales along k are mostly contiguous (sxK == 1): four blocks come as one 16-byte load, one value at a time would
+            // touch a line per row and block, more lines than fit beside the shared memory (4096^3 with a scale per
+            // column: 218 us). Batches of four loads, then four stores each into the rows of the ring.
+            struct Side
+            {
+                const Args& a;
+                const int   lane;
+                int64_t     row, col;
+
+                __device__ Side(const Args& args, int l)
+                    : a(args)
+                    , lane(l)
+                {
+                }
+                __device__ __forceinline__ void begin(int64_t r, int64_t c)
+                {
+                    row = r + lane;
+                    col = VECY ? c + lane : c + (lane & 1) * COLS;
+                }
+                // values kb .. end - 1 of N rows (32 apart from `first`) into ring[kb % group][at + 32 i + lane]
+                template <int N>
+                __device__ __forceinline__ void batch(float* ring, int at, const float* src, int64_t first, int64_t limit, int block, int64_t sRow,
+                                                      int64_t sK, bool quad, int kb, int end, bool mine)
+                {
+                    float v[N][kSideGroup];
+#pragma unroll
+                    for(int i = 0; i < N; i++)
+                    {
+                        const int64_t r = first + i * 32;
+                        const float*  p = src + (block > 1 ? r / kScaleBlock : r) * sRow + kb * sK;
+#pragma unroll
+                        for(int j = 0; j < kSideGroup; j++)
+                            v[i][j] = 0.f; // rows and columns past the result
+                        if(mine && r < limit)
+                        {
+                            if(quad && end - kb == kSideGroup)
+                            {
+                                const float4 q = __ldg(reinterpret_cast<const float4*>(p));
+                                v[i][0] = q.x, v[i][1] = q.y, v[i][2] = q.z, v[i][3] = q.w;
+                            }
+                            else
+                            {
+#pragma unroll
+                                for(int j = 0; j < kSideGroup; j++)
+                                    if(kb + j < end)
+                                        v[i][j] = __ldg(p + j * sK);
+                            }
+                        }
+                    }
+                    if(!mine)
+                        return;
+#pragma unroll
+                    for(int i = 0; i < N; i++)
+#pragma unroll
+                        for(int j = 0; j < kSideGroup; j++)
+                            if(kb + j < end)
+                                ring[(kb % kSideGroup + j) * kSide + at + i * 32 + lane] = v[i][j];
+                }
+                __device__ __forceinline__ void fetch(float* ring, int kb, int end)
+                {
+                    batch<4>(ring, 0, a.sX, row, a.rows, a.blockX, a.sxRow, a.sxK, a.quadX != 0, kb, end, true);
+                    if constexpr(VECY)
+                    {
+                        constexpr int N = TN / 32 < 4 ? TN / 32 : 4;
+#pragma unroll 1
+                        for(int i = 0; i < TN / 32; i += N)
+                            batch<N>(ring, 128 + i * 32, a.sY, col + i * 32, a.cols, 1, a.syRow, a.syK, a.quadY != 0, kb, end, true);
+                    }
+                    else
+                        batch<1>(ring, 128, a.sY, col, a.cols, kScaleBlock, a.syRow, a.syK, a.quadY != 0, kb, end, lane < 2);
+                }
+            };
+
+            const Args&  a;
+            const int    lane;
+            float*       slot;
+            int          stores; // bulk stores of this warp so far, they take the slots in turn
+            const float* ys;
+            uint64_t     s;
+            uint64_t     acc[COLS / 2];
 
             __device__ ScaledEpi(const Args& args, int w, int l, unsigned char* smem)
                 : a(args)
-                , warp(w)
                 , lane(l)
-                , slot(reinterpret_cast<float*>(smem + w * (SLOTS * 4096)))
-                , scales(reinterpret_cast<float*>(smem + 8 * SLOTS * 4096 + w * (2 * COLS * 4)))
+                , slot(reinterpret_cast<float*>(smem + (BYTES + 1023) / 1024 * 1024 + w * (SLOTS * 4096)))
                 , stores(0)
             {
             }
-            __device__ __forceinline__ void fetch(int kb, float& x, float (&y)[PER])
+            __device__ __forceinline__ void begin()
             {
-                const bool in = kb < kbEnd;
-                x             = (px && in) ? __ldg(px + kb * a.sxK) : 0.f;
-#pragma unroll
-                for(int i = 0; i < PER; i++)
-                    y[i] = (py[i] && in) ? __ldg(py[i] + kb * a.syK) : 0.f;
-            }
-            __device__ __forceinline__ void begin(int64_t row, int64_t col, int kb0, int kb1)
-            {
-                kbEnd = kb1;
-                px    = row < a.rows ? a.sX + (a.blockX > 1 ? row / kScaleBlock : row) * a.sxRow : nullptr;
-#pragma unroll
-                for(int i = 0; i < PER; i++)
-                {
-                    const int64_t c = VECY ? col + i * 32 + lane : col;
-                    py[i] = (c < a.cols && (!VECY || i * 32 + lane < COLS)) ? a.sY + (VECY ? c : c / kScaleBlock) * a.syRow : nullptr;
-                }
-                fetch(kb0, x0, y0);
-                fetch(kb0 + 1, x1, y1);
 #pragma unroll
                 for(int j = 0; j < COLS / 2; j++)
                     acc[j] = 0;
             }
-            template <class Release>
-            __device__ __forceinline__ void add(int kb, uint32_t taddr, bool, Release release)
+            __device__ __forceinline__ void side(const float* v, int row, int half)
             {
-                const float x = x0;
-                float       y[PER];
-                x0 = x1;
-#pragma unroll
-                for(int i = 0; i < PER; i++)
-                {
-                    y[i]  = y0[i];
-                    y0[i] = y1[i];
-                }
-                fetch(kb + 2, x1, y1);
-                const float* ys = scales + (kb & 1) * COLS;
-                if constexpr(VECY)
-                {
-                    // two slots in turn: the warp barrier of the next block keeps a slot until every lane has read it
-#pragma unroll
-                    for(int i = 0; i < PER; i++)
-                        if(i * 32 + lane < COLS)
-                            scales[(kb & 1) * COLS + i * 32 + lane] = y[i];
-                    __syncwarp();
-                }
-                const uint64_t s = VECY ? pack2(x, x) : pack2(x * y[0], x * y[0]);
+                const float x = v[row];
+                ys            = v + 128 + half * COLS;
+                const float m = VECY ? x : x * v[128 + half];
+                s             = pack2(m, m);
+            }
+            template <class Release>
+            __device__ __forceinline__ void add(uint32_t taddr, bool, Release release)
+            {
                 auto scaleAdd = [&](const uint32_t(&v)[CL], int c) {
 #pragma unroll
                     for(int j = 0; j < CL; j += 4)
@@ -379,30 +417,29 @@ namespace htb
             }
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
-                if constexpr(COLS >= ROUND)
+                if constexpr(BULK)
                 {
-                    if(a.tma)
-                    {
 #pragma unroll
-                        for(int c = 0; c < COLS; c += ROUND)
-                            bulkStore(c, row, col);
-                        return;
-                    }
+                    for(int c = 0; c < COLS; c += ROUND)
+                        bulkStore(c, row, col);
                 }
-#pragma unroll
-                for(int c = 0; c < COLS; c += CH)
+                else
                 {
-                    float w[CH];
 #pragma unroll
-                    for(int j = 0; j < CH; j++)
-                        w[j] = sum(c + j);
-                    store<CH>(a, slot, lane, w, row, col + c);
+                    for(int c = 0; c < COLS; c += CH)
+                    {
+                        float w[CH];
+#pragma unroll
+                        for(int j = 0; j < CH; j++)
+                            w[j] = sum(c + j);
+                        store<CH>(a, slot, lane, w, row, col + c);
+                    }
                 }
             }
             // before the block ends: the bulk stores have read their slots
             __device__ __forceinline__ void leave()
             {
-                if(a.tma && lane == 0)
+                if(BULK && lane == 0)
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             }
             // exchange zone in the stages of CTA q: [sending rank][column of q's slice][128 rows]
@@ -509,15 +546,17 @@ namespace htb
             return f;
         }
 
-        template <typename TD, bool PAIR, int TN, bool VECY>
+        template <typename TD, bool PAIR, int TN, bool VECY, bool BULK>
         cudaError_t launchTensor(const CUtensorMap& mapX, const CUtensorMap& mapY, AccArgs a, const ScaledArgs& ea, int smCount,
                                  cudaStream_t stream)
         {
-            using Epi               = ScaledEpi<TD, TN, VECY>;
+            using Epi               = ScaledEpi<TD, TN, VECY, BULK>;
             auto           kernel   = accumulate_kernel<Epi, PAIR, TN, true>;
             const uint32_t stage    = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
-            a.stages                = std::min<int>(kAccMaxStages, int((225 * 1024 - 1024 - 8 * Epi::BYTES) / stage));
-            const size_t smem       = size_t(a.stages) * stage + 1024 + 8 * Epi::BYTES;
+            // the ring of scales, two slots of 4 KiB per warp for the result, and room to align the stages
+            const uint32_t room     = (Epi::BYTES + 1023) / 1024 * 1024 + 8 * Epi::SLOTS * 4096 + 1024;
+            a.stages                = std::min<int>(kAccMaxStages, int((226 * 1024 - room) / stage));
+            const size_t smem       = size_t(a.stages) * stage + room;
             static const cudaError_t regs = accCheckRegs((const void*)kernel, TN);
             if(regs != cudaSuccess)
                 return regs;
@@ -551,12 +590,14 @@ namespace htb
                                const ScaledArgs& ea, int smCount, cudaStream_t stream)
         {
             if(f.pair)
-                return launchTensor<TD, true, 256, VECY>(mapX, mapY, a, ea, smCount, stream);
+                return ea.tma ? launchTensor<TD, true, 256, VECY, true>(mapX, mapY, a, ea, smCount, stream)
+                              : launchTensor<TD, true, 256, VECY, false>(mapX, mapY, a, ea, smCount, stream);
             if(f.tn == 128)
-                return launchTensor<TD, false, 128, VECY>(mapX, mapY, a, ea, smCount, stream);
+                return ea.tma ? launchTensor<TD, false, 128, VECY, true>(mapX, mapY, a, ea, smCount, stream)
+                              : launchTensor<TD, false, 128, VECY, false>(mapX, mapY, a, ea, smCount, stream);
             if(f.tn == 64)
-                return launchTensor<TD, false, 64, VECY>(mapX, mapY, a, ea, smCount, stream);
-            return launchTensor<TD, false, 32, VECY>(mapX, mapY, a, ea, smCount, stream);
+                return launchTensor<TD, false, 64, VECY, false>(mapX, mapY, a, ea, smCount, stream);
+            return launchTensor<TD, false, 32, VECY, false>(mapX, mapY, a, ea, smCount, stream);
         }
 
         template <typename TD>
@@ -594,6 +635,8 @@ namespace htb
                     ea.sX = f.swap ? sB : sA, ea.sY = f.swap ? sA : sB;
                     ea.sxRow = f.swap ? p.sbN : p.saM, ea.sxK = f.swap ? p.sbK : p.saK;
                     ea.syRow = f.swap ? p.saM : p.sbN, ea.syK = f.swap ? p.saK : p.sbK;
+                    auto quad = [](const float* s, int64_t sRow, int64_t sK) { return sK == 1 && sRow % 4 == 0 && (uintptr_t(s) & 15) == 0; };
+                    ea.quadX = quad(ea.sX, ea.sxRow, ea.sxK), ea.quadY = quad(ea.sY, ea.syRow, ea.syK);
                     ea.blockX = f.swap ? p.blockN : p.blockM, ea.blockY = f.swap ? p.blockM : p.blockN;
                     ea.rows = rows, ea.cols = cols;
                     ea.C = C, ea.D = D;
