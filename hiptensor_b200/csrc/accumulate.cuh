@@ -168,6 +168,7 @@ namespace htb
         //   add(taddr, first, release)      reads the chunk's sums from tensor memory, calls release, and adds them
         //   end(row, col)                   the tile's sums are complete
         //   leave()                         no tile follows
+        //   send(..), endSplit(..)          with kSplit: the exchange of a tile whose K range is cut
         // With Epi::kSide > 0, warp 3 fetches kSide floats for every K block (the scales), a group of kSideGroup blocks at a time,
         // into a ring of kSideSlots groups, ahead of the epilogue and across tiles:
         //   Side(args, lane), begin(first row of this CTA, first column), fetch(slot, first K block, past the last one)
@@ -491,7 +492,7 @@ namespace htb
                     }
                     if(!ok)
                         break;
-                    if constexpr(!PAIR)
+                    if constexpr(!PAIR && Epi::kSplit)
                     {
                         if(clustered)
                         {

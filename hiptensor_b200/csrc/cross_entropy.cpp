@@ -61,10 +61,13 @@ namespace htb
             l.hOff           = take(l.packH, T * uint64_t(l.ld) * size);
             l.stateOff       = take(!gradient, T * 12);
             l.scaleOff       = take(gradient, 8);
+            l.restOff        = take(gradient, T * 4);
             l.dhOff          = take(gradient, T * uint64_t(l.ld) * 4);
             l.wOff           = take(l.packW, n * uint64_t(l.ld) * size);
-            l.zOff           = take(true, T * n * 4);
-            l.pOff           = take(gradient && p.type != CUDA_R_32F, T * n * size);
+            const bool f32   = p.type == CUDA_R_32F;
+            l.zOff           = take(f32, T * n * 4);
+            l.partOff        = take(!f32 && !gradient, (n + headGroup(p.T) - 1) / headGroup(p.T) * T * 8);
+            l.pOff           = take(!f32 && gradient, T * n * size);
             l.dwOff          = take(gradient && p.type == CUDA_R_16F, n * uint64_t(l.ld) * 4);
             l.bytes          = at + 256; // room to align the caller's pointer
             return l;
@@ -289,11 +292,12 @@ namespace htb
         int64_t            ldh    = p.nt ? p.tStride[0] : l.ld;
         if(l.packH)
         {
-            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, stream));
+            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, nullptr, stream));
             h   = ws + l.hOff;
             ldh = l.ld;
         }
-        float* z = reinterpret_cast<float*>(ws + l.zOff);
+        const bool f32 = p.type == CUDA_R_32F;
+        float*     z   = reinterpret_cast<float*>(ws + l.zOff);
         for(int64_t v0 = 0; v0 < p.V; v0 += l.piece)
         {
             const int64_t n   = std::min(l.piece, p.V - v0);
@@ -301,15 +305,26 @@ namespace htb
             int64_t       ldw = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
-            HTB_TRY(product(Matrix{h, p.T, p.D, ldh, 1, p.type}, 0, 2, Matrix{w, n, p.D, ldw, 1, p.type}, 1, 2,
-                            Matrix{z, p.T, n, l.piece, 1, CUDA_R_32F}, 0, 1, a, 0.f, st, stream));
-            HTB_TRY(launchSoftmaxPiece(z, l.piece, p.T, v0, n, targets, state, stream));
+            if(f32)
+            {
+                HTB_TRY(product(Matrix{h, p.T, p.D, ldh, 1, p.type}, 0, 2, Matrix{w, n, p.D, ldw, 1, p.type}, 1, 2,
+                                Matrix{z, p.T, n, l.piece, 1, CUDA_R_32F}, 0, 1, a, 0.f, st, stream));
+                HTB_TRY(launchSoftmaxPiece(z, l.piece, p.T, v0, n, targets, state, stream));
+            }
+            else
+            {
+                HTB_TRY(launchHeadLoss(HeadProduct{h, w, p.T, n, p.D, ldh, ldw, p.type}, v0, targets, a, ws + l.partOff, state, st->smCount,
+                                       st->deviceStatus, stream));
+                HTB_TRY(launchLossJoin(ws + l.partOff, n, p.T, state, v0 == 0, v0 + n == p.V, p.V, p.ignore, targets, loss, lse,
+                                       st->deviceStatus, stream));
+            }
         }
-        HTB_TRY(launchLossFinish(state, p.T, p.V, p.ignore, targets, loss, lse, st->deviceStatus, stream));
+        if(f32)
+            HTB_TRY(launchLossFinish(state, p.T, p.V, p.ignore, targets, loss, lse, st->deviceStatus, stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }
 
@@ -343,7 +358,7 @@ namespace htb
         if(p.T == 0)
         {
             if(dW) // no token, no gradient
-                HTB_TRY(launchStoreRows(p.type, nullptr, 0, p.V, p.D, nullptr, dW, plainRows(p.wV, p.wD, p.V), stream));
+                HTB_TRY(launchStoreRows(p.type, nullptr, 0, p.V, p.D, nullptr, dW, plainRows(p.wV, p.wD, p.V), TargetRest{}, stream));
             return HIPTENSOR_STATUS_SUCCESS;
         }
         const CrossEntropyLayout l = layoutIn(p, true, workspace ? workspaceSize : 0);
@@ -364,11 +379,12 @@ namespace htb
             HTB_TRY(launchGradientScale(gradLoss, a, p.T, scale, stream));
         }
         void* h = ws + l.hOff;
-        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, h, targets, p.ignore, p.V, stream));
+        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, h, targets, p.ignore, p.V, st->deviceStatus, stream));
         float*       z   = reinterpret_cast<float*>(ws + l.zOff);
         void*        P   = f32 ? (void*)z : (void*)(ws + l.pOff);
         float*       dh  = reinterpret_cast<float*>(ws + l.dhOff);
         float*       dw  = reinterpret_cast<float*>(ws + l.dwOff);
+        float*       rest = reinterpret_cast<float*>(ws + l.restOff);
         const Matrix Hm{h, p.T, p.D, l.ld, 1, p.type};
         for(int64_t v0 = 0; v0 < p.V; v0 += l.piece)
         {
@@ -377,14 +393,19 @@ namespace htb
             int64_t       ldw = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
             const Matrix Wm{w, n, p.D, ldw, 1, p.type}, Pm{P, p.T, n, l.piece, 1, p.type};
-            HTB_TRY(product(Hm, 0, 2, Wm, 1, 2, Matrix{z, p.T, n, l.piece, 1, CUDA_R_32F}, 0, 1, a, 0.f, st, stream));
-            HTB_TRY(launchProbabilities(p.type, z, l.piece, p.T, v0, n, p.V, p.ignore, targets, lse, gradLoss, a, scale, P, l.piece,
-                                        st->deviceStatus, stream));
+            if(f32)
+            {
+                HTB_TRY(product(Hm, 0, 2, Wm, 1, 2, Matrix{z, p.T, n, l.piece, 1, CUDA_R_32F}, 0, 1, a, 0.f, st, stream));
+                HTB_TRY(launchProbabilities(z, l.piece, p.T, v0, n, p.V, p.ignore, targets, lse, gradLoss, a, stream));
+            }
+            else
+                HTB_TRY(launchHeadGradient(HeadProduct{h, w, p.T, n, p.D, l.ld, ldw, p.type}, v0, p.V, p.ignore, targets, lse, gradLoss, a,
+                                           scale, P, l.piece, rest, st->smCount, st->deviceStatus, stream));
             if(dH)
                 HTB_TRY(product(Pm, 0, 1, Wm, 1, 2, Matrix{dh, p.T, p.D, l.ld, 1, CUDA_R_32F}, 0, 2, 1.f, v0 ? 1.f : 0.f, st, stream));
             if(dW)
@@ -393,14 +414,15 @@ namespace htb
                 if(scale)
                 {
                     HTB_TRY(product(Pm, 0, 1, Hm, 0, 2, Matrix{dw, n, p.D, l.ld, 1, CUDA_R_32F}, 1, 2, 1.f, 0.f, st, stream));
-                    HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), stream));
+                    HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, stream));
                 }
                 else
                     HTB_TRY(product(Pm, 0, 1, Hm, 0, 2, Matrix{out, n, p.D, p.wV, p.wD, p.type}, 1, 2, 1.f, 0.f, st, stream));
             }
         }
         if(dH)
-            HTB_TRY(launchStoreRows(p.type, dh, l.ld, p.T, p.D, scale, dH, rowsOfH(p), stream));
+            HTB_TRY(launchStoreRows(p.type, dh, l.ld, p.T, p.D, scale, dH, rowsOfH(p),
+                                    f32 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }
 } // namespace htb

@@ -29,7 +29,7 @@ namespace htb
         bool     packH, packW; // operands copied into the workspace as packed rows of ld elements
         int64_t  ld;
         int64_t  piece; // classes of a piece (a multiple of kPieceUnit, or all of them)
-        uint64_t hOff, wOff, stateOff, zOff, pOff, dhOff, dwOff, scaleOff;
+        uint64_t hOff, wOff, stateOff, zOff, partOff, pOff, dhOff, dwOff, scaleOff, restOff;
         uint64_t bytes;
     };
 
@@ -44,24 +44,52 @@ namespace htb
         int64_t ext[kMaxGroup], stride[kMaxGroup];
         int64_t elem; // stride along the contracted mode
     };
-    // X2[r, 0 .. ld) = X[row r, 0 .. cols), zeros behind; rows whose target is `ignore` or outside [0, V) become zeros when
-    // targets are given
+    // X2[r, 0 .. ld) = X[row r, 0 .. cols), zeros behind. With targets: rows whose target is `ignore` or no class become zeros,
+    // and the latter raise the status word.
     cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t cols, int64_t ld, void* X2,
-                               const int64_t* targets, int64_t ignore, int64_t V, cudaStream_t stream);
+                               const int64_t* targets, int64_t ignore, int64_t V, int* status, cudaStream_t stream);
+
+    // f16 / bf16: logits of n classes from v0 on, used where they are made
+    struct HeadProduct
+    {
+        const void *H, *W; // rows of D elements, ldh / ldw apart, at multiples of 16 bytes
+        int64_t     T, n, D, ldh, ldw;
+        int         type;
+    };
+    int headGroup(int64_t T); // classes that share one partial maximum and sum
+    // part: ceil(n / headGroup) x T pairs of floats; the target logits go to state[2T .. 3T)
+    cudaError_t launchHeadLoss(const HeadProduct& h, int64_t v0, const int64_t* targets, float alpha, void* part, float* state, int smCount,
+                               int* status, cudaStream_t stream);
+    // joins a piece's partial results with state[0 .. 2T) (maximum, sum in powers of two); after the last piece loss and lse
+    cudaError_t launchLossJoin(const void* part, int64_t n, int64_t T, float* state, bool first, bool last, int64_t V, int64_t ignore,
+                               const int64_t* targets, float* loss, float* lse, int* status, cudaStream_t stream);
+    // P[t, v] = (exp(z - lse) - [v0 + v == target]) * g * alpha (* scale[0]); rest[t]: what rounding took from the target's entry
+    cudaError_t launchHeadGradient(const HeadProduct& h, int64_t v0, int64_t V, int64_t ignore, const int64_t* targets, const float* lse,
+                                   const float* g, float alpha, const float* scale, void* P, int64_t ldp, float* rest, int smCount, int* status,
+                                   cudaStream_t stream);
+
+    // f32: logits of a piece in memory, z[t, v] with rows ldz apart
     // running maximum / sum / target logit per token: state[0 .. T), [T .. 2T), [2T .. 3T)
     cudaError_t launchSoftmaxPiece(const float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, const int64_t* targets, float* state,
                                    cudaStream_t stream);
     cudaError_t launchLossFinish(const float* state, int64_t T, int64_t V, int64_t ignore, const int64_t* targets, float* loss, float* lse,
                                  int* deviceStatus, cudaStream_t stream);
-    // scale[0] = a power of two that brings max |g * alpha| close to the top of f16's range, scale[1] = its reciprocal
+    // z becomes P in place
+    cudaError_t launchProbabilities(float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, int64_t V, int64_t ignore,
+                                    const int64_t* targets, const float* lse, const float* g, float alpha, cudaStream_t stream);
+
+    // f16: scale[0] = a power of two that brings max |g * alpha| close to the top of the range, scale[1] = its reciprocal
     cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, float* scale, cudaStream_t stream);
-    // P[t, v] = (exp(z - lse) - [v0 + v == target]) * g * alpha (* scale[0])
-    cudaError_t launchProbabilities(int type, const float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, int64_t V, int64_t ignore,
-                                    const int64_t* targets, const float* lse, const float* g, float alpha, const float* scale, void* P,
-                                    int64_t ldp, int* deviceStatus, cudaStream_t stream);
-    // Y[row r, c] = X[r, c] (* scale[1]) rounded to `type`
+    // Y[row r, c] = (X[r, c] + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; X null: zeros; rest null: none
+    struct TargetRest
+    {
+        const float*   rest;
+        const int64_t* targets;
+        int64_t        ignore, V, wV, wD;
+        const void*    W;
+    };
     cudaError_t launchStoreRows(int type, const float* X, int64_t ldx, int64_t count, int64_t cols, const float* scale, void* Y,
-                                const TokenRows& rows, cudaStream_t stream);
+                                const TokenRows& rows, const TargetRest& rest, cudaStream_t stream);
 
     int crossEntropy(const hiptensorHandle_t* handle, const CrossEntropyPlan* plan, const void* alpha, const void* H, const void* W,
                      const int64_t* targets, float* loss, float* lse, void* workspace, uint64_t workspaceSize, void* stream);
