@@ -7,7 +7,7 @@
 //     4096 elements are short by 3.6e-6 of their value), so a long sum is made of chunks of 1024 whose sums are added with
 //     rounding.
 //
-// Roles: warp 0 loads by TMA, one thread each of warps 1 and 2 issues the MMAs, warps 4 .. 11 are the epilogue. Tensor memory holds two
+// Roles: warp 0 loads by TMA, one thread of warp 1 (8 bit: of warps 1 and 2) issues the MMAs, warp 3 fetches scales, warps 4 .. 11 are the epilogue. Tensor memory holds two
 // chunks: while one is read, the next is summed. Epilogue warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and half
 // (w - 4) / 4 of the columns, so a thread owns one row and TN / 2 neighbouring columns of the tile.
 //
@@ -115,6 +115,18 @@ namespace htb
                          "[%2];" ::"r"(dst),
                          "l"(map), "r"(bar), "r"(c0), "r"(c1)
                          : "memory");
+        }
+
+        __device__ __forceinline__ bool mbarTest(uint32_t bar, uint32_t parity)
+        {
+            uint32_t done;
+            asm volatile("{\n\t.reg .pred p;\n\t"
+                         "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                         "selp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(done)
+                         : "r"(bar), "r"(parity)
+                         : "memory");
+            return done != 0;
         }
 
         template <bool PAIR, bool F8>
@@ -318,56 +330,68 @@ namespace htb
             }
             else if(warp <= 2)
             {
-                // Two issuers: warp 1 takes the even chunks (first accumulator), warp 2 the odd ones. An MMA is accepted only
-                // shortly before the one ahead of it is done, so what a thread does between its MMAs (the waits, the
-                // commits: 700 cycles around 512 of MMAs for a chunk of one block) would leave the tensor cores idle.
-                if(lane == 0 && leader)
+                // 8 bit: two issuers, warp 1 takes the even chunks (first accumulator), warp 2 the odd ones. An MMA is accepted
+                // only shortly before the one ahead of it is done, so what a thread does between its MMAs (the waits, the
+                // commits: 700 cycles around 512 of MMAs for a chunk of one block) would leave the tensor cores idle. A
+                // barrier tells apart two rounds of the stages only, so neither issuer may look more than a round ahead: a
+                // chunk begins after the one two before it was read, hence (in order) all before that, and with four
+                // stages or more (checked by the launcher) that covers the stage's last use.
+                // Half precision: long chunks, one issuer.
+                constexpr uint32_t ISSUERS = F8 ? 2 : 1;
+                if(lane == 0 && leader && uint32_t(warp) <= ISSUERS)
                 {
                     const uint64_t descX = smemDesc(tilesAddr), descY = smemDesc(tilesAddr + 16384);
-                    const uint32_t buf = uint32_t(warp) - 1, d = tmem + buf * TN;
+                    const uint32_t self = uint32_t(warp) - 1;
                     uint32_t       stage = 0, phase = 0, bufPhase = 0, seq = 0;
                     bool           ok = true;
                     for(int u = clusterId; ok && u < units; u += numClusters)
                         for(int kb = kbBegin; ok && kb < kbEnd; kb += a.chunk, seq++)
                         {
-                            const int end = min(kb + a.chunk, kbEnd);
-                            if((seq & 1) != buf)
+                            const uint32_t buf = seq & 1;
+                            if(ISSUERS == 2 && buf != self)
                             {
-                                // the other issuer's stages
-                                stage += uint32_t(end - kb);
-                                while(stage >= uint32_t(a.stages))
+                                if(++stage == uint32_t(a.stages)) // the other issuer's stage (a chunk is one block)
                                 {
-                                    stage -= uint32_t(a.stages);
+                                    stage = 0;
                                     phase ^= 1;
                                 }
                                 continue;
                             }
+                            const int      end = min(kb + a.chunk, kbEnd);
+                            const uint32_t d   = tmem + buf * TN;
                             // the first stage before the accumulator: the latter is what comes late, and nothing should
                             // stand between its release and the MMAs
                             ok = mbarWaitTight(fullAddr + 8 * stage, phase, abortP)
                                  && mbarWaitTight(smemAddr(&tmemEmptyBar[buf]), bufPhase ^ 1, abortP);
                             if(!ok)
                                 break;
-                            bufPhase ^= 1;
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            if(ISSUERS == 2 || buf == 1)
+                                bufPhase ^= 1;
                             for(int k = kb; k < end; k++)
                             {
-                                ok = k == kb || mbarWaitTight(fullAddr + 8 * stage, phase, abortP);
-                                if(!ok)
-                                    break;
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                                 const uint64_t off = uint64_t((stage * kStage) >> 4);
-#pragma unroll
-                                for(int s = 0; s < 4; s++) // 32 bytes of K each
-                                    issueMma<PAIR, F8>(d, descX + off + 2 * s, descY + off + 2 * s, a.idesc, (k != kb || s != 0) ? 1u : 0u);
-                                // frees the stage once these MMAs have read it, which with one block a chunk (F8) also says
-                                // that the chunk is summed
-                                commitTo<PAIR>(emptyAddr + 8 * stage);
+                                const uint32_t now = stage;
                                 if(++stage == uint32_t(a.stages))
                                 {
                                     stage = 0;
                                     phase ^= 1;
                                 }
+                                bool ready = false;
+#pragma unroll
+                                for(int s = 0; s < 4; s++) // 32 bytes of K each
+                                {
+                                    if(s == 2 && k + 1 < end) // a look at the next stage while MMAs are queued
+                                        ready = mbarTest(fullAddr + 8 * stage, phase);
+                                    issueMma<PAIR, F8>(d, descX + off + 2 * s, descY + off + 2 * s, a.idesc, (k != kb || s != 0) ? 1u : 0u);
+                                }
+                                // frees the stage once these MMAs have read it, which with one block a chunk (F8) also says
+                                // that the chunk is summed
+                                commitTo<PAIR>(emptyAddr + 8 * now);
+                                if(k + 1 < end && !ready)
+                                    ok = mbarWaitTight(fullAddr + 8 * stage, phase, abortP);
+                                if(!ok)
+                                    break;
                             }
                             if(!F8 && ok)
                                 commitTo<PAIR>(smemAddr(&tmemFullBar[buf]));
@@ -516,6 +540,14 @@ namespace htb
 
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncthreads();
+            if(abortFlag)
+            {
+                // a wait ran out: loads and MMAs may still be on their way into memory that is given up below (about a
+                // millisecond is many times what they can take)
+                const long long t0 = clock64();
+                while(clock64() - t0 < 2000000)
+                    ;
+            }
             if(clustered)
                 clusterSync(); // all CTAs are done with tensor memory and with each other's barriers and shared memory
             if(threadIdx.x == 0 && abortFlag && a.status)

@@ -555,8 +555,10 @@ namespace htb
             auto           kernel   = accumulate_kernel<Epi, PAIR, TN, true>;
             const uint32_t stage    = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
             // the ring of scales, two slots of 4 KiB per warp for the result, and room to align the stages
-            const uint32_t room     = (Epi::BYTES + 1023) / 1024 * 1024 + 8 * Epi::SLOTS * 4096 + 1024;
+            constexpr uint32_t room = (Epi::BYTES + 1023) / 1024 * 1024 + 8 * Epi::SLOTS * 4096 + 1024;
             a.stages                = std::min<int>(kAccMaxStages, int((226 * 1024 - room) / stage));
+            static_assert((226 * 1024 - ((Epi::BYTES + 1023) / 1024 * 1024 + 8 * Epi::SLOTS * 4096 + 1024)) / (16384 + (PAIR ? 128 : TN) * 128) >= 4,
+                          "two issuers need four stages");
             const size_t smem       = size_t(a.stages) * stage + room;
             static const cudaError_t regs = accCheckRegs((const void*)kernel, TN);
             if(regs != cudaSuccess)
