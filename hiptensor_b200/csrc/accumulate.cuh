@@ -28,7 +28,7 @@ namespace htb
         // the first warpgroup gives some back, the epilogue takes them: 128 x 72 + 256 x 216 = 64512.
         constexpr int kAccRegs = 168, kAccRegsLoad = 72, kAccRegsEpi = 216;
         static_assert(128 * kAccRegsLoad + 256 * kAccRegsEpi <= kAccThreads * kAccRegs, "the shares exceed what the launch has");
-        constexpr int kAccMaxStages = 12;
+        constexpr int kAccMaxStages = 16;
         constexpr int kSideSlots    = 2; // groups of kSideGroup K blocks in the side ring
         constexpr int kSideGroup    = 4;
 
@@ -39,8 +39,10 @@ namespace htb
             int      kBlocks; // 128-byte blocks along K
             int      chunk; // K blocks per chunk (1 for 8-bit operands)
             int      kElems; // elements of a 128-byte block: 128 (8 bit) or 64
+            int      xRows; // not PAIR: rows of X that are loaded, a multiple of 8
             int      ksplit; // CTAs of a cluster that share a tile (not PAIR)
             int      stages;
+            uint32_t stageBytes; // of all stages, and what the MMAs may read behind them: a multiple of 1024
             uint32_t idesc;
             int*     status;
             int      statusCode;
@@ -197,13 +199,18 @@ namespace htb
             return at.numRegs >= kAccRegs ? cudaSuccess : cudaErrorInvalidKernelImage;
         }
 
-        template <class Epi, bool PAIR, int TN, bool F8>
+        // MN: both operands are contiguous along their rows (X^T Y of matrices with one row per k; half precision): 64-row chunks of
+        // [64 k][128 bytes] instead of rows of 128 bytes along k, transposed descriptors.
+        template <class Epi, bool PAIR, int TN, bool F8, bool MN = false>
         __global__ void __launch_bounds__(kAccThreads, 1)
             accumulate_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapY, const __grid_constant__ AccArgs a,
                               const __grid_constant__ typename Epi::Args ea)
         {
             constexpr int      ROWS   = PAIR ? 256 : 128;
-            constexpr uint32_t kStage = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u; // 128 rows of X, this CTA's rows of Y
+            // A stage: PAIR 128 rows of X, then this CTA's 128 rows of Y; else TN rows of Y, then the rows of X that there are
+            // (a.xRows: a few tokens need not fill 128 rows, the MMAs read what lies behind and nobody looks at those rows)
+            constexpr uint32_t yOff   = PAIR ? 16384u : uint32_t(TN) * 128u;
+            const uint32_t     kStage = PAIR ? 32768u : yOff + uint32_t(a.xRows) * 128u;
             constexpr uint32_t kCols  = 2 * TN < 32 ? 32 : 2 * TN;
             extern __shared__ unsigned char smemRaw[];
             unsigned char* tiles = (unsigned char*)((uintptr_t(smemRaw) + 1023) & ~uintptr_t(1023));
@@ -302,7 +309,15 @@ namespace htb
                             if(leader)
                                 mbarArriveExpectTx(fullAddr + 8 * stage, (PAIR ? 2 : 1) * kStage);
                             const int k0 = kb * a.kElems;
-                            if constexpr(PAIR)
+                            if constexpr(MN)
+                            {
+                                static_assert(!MN || (PAIR && !F8), "only pairs on half precision");
+                                tmaLoadPair2(dst, &mapX, bar, x0, k0);
+                                tmaLoadPair2(dst + 8192, &mapX, bar, x0 + 64, k0);
+                                tmaLoadPair2(dst + 16384, &mapY, bar, y0, k0);
+                                tmaLoadPair2(dst + 16384 + 8192, &mapY, bar, y0 + 64, k0);
+                            }
+                            else if constexpr(PAIR)
                             {
                                 tmaLoadPair2(dst, &mapX, bar, k0, x0);
                                 tmaLoadPair2(dst + 16384, &mapY, bar, k0, y0);
@@ -310,8 +325,8 @@ namespace htb
                             else
                             {
                                 const int cx[2] = {k0, x0}, cy[2] = {k0, y0};
-                                tmaLoad<2>(dst, &mapX, bar, cx);
-                                tmaLoad<2>(dst + 16384, &mapY, bar, cy);
+                                tmaLoad<2>(dst + yOff, &mapX, bar, cx);
+                                tmaLoad<2>(dst, &mapY, bar, cy);
                             }
                             if(++stage == uint32_t(a.stages))
                             {
@@ -340,7 +355,9 @@ namespace htb
                 constexpr uint32_t ISSUERS = F8 ? 2 : 1;
                 if(lane == 0 && leader && uint32_t(warp) <= ISSUERS)
                 {
-                    const uint64_t descX = smemDesc(tilesAddr), descY = smemDesc(tilesAddr + 16384);
+                    const uint64_t descX = MN ? smemDescMn(tilesAddr) : smemDesc(tilesAddr + (PAIR ? 0u : yOff));
+                    const uint64_t descY = MN ? smemDescMn(tilesAddr + 16384) : smemDesc(tilesAddr + (PAIR ? 16384u : 0u));
+                    constexpr int  step  = MN ? 128 : 2; // a K step of 32 bytes (MN: of 16 rows), in units of 16 bytes
                     const uint32_t self = uint32_t(warp) - 1;
                     uint32_t       stage = 0, phase = 0, bufPhase = 0, seq = 0;
                     bool           ok = true;
@@ -383,7 +400,7 @@ namespace htb
                                 {
                                     if(s == 2 && k + 1 < end) // a look at the next stage while MMAs are queued
                                         ready = mbarTest(fullAddr + 8 * stage, phase);
-                                    issueMma<PAIR, F8>(d, descX + off + 2 * s, descY + off + 2 * s, a.idesc, (k != kb || s != 0) ? 1u : 0u);
+                                    issueMma<PAIR, F8>(d, descX + off + step * s, descY + off + step * s, a.idesc, (k != kb || s != 0) ? 1u : 0u);
                                 }
                                 // frees the stage once these MMAs have read it, which with one block a chunk (F8) also says
                                 // that the chunk is summed
@@ -408,7 +425,7 @@ namespace htb
             {
                 if constexpr(Epi::kSide > 0)
                 {
-                    float* const       ring = reinterpret_cast<float*>(tiles + size_t(a.stages) * kStage);
+                    float* const       ring = reinterpret_cast<float*>(tiles + a.stageBytes);
                     typename Epi::Side side(ea, lane);
                     uint32_t           slot = 0, phase = 0;
                     bool               ok = true;
@@ -447,10 +464,10 @@ namespace htb
                 if constexpr(kMoreRegs)
                     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAccRegsEpi));
                 const int quad = warp & 3, half = (warp - 4) >> 2;
-                Epi       epi(ea, warp - 4, lane, tiles + size_t(a.stages) * kStage);
+                Epi       epi(ea, warp - 4, lane, tiles + a.stageBytes);
                 uint32_t  buf = 0, bufPhase = 0, stage = 0, phase = 0; // stage and phase: F8, a chunk is one stage
                 uint32_t  slot = 0, slotPhase = 0;
-                const float* ring = reinterpret_cast<const float*>(tiles + size_t(a.stages) * kStage);
+                const float* ring = reinterpret_cast<const float*>(tiles + a.stageBytes);
                 bool      ok = true;
                 int       syncs = 0;
                 const uint32_t emptyLeader = PAIR ? mapToRank(smemAddr(&tmemEmptyBar[0]), 0) : smemAddr(&tmemEmptyBar[0]);

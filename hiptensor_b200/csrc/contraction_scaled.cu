@@ -565,6 +565,8 @@ namespace htb
                 return regs;
             if(cudaError_t e = ensureDynamicSmem((const void*)kernel, int(smem)))
                 return e;
+            a.xRows                   = 128;
+            a.stageBytes              = uint32_t(a.stages) * stage;
             const int           csize = PAIR ? 2 : a.ksplit;
             cudaLaunchConfig_t  cfg{};
             cudaLaunchAttribute attr[2];

@@ -58,17 +58,17 @@ namespace htb
                 return here;
             };
             const uint64_t T = uint64_t(p.T), n = uint64_t(piece);
-            l.hOff           = take(l.packH, T * uint64_t(l.ld) * size);
+            const bool f32   = p.type == CUDA_R_32F, two = gradient && !f32 && splitProbabilities(p.T);
+            l.hOff           = take(l.packH, (two ? 2 : 1) * T * uint64_t(l.ld) * size);
             l.stateOff       = take(!gradient, T * 12);
             l.scaleOff       = take(gradient, 8);
             l.restOff        = take(gradient, T * 4);
             l.dhOff          = take(gradient, T * uint64_t(l.ld) * 4);
             l.wOff           = take(l.packW, n * uint64_t(l.ld) * size);
-            const bool f32   = p.type == CUDA_R_32F;
             l.zOff           = take(f32, T * n * 4);
             l.partOff        = take(!f32 && !gradient, (n + headGroup(p.T) - 1) / headGroup(p.T) * T * 8);
-            l.pOff           = take(!f32 && gradient, T * n * size);
-            l.dwOff          = take(gradient && p.type == CUDA_R_16F, n * uint64_t(l.ld) * 4);
+            l.pOff           = take(!f32 && gradient, (two ? 2 : 1) * T * n * size);
+            l.dwOff          = take(gradient && !f32 && l.packW, n * uint64_t(l.ld) * 4);
             l.bytes          = at + 256; // room to align the caller's pointer
             return l;
         }
@@ -292,7 +292,7 @@ namespace htb
         int64_t            ldh    = p.nt ? p.tStride[0] : l.ld;
         if(l.packH)
         {
-            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, nullptr, stream));
+            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, nullptr, false, stream));
             h   = ws + l.hOff;
             ldh = l.ld;
         }
@@ -305,7 +305,7 @@ namespace htb
             int64_t       ldw = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, false, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
@@ -349,7 +349,7 @@ namespace htb
         if(!dH && !dW)
             return HIPTENSOR_STATUS_SUCCESS;
         if((p.T > 0 && (!alpha || !H || !W || !targets || !lse || !gradLoss)) || ((uintptr_t(H) | uintptr_t(W)) & 15)
-           || (uintptr_t(targets) & 7) || ((uintptr_t(lse) | uintptr_t(gradLoss)) & 3) || (uintptr_t(dH) % size) || (uintptr_t(dW) % size))
+           || ((uintptr_t(dH) | uintptr_t(dW)) & 15) || (uintptr_t(targets) & 7) || ((uintptr_t(lse) | uintptr_t(gradLoss)) & 3))
         {
             HTB_LOG_ERROR(fn, "Input Parameter Error : a required pointer is nullptr or not aligned (%s)",
                           hiptensorGetErrorString(HIPTENSOR_STATUS_INVALID_VALUE));
@@ -378,8 +378,10 @@ namespace htb
             scale = reinterpret_cast<float*>(ws + l.scaleOff);
             HTB_TRY(launchGradientScale(gradLoss, a, p.T, scale, stream));
         }
-        void* h = ws + l.hOff;
-        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, h, targets, p.ignore, p.V, st->deviceStatus, stream));
+        const bool    two   = !f32 && splitProbabilities(p.T);
+        const int64_t rowsK = two ? 2 * p.T : p.T; // of P and H in the weights' product
+        void*         h     = ws + l.hOff;
+        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, h, targets, p.ignore, p.V, st->deviceStatus, two, stream));
         float*       z   = reinterpret_cast<float*>(ws + l.zOff);
         void*        P   = f32 ? (void*)z : (void*)(ws + l.pOff);
         float*       dh  = reinterpret_cast<float*>(ws + l.dhOff);
@@ -393,7 +395,7 @@ namespace htb
             int64_t       ldw = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, false, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
@@ -411,9 +413,14 @@ namespace htb
             if(dW)
             {
                 unsigned char* out = static_cast<unsigned char*>(dW) + v0 * p.wV * size;
-                if(scale)
+                if(!f32 && !l.packW)
+                    HTB_TRY(launchWeightGradient(p.type, P, l.piece, h, l.ld, rowsK, n, p.D, scale, out, p.wV, st->smCount, st->deviceStatus,
+                                                 stream));
+                else if(!f32)
                 {
-                    HTB_TRY(product(Pm, 0, 1, Hm, 0, 2, Matrix{dw, n, p.D, l.ld, 1, CUDA_R_32F}, 1, 2, 1.f, 0.f, st, stream));
+                    // rows of W that no bulk store can write: through f32 in the workspace
+                    const Matrix P2{P, rowsK, n, l.piece, 1, p.type}, H2{h, rowsK, p.D, l.ld, 1, p.type};
+                    HTB_TRY(product(P2, 0, 1, H2, 0, 2, Matrix{dw, n, p.D, l.ld, 1, CUDA_R_32F}, 1, 2, 1.f, 0.f, st, stream));
                     HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, stream));
                 }
                 else

@@ -60,7 +60,7 @@ namespace htb
 
         template <typename T>
         __global__ void pack_rows_kernel(const T* __restrict__ X, const __grid_constant__ TokenRows rows, int64_t count, int64_t cols, int64_t ld,
-                                         T* __restrict__ X2, const int64_t* __restrict__ targets, int64_t ignore, int64_t V, int* status)
+                                         T* __restrict__ X2, const int64_t* __restrict__ targets, int64_t ignore, int64_t V, int* status, bool twice)
         {
             for(int64_t r = blockIdx.x; r < count; r += gridDim.x)
             {
@@ -69,7 +69,12 @@ namespace htb
                 if(!live && targets[r] != ignore && threadIdx.x == 0)
                     atomicExch_system(status, kStatusBadTarget);
                 for(int64_t c = threadIdx.x; c < ld; c += blockDim.x)
-                    X2[r * ld + c] = (live && c < cols) ? src[c * rows.elem] : narrow<T>(0.f);
+                {
+                    const T x      = (live && c < cols) ? src[c * rows.elem] : narrow<T>(0.f);
+                    X2[r * ld + c] = x;
+                    if(twice)
+                        X2[(count + r) * ld + c] = x;
+                }
             }
         }
 
@@ -252,7 +257,8 @@ namespace htb
             // gradient
             const float *lse, *g, *scale;
             float*       rest; // what rounding took from the target's entry of P
-            CUtensorMap  mapP;
+            int          two; // P as a sum of two numbers of the type: what rounding took from every entry goes to mapLow
+            CUtensorMap  mapP, mapLow;
         };
 
         // Common to both: the sums of a chunk of up to 1024 elements are added to the running ones with rounding (the
@@ -427,8 +433,105 @@ namespace htb
                     const float p = (exp2f(x) - 1.f) * f;
                     a.rest[row]   = p - widen(narrow<TP>(p));
                 }
+                const int lows = TN == 64 ? a.two : 0;
+                for(int low = 0; low <= lows; low++)
 #pragma unroll
-                for(int r = 0; r < COLS; r += ROUND)
+                    for(int r = 0; r < COLS; r += ROUND)
+                    {
+                        const uint32_t at = slot + uint32_t((stores % SLOTS) * 4096);
+                        if(lane == 0)
+                            asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(SLOTS - 1) : "memory"); // the slot's last store has read it
+                        __syncwarp();
+                        stores++;
+#pragma unroll
+                        for(int u = 0; u < ROUND / 8; u++)
+                        {
+                            uint32_t q[4];
+#pragma unroll
+                            for(int j = 0; j < 4; j++)
+                            {
+                                const int    k = r + 8 * u + 2 * j;
+                                const float2 x = unpack2(fma2(acc[k / 2], c2, l2));
+                                float        p0 = exp2f(x.x), p1 = exp2f(x.y);
+                                if(t == k)
+                                    p0 -= 1.f;
+                                if(t == k + 1)
+                                    p1 -= 1.f;
+                                p0 = live ? p0 * f : 0.f;
+                                p1 = live ? p1 * f : 0.f;
+                                TP lo = narrow<TP>(p0), hi = narrow<TP>(p1);
+                                if(TN == 64 && low)
+                                {
+                                    lo = narrow<TP>(p0 - widen(lo));
+                                    hi = narrow<TP>(p1 - widen(hi));
+                                }
+                                q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo))
+                                       | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
+                            }
+                            // 16-byte units permuted as the map's swizzle has them (rows of 64 bytes are not swizzled)
+                            const uint32_t unit = ROUND == 64 ? uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4)) : uint32_t(lane * ROUND * 2 + (u << 4));
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + unit), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                                         : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if(lane == 0)
+                        {
+                            // a block that begins outside P has nothing to store (one that ends outside is clipped)
+                            if(row < a.T && col + r < a.n)
+                                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(low ? &a.mapLow : &a.mapP),
+                                             "r"(at), "r"(int(col + r)), "r"(int(row))
+                                             : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                    }
+            }
+            __device__ __forceinline__ void leave()
+            {
+                if(lane == 0)
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+        };
+
+        // dW = P^T H of a piece: the sums (times scale[1]) rounded once, out by bulk stores while the next tile is summed.
+        struct WeightArgs
+        {
+            int64_t      rows, cols;
+            const float* scale;
+            CUtensorMap  mapD;
+        };
+        template <typename TD>
+        struct WeightEpi : HeadSums<256>
+        {
+            using Args                   = WeightArgs;
+            static constexpr int  kSide  = 0;
+            static constexpr bool kSplit = false;
+            static constexpr int  SLOTS  = 2;
+            static constexpr int  ROOM   = 8 * SLOTS * 4096;
+            const Args&           a;
+            const int             lane;
+            const uint32_t        slot;
+            int                   stores;
+
+            __device__ WeightEpi(const Args& args, int w, int l, unsigned char* smem)
+                : a(args)
+                , lane(l)
+                , slot(smemAddr(smem) + uint32_t(w * SLOTS * 4096))
+                , stores(0)
+            {
+            }
+            __device__ __forceinline__ void begin() {}
+            template <class Release>
+            __device__ __forceinline__ void add(uint32_t taddr, bool first, Release release)
+            {
+                addSums(taddr, first, release);
+            }
+            __device__ __forceinline__ void end(int64_t row, int64_t col)
+            {
+                const float    f  = a.scale ? a.scale[1] : 1.f;
+                const uint64_t f2 = pack2(f, f);
+#pragma unroll
+                for(int r = 0; r < COLS; r += 64)
                 {
                     const uint32_t at = slot + uint32_t((stores % SLOTS) * 4096);
                     if(lane == 0)
@@ -436,34 +539,26 @@ namespace htb
                     __syncwarp();
                     stores++;
 #pragma unroll
-                    for(int u = 0; u < ROUND / 8; u++)
+                    for(int u = 0; u < 8; u++)
                     {
                         uint32_t q[4];
 #pragma unroll
                         for(int j = 0; j < 4; j++)
                         {
-                            const int    k = r + 8 * u + 2 * j;
-                            const float2 x = unpack2(fma2(acc[k / 2], c2, l2));
-                            float        p0 = exp2f(x.x), p1 = exp2f(x.y);
-                            if(t == k)
-                                p0 -= 1.f;
-                            if(t == k + 1)
-                                p1 -= 1.f;
-                            const TP lo = narrow<TP>(live ? p0 * f : 0.f), hi = narrow<TP>(live ? p1 * f : 0.f);
+                            const float2 x = unpack2(mul2(acc[(r + 8 * u + 2 * j) / 2], f2));
+                            const TD     lo = narrow<TD>(x.x), hi = narrow<TD>(x.y);
                             q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo)) | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
                         }
-                        // 16-byte units permuted as the map's swizzle has them (rows of 64 bytes are not swizzled)
-                        const uint32_t unit = ROUND == 64 ? uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4)) : uint32_t(lane * ROUND * 2 + (u << 4));
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + unit), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))),
+                                     "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
                                      : "memory");
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if(lane == 0)
                     {
-                        // a block that begins outside P has nothing to store (one that ends outside is clipped)
-                        if(row < a.T && col + r < a.n)
-                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&a.mapP), "r"(at),
+                        if(row < a.rows && col + r < a.cols)
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&a.mapD), "r"(at),
                                          "r"(int(col + r)), "r"(int(row))
                                          : "memory");
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -550,33 +645,15 @@ namespace htb
                    == CUDA_SUCCESS;
         }
 
-        template <class Epi, bool PAIR, int TN>
-        cudaError_t launchHeadForm(const HeadProduct& h, HeadArgs& ea, int smCount, int* status, cudaStream_t stream, const char* name)
+        template <class Epi, bool PAIR, int TN, bool MN>
+        cudaError_t launchAccumulate(const CUtensorMap& mapX, const CUtensorMap& mapY, const AccArgs& a, const typename Epi::Args& ea, int smCount,
+                                     cudaStream_t stream, const char* name)
         {
-            PFN_encodeTiled encode = tensorMapEncoder();
-            auto            kernel = accumulate_kernel<Epi, PAIR, TN, false>;
-            static const cudaError_t regs = accCheckRegs((const void*)kernel, TN);
-            if(!encode || regs != cudaSuccess)
-                return encode ? regs : cudaErrorNotSupported;
-            CUtensorMap mapX, mapY;
-            if(!encodeMatrix(encode, &mapX, h.H, h.D, h.T, h.ldh, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)
-               || !encodeMatrix(encode, &mapY, h.W, h.D, h.n, h.ldw, 64, PAIR ? 128 : TN, CU_TENSOR_MAP_SWIZZLE_128B))
-                return cudaErrorNotSupported;
-            constexpr int  rows  = PAIR ? 256 : 128;
-            const uint32_t stage = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
-            AccArgs        a{};
-            a.tilesM     = int((h.T + rows - 1) / rows);
-            a.tilesN     = int((h.n + TN - 1) / TN);
-            a.kBlocks    = int((h.D + 63) / 64);
-            a.chunk      = 16;
-            a.kElems     = 64;
-            a.ksplit     = 1;
-            a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (rows * h.D * 2))));
-            a.stages     = std::min<int>(kAccMaxStages, int((226 * 1024 - 1024 - Epi::ROOM) / stage));
-            a.idesc      = (1u << 4) | (h.type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TN >> 3) << 17) | (uint32_t(rows >> 4) << 24);
-            a.status     = status;
-            a.statusCode = kStatusSoftmax;
-            const size_t smem = size_t(a.stages) * stage + 1024 + Epi::ROOM;
+            auto                     kernel = accumulate_kernel<Epi, PAIR, TN, false, MN>;
+            static const cudaError_t regs   = accCheckRegs((const void*)kernel, TN);
+            if(regs != cudaSuccess)
+                return regs;
+            const size_t smem = size_t(a.stageBytes) + 1024 + Epi::ROOM;
             if(cudaError_t e = ensureDynamicSmem((const void*)kernel, int(smem)))
                 return e;
             const int           csize = PAIR ? 2 : 1;
@@ -599,6 +676,36 @@ namespace htb
                 noteLaunch(name);
             return e;
         }
+
+        template <class Epi, bool PAIR, int TN>
+        cudaError_t launchHeadForm(const HeadProduct& h, HeadArgs& ea, int smCount, int* status, cudaStream_t stream, const char* name)
+        {
+            PFN_encodeTiled encode = tensorMapEncoder();
+            if(!encode)
+                return cudaErrorNotSupported;
+            constexpr int rows  = PAIR ? 256 : 128;
+            const int     xRows = PAIR ? 128 : int(std::min<int64_t>(128, (h.T + 7) / 8 * 8)); // no more rows of H than there are tokens
+            const uint32_t stage = (uint32_t(xRows) + (PAIR ? 128u : uint32_t(TN))) * 128u, behind = uint32_t(128 - xRows) * 128u;
+            CUtensorMap mapX, mapY;
+            if(!encodeMatrix(encode, &mapX, h.H, h.D, h.T, h.ldh, 64, xRows, CU_TENSOR_MAP_SWIZZLE_128B)
+               || !encodeMatrix(encode, &mapY, h.W, h.D, h.n, h.ldw, 64, PAIR ? 128 : TN, CU_TENSOR_MAP_SWIZZLE_128B))
+                return cudaErrorNotSupported;
+            AccArgs        a{};
+            a.tilesM     = int((h.T + rows - 1) / rows);
+            a.tilesN     = int((h.n + TN - 1) / TN);
+            a.kBlocks    = int((h.D + 63) / 64);
+            a.chunk      = 16;
+            a.kElems     = 64;
+            a.ksplit     = 1;
+            a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (rows * h.D * 2))));
+            a.xRows      = xRows;
+            a.stages     = std::min<int>(kAccMaxStages, int((226 * 1024 - 1024 - Epi::ROOM - behind) / stage));
+            a.stageBytes = (uint32_t(a.stages) * stage + behind + 1023) / 1024 * 1024;
+            a.idesc      = (1u << 4) | (h.type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TN >> 3) << 17) | (uint32_t(rows >> 4) << 24);
+            a.status     = status;
+            a.statusCode = kStatusSoftmax;
+            return launchAccumulate<Epi, PAIR, TN, false>(mapX, mapY, a, ea, smCount, stream, name);
+        }
         // Up to 128 tokens the classes' rows are the traffic and a tile of 128 tokens is enough: 128 x 64 tiles, which
         // spread a vocabulary evenly over the SMs. Beyond, 256 x 256 tiles of CTA pairs.
         bool narrowHead(int64_t T)
@@ -619,6 +726,44 @@ namespace htb
         }
     } // namespace
 
+    cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
+                                     const float* scale, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream)
+    {
+        PFN_encodeTiled encode = tensorMapEncoder();
+        WeightArgs      ea{};
+        ea.rows = n, ea.cols = D, ea.scale = scale;
+        CUtensorMap mapX, mapY;
+        if(!encode || !encodeMatrix(encode, &mapX, P, n, K, ldp, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
+           || !encodeMatrix(encode, &mapY, H, D, K, ldh, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
+           || !encodeMatrix(encode, &ea.mapD, dW, D, n, ldw, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+            return cudaErrorNotSupported;
+        AccArgs a{};
+        a.tilesM     = int((n + 255) / 256);
+        a.tilesN     = int((D + 255) / 256);
+        a.kBlocks    = int((K + 63) / 64);
+        a.chunk      = 16;
+        a.kElems     = 64;
+        a.xRows      = 128;
+        a.ksplit     = 1;
+        a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (256 * K * 2))));
+        a.stages     = int((226 * 1024 - 1024 - WeightEpi<__half>::ROOM) / 32768);
+        a.stageBytes = uint32_t(a.stages) * 32768u;
+        // f32 sums, both operands transposed (contiguous along their rows)
+        a.idesc = (1u << 4) | (type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | (uint32_t(256 >> 3) << 17)
+                  | (uint32_t(256 >> 4) << 24);
+        a.status     = status;
+        a.statusCode = kStatusSoftmax;
+        return type == CUDA_R_16F ? launchAccumulate<WeightEpi<__half>, true, 256, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight")
+                                  : launchAccumulate<WeightEpi<__nv_bfloat16>, true, 256, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight");
+    }
+
+    // A row of dW is a sum over the tokens of which the class's own ones outweigh the others: over few tokens the rounding of
+    // P does not average out (up to 1.5 times the rounding of dW itself). P is then handed over as two numbers, which
+    // doubles a short sum that is bound by the bytes of dW all the same.
+    bool splitProbabilities(int64_t T)
+    {
+        return T <= 64;
+    }
     int headGroup(int64_t T)
     {
         return narrowHead(T) ? 32 : 128;
@@ -657,6 +802,10 @@ namespace htb
         const bool      narrow = narrowHead(h.T);
         if(!encode || !encodeMatrix(encode, &ea.mapP, P, h.n, h.T, ldp, narrow ? 32 : 64, 32, narrow ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
             return cudaErrorNotSupported;
+        ea.two = splitProbabilities(h.T) ? 1 : 0;
+        if(ea.two
+           && !encodeMatrix(encode, &ea.mapLow, static_cast<const char*>(P) + h.T * ldp * 2, h.n, h.T, ldp, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE))
+            return cudaErrorNotSupported;
         if(h.type == CUDA_R_16F)
             return narrow ? launchHeadForm<ProbabilityEpi<__half, 64>, false, 64>(h, ea, smCount, status, stream, "cross_entropy_head_gradient")
                           : launchHeadForm<ProbabilityEpi<__half, 256>, true, 256>(h, ea, smCount, status, stream, "cross_entropy_head_gradient_pair");
@@ -665,16 +814,16 @@ namespace htb
     }
 
     cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t cols, int64_t ld, void* X2,
-                               const int64_t* targets, int64_t ignore, int64_t V, int* status, cudaStream_t stream)
+                               const int64_t* targets, int64_t ignore, int64_t V, int* status, bool twice, cudaStream_t stream)
     {
         const int grid = rowGrid(count);
         if(type == CUDA_R_32F)
-            pack_rows_kernel<float><<<grid, 256, 0, stream>>>((const float*)X, rows, count, cols, ld, (float*)X2, targets, ignore, V, status);
+            pack_rows_kernel<float><<<grid, 256, 0, stream>>>((const float*)X, rows, count, cols, ld, (float*)X2, targets, ignore, V, status, twice);
         else if(type == CUDA_R_16F)
-            pack_rows_kernel<__half><<<grid, 256, 0, stream>>>((const __half*)X, rows, count, cols, ld, (__half*)X2, targets, ignore, V, status);
+            pack_rows_kernel<__half><<<grid, 256, 0, stream>>>((const __half*)X, rows, count, cols, ld, (__half*)X2, targets, ignore, V, status, twice);
         else
             pack_rows_kernel<__nv_bfloat16>
-                <<<grid, 256, 0, stream>>>((const __nv_bfloat16*)X, rows, count, cols, ld, (__nv_bfloat16*)X2, targets, ignore, V, status);
+                <<<grid, 256, 0, stream>>>((const __nv_bfloat16*)X, rows, count, cols, ld, (__nv_bfloat16*)X2, targets, ignore, V, status, twice);
         return noted("cross_entropy_pack");
     }
 

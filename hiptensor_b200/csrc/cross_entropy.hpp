@@ -45,9 +45,9 @@ namespace htb
         int64_t elem; // stride along the contracted mode
     };
     // X2[r, 0 .. ld) = X[row r, 0 .. cols), zeros behind. With targets: rows whose target is `ignore` or no class become zeros,
-    // and the latter raise the status word.
+    // and the latter raise the status word. twice: the rows again behind the first `count`.
     cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t cols, int64_t ld, void* X2,
-                               const int64_t* targets, int64_t ignore, int64_t V, int* status, cudaStream_t stream);
+                               const int64_t* targets, int64_t ignore, int64_t V, int* status, bool twice, cudaStream_t stream);
 
     // f16 / bf16: logits of n classes from v0 on, used where they are made
     struct HeadProduct
@@ -63,10 +63,16 @@ namespace htb
     // joins a piece's partial results with state[0 .. 2T) (maximum, sum in powers of two); after the last piece loss and lse
     cudaError_t launchLossJoin(const void* part, int64_t n, int64_t T, float* state, bool first, bool last, int64_t V, int64_t ignore,
                                const int64_t* targets, float* loss, float* lse, int* status, cudaStream_t stream);
-    // P[t, v] = (exp(z - lse) - [v0 + v == target]) * g * alpha (* scale[0]); rest[t]: what rounding took from the target's entry
+    // P[t, v] = (exp(z - lse) - [v0 + v == target]) * g * alpha (* scale[0]); rest[t]: what rounding took from the target's entry;
+    // with splitProbabilities(T) what it took from every entry in T more rows
+    bool splitProbabilities(int64_t T);
     cudaError_t launchHeadGradient(const HeadProduct& h, int64_t v0, int64_t V, int64_t ignore, const int64_t* targets, const float* lse,
                                    const float* g, float alpha, const float* scale, void* P, int64_t ldp, float* rest, int smCount, int* status,
                                    cudaStream_t stream);
+
+    // dW[v, d] = sum over K rows of P[k, v] H[k, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes
+    cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
+                                     const float* scale, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream);
 
     // f32: logits of a piece in memory, z[t, v] with rows ldz apart
     // running maximum / sum / target logit per token: state[0 .. T), [T .. 2T), [2T .. 3T)

@@ -166,8 +166,8 @@ int htScaledContraction(const htHandle* handle, const htScaledContractionPlan* p
  *
  * Logits z = alpha * (H contracted with W) are never kept: they are made, used and dropped piece by piece of the
  * vocabulary. The modes that H and W share are contracted, H's other modes are the tokens (numbered in modeH's order, the
- * last one fastest), W's other modes the classes (numbered likewise). H and W are f16, bf16 or f32, both the same, and start at
- * multiples of 16 bytes; targets are int64, loss, lse and gradLoss f32, one packed value for each token.
+ * last one fastest), W's other modes the classes (numbered likewise). H and W are f16, bf16 or f32, both the same; they and
+ * dH and dW start at multiples of 16 bytes; targets are int64, loss, lse and gradLoss f32, one packed value for each token.
  *     lse = log sum over classes of exp z,   loss = lse - z[target];   loss = 0 where target == ignoreIndex
  *     P = (exp(z - lse) - [class == target]) * gradLoss * alpha, 0 where target == ignoreIndex
  *     dH = P contracted with W (laid out like H),   dW = P contracted with H (laid out like W)
