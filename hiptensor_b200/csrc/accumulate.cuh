@@ -38,6 +38,8 @@ namespace htb
             int      groupM; // tiles of M that are walked together, for the sake of L2
             int      kBlocks; // 128-byte blocks along K
             int      chunk; // K blocks per chunk (1 for 8-bit operands)
+            int      sub; // K blocks per stage (1 for 8-bit operands); chunks are multiples of it
+            int      kParts; // > 1: one tile of rows, and tm counts parts of the K range whose sums stay apart
             int      kElems; // elements of a 128-byte block: 128 (8 bit) or 64
             int      xRows; // not PAIR: rows of X that are loaded, a multiple of 8
             int      ksplit; // CTAs of a cluster that share a tile (not PAIR)
@@ -199,18 +201,19 @@ namespace htb
             return at.numRegs >= kAccRegs ? cudaSuccess : cudaErrorInvalidKernelImage;
         }
 
-        // MN: both operands are contiguous along their rows (X^T Y of matrices with one row per k; half precision): 64-row chunks of
+        // XMN, YMN: the operand is contiguous along its rows (a matrix with one row per k; half precision): 64-row chunks of
         // [64 k][128 bytes] instead of rows of 128 bytes along k, transposed descriptors.
-        template <class Epi, bool PAIR, int TN, bool F8, bool MN = false>
+        template <class Epi, bool PAIR, int TN, bool F8, bool XMN = false, bool YMN = false>
         __global__ void __launch_bounds__(kAccThreads, 1)
             accumulate_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapY, const __grid_constant__ AccArgs a,
                               const __grid_constant__ typename Epi::Args ea)
         {
             constexpr int      ROWS   = PAIR ? 256 : 128;
-            // A stage: PAIR 128 rows of X, then this CTA's 128 rows of Y; else TN rows of Y, then the rows of X that there are
+            // A K block: PAIR 128 rows of X, then this CTA's 128 rows of Y; else TN rows of Y, then the rows of X that there are
             // (a.xRows: a few tokens need not fill 128 rows, the MMAs read what lies behind and nobody looks at those rows)
             constexpr uint32_t yOff   = PAIR ? 16384u : uint32_t(TN) * 128u;
-            const uint32_t     kStage = PAIR ? 32768u : yOff + uint32_t(a.xRows) * 128u;
+            const uint32_t     kBlock = PAIR ? 32768u : yOff + uint32_t(a.xRows) * 128u; // of one K block
+            const uint32_t     kStage = kBlock * uint32_t(a.sub);
             constexpr uint32_t kCols  = 2 * TN < 32 ? 32 : 2 * TN;
             extern __shared__ unsigned char smemRaw[];
             unsigned char* tiles = (unsigned char*)((uintptr_t(smemRaw) + 1023) & ~uintptr_t(1023));
@@ -278,8 +281,16 @@ namespace htb
             const uint32_t tilesAddr = smemAddr(tiles), fullAddr = smemAddr(&fullBar[0]), emptyAddr = smemAddr(&emptyBar[0]);
             const int      units = a.tilesM * a.tilesN;
             // K blocks of this CTA: all, or its part of a split tile
-            const int kbBegin = PAIR ? 0 : int((long long)a.kBlocks * int(rank) / a.ksplit);
-            const int kbEnd   = PAIR ? a.kBlocks : int((long long)a.kBlocks * (int(rank) + 1) / a.ksplit);
+            int  kbBegin = PAIR ? 0 : int((long long)a.kBlocks * int(rank) / a.ksplit);
+            int  kbEnd   = PAIR ? a.kBlocks : int((long long)a.kBlocks * (int(rank) + 1) / a.ksplit);
+            auto part    = [&](int& tm) { // kParts: the K range is the tile's, the rows are the first ones
+                if(!PAIR && a.kParts > 1)
+                {
+                    kbBegin = int((long long)a.kBlocks * tm / a.kParts);
+                    kbEnd   = int((long long)a.kBlocks * (tm + 1) / a.kParts);
+                    tm      = 0;
+                }
+            };
             // global memory is read and written from here on: the grid ahead of this one must be complete
             asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -299,34 +310,55 @@ namespace htb
                     {
                         int tm, tn;
                         tileOf(a, u, tm, tn);
+                        part(tm);
                         const int x0 = tm * ROWS + (PAIR ? int(rank) * 128 : 0), y0 = tn * TN + (PAIR ? int(rank) * 128 : 0);
-                        for(int kb = kbBegin; kb < kbEnd; kb++)
+                        for(int kb = kbBegin; kb < kbEnd; kb += a.sub)
                         {
                             ok = mbarWaitTight(emptyAddr + 8 * stage, phase ^ 1, abortP);
                             if(!ok)
                                 break;
-                            const uint32_t dst = tilesAddr + stage * kStage, bar = leaderFull + 8 * stage;
+                            const uint32_t bar = leaderFull + 8 * stage;
+                            const int      blocks = min(a.sub, kbEnd - kb);
                             if(leader)
-                                mbarArriveExpectTx(fullAddr + 8 * stage, (PAIR ? 2 : 1) * kStage);
-                            const int k0 = kb * a.kElems;
-                            if constexpr(MN)
+                                mbarArriveExpectTx(fullAddr + 8 * stage, (PAIR ? 2 : 1) * kBlock * uint32_t(blocks));
+                            for(int i = 0; i < blocks; i++)
                             {
-                                static_assert(!MN || (PAIR && !F8), "only pairs on half precision");
-                                tmaLoadPair2(dst, &mapX, bar, x0, k0);
-                                tmaLoadPair2(dst + 8192, &mapX, bar, x0 + 64, k0);
-                                tmaLoadPair2(dst + 16384, &mapY, bar, y0, k0);
-                                tmaLoadPair2(dst + 16384 + 8192, &mapY, bar, y0 + 64, k0);
-                            }
-                            else if constexpr(PAIR)
-                            {
-                                tmaLoadPair2(dst, &mapX, bar, k0, x0);
-                                tmaLoadPair2(dst + 16384, &mapY, bar, k0, y0);
-                            }
-                            else
-                            {
-                                const int cx[2] = {k0, x0}, cy[2] = {k0, y0};
-                                tmaLoad<2>(dst + yOff, &mapX, bar, cx);
-                                tmaLoad<2>(dst, &mapY, bar, cy);
+                                const uint32_t dst = tilesAddr + stage * kStage + i * kBlock;
+                                const uint32_t dstX = PAIR ? dst : dst + yOff, dstY = PAIR ? dst + 16384 : dst;
+                                const int      k0 = (kb + i) * a.kElems;
+                                static_assert(!(XMN || YMN) || !F8, "only half precision");
+                                static_assert(!XMN || PAIR, "128 rows of X in two chunks");
+                                if constexpr(XMN)
+                                {
+                                    tmaLoadPair2(dstX, &mapX, bar, x0, k0);
+                                    tmaLoadPair2(dstX + 8192, &mapX, bar, x0 + 64, k0);
+                                }
+                                else if constexpr(PAIR)
+                                    tmaLoadPair2(dstX, &mapX, bar, k0, x0);
+                                else
+                                {
+                                    const int c[2] = {k0, x0};
+                                    tmaLoad<2>(dstX, &mapX, bar, c);
+                                }
+                                if constexpr(YMN)
+                                {
+#pragma unroll
+                                    for(int c0 = 0; c0 < (PAIR ? 128 : TN); c0 += 64)
+                                    {
+                                        const int c[2] = {y0 + c0, k0};
+                                        if constexpr(PAIR)
+                                            tmaLoadPair2(dstY + c0 * 128, &mapY, bar, c[0], c[1]);
+                                        else
+                                            tmaLoad<2>(dstY + c0 * 128, &mapY, bar, c);
+                                    }
+                                }
+                                else if constexpr(PAIR)
+                                    tmaLoadPair2(dstY, &mapY, bar, k0, y0);
+                                else
+                                {
+                                    const int c[2] = {k0, y0};
+                                    tmaLoad<2>(dstY, &mapY, bar, c);
+                                }
                             }
                             if(++stage == uint32_t(a.stages))
                             {
@@ -355,13 +387,17 @@ namespace htb
                 constexpr uint32_t ISSUERS = F8 ? 2 : 1;
                 if(lane == 0 && leader && uint32_t(warp) <= ISSUERS)
                 {
-                    const uint64_t descX = MN ? smemDescMn(tilesAddr) : smemDesc(tilesAddr + (PAIR ? 0u : yOff));
-                    const uint64_t descY = MN ? smemDescMn(tilesAddr + 16384) : smemDesc(tilesAddr + (PAIR ? 16384u : 0u));
-                    constexpr int  step  = MN ? 128 : 2; // a K step of 32 bytes (MN: of 16 rows), in units of 16 bytes
+                    const uint32_t addrX = tilesAddr + (PAIR ? 0u : yOff), addrY = tilesAddr + (PAIR ? 16384u : 0u);
+                    const uint64_t descX = XMN ? smemDescMn(addrX) : smemDesc(addrX), descY = YMN ? smemDescMn(addrY) : smemDesc(addrY);
+                    constexpr int  stepX = XMN ? 128 : 2, stepY = YMN ? 128 : 2; // a K step of 32 bytes (MN: of 16 rows), in 16 bytes
                     const uint32_t self = uint32_t(warp) - 1;
                     uint32_t       stage = 0, phase = 0, bufPhase = 0, seq = 0;
                     bool           ok = true;
                     for(int u = clusterId; ok && u < units; u += numClusters)
+                    {
+                        int tm, tn;
+                        tileOf(a, u, tm, tn);
+                        part(tm);
                         for(int kb = kbBegin; ok && kb < kbEnd; kb += a.chunk, seq++)
                         {
                             const uint32_t buf = seq & 1;
@@ -384,28 +420,33 @@ namespace htb
                                 break;
                             if(ISSUERS == 2 || buf == 1)
                                 bufPhase ^= 1;
-                            for(int k = kb; k < end; k++)
+                            for(int k = kb; k < end; k += a.sub)
                             {
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                                const uint64_t off = uint64_t((stage * kStage) >> 4);
                                 const uint32_t now = stage;
                                 if(++stage == uint32_t(a.stages))
                                 {
                                     stage = 0;
                                     phase ^= 1;
                                 }
-                                bool ready = false;
-#pragma unroll
-                                for(int s = 0; s < 4; s++) // 32 bytes of K each
+                                bool      ready  = false;
+                                const int blocks = min(a.sub, end - k);
+                                for(int i = 0; i < blocks; i++)
                                 {
-                                    if(s == 2 && k + 1 < end) // a look at the next stage while MMAs are queued
-                                        ready = mbarTest(fullAddr + 8 * stage, phase);
-                                    issueMma<PAIR, F8>(d, descX + off + step * s, descY + off + step * s, a.idesc, (k != kb || s != 0) ? 1u : 0u);
+                                    const uint64_t off = uint64_t((now * kStage + i * kBlock) >> 4);
+#pragma unroll
+                                    for(int s = 0; s < 4; s++) // 32 bytes of K each
+                                    {
+                                        if(s == 2 && i + 1 == blocks && k + a.sub < end) // a look at the next stage while MMAs are queued
+                                            ready = mbarTest(fullAddr + 8 * stage, phase);
+                                        issueMma<PAIR, F8>(d, descX + off + stepX * s, descY + off + stepY * s, a.idesc,
+                                                           (k != kb || i != 0 || s != 0) ? 1u : 0u);
+                                    }
                                 }
                                 // frees the stage once these MMAs have read it, which with one block a chunk (F8) also says
                                 // that the chunk is summed
                                 commitTo<PAIR>(emptyAddr + 8 * now);
-                                if(k + 1 < end && !ready)
+                                if(k + a.sub < end && !ready)
                                     ok = mbarWaitTight(fullAddr + 8 * stage, phase, abortP);
                                 if(!ok)
                                     break;
@@ -413,6 +454,7 @@ namespace htb
                             if(!F8 && ok)
                                 commitTo<PAIR>(smemAddr(&tmemFullBar[buf]));
                         }
+                    }
                 }
                 if(!PAIR && clustered)
                 {
@@ -433,6 +475,7 @@ namespace htb
                     {
                         int tm, tn;
                         tileOf(a, u, tm, tn);
+                        part(tm);
                         side.begin(int64_t(tm) * ROWS + (PAIR ? int(rank) * 128 : 0), int64_t(tn) * TN);
                         for(int kb = kbBegin; kb < kbEnd;)
                         {
@@ -475,8 +518,10 @@ namespace htb
                 {
                     int tm, tn;
                     tileOf(a, u, tm, tn);
+                    const int tile = tm; // with kParts the rows of the parts' results follow each other
+                    part(tm);
                     const int     row = quad * 32 + lane;
-                    const int64_t r = int64_t(tm) * ROWS + (PAIR ? int(rank) * 128 : 0) + row, c = int64_t(tn) * TN + half * (TN / 2);
+                    const int64_t r = int64_t(tile) * ROWS + (PAIR ? int(rank) * 128 : 0) + row, c = int64_t(tn) * TN + half * (TN / 2);
                     epi.begin();
                     for(int kb = kbBegin; kb < kbEnd; kb += a.chunk)
                     {

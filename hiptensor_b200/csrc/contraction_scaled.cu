@@ -627,6 +627,8 @@ namespace htb
                     a.tilesN     = int(tilesN);
                     a.kBlocks    = int((p.K + 127) / 128);
                     a.chunk      = 1;
+                    a.sub        = 1;
+                    a.kParts     = 1;
                     a.kElems     = 128;
                     a.ksplit     = f.ksplit;
                     a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(tilesM, (int64_t(32) << 20) / (tileRows * p.K))));

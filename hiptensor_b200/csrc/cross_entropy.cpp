@@ -63,7 +63,8 @@ namespace htb
             l.stateOff       = take(!gradient, T * 12);
             l.scaleOff       = take(gradient, 8);
             l.restOff        = take(gradient, T * 4);
-            l.dhOff          = take(gradient, T * uint64_t(l.ld) * 4);
+            l.parts          = f32 ? 1 : hiddenParts(p.T, l.ld, piece, 0);
+            l.dhOff          = take(gradient, uint64_t(l.parts) * T * uint64_t(l.ld) * 4);
             l.wOff           = take(l.packW, n * uint64_t(l.ld) * size);
             l.zOff           = take(f32, T * n * 4);
             l.partOff        = take(!f32 && !gradient, (n + headGroup(p.T) - 1) / headGroup(p.T) * T * 8);
@@ -358,7 +359,7 @@ namespace htb
         if(p.T == 0)
         {
             if(dW) // no token, no gradient
-                HTB_TRY(launchStoreRows(p.type, nullptr, 0, p.V, p.D, nullptr, dW, plainRows(p.wV, p.wD, p.V), TargetRest{}, stream));
+                HTB_TRY(launchStoreRows(p.type, nullptr, 0, p.V, p.D, nullptr, dW, plainRows(p.wV, p.wD, p.V), TargetRest{}, 0, stream));
             return HIPTENSOR_STATUS_SUCCESS;
         }
         const CrossEntropyLayout l = layoutIn(p, true, workspace ? workspaceSize : 0);
@@ -408,7 +409,10 @@ namespace htb
             else
                 HTB_TRY(launchHeadGradient(HeadProduct{h, w, p.T, n, p.D, l.ld, ldw, p.type}, v0, p.V, p.ignore, targets, lse, gradLoss, a,
                                            scale, P, l.piece, rest, st->smCount, st->deviceStatus, stream));
-            if(dH)
+            if(dH && !f32 && narrowTokens(p.T))
+                HTB_TRY(launchHiddenGradient(p.type, P, l.piece, w, ldw, p.T, n, p.D, l.parts, dh, l.ld, v0 > 0, st->smCount, st->deviceStatus,
+                                             stream));
+            else if(dH)
                 HTB_TRY(product(Pm, 0, 1, Wm, 1, 2, Matrix{dh, p.T, p.D, l.ld, 1, CUDA_R_32F}, 0, 2, 1.f, v0 ? 1.f : 0.f, st, stream));
             if(dW)
             {
@@ -421,7 +425,7 @@ namespace htb
                     // rows of W that no bulk store can write: through f32 in the workspace
                     const Matrix P2{P, rowsK, n, l.piece, 1, p.type}, H2{h, rowsK, p.D, l.ld, 1, p.type};
                     HTB_TRY(product(P2, 0, 1, H2, 0, 2, Matrix{dw, n, p.D, l.ld, 1, CUDA_R_32F}, 1, 2, 1.f, 0.f, st, stream));
-                    HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, stream));
+                    HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, 1, stream));
                 }
                 else
                     HTB_TRY(product(Pm, 0, 1, Hm, 0, 2, Matrix{out, n, p.D, p.wV, p.wD, p.type}, 1, 2, 1.f, 0.f, st, stream));
@@ -429,7 +433,7 @@ namespace htb
         }
         if(dH)
             HTB_TRY(launchStoreRows(p.type, dh, l.ld, p.T, p.D, scale, dH, rowsOfH(p),
-                                    f32 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, stream));
+                                    f32 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, l.parts, stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }
 } // namespace htb

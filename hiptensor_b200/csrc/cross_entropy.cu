@@ -203,7 +203,7 @@ namespace htb
 
         template <typename T>
         __global__ void store_rows_kernel(const float* __restrict__ X, int64_t ldx, int64_t count, int64_t cols, const float* __restrict__ scale,
-                                          T* __restrict__ Y, const __grid_constant__ TokenRows rows, const __grid_constant__ TargetRest rest)
+                                          T* __restrict__ Y, const __grid_constant__ TokenRows rows, const __grid_constant__ TargetRest rest, int parts)
         {
             const float f = scale ? scale[1] : 1.f;
             for(int64_t r = blockIdx.x; r < count; r += gridDim.x)
@@ -222,7 +222,9 @@ namespace htb
                 }
                 for(int64_t c = threadIdx.x; c < cols; c += blockDim.x)
                 {
-                    float x = X ? X[r * ldx + c] : 0.f;
+                    float x = 0.f;
+                    for(int i = 0; i < parts; i++)
+                        x += X[(int64_t(i) * count + r) * ldx + c];
                     if(w)
                         x = fmaf(e, widen(w[c * rest.wD]), x);
                     dst[c * rows.elem] = narrow<T>(x * f);
@@ -389,7 +391,7 @@ namespace htb
             static constexpr int kSide = 0;
             static constexpr bool kSplit = false;
             static constexpr int ROUND = COLS < 64 ? COLS : 64; // columns of a slot: rows of 128 bytes (64 with TN = 64)
-            static constexpr int SLOTS = 2;
+            static constexpr int SLOTS = 1;
             static constexpr int ROOM  = 8 * SLOTS * 4096;
             const Args&          a;
             const int            lane;
@@ -506,7 +508,7 @@ namespace htb
             using Args                   = WeightArgs;
             static constexpr int  kSide  = 0;
             static constexpr bool kSplit = false;
-            static constexpr int  SLOTS  = 2;
+            static constexpr int  SLOTS  = 1;
             static constexpr int  ROOM   = 8 * SLOTS * 4096;
             const Args&           a;
             const int             lane;
@@ -570,6 +572,54 @@ namespace htb
                 if(lane == 0)
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             }
+        };
+
+        // dH = P W over parts of the classes, for up to 128 tokens: f32 sums of every part, [part][T][ld]
+        struct HiddenArgs
+        {
+            int64_t T, ld, cols;
+            float*  out;
+            int     add; // to what the pieces before left there
+        };
+        struct HiddenEpi : HeadSums<128>
+        {
+            using Args                   = HiddenArgs;
+            static constexpr int  kSide  = 0;
+            static constexpr bool kSplit = false;
+            static constexpr int  ROOM   = 0;
+            const Args&           a;
+
+            __device__ HiddenEpi(const Args& args, int, int, unsigned char*)
+                : a(args)
+            {
+            }
+            __device__ __forceinline__ void begin() {}
+            template <class Release>
+            __device__ __forceinline__ void add(uint32_t taddr, bool first, Release release)
+            {
+                addSums(taddr, first, release);
+            }
+            __device__ __forceinline__ void end(int64_t row, int64_t col)
+            {
+                const int64_t t = row & 127;
+                if(t >= a.T)
+                    return;
+                float* out = a.out + ((row >> 7) * a.T + t) * a.ld + col; // ld is a multiple of eight
+#pragma unroll
+                for(int j = 0; j < COLS; j += 4)
+                    if(col + j < a.ld)
+                    {
+                        const float2 x = unpack2(acc[j / 2]), y = unpack2(acc[j / 2 + 1]);
+                        float4       v = make_float4(x.x, x.y, y.x, y.y);
+                        if(a.add)
+                        {
+                            const float4 o = *reinterpret_cast<const float4*>(out + j);
+                            v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+                        }
+                        *reinterpret_cast<float4*>(out + j) = v;
+                    }
+            }
+            __device__ __forceinline__ void leave() {}
         };
 
         // Joins the partial maxima and sums of a piece, 32 tokens a block, a slice of the classes a warp (in the order of the
@@ -645,11 +695,11 @@ namespace htb
                    == CUDA_SUCCESS;
         }
 
-        template <class Epi, bool PAIR, int TN, bool MN>
+        template <class Epi, bool PAIR, int TN, bool XMN, bool YMN>
         cudaError_t launchAccumulate(const CUtensorMap& mapX, const CUtensorMap& mapY, const AccArgs& a, const typename Epi::Args& ea, int smCount,
                                      cudaStream_t stream, const char* name)
         {
-            auto                     kernel = accumulate_kernel<Epi, PAIR, TN, false, MN>;
+            auto                     kernel = accumulate_kernel<Epi, PAIR, TN, false, XMN, YMN>;
             static const cudaError_t regs   = accCheckRegs((const void*)kernel, TN);
             if(regs != cudaSuccess)
                 return regs;
@@ -699,12 +749,16 @@ namespace htb
             a.ksplit     = 1;
             a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (rows * h.D * 2))));
             a.xRows      = xRows;
-            a.stages     = std::min<int>(kAccMaxStages, int((226 * 1024 - 1024 - Epi::ROOM - behind) / stage));
-            a.stageBytes = (uint32_t(a.stages) * stage + behind + 1023) / 1024 * 1024;
+            // Waits and commits between MMAs cost the issuing thread several hundred cycles: two K blocks a stage for a pair's
+            // tiles (512 cycles of MMAs each), four for narrow ones (128)
+            a.sub        = PAIR ? 2 : 4;
+            a.kParts     = 1;
+            a.stages     = std::min<int>(kAccMaxStages, int((226 * 1024 - 1024 - Epi::ROOM - behind) / (stage * a.sub)));
+            a.stageBytes = (uint32_t(a.stages * a.sub) * stage + behind + 1023) / 1024 * 1024;
             a.idesc      = (1u << 4) | (h.type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TN >> 3) << 17) | (uint32_t(rows >> 4) << 24);
             a.status     = status;
             a.statusCode = kStatusSoftmax;
-            return launchAccumulate<Epi, PAIR, TN, false>(mapX, mapY, a, ea, smCount, stream, name);
+            return launchAccumulate<Epi, PAIR, TN, false, false>(mapX, mapY, a, ea, smCount, stream, name);
         }
         // Up to 128 tokens the classes' rows are the traffic and a tile of 128 tokens is enough: 128 x 64 tiles, which
         // spread a vocabulary evenly over the SMs. Beyond, 256 x 256 tiles of CTA pairs.
@@ -726,6 +780,49 @@ namespace htb
         }
     } // namespace
 
+    // Parts of the classes whose products run side by side: tiles of 128 columns alone would leave most SMs idle. One unit
+    // each for about every SM.
+    int hiddenParts(int64_t T, int64_t D, int64_t piece, int smCount)
+    {
+        if(!narrowHead(T))
+            return 1;
+        const int64_t tiles = (D + 127) / 128, sms = smCount > 0 ? smCount : 148;
+        return int(std::max<int64_t>(1, std::min<int64_t>((sms + tiles / 2) / tiles, piece / 1024)));
+    }
+
+    cudaError_t launchHiddenGradient(int type, const void* P, int64_t ldp, const void* W, int64_t ldw, int64_t T, int64_t n, int64_t D, int parts,
+                                     float* out, int64_t ldo, bool add, int smCount, int* status, cudaStream_t stream)
+    {
+        PFN_encodeTiled encode = tensorMapEncoder();
+        HiddenArgs      ea{};
+        ea.T = T, ea.ld = ldo, ea.cols = D, ea.out = out, ea.add = add;
+        const int   xRows = int((T + 7) / 8 * 8);
+        CUtensorMap mapX, mapY;
+        if(!encode || !encodeMatrix(encode, &mapX, P, n, T, ldp, 64, xRows, CU_TENSOR_MAP_SWIZZLE_128B)
+           || !encodeMatrix(encode, &mapY, W, D, n, ldw, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B))
+            return cudaErrorNotSupported;
+        const uint32_t block = (uint32_t(xRows) + 128u) * 128u, behind = uint32_t(128 - xRows) * 128u;
+        parts = int(std::min<int64_t>(parts, (n + 63) / 64)); // a short last piece: every part has something to add
+        AccArgs a{};
+        a.tilesM     = parts;
+        a.tilesN     = int((D + 127) / 128);
+        a.kBlocks    = int((n + 63) / 64);
+        a.chunk      = 16;
+        a.sub        = 2;
+        a.kParts     = parts;
+        a.kElems     = 64;
+        a.xRows      = xRows;
+        a.ksplit     = 1;
+        a.groupM     = parts;
+        a.stages     = std::min<int>(kAccMaxStages, int((226 * 1024 - 1024 - behind) / (block * a.sub)));
+        a.stageBytes = (uint32_t(a.stages * a.sub) * block + behind + 1023) / 1024 * 1024;
+        a.idesc      = (1u << 4) | (type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | (uint32_t(128 >> 3) << 17)
+                  | (uint32_t(128 >> 4) << 24); // Y transposed
+        a.status     = status;
+        a.statusCode = kStatusSoftmax;
+        return launchAccumulate<HiddenEpi, false, 128, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden");
+    }
+
     cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
                                      const float* scale, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream)
     {
@@ -746,15 +843,17 @@ namespace htb
         a.xRows      = 128;
         a.ksplit     = 1;
         a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (256 * K * 2))));
-        a.stages     = int((226 * 1024 - 1024 - WeightEpi<__half>::ROOM) / 32768);
-        a.stageBytes = uint32_t(a.stages) * 32768u;
+        a.sub        = 2;
+        a.kParts     = 1;
+        a.stages     = int((226 * 1024 - 1024 - WeightEpi<__half>::ROOM) / 65536);
+        a.stageBytes = uint32_t(a.stages) * 65536u;
         // f32 sums, both operands transposed (contiguous along their rows)
         a.idesc = (1u << 4) | (type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | (uint32_t(256 >> 3) << 17)
                   | (uint32_t(256 >> 4) << 24);
         a.status     = status;
         a.statusCode = kStatusSoftmax;
-        return type == CUDA_R_16F ? launchAccumulate<WeightEpi<__half>, true, 256, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight")
-                                  : launchAccumulate<WeightEpi<__nv_bfloat16>, true, 256, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight");
+        return type == CUDA_R_16F ? launchAccumulate<WeightEpi<__half>, true, 256, true, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight")
+                                  : launchAccumulate<WeightEpi<__nv_bfloat16>, true, 256, true, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight");
     }
 
     // A row of dW is a sum over the tokens of which the class's own ones outweigh the others: over few tokens the rounding of
@@ -763,6 +862,10 @@ namespace htb
     bool splitProbabilities(int64_t T)
     {
         return T <= 64;
+    }
+    bool narrowTokens(int64_t T)
+    {
+        return narrowHead(T);
     }
     int headGroup(int64_t T)
     {
@@ -855,15 +958,15 @@ namespace htb
     }
 
     cudaError_t launchStoreRows(int type, const float* X, int64_t ldx, int64_t count, int64_t cols, const float* scale, void* Y,
-                                const TokenRows& rows, const TargetRest& rest, cudaStream_t stream)
+                                const TokenRows& rows, const TargetRest& rest, int parts, cudaStream_t stream)
     {
         const int grid = rowGrid(count);
         if(type == CUDA_R_32F)
-            store_rows_kernel<float><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (float*)Y, rows, rest);
+            store_rows_kernel<float><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (float*)Y, rows, rest, parts);
         else if(type == CUDA_R_16F)
-            store_rows_kernel<__half><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (__half*)Y, rows, rest);
+            store_rows_kernel<__half><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (__half*)Y, rows, rest, parts);
         else
-            store_rows_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (__nv_bfloat16*)Y, rows, rest);
+            store_rows_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (__nv_bfloat16*)Y, rows, rest, parts);
         return noted("cross_entropy_store");
     }
 } // namespace htb

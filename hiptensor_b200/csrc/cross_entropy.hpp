@@ -28,6 +28,7 @@ namespace htb
     {
         bool     packH, packW; // operands copied into the workspace as packed rows of ld elements
         int64_t  ld;
+        int      parts; // sums of dH that are kept apart
         int64_t  piece; // classes of a piece (a multiple of kPieceUnit, or all of them)
         uint64_t hOff, wOff, stateOff, zOff, partOff, pOff, dhOff, dwOff, scaleOff, restOff;
         uint64_t bytes;
@@ -70,6 +71,11 @@ namespace htb
                                    const float* g, float alpha, const float* scale, void* P, int64_t ldp, float* rest, int smCount, int* status,
                                    cudaStream_t stream);
 
+    // up to 128 tokens: out[part][t, d] = (add: +=) sum over a part of the classes of P[t, v] W[v, d], `parts` of them side by side
+    int         hiddenParts(int64_t T, int64_t D, int64_t piece, int smCount);
+    cudaError_t launchHiddenGradient(int type, const void* P, int64_t ldp, const void* W, int64_t ldw, int64_t T, int64_t n, int64_t D, int parts,
+                                     float* out, int64_t ldo, bool add, int smCount, int* status, cudaStream_t stream);
+    bool        narrowTokens(int64_t T);
     // dW[v, d] = sum over K rows of P[k, v] H[k, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes
     cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
                                      const float* scale, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream);
@@ -86,7 +92,7 @@ namespace htb
 
     // f16: scale[0] = a power of two that brings max |g * alpha| close to the top of the range, scale[1] = its reciprocal
     cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, float* scale, cudaStream_t stream);
-    // Y[row r, c] = (X[r, c] + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; X null: zeros; rest null: none
+    // Y[row r, c] = (sum of `parts` X[r, c] + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; parts 0: zeros; rest null: none
     struct TargetRest
     {
         const float*   rest;
@@ -95,7 +101,7 @@ namespace htb
         const void*    W;
     };
     cudaError_t launchStoreRows(int type, const float* X, int64_t ldx, int64_t count, int64_t cols, const float* scale, void* Y,
-                                const TokenRows& rows, const TargetRest& rest, cudaStream_t stream);
+                                const TokenRows& rows, const TargetRest& rest, int parts, cudaStream_t stream);
 
     int crossEntropy(const hiptensorHandle_t* handle, const CrossEntropyPlan* plan, const void* alpha, const void* H, const void* W,
                      const int64_t* targets, float* loss, float* lse, void* workspace, uint64_t workspaceSize, void* stream);
