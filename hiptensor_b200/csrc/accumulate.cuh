@@ -39,7 +39,7 @@ namespace htb
             int      kBlocks; // 128-byte blocks along K
             int      chunk; // K blocks per chunk (1 for 8-bit operands)
             int      sub; // K blocks per stage (1 for 8-bit operands); chunks are multiples of it
-            int      kParts; // > 1: one tile of rows, and tm counts parts of the K range whose sums stay apart
+            int      kParts; // not PAIR: parts of the K range whose sums stay apart; tm counts the tiles of rows part by part
             int      kElems; // elements of a 128-byte block: 128 (8 bit) or 64
             int      xRows; // not PAIR: rows of X that are loaded, a multiple of 8
             int      ksplit; // CTAs of a cluster that share a tile (not PAIR)
@@ -283,12 +283,13 @@ namespace htb
             // K blocks of this CTA: all, or its part of a split tile
             int  kbBegin = PAIR ? 0 : int((long long)a.kBlocks * int(rank) / a.ksplit);
             int  kbEnd   = PAIR ? a.kBlocks : int((long long)a.kBlocks * (int(rank) + 1) / a.ksplit);
-            auto part    = [&](int& tm) { // kParts: the K range is the tile's, the rows are the first ones
+            auto part    = [&](int& tm) { // kParts: the K range is the tile's
                 if(!PAIR && a.kParts > 1)
                 {
-                    kbBegin = int((long long)a.kBlocks * tm / a.kParts);
-                    kbEnd   = int((long long)a.kBlocks * (tm + 1) / a.kParts);
-                    tm      = 0;
+                    const int tiles = a.tilesM / a.kParts, p = tm / tiles;
+                    kbBegin = int((long long)a.kBlocks * p / a.kParts);
+                    kbEnd   = int((long long)a.kBlocks * (p + 1) / a.kParts);
+                    tm -= p * tiles;
                 }
             };
             // global memory is read and written from here on: the grid ahead of this one must be complete

@@ -43,7 +43,8 @@ namespace htb
             const uint64_t     size = uint64_t(dtypeSize(p.type));
             const int64_t      unit = 16 / int64_t(size);
             const bool wordsH = p.nt <= 1 && p.hD == 1 && (p.T == 1 || (p.tStride[0] % unit == 0 && p.tStride[0] >= p.D));
-            const bool wordsW = p.wD == 1 && (p.V == 1 || (p.wV % unit == 0 && p.wV >= p.D));
+            // (the gradient's products read W along its rows, too: their length has to be one of whole 16-byte words)
+            const bool wordsW = p.wD == 1 && (p.V == 1 || (p.wV % unit == 0 && p.wV >= p.D)) && (!gradient || p.D % unit == 0);
             // the gradient reads a copy of H whose rows of ignored tokens are zeros: what lies there (padding, NaN) must not
             // reach dW through 0 * NaN
             l.packH  = gradient || !wordsH;
@@ -63,11 +64,11 @@ namespace htb
             l.stateOff       = take(!gradient, T * 12);
             l.scaleOff       = take(gradient, 8);
             l.restOff        = take(gradient, T * 4);
-            l.parts          = f32 ? 1 : hiddenParts(p.T, l.ld, piece, 0);
-            l.dhOff          = take(gradient, uint64_t(l.parts) * T * uint64_t(l.ld) * 4);
+            l.parts          = f32 ? 0 : hiddenParts(p.T, l.ld, piece);
+            l.dhOff          = take(gradient, uint64_t(std::max(l.parts, 1)) * T * uint64_t(l.ld) * 4);
             l.wOff           = take(l.packW, n * uint64_t(l.ld) * size);
             l.zOff           = take(f32, T * n * 4);
-            l.partOff        = take(!f32 && !gradient, (n + headGroup(p.T) - 1) / headGroup(p.T) * T * 8);
+            l.partOff        = take(!f32 && !gradient, (n + kHeadGroup - 1) / kHeadGroup * T * 8);
             l.pOff           = take(!f32 && gradient, (two ? 2 : 1) * T * n * size);
             l.dwOff          = take(gradient && !f32 && l.packW, n * uint64_t(l.ld) * 4);
             l.bytes          = at + 256; // room to align the caller's pointer
@@ -388,7 +389,8 @@ namespace htb
         float*       dh  = reinterpret_cast<float*>(ws + l.dhOff);
         float*       dw  = reinterpret_cast<float*>(ws + l.dwOff);
         float*       rest = reinterpret_cast<float*>(ws + l.restOff);
-        const Matrix Hm{h, p.T, p.D, l.ld, 1, p.type};
+        // the copies are as wide as their rows (zeros behind D), and so are the results' buffers
+        const Matrix Hm{h, p.T, l.ld, l.ld, 1, p.type};
         for(int64_t v0 = 0; v0 < p.V; v0 += l.piece)
         {
             const int64_t n   = std::min(l.piece, p.V - v0);
@@ -400,7 +402,7 @@ namespace htb
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
-            const Matrix Wm{w, n, p.D, ldw, 1, p.type}, Pm{P, p.T, n, l.piece, 1, p.type};
+            const Matrix Wm{w, n, l.ld, ldw, 1, p.type}, Pm{P, p.T, n, l.piece, 1, p.type};
             if(f32)
             {
                 HTB_TRY(product(Hm, 0, 2, Wm, 1, 2, Matrix{z, p.T, n, l.piece, 1, CUDA_R_32F}, 0, 1, a, 0.f, st, stream));
@@ -409,11 +411,11 @@ namespace htb
             else
                 HTB_TRY(launchHeadGradient(HeadProduct{h, w, p.T, n, p.D, l.ld, ldw, p.type}, v0, p.V, p.ignore, targets, lse, gradLoss, a,
                                            scale, P, l.piece, rest, st->smCount, st->deviceStatus, stream));
-            if(dH && !f32 && narrowTokens(p.T))
-                HTB_TRY(launchHiddenGradient(p.type, P, l.piece, w, ldw, p.T, n, p.D, l.parts, dh, l.ld, v0 > 0, st->smCount, st->deviceStatus,
+            if(dH && l.parts > 0)
+                HTB_TRY(launchHiddenGradient(p.type, P, l.piece, w, ldw, p.T, n, l.ld, l.parts, dh, l.ld, v0 > 0, st->smCount, st->deviceStatus,
                                              stream));
             else if(dH)
-                HTB_TRY(product(Pm, 0, 1, Wm, 1, 2, Matrix{dh, p.T, p.D, l.ld, 1, CUDA_R_32F}, 0, 2, 1.f, v0 ? 1.f : 0.f, st, stream));
+                HTB_TRY(product(Pm, 0, 1, Wm, 1, 2, Matrix{dh, p.T, l.ld, l.ld, 1, CUDA_R_32F}, 0, 2, 1.f, v0 ? 1.f : 0.f, st, stream));
             if(dW)
             {
                 unsigned char* out = static_cast<unsigned char*>(dW) + v0 * p.wV * size;
@@ -423,17 +425,17 @@ namespace htb
                 else if(!f32)
                 {
                     // rows of W that no bulk store can write: through f32 in the workspace
-                    const Matrix P2{P, rowsK, n, l.piece, 1, p.type}, H2{h, rowsK, p.D, l.ld, 1, p.type};
-                    HTB_TRY(product(P2, 0, 1, H2, 0, 2, Matrix{dw, n, p.D, l.ld, 1, CUDA_R_32F}, 1, 2, 1.f, 0.f, st, stream));
+                    const Matrix P2{P, rowsK, n, l.piece, 1, p.type}, H2{h, rowsK, l.ld, l.ld, 1, p.type};
+                    HTB_TRY(product(P2, 0, 1, H2, 0, 2, Matrix{dw, n, l.ld, l.ld, 1, CUDA_R_32F}, 1, 2, 1.f, 0.f, st, stream));
                     HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, 1, stream));
                 }
                 else
-                    HTB_TRY(product(Pm, 0, 1, Hm, 0, 2, Matrix{out, n, p.D, p.wV, p.wD, p.type}, 1, 2, 1.f, 0.f, st, stream));
+                    HTB_TRY(product(Pm, 0, 1, Matrix{h, p.T, p.D, l.ld, 1, p.type}, 0, 2, Matrix{out, n, p.D, p.wV, p.wD, p.type}, 1, 2, 1.f, 0.f, st, stream));
             }
         }
         if(dH)
             HTB_TRY(launchStoreRows(p.type, dh, l.ld, p.T, p.D, scale, dH, rowsOfH(p),
-                                    f32 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, l.parts, stream));
+                                    f32 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, std::max(l.parts, 1), stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }
 } // namespace htb

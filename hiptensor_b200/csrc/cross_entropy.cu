@@ -253,13 +253,12 @@ namespace htb
             int64_t        ignore;
             const int64_t* targets;
             float          alpha;
-            // forward: partial (maximum, sum) of TN / 2 classes each, [classes][T], in powers of two; target logits
+            // forward: partial (maximum, sum) of 128 classes each, [classes][T], in powers of two; target logits
             float2* part;
             float*  targetLogit;
             // gradient
             const float *lse, *g, *scale;
             float*       rest; // what rounding took from the target's entry of P
-            int          two; // P as a sum of two numbers of the type: what rounding took from every entry goes to mapLow
             CUtensorMap  mapP, mapLow;
         };
 
@@ -314,14 +313,11 @@ namespace htb
         };
 
         // Loss: one pass over a tile's logits in registers, maximum then sum of powers of two; what leaves the SM are two
-        // floats for TN / 2 logits.
-        template <int TN>
-        struct LossEpi : HeadSums<TN>
+        // floats for 128 logits.
+        struct LossEpi : HeadSums<256>
         {
             using Args                 = HeadArgs;
-            using Sums                 = HeadSums<TN>;
-            using Sums::acc;
-            static constexpr int COLS  = TN / 2;
+            using Sums                 = HeadSums<256>;
             static constexpr int kSide = 0;
             static constexpr bool kSplit = false;
             static constexpr int ROOM  = 0; // shared memory behind the stages
@@ -381,16 +377,15 @@ namespace htb
         // that follow (the products' sums are f32; a rounding of 2^-9 or 2^-12 of each entry is about what the rounding of
         // the results to the same type costs). The target's entry outweighs the others: what its rounding takes is kept and
         // added to dH in f32.
-        template <typename TP, int TN>
-        struct ProbabilityEpi : HeadSums<TN>
+        // PARTS = 2: P as a sum of two numbers of the type, what rounding took from every entry goes to mapLow.
+        template <typename TP, int PARTS>
+        struct ProbabilityEpi : HeadSums<256>
         {
             using Args                 = HeadArgs;
-            using Sums                 = HeadSums<TN>;
-            using Sums::acc;
-            static constexpr int COLS  = TN / 2;
+            using Sums                 = HeadSums<256>;
             static constexpr int kSide = 0;
             static constexpr bool kSplit = false;
-            static constexpr int ROUND = COLS < 64 ? COLS : 64; // columns of a slot: rows of 128 bytes (64 with TN = 64)
+            static constexpr int ROUND = 64; // columns of a slot: rows of 128 bytes
             static constexpr int SLOTS = 1;
             static constexpr int ROOM  = 8 * SLOTS * 4096;
             const Args&          a;
@@ -435,8 +430,8 @@ namespace htb
                     const float p = (exp2f(x) - 1.f) * f;
                     a.rest[row]   = p - widen(narrow<TP>(p));
                 }
-                const int lows = TN == 64 ? a.two : 0;
-                for(int low = 0; low <= lows; low++)
+#pragma unroll 1
+                for(int low = 0; low < PARTS; low++)
 #pragma unroll
                     for(int r = 0; r < COLS; r += ROUND)
                     {
@@ -462,7 +457,7 @@ namespace htb
                                 p0 = live ? p0 * f : 0.f;
                                 p1 = live ? p1 * f : 0.f;
                                 TP lo = narrow<TP>(p0), hi = narrow<TP>(p1);
-                                if(TN == 64 && low)
+                                if(low)
                                 {
                                     lo = narrow<TP>(p0 - widen(lo));
                                     hi = narrow<TP>(p1 - widen(hi));
@@ -470,9 +465,8 @@ namespace htb
                                 q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo))
                                        | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
                             }
-                            // 16-byte units permuted as the map's swizzle has them (rows of 64 bytes are not swizzled)
-                            const uint32_t unit = ROUND == 64 ? uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4)) : uint32_t(lane * ROUND * 2 + (u << 4));
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + unit), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                            // 16-byte units permuted as the map's swizzle has them
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
                                          : "memory");
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -574,14 +568,15 @@ namespace htb
             }
         };
 
-        // dH = P W over parts of the classes, for up to 128 tokens: f32 sums of every part, [part][T][ld]
+        // dH = P W over parts of the classes: f32 sums of every part, [part][T][ld]
         struct HiddenArgs
         {
-            int64_t T, ld, cols;
+            int64_t T, ld;
+            int     tiles; // of 128 tokens: tile rows of a part
             float*  out;
             int     add; // to what the pieces before left there
         };
-        struct HiddenEpi : HeadSums<128>
+        struct HiddenEpi : HeadSums<256>
         {
             using Args                   = HiddenArgs;
             static constexpr int  kSide  = 0;
@@ -601,10 +596,11 @@ namespace htb
             }
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
-                const int64_t t = row & 127;
+                const int64_t tile = row >> 7, part = tile / a.tiles;
+                const int64_t t    = row - part * a.tiles * 128;
                 if(t >= a.T)
                     return;
-                float* out = a.out + ((row >> 7) * a.T + t) * a.ld + col; // ld is a multiple of eight
+                float* out = a.out + (part * a.T + t) * a.ld + col; // ld is a multiple of eight
 #pragma unroll
                 for(int j = 0; j < COLS; j += 4)
                     if(col + j < a.ld)
@@ -727,13 +723,13 @@ namespace htb
             return e;
         }
 
-        template <class Epi, bool PAIR, int TN>
+        template <class Epi, bool PAIR>
         cudaError_t launchHeadForm(const HeadProduct& h, HeadArgs& ea, int smCount, int* status, cudaStream_t stream, const char* name)
         {
             PFN_encodeTiled encode = tensorMapEncoder();
             if(!encode)
                 return cudaErrorNotSupported;
-            constexpr int rows  = PAIR ? 256 : 128;
+            constexpr int rows = PAIR ? 256 : 128, TN = 256;
             const int     xRows = PAIR ? 128 : int(std::min<int64_t>(128, (h.T + 7) / 8 * 8)); // no more rows of H than there are tokens
             const uint32_t stage = (uint32_t(xRows) + (PAIR ? 128u : uint32_t(TN))) * 128u, behind = uint32_t(128 - xRows) * 128u;
             CUtensorMap mapX, mapY;
@@ -749,19 +745,21 @@ namespace htb
             a.ksplit     = 1;
             a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (rows * h.D * 2))));
             a.xRows      = xRows;
-            // Waits and commits between MMAs cost the issuing thread several hundred cycles: two K blocks a stage for a pair's
-            // tiles (512 cycles of MMAs each), four for narrow ones (128)
-            a.sub        = PAIR ? 2 : 4;
-            a.kParts     = 1;
-            a.stages     = std::min<int>(kAccMaxStages, int((226 * 1024 - 1024 - Epi::ROOM - behind) / (stage * a.sub)));
+            // Waits and commits between MMAs cost the issuing thread several hundred cycles: two K blocks a stage (1024 cycles
+            // of MMAs) where three stages of them fit
+            const int room = 226 * 1024 - 1024 - Epi::ROOM - int(behind);
+            a.sub          = room / int(2 * stage) >= 3 ? 2 : 1;
+            a.kParts       = 1;
+            a.stages       = std::min<int>(kAccMaxStages, room / int(stage * a.sub));
             a.stageBytes = (uint32_t(a.stages * a.sub) * stage + behind + 1023) / 1024 * 1024;
             a.idesc      = (1u << 4) | (h.type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TN >> 3) << 17) | (uint32_t(rows >> 4) << 24);
             a.status     = status;
             a.statusCode = kStatusSoftmax;
             return launchAccumulate<Epi, PAIR, TN, false, false>(mapX, mapY, a, ea, smCount, stream, name);
         }
-        // Up to 128 tokens the classes' rows are the traffic and a tile of 128 tokens is enough: 128 x 64 tiles, which
-        // spread a vocabulary evenly over the SMs. Beyond, 256 x 256 tiles of CTA pairs.
+        // Up to 128 tokens the classes' rows are the traffic and a tile of 128 tokens is enough: 128 x 256 tiles of one CTA each.
+        // (1 token, 32000 x 4096: 56 us; tiles of 128 classes 60, of 64 94, of 32 146: a K block costs the same however narrow.)
+        // Beyond, 256 x 256 tiles of CTA pairs.
         bool narrowHead(int64_t T)
         {
             return T <= 128;
@@ -780,14 +778,15 @@ namespace htb
         }
     } // namespace
 
-    // Parts of the classes whose products run side by side: tiles of 128 columns alone would leave most SMs idle. One unit
-    // each for about every SM.
-    int hiddenParts(int64_t T, int64_t D, int64_t piece, int smCount)
+    // How many parts of the classes dH's products run in, side by side: tiles of 128 x 256 of [T, D] alone would leave SMs idle
+    // when there are few tokens. About one unit for every SM, each of at least 1024 classes. 0: many tokens, the general
+    // contraction has enough tiles.
+    int hiddenParts(int64_t T, int64_t D, int64_t piece)
     {
-        if(!narrowHead(T))
-            return 1;
-        const int64_t tiles = (D + 127) / 128, sms = smCount > 0 ? smCount : 148;
-        return int(std::max<int64_t>(1, std::min<int64_t>((sms + tiles / 2) / tiles, piece / 1024)));
+        if(T > 384)
+            return 0;
+        const int64_t tiles = (D + 255) / 256 * ((T + 127) / 128);
+        return int(std::max<int64_t>(1, std::min<int64_t>((148 + tiles / 2) / tiles, piece / 1024)));
     }
 
     cudaError_t launchHiddenGradient(int type, const void* P, int64_t ldp, const void* W, int64_t ldw, int64_t T, int64_t n, int64_t D, int parts,
@@ -795,32 +794,33 @@ namespace htb
     {
         PFN_encodeTiled encode = tensorMapEncoder();
         HiddenArgs      ea{};
-        ea.T = T, ea.ld = ldo, ea.cols = D, ea.out = out, ea.add = add;
-        const int   xRows = int((T + 7) / 8 * 8);
+        const int       tiles = int((T + 127) / 128), xRows = int(std::min<int64_t>(128, (T + 7) / 8 * 8));
+        ea.T = T, ea.ld = ldo, ea.tiles = tiles, ea.out = out, ea.add = add;
         CUtensorMap mapX, mapY;
         if(!encode || !encodeMatrix(encode, &mapX, P, n, T, ldp, 64, xRows, CU_TENSOR_MAP_SWIZZLE_128B)
            || !encodeMatrix(encode, &mapY, W, D, n, ldw, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B))
             return cudaErrorNotSupported;
-        const uint32_t block = (uint32_t(xRows) + 128u) * 128u, behind = uint32_t(128 - xRows) * 128u;
-        parts = int(std::min<int64_t>(parts, (n + 63) / 64)); // a short last piece: every part has something to add
+        const uint32_t block = (uint32_t(xRows) + 256u) * 128u, behind = uint32_t(128 - xRows) * 128u;
+        const int      room  = 226 * 1024 - 1024 - int(behind);
+        parts                = int(std::min<int64_t>(parts, (n + 63) / 64)); // a short last piece: every part has something to add
         AccArgs a{};
-        a.tilesM     = parts;
-        a.tilesN     = int((D + 127) / 128);
+        a.tilesM     = parts * tiles;
+        a.tilesN     = int((D + 255) / 256);
         a.kBlocks    = int((n + 63) / 64);
         a.chunk      = 16;
-        a.sub        = 2;
+        a.sub        = room / int(2 * block) >= 3 ? 2 : 1;
         a.kParts     = parts;
         a.kElems     = 64;
         a.xRows      = xRows;
         a.ksplit     = 1;
-        a.groupM     = parts;
-        a.stages     = std::min<int>(kAccMaxStages, int((226 * 1024 - 1024 - behind) / (block * a.sub)));
+        a.groupM     = a.tilesM;
+        a.stages     = std::min<int>(kAccMaxStages, room / int(block * a.sub));
         a.stageBytes = (uint32_t(a.stages * a.sub) * block + behind + 1023) / 1024 * 1024;
-        a.idesc      = (1u << 4) | (type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | (uint32_t(128 >> 3) << 17)
+        a.idesc      = (1u << 4) | (type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | (uint32_t(256 >> 3) << 17)
                   | (uint32_t(128 >> 4) << 24); // Y transposed
         a.status     = status;
         a.statusCode = kStatusSoftmax;
-        return launchAccumulate<HiddenEpi, false, 128, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden");
+        return launchAccumulate<HiddenEpi, false, 256, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden");
     }
 
     cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
@@ -863,14 +863,6 @@ namespace htb
     {
         return T <= 64;
     }
-    bool narrowTokens(int64_t T)
-    {
-        return narrowHead(T);
-    }
-    int headGroup(int64_t T)
-    {
-        return narrowHead(T) ? 32 : 128;
-    }
 
     cudaError_t launchHeadLoss(const HeadProduct& h, int64_t v0, const int64_t* targets, float alpha, void* part, float* state, int smCount,
                                int* status, cudaStream_t stream)
@@ -881,14 +873,14 @@ namespace htb
         ea.alpha       = alpha;
         ea.part        = static_cast<float2*>(part);
         ea.targetLogit = state + 2 * h.T;
-        return narrowHead(h.T) ? launchHeadForm<LossEpi<64>, false, 64>(h, ea, smCount, status, stream, "cross_entropy_head")
-                               : launchHeadForm<LossEpi<256>, true, 256>(h, ea, smCount, status, stream, "cross_entropy_head_pair");
+        return narrowHead(h.T) ? launchHeadForm<LossEpi, false>(h, ea, smCount, status, stream, "cross_entropy_head")
+                               : launchHeadForm<LossEpi, true>(h, ea, smCount, status, stream, "cross_entropy_head_pair");
     }
 
     cudaError_t launchLossJoin(const void* part, int64_t n, int64_t T, float* state, bool first, bool last, int64_t V, int64_t ignore,
                                const int64_t* targets, float* loss, float* lse, int* status, cudaStream_t stream)
     {
-        const int group = headGroup(T);
+        const int group = kHeadGroup;
         join_kernel<<<unsigned((T + 31) / 32), 32 * kJoinWarps, 0, stream>>>(static_cast<const float2*>(part), (n + group - 1) / group, T, state, first,
                                                                             last, V, ignore, targets, loss, lse, status);
         return noted("cross_entropy_join");
@@ -902,18 +894,19 @@ namespace htb
         ea.T = h.T, ea.n = h.n, ea.v0 = v0, ea.V = V, ea.ignore = ignore;
         ea.targets = targets, ea.alpha = alpha, ea.lse = lse, ea.g = g, ea.scale = scale, ea.rest = rest;
         PFN_encodeTiled encode = tensorMapEncoder();
-        const bool      narrow = narrowHead(h.T);
-        if(!encode || !encodeMatrix(encode, &ea.mapP, P, h.n, h.T, ldp, narrow ? 32 : 64, 32, narrow ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
+        const bool      two    = splitProbabilities(h.T), half = h.type == CUDA_R_16F;
+        if(!encode || !encodeMatrix(encode, &ea.mapP, P, h.n, h.T, ldp, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B)
+           || !encodeMatrix(encode, &ea.mapLow, static_cast<const char*>(P) + (two ? h.T * ldp * 2 : 0), h.n, h.T, ldp, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
             return cudaErrorNotSupported;
-        ea.two = splitProbabilities(h.T) ? 1 : 0;
-        if(ea.two
-           && !encodeMatrix(encode, &ea.mapLow, static_cast<const char*>(P) + h.T * ldp * 2, h.n, h.T, ldp, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE))
-            return cudaErrorNotSupported;
-        if(h.type == CUDA_R_16F)
-            return narrow ? launchHeadForm<ProbabilityEpi<__half, 64>, false, 64>(h, ea, smCount, status, stream, "cross_entropy_head_gradient")
-                          : launchHeadForm<ProbabilityEpi<__half, 256>, true, 256>(h, ea, smCount, status, stream, "cross_entropy_head_gradient_pair");
-        return narrow ? launchHeadForm<ProbabilityEpi<__nv_bfloat16, 64>, false, 64>(h, ea, smCount, status, stream, "cross_entropy_head_gradient")
-                      : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 256>, true, 256>(h, ea, smCount, status, stream, "cross_entropy_head_gradient_pair");
+        const char* name = "cross_entropy_head_gradient";
+        if(two)
+            return half ? launchHeadForm<ProbabilityEpi<__half, 2>, false>(h, ea, smCount, status, stream, name)
+                        : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 2>, false>(h, ea, smCount, status, stream, name);
+        if(narrowHead(h.T))
+            return half ? launchHeadForm<ProbabilityEpi<__half, 1>, false>(h, ea, smCount, status, stream, name)
+                        : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 1>, false>(h, ea, smCount, status, stream, name);
+        return half ? launchHeadForm<ProbabilityEpi<__half, 1>, true>(h, ea, smCount, status, stream, "cross_entropy_head_gradient_pair")
+                    : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 1>, true>(h, ea, smCount, status, stream, "cross_entropy_head_gradient_pair");
     }
 
     cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t cols, int64_t ld, void* X2,

@@ -57,8 +57,8 @@ namespace htb
         int64_t     T, n, D, ldh, ldw;
         int         type;
     };
-    int headGroup(int64_t T); // classes that share one partial maximum and sum
-    // part: ceil(n / headGroup) x T pairs of floats; the target logits go to state[2T .. 3T)
+    constexpr int kHeadGroup = 128; // classes that share one partial maximum and sum
+    // part: ceil(n / kHeadGroup) x T pairs of floats; the target logits go to state[2T .. 3T)
     cudaError_t launchHeadLoss(const HeadProduct& h, int64_t v0, const int64_t* targets, float alpha, void* part, float* state, int smCount,
                                int* status, cudaStream_t stream);
     // joins a piece's partial results with state[0 .. 2T) (maximum, sum in powers of two); after the last piece loss and lse
@@ -71,11 +71,10 @@ namespace htb
                                    const float* g, float alpha, const float* scale, void* P, int64_t ldp, float* rest, int smCount, int* status,
                                    cudaStream_t stream);
 
-    // up to 128 tokens: out[part][t, d] = (add: +=) sum over a part of the classes of P[t, v] W[v, d], `parts` of them side by side
-    int         hiddenParts(int64_t T, int64_t D, int64_t piece, int smCount);
+    // out[part][t, d] = (add: +=) sum over a part of the classes of P[t, v] W[v, d], `parts` of them side by side
+    int         hiddenParts(int64_t T, int64_t D, int64_t piece);
     cudaError_t launchHiddenGradient(int type, const void* P, int64_t ldp, const void* W, int64_t ldw, int64_t T, int64_t n, int64_t D, int parts,
                                      float* out, int64_t ldo, bool add, int smCount, int* status, cudaStream_t stream);
-    bool        narrowTokens(int64_t T);
     // dW[v, d] = sum over K rows of P[k, v] H[k, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes
     cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
                                      const float* scale, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream);
