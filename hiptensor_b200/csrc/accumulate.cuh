@@ -39,8 +39,14 @@ namespace htb
             int      kBlocks; // 128-byte blocks along K
             int      chunk; // K blocks per chunk (1 for 8-bit operands)
             int      sub; // K blocks per stage (1 for 8-bit operands); chunks are multiples of it
-            int      kParts; // not PAIR: parts of the K range whose sums stay apart; tm counts the tiles of rows part by part
+            int      kParts; // parts of the K range whose sums stay apart; tm counts the tiles of rows part by part
             int      kElems; // elements of a 128-byte block: 128 (8 bit) or 64
+            // Operands that are sums of several matrices (f32 numbers as three bf16 ones, [segment][rows][cols]): the K range is a
+            // list of pairs of segments, segBlocks K blocks each; bits 4 i .. of segX / segY name the pair's segments, which
+            // lie xSegR / ySegR rows of the tile's side or xSegK / ySegK elements of K apart. One pair: segBlocks = kBlocks.
+            int      segBlocks;
+            uint32_t segX, segY;
+            int      xSegR, xSegK, ySegR, ySegK;
             int      xRows; // not PAIR: rows of X that are loaded, a multiple of 8
             int      ksplit; // CTAs of a cluster that share a tile (not PAIR)
             int      stages;
@@ -284,7 +290,7 @@ namespace htb
             int  kbBegin = PAIR ? 0 : int((long long)a.kBlocks * int(rank) / a.ksplit);
             int  kbEnd   = PAIR ? a.kBlocks : int((long long)a.kBlocks * (int(rank) + 1) / a.ksplit);
             auto part    = [&](int& tm) { // kParts: the K range is the tile's
-                if(!PAIR && a.kParts > 1)
+                if(a.kParts > 1)
                 {
                     const int tiles = a.tilesM / a.kParts, p = tm / tiles;
                     kbBegin = int((long long)a.kBlocks * p / a.kParts);
@@ -326,19 +332,26 @@ namespace htb
                             {
                                 const uint32_t dst = tilesAddr + stage * kStage + i * kBlock;
                                 const uint32_t dstX = PAIR ? dst : dst + yOff, dstY = PAIR ? dst + 16384 : dst;
-                                const int      k0 = (kb + i) * a.kElems;
+                                int k0 = (kb + i) * a.kElems, xr = x0, yr = y0, kx = k0, ky = k0;
+                                if(!F8 && a.segBlocks != a.kBlocks)
+                                {
+                                    const int pair = (kb + i) / a.segBlocks, sx = int(a.segX >> (4 * pair)) & 15, sy = int(a.segY >> (4 * pair)) & 15;
+                                    k0 -= pair * a.segBlocks * a.kElems;
+                                    kx = k0 + sx * a.xSegK, xr += sx * a.xSegR;
+                                    ky = k0 + sy * a.ySegK, yr += sy * a.ySegR;
+                                }
                                 static_assert(!(XMN || YMN) || !F8, "only half precision");
                                 static_assert(!XMN || PAIR, "128 rows of X in two chunks");
                                 if constexpr(XMN)
                                 {
-                                    tmaLoadPair2(dstX, &mapX, bar, x0, k0);
-                                    tmaLoadPair2(dstX + 8192, &mapX, bar, x0 + 64, k0);
+                                    tmaLoadPair2(dstX, &mapX, bar, xr, kx);
+                                    tmaLoadPair2(dstX + 8192, &mapX, bar, xr + 64, kx);
                                 }
                                 else if constexpr(PAIR)
-                                    tmaLoadPair2(dstX, &mapX, bar, k0, x0);
+                                    tmaLoadPair2(dstX, &mapX, bar, kx, xr);
                                 else
                                 {
-                                    const int c[2] = {k0, x0};
+                                    const int c[2] = {kx, xr};
                                     tmaLoad<2>(dstX, &mapX, bar, c);
                                 }
                                 if constexpr(YMN)
@@ -346,7 +359,7 @@ namespace htb
 #pragma unroll
                                     for(int c0 = 0; c0 < (PAIR ? 128 : TN); c0 += 64)
                                     {
-                                        const int c[2] = {y0 + c0, k0};
+                                        const int c[2] = {yr + c0, ky};
                                         if constexpr(PAIR)
                                             tmaLoadPair2(dstY + c0 * 128, &mapY, bar, c[0], c[1]);
                                         else
@@ -354,10 +367,10 @@ namespace htb
                                     }
                                 }
                                 else if constexpr(PAIR)
-                                    tmaLoadPair2(dstY, &mapY, bar, k0, y0);
+                                    tmaLoadPair2(dstY, &mapY, bar, ky, yr);
                                 else
                                 {
-                                    const int c[2] = {k0, y0};
+                                    const int c[2] = {ky, yr};
                                     tmaLoad<2>(dstY, &mapY, bar, c);
                                 }
                             }

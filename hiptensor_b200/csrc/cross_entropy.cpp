@@ -1,5 +1,5 @@
 // Host side of the linear cross entropy and its gradient: mode folding, the layout of the workspace, the walk over the
-// pieces of the vocabulary. The products are this library's own contractions.
+// pieces of the vocabulary.
 #include <algorithm>
 
 #include <hiptensor/hiptensor.hpp>
@@ -11,7 +11,7 @@ namespace htb
 {
     namespace
     {
-        constexpr int64_t  kPieceUnit   = 256; // classes; a piece's rows then start at multiples of 16 bytes in every type
+        constexpr int64_t  kPieceUnit   = 256; // classes: a tile's columns
         constexpr uint64_t kRecommended = uint64_t(512) << 20; // bytes of the pieces' buffers under WORKSPACE_RECOMMENDED
 
         int64_t roundUp(int64_t n, int64_t to)
@@ -40,17 +40,22 @@ namespace htb
         CrossEntropyLayout layoutFor(const CrossEntropyPlan& p, bool gradient, int64_t piece)
         {
             CrossEntropyLayout l{};
-            const uint64_t     size = uint64_t(dtypeSize(p.type));
-            const int64_t      unit = 16 / int64_t(size);
+            const int64_t      unit = 16 / dtypeSize(p.type);
+            const bool         f32  = p.type == CUDA_R_32F;
             const bool wordsH = p.nt <= 1 && p.hD == 1 && (p.T == 1 || (p.tStride[0] % unit == 0 && p.tStride[0] >= p.D));
-            // (the gradient's products read W along its rows, too: their length has to be one of whole 16-byte words)
-            const bool wordsW = p.wD == 1 && (p.V == 1 || (p.wV % unit == 0 && p.wV >= p.D)) && (!gradient || p.D % unit == 0);
+            const bool wordsW = p.wD == 1 && (p.V == 1 || (p.wV % unit == 0 && p.wV >= p.D));
             // the gradient reads a copy of H whose rows of ignored tokens are zeros: what lies there (padding, NaN) must not
             // reach dW through 0 * NaN
-            l.packH  = gradient || !wordsH;
-            l.packW  = !wordsW;
-            l.ld     = roundUp(p.D, unit);
-            l.piece  = piece;
+            l.packH    = gradient || f32 || !wordsH;
+            l.packW    = f32 || !wordsW;
+            l.direct   = wordsW;
+            l.segments = f32 ? 3 : 1;
+            l.ld       = roundUp(p.D, 8);
+            l.piece    = piece;
+            const int partsP = gradient ? probabilityParts(p.type, p.T) : 1;
+            // segments of tokens are contracted in blocks of 64: zeros up to there
+            l.rowsT = l.segments > 1 || partsP > 1 ? roundUp(p.T, 64) : p.T;
+            l.parts = gradient ? hiddenParts(p.T, p.D, piece) : 1;
             uint64_t at   = 0;
             auto     take = [&](bool wanted, uint64_t bytes) {
                 const uint64_t here = at;
@@ -58,19 +63,16 @@ namespace htb
                     at += (bytes + 255) / 256 * 256;
                 return here;
             };
-            const uint64_t T = uint64_t(p.T), n = uint64_t(piece);
-            const bool f32   = p.type == CUDA_R_32F, two = gradient && !f32 && splitProbabilities(p.T);
-            l.hOff           = take(l.packH, (two ? 2 : 1) * T * uint64_t(l.ld) * size);
+            const uint64_t T = uint64_t(p.T), n = uint64_t(piece), ld = uint64_t(l.ld), seg = uint64_t(l.segments);
+            l.hOff           = take(l.packH, seg * uint64_t(l.rowsT) * ld * 2);
             l.stateOff       = take(!gradient, T * 12);
             l.scaleOff       = take(gradient, 8);
             l.restOff        = take(gradient, T * 4);
-            l.parts          = f32 ? 0 : hiddenParts(p.T, l.ld, piece);
-            l.dhOff          = take(gradient, uint64_t(std::max(l.parts, 1)) * T * uint64_t(l.ld) * 4);
-            l.wOff           = take(l.packW, n * uint64_t(l.ld) * size);
-            l.zOff           = take(f32, T * n * 4);
-            l.partOff        = take(!f32 && !gradient, (n + kHeadGroup - 1) / kHeadGroup * T * 8);
-            l.pOff           = take(!f32 && gradient, (two ? 2 : 1) * T * n * size);
-            l.dwOff          = take(gradient && !f32 && l.packW, n * uint64_t(l.ld) * 4);
+            l.dhOff          = take(gradient, uint64_t(l.parts) * T * ld * 4);
+            l.wOff           = take(l.packW, seg * n * ld * 2);
+            l.partOff        = take(!gradient, n / kHeadGroup * T * 8);
+            l.pOff           = take(gradient, uint64_t(partsP) * uint64_t(l.rowsT) * n * 2);
+            l.dwOff          = take(gradient && !l.direct, n * ld * 4);
             l.bytes          = at + 256; // room to align the caller's pointer
             return l;
         }
@@ -117,28 +119,11 @@ namespace htb
             return r;
         }
 
-        // D[m, n] = alpha * sum_k A B + beta * D through the library's contraction planner: matrices given by extents and
-        // the strides of their two modes
-        struct Matrix
+        int64_t rowStride(const CrossEntropyPlan& p, const CrossEntropyLayout& l)
         {
-            const void* data;
-            int64_t     rows, cols, sRow, sCol;
-            int         type;
-        };
-        cudaError_t product(const Matrix& A, int aRow, int aCol, const Matrix& B, int bRow, int bCol, const Matrix& D, int dRow, int dCol,
-                            float alpha, float beta, const HandleState* st, cudaStream_t stream)
-        {
-            const int64_t   lA[2] = {A.rows, A.cols}, sA[2] = {A.sRow, A.sCol}, lB[2] = {B.rows, B.cols}, sB[2] = {B.sRow, B.sCol},
-                          lD[2] = {D.rows, D.cols}, sD[2] = {D.sRow, D.sCol};
-            const int32_t   mA[2] = {aRow, aCol}, mB[2] = {bRow, bCol}, mD[2] = {dRow, dCol};
-            ContractionPlan plan;
-            const int rc = planContraction(TensorView{2, lA, sA, mA, A.type}, TensorView{2, lB, sB, mB, B.type},
-                                           TensorView{2, lD, sD, mD, D.type}, D.type, beta != 0.f, HIPTENSOR_COMPUTE_32F, st->smCount, &plan, 0);
-            if(rc != PLAN_OK)
-                return cudaErrorNotSupported;
-            return launchContraction(plan, alpha, A.data, B.data, beta, beta != 0.f ? D.data : nullptr, const_cast<void*>(D.data), nullptr, 0,
-                                     st->smCount, st->deviceStatus, stream);
+            return p.T > 1 ? p.tStride[0] : l.ld;
         }
+
 #define HTB_TRY(call)                    \
     do                                   \
     {                                    \
@@ -235,7 +220,7 @@ namespace htb
             return HIPTENSOR_STATUS_INVALID_VALUE;
         if(empty)
             p.T = 0;
-        if(p.V >= (int64_t(1) << 31) - 512 || p.T >= (int64_t(1) << 31) - 512 || p.D >= (int64_t(1) << 31) - 512)
+        if(p.V >= (int64_t(1) << 31) - 512 || p.T >= (int64_t(1) << 31) - 512 || p.D > (int64_t(1) << 26))
             return HIPTENSOR_STATUS_NOT_SUPPORTED;
         *out = p;
         return HIPTENSOR_STATUS_SUCCESS;
@@ -289,17 +274,16 @@ namespace htb
         unsigned char*     ws     = reinterpret_cast<unsigned char*>((uintptr_t(workspace) + 255) & ~uintptr_t(255));
         const float        a      = *(const float*)alpha;
         const int64_t      size   = dtypeSize(p.type);
+        const int          type16 = p.type == CUDA_R_16F ? CUDA_R_16F : CUDA_R_16BF;
         float*             state  = reinterpret_cast<float*>(ws + l.stateOff);
         const void*        h      = H;
-        int64_t            ldh    = p.nt ? p.tStride[0] : l.ld;
+        int64_t            ldh    = rowStride(p, l);
         if(l.packH)
         {
-            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, nullptr, false, stream));
+            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, l.rowsT, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, nullptr, stream));
             h   = ws + l.hOff;
             ldh = l.ld;
         }
-        const bool f32 = p.type == CUDA_R_32F;
-        float*     z   = reinterpret_cast<float*>(ws + l.zOff);
         for(int64_t v0 = 0; v0 < p.V; v0 += l.piece)
         {
             const int64_t n   = std::min(l.piece, p.V - v0);
@@ -307,26 +291,15 @@ namespace htb
             int64_t       ldw = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, false, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
-            if(f32)
-            {
-                HTB_TRY(product(Matrix{h, p.T, p.D, ldh, 1, p.type}, 0, 2, Matrix{w, n, p.D, ldw, 1, p.type}, 1, 2,
-                                Matrix{z, p.T, n, l.piece, 1, CUDA_R_32F}, 0, 1, a, 0.f, st, stream));
-                HTB_TRY(launchSoftmaxPiece(z, l.piece, p.T, v0, n, targets, state, stream));
-            }
-            else
-            {
-                HTB_TRY(launchHeadLoss(HeadProduct{h, w, p.T, n, p.D, ldh, ldw, p.type}, v0, targets, a, ws + l.partOff, state, st->smCount,
-                                       st->deviceStatus, stream));
-                HTB_TRY(launchLossJoin(ws + l.partOff, n, p.T, state, v0 == 0, v0 + n == p.V, p.V, p.ignore, targets, loss, lse,
-                                       st->deviceStatus, stream));
-            }
+            HTB_TRY(launchHeadLoss(HeadProduct{h, w, p.T, n, p.D, ldh, ldw, type16, l.segments, l.rowsT, n}, v0, targets, a, ws + l.partOff, state,
+                                   st->smCount, st->deviceStatus, stream));
+            HTB_TRY(launchLossJoin(ws + l.partOff, n, p.T, state, v0 == 0, v0 + n == p.V, p.V, p.ignore, targets, loss, lse, st->deviceStatus,
+                                   stream));
         }
-        if(f32)
-            HTB_TRY(launchLossFinish(state, p.T, p.V, p.ignore, targets, loss, lse, st->deviceStatus, stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }
 
@@ -371,71 +344,54 @@ namespace htb
                           hiptensorGetErrorString(HIPTENSOR_STATUS_INSUFFICIENT_WORKSPACE));
             return HIPTENSOR_STATUS_INSUFFICIENT_WORKSPACE;
         }
-        unsigned char* ws    = reinterpret_cast<unsigned char*>((uintptr_t(workspace) + 255) & ~uintptr_t(255));
-        const float    a     = *(const float*)alpha;
-        const bool     f32   = p.type == CUDA_R_32F;
-        float*         scale = nullptr;
+        unsigned char* ws     = reinterpret_cast<unsigned char*>((uintptr_t(workspace) + 255) & ~uintptr_t(255));
+        const float    a      = *(const float*)alpha;
+        const int      type16 = p.type == CUDA_R_16F ? CUDA_R_16F : CUDA_R_16BF;
+        float*         scale  = nullptr;
         if(p.type == CUDA_R_16F)
         {
             scale = reinterpret_cast<float*>(ws + l.scaleOff);
             HTB_TRY(launchGradientScale(gradLoss, a, p.T, scale, stream));
         }
-        const bool    two   = !f32 && splitProbabilities(p.T);
-        const int64_t rowsK = two ? 2 * p.T : p.T; // of P and H in the weights' product
-        void*         h     = ws + l.hOff;
-        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, p.D, l.ld, h, targets, p.ignore, p.V, st->deviceStatus, two, stream));
-        float*       z   = reinterpret_cast<float*>(ws + l.zOff);
-        void*        P   = f32 ? (void*)z : (void*)(ws + l.pOff);
-        float*       dh  = reinterpret_cast<float*>(ws + l.dhOff);
-        float*       dw  = reinterpret_cast<float*>(ws + l.dwOff);
-        float*       rest = reinterpret_cast<float*>(ws + l.restOff);
-        // the copies are as wide as their rows (zeros behind D), and so are the results' buffers
-        const Matrix Hm{h, p.T, l.ld, l.ld, 1, p.type};
+        void* h = ws + l.hOff;
+        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, l.rowsT, p.D, l.ld, h, targets, p.ignore, p.V, st->deviceStatus, stream));
+        float*              dh   = reinterpret_cast<float*>(ws + l.dhOff);
+        float*              dw   = reinterpret_cast<float*>(ws + l.dwOff);
+        float*              rest = reinterpret_cast<float*>(ws + l.restOff);
+        const Probabilities P{ws + l.pOff, probabilityParts(p.type, p.T), l.rowsT, l.piece};
         for(int64_t v0 = 0; v0 < p.V; v0 += l.piece)
         {
-            const int64_t n   = std::min(l.piece, p.V - v0);
-            const void*   w   = static_cast<const unsigned char*>(W) + v0 * p.wV * size;
-            int64_t       ldw = p.wV;
+            const int64_t n = std::min(l.piece, p.V - v0);
+            // segments of classes are contracted in blocks of 64: zeros up to there
+            const int64_t rowsW = l.segments > 1 ? roundUp(n, 64) : n;
+            const void*   w     = static_cast<const unsigned char*>(W) + v0 * p.wV * size;
+            int64_t       ldw   = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, false, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, rowsW, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
-            const Matrix Wm{w, n, l.ld, ldw, 1, p.type}, Pm{P, p.T, n, l.piece, 1, p.type};
-            if(f32)
-            {
-                HTB_TRY(product(Hm, 0, 2, Wm, 1, 2, Matrix{z, p.T, n, l.piece, 1, CUDA_R_32F}, 0, 1, a, 0.f, st, stream));
-                HTB_TRY(launchProbabilities(z, l.piece, p.T, v0, n, p.V, p.ignore, targets, lse, gradLoss, a, stream));
-            }
-            else
-                HTB_TRY(launchHeadGradient(HeadProduct{h, w, p.T, n, p.D, l.ld, ldw, p.type}, v0, p.V, p.ignore, targets, lse, gradLoss, a,
-                                           scale, P, l.piece, rest, st->smCount, st->deviceStatus, stream));
-            if(dH && l.parts > 0)
-                HTB_TRY(launchHiddenGradient(p.type, P, l.piece, w, ldw, p.T, n, l.ld, l.parts, dh, l.ld, v0 > 0, st->smCount, st->deviceStatus,
-                                             stream));
-            else if(dH)
-                HTB_TRY(product(Pm, 0, 1, Wm, 1, 2, Matrix{dh, p.T, l.ld, l.ld, 1, CUDA_R_32F}, 0, 2, 1.f, v0 ? 1.f : 0.f, st, stream));
+            const HeadProduct head{h, w, p.T, n, p.D, l.ld, ldw, type16, l.segments, l.rowsT, rowsW};
+            HTB_TRY(launchHeadGradient(head, v0, p.V, p.ignore, targets, lse, gradLoss, a, scale, P, rest, st->smCount, st->deviceStatus, stream));
+            if(dH)
+                HTB_TRY(launchHiddenGradient(head, P, l.parts, dh, l.ld, v0 > 0, st->smCount, st->deviceStatus, stream));
             if(dW)
             {
                 unsigned char* out = static_cast<unsigned char*>(dW) + v0 * p.wV * size;
-                if(!f32 && !l.packW)
-                    HTB_TRY(launchWeightGradient(p.type, P, l.piece, h, l.ld, rowsK, n, p.D, scale, out, p.wV, st->smCount, st->deviceStatus,
-                                                 stream));
-                else if(!f32)
+                if(l.direct)
+                    HTB_TRY(launchWeightGradient(head, P, scale, p.type, out, p.wV, st->smCount, st->deviceStatus, stream));
+                else
                 {
                     // rows of W that no bulk store can write: through f32 in the workspace
-                    const Matrix P2{P, rowsK, n, l.piece, 1, p.type}, H2{h, rowsK, l.ld, l.ld, 1, p.type};
-                    HTB_TRY(product(P2, 0, 1, H2, 0, 2, Matrix{dw, n, l.ld, l.ld, 1, CUDA_R_32F}, 1, 2, 1.f, 0.f, st, stream));
+                    HTB_TRY(launchWeightGradient(head, P, nullptr, CUDA_R_32F, dw, l.ld, st->smCount, st->deviceStatus, stream));
                     HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, 1, stream));
                 }
-                else
-                    HTB_TRY(product(Pm, 0, 1, Matrix{h, p.T, p.D, l.ld, 1, p.type}, 0, 2, Matrix{out, n, p.D, p.wV, p.wD, p.type}, 1, 2, 1.f, 0.f, st, stream));
             }
         }
         if(dH)
             HTB_TRY(launchStoreRows(p.type, dh, l.ld, p.T, p.D, scale, dH, rowsOfH(p),
-                                    f32 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, std::max(l.parts, 1), stream));
+                                    P.parts == 3 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, l.parts, stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }
 } // namespace htb

@@ -1,4 +1,7 @@
-// Kernels of the linear cross entropy around the library's contractions.
+// Kernels of the linear cross entropy and its gradient. All products run on the shared pipeline of accumulate.cuh; logits and
+// probabilities are made in the epilogue of the product that needs them. f32 operands are sums of three bf16 numbers each, of
+// whose nine products the six that matter are added (2^-26 of the whole is left out): the rate is a sixth of bf16's, as with the
+// TF32 split of the f32 contraction, and everything else is shared.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -58,104 +61,63 @@ namespace htb
             return target != ignore && target >= 0 && target < V;
         }
 
-        template <typename T>
-        __global__ void pack_rows_kernel(const T* __restrict__ X, const __grid_constant__ TokenRows rows, int64_t count, int64_t cols, int64_t ld,
-                                         T* __restrict__ X2, const int64_t* __restrict__ targets, int64_t ignore, int64_t V, int* status, bool twice)
+        // Rows of a strided tensor as packed rows of ld 16-bit elements, eight elements a thread. SPLIT: f32 numbers as three bf16
+        // ones, x = h + m + l up to 2^-27 of x, [3][rows][ld] (an infinity or NaN stays in h).
+        template <typename T, bool SPLIT>
+        __global__ void pack_rows_kernel(const T* __restrict__ X, const __grid_constant__ TokenRows rows, int64_t count, int64_t total, int64_t cols,
+                                         int64_t ld, unsigned short* __restrict__ X2, const int64_t* __restrict__ targets, int64_t ignore,
+                                         int64_t V, int* status, bool vec)
         {
-            for(int64_t r = blockIdx.x; r < count; r += gridDim.x)
+            const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
+            for(int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; r < total; r += int64_t(gridDim.x) * blockDim.y)
             {
-                const bool    live = !targets || counts(targets[r], ignore, V);
-                const T*      src  = X + rowOffset(rows, r);
-                if(!live && targets[r] != ignore && threadIdx.x == 0)
-                    atomicExch_system(status, kStatusBadTarget);
-                for(int64_t c = threadIdx.x; c < ld; c += blockDim.x)
+                if(c >= ld)
+                    continue;
+                bool live = r < count;
+                if(live && targets)
                 {
-                    const T x      = (live && c < cols) ? src[c * rows.elem] : narrow<T>(0.f);
-                    X2[r * ld + c] = x;
-                    if(twice)
-                        X2[(count + r) * ld + c] = x;
+                    const int64_t target = targets[r];
+                    live                 = counts(target, ignore, V);
+                    if(!live && target != ignore && c == 0)
+                        atomicExch_system(status, kStatusBadTarget);
                 }
-            }
-        }
-
-        // one block per token
-        __global__ void __launch_bounds__(256) softmax_piece_kernel(const float* __restrict__ z, int64_t ldz, int64_t T, int64_t v0, int64_t count,
-                                                                    const int64_t* __restrict__ targets, float* state)
-        {
-            __shared__ float part[8];
-            for(int64_t t = blockIdx.x; t < T; t += gridDim.x)
-            {
-                const float* row = z + t * ldz;
-                float        m   = -INFINITY;
-                for(int64_t v = threadIdx.x; v < count; v += 256)
+                T x[8];
+                if(live && vec && c + 8 <= cols)
                 {
-                    const float x = row[v];
-                    m             = (x > m || x != x) ? x : m; // a NaN stays
+                    const uint4* src = reinterpret_cast<const uint4*>(X + rowOffset(rows, r) + c);
+#pragma unroll
+                    for(int w = 0; w < int(sizeof(T)) / 2; w++)
+                        reinterpret_cast<uint4*>(x)[w] = __ldg(src + w);
                 }
-                for(int s = 16; s; s >>= 1)
+                else
                 {
-                    const float o = __shfl_xor_sync(0xffffffffu, m, s);
-                    m             = (o > m || o != o) ? o : m;
+                    const T* src = X + (live ? rowOffset(rows, r) + c * rows.elem : 0);
+#pragma unroll
+                    for(int j = 0; j < 8; j++)
+                        x[j] = (live && c + j < cols) ? src[j * rows.elem] : narrow<T>(0.f);
                 }
-                __syncthreads();
-                if((threadIdx.x & 31) == 0)
-                    part[threadIdx.x >> 5] = m;
-                __syncthreads();
-                for(int i = 0; i < 8; i++)
-                    m = (part[i] > m || part[i] != part[i]) ? part[i] : m;
-                const float ref = fabsf(m) == INFINITY ? 0.f : m;
-                float       sum = 0.f;
-                for(int64_t v = threadIdx.x; v < count; v += 256)
-                    sum += expf(row[v] - ref);
-                for(int s = 16; s; s >>= 1)
-                    sum += __shfl_xor_sync(0xffffffffu, sum, s);
-                __syncthreads();
-                if((threadIdx.x & 31) == 0)
-                    part[threadIdx.x >> 5] = sum;
-                __syncthreads();
-                if(threadIdx.x == 0)
+                if constexpr(!SPLIT)
+                    *reinterpret_cast<uint4*>(X2 + r * ld + c) = *reinterpret_cast<const uint4*>(x);
+                else
                 {
-                    sum = 0.f;
-                    for(int i = 0; i < 8; i++)
-                        sum += part[i];
-                    const int64_t target = targets[t];
-                    if(target >= v0 && target < v0 + count)
-                        state[2 * T + t] = row[target - v0];
-                    if(v0)
+                    __nv_bfloat16 part[3][8];
+#pragma unroll
+                    for(int j = 0; j < 8; j++)
                     {
-                        const float m1 = state[t], s1 = state[T + t];
-                        const float top = (m1 > m || m1 != m1) ? m1 : m;
-                        const float r2  = fabsf(top) == INFINITY ? 0.f : top;
-                        // each sum was taken relative to its own reference
-                        const float f1 = fabsf(m1) == INFINITY ? 0.f : m1;
-                        sum            = s1 * expf(f1 - r2) + sum * expf(ref - r2);
-                        m              = top;
+                        float       left = x[j];
+                        const float whole = widen(narrow<__nv_bfloat16>(left));
+#pragma unroll
+                        for(int k = 0; k < 3; k++)
+                        {
+                            part[k][j] = narrow<__nv_bfloat16>(left);
+                            left       = fabsf(whole) < INFINITY ? left - widen(part[k][j]) : 0.f;
+                        }
                     }
-                    state[t]     = m;
-                    state[T + t] = sum;
+#pragma unroll
+                    for(int k = 0; k < 3; k++)
+                        *reinterpret_cast<uint4*>(X2 + (k * total + r) * ld + c) = *reinterpret_cast<const uint4*>(part[k]);
                 }
             }
-        }
-
-        __global__ void loss_finish_kernel(const float* __restrict__ state, int64_t T, int64_t V, int64_t ignore,
-                                           const int64_t* __restrict__ targets, float* loss, float* lse, int* status)
-        {
-            const int64_t t = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-            if(t >= T)
-                return;
-            const float   m = state[t], ref = fabsf(m) == INFINITY ? 0.f : m;
-            const float   l = ref + logf(state[T + t]);
-            const int64_t target = targets[t];
-            lse[t] = l;
-            if(target == ignore)
-                loss[t] = 0.f;
-            else if(target < 0 || target >= V)
-            {
-                loss[t] = __int_as_float(0x7fc00000);
-                atomicExch_system(status, kStatusBadTarget);
-            }
-            else
-                loss[t] = l - state[2 * T + t];
         }
 
         __global__ void __launch_bounds__(1024) gradient_scale_kernel(const float* __restrict__ g, float alpha, int64_t T, float* scale)
@@ -182,57 +144,83 @@ namespace htb
             }
         }
 
-        __global__ void probabilities_kernel(float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, int64_t V, int64_t ignore,
-                                             const int64_t* __restrict__ targets, const float* __restrict__ lse, const float* __restrict__ g,
-                                             float alpha)
-        {
-            for(int64_t t = blockIdx.x; t < T; t += gridDim.x)
-            {
-                const int64_t target = targets[t];
-                const bool    live   = counts(target, ignore, V);
-                const float   l = lse[t], f = g[t] * alpha;
-                for(int64_t v = threadIdx.x; v < count; v += blockDim.x)
-                {
-                    float p = expf(z[t * ldz + v] - l);
-                    if(v0 + v == target)
-                        p -= 1.f;
-                    z[t * ldz + v] = live ? p * f : 0.f;
-                }
-            }
-        }
-
+        // Y[row r, c] = (sum of the parts' X[r, c] + rest[r] * W[target of r, c]) * scale[1]; four columns a thread
         template <typename T>
         __global__ void store_rows_kernel(const float* __restrict__ X, int64_t ldx, int64_t count, int64_t cols, const float* __restrict__ scale,
-                                          T* __restrict__ Y, const __grid_constant__ TokenRows rows, const __grid_constant__ TargetRest rest, int parts)
+                                          T* __restrict__ Y, const __grid_constant__ TokenRows rows, const __grid_constant__ TargetRest rest, int parts,
+                                          bool vec)
         {
-            const float f = scale ? scale[1] : 1.f;
-            for(int64_t r = blockIdx.x; r < count; r += gridDim.x)
+            const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 4;
+            const float   f = scale ? scale[1] : 1.f;
+            for(int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; r < count; r += int64_t(gridDim.x) * blockDim.y)
             {
-                T*       dst = Y + rowOffset(rows, r);
-                const T* w   = nullptr; // the target's row of W, times what rounding took from its entry of P
-                float    e   = 0.f;
+                if(c >= cols)
+                    continue;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                for(int i = 0; i < parts; i++)
+                {
+                    const float4 v = *reinterpret_cast<const float4*>(X + (int64_t(i) * count + r) * ldx + c); // ldx is a multiple of eight
+                    x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+                }
+                float y[4] = {x.x, x.y, x.z, x.w};
                 if(rest.rest)
                 {
                     const int64_t target = rest.targets[r];
                     if(counts(target, rest.ignore, rest.V))
                     {
-                        w = static_cast<const T*>(rest.W) + target * rest.wV;
-                        e = rest.rest[r];
+                        const T*    w = static_cast<const T*>(rest.W) + target * rest.wV + c * rest.wD;
+                        const float e = rest.rest[r];
+#pragma unroll
+                        for(int j = 0; j < 4; j++)
+                            if(c + j < cols)
+                                y[j] = fmaf(e, widen(w[j * rest.wD]), y[j]);
                     }
                 }
-                for(int64_t c = threadIdx.x; c < cols; c += blockDim.x)
+                T* dst = Y + rowOffset(rows, r) + c * rows.elem;
+                if(vec && c + 4 <= cols)
                 {
-                    float x = 0.f;
-                    for(int i = 0; i < parts; i++)
-                        x += X[(int64_t(i) * count + r) * ldx + c];
-                    if(w)
-                        x = fmaf(e, widen(w[c * rest.wD]), x);
-                    dst[c * rows.elem] = narrow<T>(x * f);
+                    struct alignas(4 * sizeof(T)) Four
+                    {
+                        T e[4];
+                    } o;
+#pragma unroll
+                    for(int j = 0; j < 4; j++)
+                        o.e[j] = narrow<T>(y[j] * f);
+                    *reinterpret_cast<Four*>(dst) = o;
+                }
+                else
+                {
+#pragma unroll
+                    for(int j = 0; j < 4; j++)
+                        if(c + j < cols)
+                            dst[j * rows.elem] = narrow<T>(y[j] * f);
                 }
             }
         }
 
-        // ------------------------------------------------------------------ f16 / bf16: logits that stay on the chip
+        // threads along a row and rows side by side for kernels of `units` threads a row
+        struct RowShape
+        {
+            dim3 grid, block;
+        };
+        RowShape rowShape(int64_t rows, int64_t units)
+        {
+            unsigned tx = 8;
+            while(tx < 256 && tx < units)
+                tx *= 2;
+            const unsigned ty = 256 / tx;
+            return RowShape{dim3(unsigned(std::min<int64_t>((rows + ty - 1) / ty, 1 << 20)), unsigned((units + tx - 1) / tx)), dim3(tx, ty)};
+        }
+        // every row of a strided tensor starts at a multiple of `unit` elements
+        bool rowsAligned(const TokenRows& rows, const void* base, int64_t unit, int64_t size)
+        {
+            bool ok = rows.elem == 1 && uintptr_t(base) % uintptr_t(unit * size) == 0;
+            for(int i = 0; i < rows.nt; i++)
+                ok = ok && rows.stride[i] % unit == 0;
+            return ok;
+        }
+
+        // ------------------------------------------------------------------ logits that stay on the chip
         constexpr float kLog2e = 1.4426950408889634f;
 
         __device__ __forceinline__ float maxNan(float a, float b)
@@ -253,13 +241,14 @@ namespace htb
             int64_t        ignore;
             const int64_t* targets;
             float          alpha;
-            // forward: partial (maximum, sum) of 128 classes each, [classes][T], in powers of two; target logits
+            // loss: partial (maximum, sum) of 128 classes each, [classes][T], in powers of two; target logits
             float2* part;
             float*  targetLogit;
             // gradient
             const float *lse, *g, *scale;
             float*       rest; // what rounding took from the target's entry of P
-            CUtensorMap  mapP, mapLow;
+            int64_t      rowsP; // of a segment of P
+            CUtensorMap  mapP;
         };
 
         // Common to both: the sums of a chunk of up to 1024 elements are added to the running ones with rounding (the
@@ -376,8 +365,8 @@ namespace htb
         // Gradient: P = (exp(z - lse) - [class is the target]) * g * alpha, rounded to the operands' type for the two products
         // that follow (the products' sums are f32; a rounding of 2^-9 or 2^-12 of each entry is about what the rounding of
         // the results to the same type costs). The target's entry outweighs the others: what its rounding takes is kept and
-        // added to dH in f32.
-        // PARTS = 2: P as a sum of two numbers of the type, what rounding took from every entry goes to mapLow.
+        // added to dH in f32. PARTS > 1: P as a sum of that many numbers, each what rounding took from the ones before, in
+        // segments of rowsP rows (a multiple of 32; rows past the tokens hold zeros there).
         template <typename TP, int PARTS>
         struct ProbabilityEpi : HeadSums<256>
         {
@@ -428,7 +417,8 @@ namespace htb
                 {
                     const float x = unpack2(fma2(pack2(Sums::at(int(t)), 0.f), c2, l2)).x;
                     const float p = (exp2f(x) - 1.f) * f;
-                    a.rest[row]   = p - widen(narrow<TP>(p));
+                    if constexpr(PARTS < 3)
+                        a.rest[row] = p - widen(narrow<TP>(p));
                 }
 #pragma unroll 1
                 for(int low = 0; low < PARTS; low++)
@@ -456,27 +446,30 @@ namespace htb
                                     p1 -= 1.f;
                                 p0 = live ? p0 * f : 0.f;
                                 p1 = live ? p1 * f : 0.f;
-                                TP lo = narrow<TP>(p0), hi = narrow<TP>(p1);
-                                if(low)
-                                {
-                                    lo = narrow<TP>(p0 - widen(lo));
-                                    hi = narrow<TP>(p1 - widen(hi));
-                                }
+                                if constexpr(PARTS > 1)
+                                    for(int i = 0; i < low; i++)
+                                    {
+                                        p0 -= widen(narrow<TP>(p0));
+                                        p1 -= widen(narrow<TP>(p1));
+                                    }
+                                const TP lo = narrow<TP>(p0), hi = narrow<TP>(p1);
                                 q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo))
                                        | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
                             }
                             // 16-byte units permuted as the map's swizzle has them
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))),
+                                         "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
                                          : "memory");
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if(lane == 0)
                         {
-                            // a block that begins outside P has nothing to store (one that ends outside is clipped)
-                            if(row < a.T && col + r < a.n)
-                                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(low ? &a.mapLow : &a.mapP),
-                                             "r"(at), "r"(int(col + r)), "r"(int(row))
+                            // a block that begins outside has nothing to store; of one that ends outside the map clips the
+                            // columns and, with one part, the rows (more parts: rowsP is a multiple of 32)
+                            if(row < a.rowsP && col + r < a.n)
+                                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&a.mapP), "r"(at),
+                                             "r"(int(col + r)), "r"(int(low * a.rowsP + row))
                                              : "memory");
                             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
@@ -503,6 +496,7 @@ namespace htb
             static constexpr int  kSide  = 0;
             static constexpr bool kSplit = false;
             static constexpr int  SLOTS  = 1;
+            static constexpr int  ROUND  = 128 / int(sizeof(TD)); // columns of a slot: rows of 128 bytes
             static constexpr int  ROOM   = 8 * SLOTS * 4096;
             const Args&           a;
             const int             lane;
@@ -527,7 +521,7 @@ namespace htb
                 const float    f  = a.scale ? a.scale[1] : 1.f;
                 const uint64_t f2 = pack2(f, f);
 #pragma unroll
-                for(int r = 0; r < COLS; r += 64)
+                for(int r = 0; r < COLS; r += ROUND)
                 {
                     const uint32_t at = slot + uint32_t((stores % SLOTS) * 4096);
                     if(lane == 0)
@@ -541,9 +535,18 @@ namespace htb
 #pragma unroll
                         for(int j = 0; j < 4; j++)
                         {
-                            const float2 x = unpack2(mul2(acc[(r + 8 * u + 2 * j) / 2], f2));
-                            const TD     lo = narrow<TD>(x.x), hi = narrow<TD>(x.y);
-                            q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo)) | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
+                            if constexpr(sizeof(TD) == 4)
+                            {
+                                const float2 x = unpack2(mul2(acc[(r + 4 * u + j) / 2], f2));
+                                q[j]           = __float_as_uint((j & 1) ? x.y : x.x);
+                            }
+                            else
+                            {
+                                const float2 x = unpack2(mul2(acc[(r + 8 * u + 2 * j) / 2], f2));
+                                const TD     lo = narrow<TD>(x.x), hi = narrow<TD>(x.y);
+                                q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo))
+                                       | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
+                            }
                         }
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))),
                                      "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
@@ -572,7 +575,7 @@ namespace htb
         struct HiddenArgs
         {
             int64_t T, ld;
-            int     tiles; // of 128 tokens: tile rows of a part
+            int64_t rows; // of a part, in whole tiles
             float*  out;
             int     add; // to what the pieces before left there
         };
@@ -596,8 +599,7 @@ namespace htb
             }
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
-                const int64_t tile = row >> 7, part = tile / a.tiles;
-                const int64_t t    = row - part * a.tiles * 128;
+                const int64_t part = row / a.rows, t = row - part * a.rows;
                 if(t >= a.T)
                     return;
                 float* out = a.out + (part * a.T + t) * a.ld + col; // ld is a multiple of eight
@@ -682,21 +684,73 @@ namespace htb
         }
 
         bool encodeMatrix(PFN_encodeTiled encode, CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int boxCols, int boxRows,
-                          CUtensorMapSwizzle swizzle)
+                          bool f32 = false)
         {
-            cuuint64_t gdim[2] = {cuuint64_t(cols), cuuint64_t(rows)}, gstr[1] = {rows > 1 ? cuuint64_t(ld) * 2 : cuuint64_t((cols + 7) / 8 * 16)};
-            cuuint32_t bx[2] = {cuuint32_t(boxCols), cuuint32_t(boxRows)}, estr[2] = {1, 1};
-            return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), gdim, gstr, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+            const int64_t size    = f32 ? 4 : 2, unit = 16 / size;
+            cuuint64_t    gdim[2] = {cuuint64_t(cols), cuuint64_t(rows)}, gstr[1] = {cuuint64_t((rows > 1 ? ld : (cols + unit - 1) / unit * unit) * size)};
+            cuuint32_t    bx[2] = {cuuint32_t(boxCols), cuuint32_t(boxRows)}, estr[2] = {1, 1};
+            return encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), gdim, gstr, bx, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
                    == CUDA_SUCCESS;
         }
 
-        template <class Epi, bool PAIR, int TN, bool XMN, bool YMN>
+        // The pairs of segments that are multiplied when X is a sum of nx numbers and Y of ny: the products that are left out
+        // are below 2^-26 of the whole.
+        void segmentPairs(int nx, int ny, AccArgs& a, int kBlocksOfOne)
+        {
+            int pairs = 0;
+            a.segX = a.segY = 0;
+            for(int sum = std::min(nx + ny - 2, 2); sum >= 0; sum--) // small products first
+                for(int x = 0; x < nx; x++)
+                {
+                    const int y = sum - x;
+                    if(y < 0 || y >= ny)
+                        continue;
+                    a.segX |= uint32_t(x) << (4 * pairs);
+                    a.segY |= uint32_t(y) << (4 * pairs);
+                    pairs++;
+                }
+            a.segBlocks = kBlocksOfOne;
+            a.kBlocks   = pairs * kBlocksOfOne;
+        }
+
+        // what every launch has in common; xRows: rows of X that a CTA loads
+        template <class Epi, bool PAIR>
+        void fillCommon(AccArgs& a, int64_t rows, int64_t cols, int xRows, int64_t bytesOfRow, int* status)
+        {
+            constexpr int  TILE   = PAIR ? 256 : 128;
+            const uint32_t block  = (uint32_t(xRows) + (PAIR ? 128u : 256u)) * 128u, behind = uint32_t(128 - xRows) * 128u;
+            const int      room   = 226 * 1024 - 1024 - Epi::ROOM - int(behind);
+            a.tilesM     = int((rows + TILE - 1) / TILE);
+            a.tilesN     = int((cols + 255) / 256);
+            a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (TILE * bytesOfRow))));
+            a.chunk      = 16;
+            a.kElems     = 64;
+            a.xRows      = xRows;
+            a.ksplit     = 1;
+            a.kParts     = 1;
+            // Waits and commits between MMAs cost the issuing thread several hundred cycles: two K blocks a stage (1024 cycles
+            // of MMAs) where three stages of them fit
+            a.sub        = room / int(2 * block) >= 3 ? 2 : 1;
+            a.stages     = std::min<int>(kAccMaxStages, room / int(block * a.sub));
+            a.stageBytes = (uint32_t(a.stages * a.sub) * block + behind + 1023) / 1024 * 1024;
+            a.status     = status;
+            a.statusCode = kStatusSoftmax;
+        }
+        // f32 sums, both operands f16 or bf16, transposed ones, N / 8, M / 16
+        uint32_t instruction(bool f16, bool pair, bool xMn, bool yMn)
+        {
+            return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (xMn ? 1u << 15 : 0u) | (yMn ? 1u << 16 : 0u) | (uint32_t(256 >> 3) << 17)
+                   | (uint32_t((pair ? 256 : 128) >> 4) << 24);
+        }
+
+        template <class Epi, bool PAIR, bool XMN, bool YMN>
         cudaError_t launchAccumulate(const CUtensorMap& mapX, const CUtensorMap& mapY, const AccArgs& a, const typename Epi::Args& ea, int smCount,
                                      cudaStream_t stream, const char* name)
         {
-            auto                     kernel = accumulate_kernel<Epi, PAIR, TN, false, XMN, YMN>;
-            static const cudaError_t regs   = accCheckRegs((const void*)kernel, TN);
+            auto                     kernel = accumulate_kernel<Epi, PAIR, 256, false, XMN, YMN>;
+            static const cudaError_t regs   = accCheckRegs((const void*)kernel, 256);
             if(regs != cudaSuccess)
                 return regs;
             const size_t smem = size_t(a.stageBytes) + 1024 + Epi::ROOM;
@@ -723,52 +777,35 @@ namespace htb
             return e;
         }
 
-        template <class Epi, bool PAIR>
-        cudaError_t launchHeadForm(const HeadProduct& h, HeadArgs& ea, int smCount, int* status, cudaStream_t stream, const char* name)
-        {
-            PFN_encodeTiled encode = tensorMapEncoder();
-            if(!encode)
-                return cudaErrorNotSupported;
-            constexpr int rows = PAIR ? 256 : 128, TN = 256;
-            const int     xRows = PAIR ? 128 : int(std::min<int64_t>(128, (h.T + 7) / 8 * 8)); // no more rows of H than there are tokens
-            const uint32_t stage = (uint32_t(xRows) + (PAIR ? 128u : uint32_t(TN))) * 128u, behind = uint32_t(128 - xRows) * 128u;
-            CUtensorMap mapX, mapY;
-            if(!encodeMatrix(encode, &mapX, h.H, h.D, h.T, h.ldh, 64, xRows, CU_TENSOR_MAP_SWIZZLE_128B)
-               || !encodeMatrix(encode, &mapY, h.W, h.D, h.n, h.ldw, 64, PAIR ? 128 : TN, CU_TENSOR_MAP_SWIZZLE_128B))
-                return cudaErrorNotSupported;
-            AccArgs        a{};
-            a.tilesM     = int((h.T + rows - 1) / rows);
-            a.tilesN     = int((h.n + TN - 1) / TN);
-            a.kBlocks    = int((h.D + 63) / 64);
-            a.chunk      = 16;
-            a.kElems     = 64;
-            a.ksplit     = 1;
-            a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (rows * h.D * 2))));
-            a.xRows      = xRows;
-            // Waits and commits between MMAs cost the issuing thread several hundred cycles: two K blocks a stage (1024 cycles
-            // of MMAs) where three stages of them fit
-            const int room = 226 * 1024 - 1024 - Epi::ROOM - int(behind);
-            a.sub          = room / int(2 * stage) >= 3 ? 2 : 1;
-            a.kParts       = 1;
-            a.stages       = std::min<int>(kAccMaxStages, room / int(stage * a.sub));
-            a.stageBytes = (uint32_t(a.stages * a.sub) * stage + behind + 1023) / 1024 * 1024;
-            a.idesc      = (1u << 4) | (h.type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TN >> 3) << 17) | (uint32_t(rows >> 4) << 24);
-            a.status     = status;
-            a.statusCode = kStatusSoftmax;
-            return launchAccumulate<Epi, PAIR, TN, false, false>(mapX, mapY, a, ea, smCount, stream, name);
-        }
         // Up to 128 tokens the classes' rows are the traffic and a tile of 128 tokens is enough: 128 x 256 tiles of one CTA each.
-        // (1 token, 32000 x 4096: 56 us; tiles of 128 classes 60, of 64 94, of 32 146: a K block costs the same however narrow.)
+        // (1 token, 32000 x 4096: 54 us; tiles of 128 classes 60, of 64 94, of 32 146: a K block costs the same however narrow.)
         // Beyond, 256 x 256 tiles of CTA pairs.
         bool narrowHead(int64_t T)
         {
             return T <= 128;
         }
-
-        int rowGrid(int64_t rows)
+        int rowsLoaded(int64_t T) // no more rows than there are tokens
         {
-            return int(std::min<int64_t>(rows, 148 * 64));
+            return int(std::min<int64_t>(128, (T + 7) / 8 * 8));
         }
+
+        template <class Epi, bool PAIR>
+        cudaError_t launchHeadForm(const HeadProduct& h, HeadArgs& ea, int smCount, int* status, cudaStream_t stream, const char* name)
+        {
+            PFN_encodeTiled encode = tensorMapEncoder();
+            const int       xRows  = PAIR ? 128 : rowsLoaded(h.T);
+            CUtensorMap     mapX, mapY;
+            if(!encode || !encodeMatrix(encode, &mapX, h.H, h.D, h.segments > 1 ? h.segments * h.segH : h.T, h.ldh, 64, xRows)
+               || !encodeMatrix(encode, &mapY, h.W, h.D, h.segments > 1 ? h.segments * h.segW : h.n, h.ldw, 64, PAIR ? 128 : 256))
+                return cudaErrorNotSupported;
+            AccArgs a{};
+            fillCommon<Epi, PAIR>(a, h.T, h.n, xRows, h.D * 2 * h.segments, status);
+            segmentPairs(h.segments, h.segments, a, int((h.D + 63) / 64));
+            a.xSegR = int(h.segH), a.ySegR = int(h.segW);
+            a.idesc = instruction(h.type == CUDA_R_16F, PAIR, false, false);
+            return launchAccumulate<Epi, PAIR, false, false>(mapX, mapY, a, ea, smCount, stream, name);
+        }
+
         cudaError_t noted(const char* name)
         {
             const cudaError_t e = cudaGetLastError();
@@ -778,90 +815,12 @@ namespace htb
         }
     } // namespace
 
-    // How many parts of the classes dH's products run in, side by side: tiles of 128 x 256 of [T, D] alone would leave SMs idle
-    // when there are few tokens. About one unit for every SM, each of at least 1024 classes. 0: many tokens, the general
-    // contraction has enough tiles.
-    int hiddenParts(int64_t T, int64_t D, int64_t piece)
+    int probabilityParts(int type, int64_t T)
     {
-        if(T > 384)
-            return 0;
-        const int64_t tiles = (D + 255) / 256 * ((T + 127) / 128);
-        return int(std::max<int64_t>(1, std::min<int64_t>((148 + tiles / 2) / tiles, piece / 1024)));
-    }
-
-    cudaError_t launchHiddenGradient(int type, const void* P, int64_t ldp, const void* W, int64_t ldw, int64_t T, int64_t n, int64_t D, int parts,
-                                     float* out, int64_t ldo, bool add, int smCount, int* status, cudaStream_t stream)
-    {
-        PFN_encodeTiled encode = tensorMapEncoder();
-        HiddenArgs      ea{};
-        const int       tiles = int((T + 127) / 128), xRows = int(std::min<int64_t>(128, (T + 7) / 8 * 8));
-        ea.T = T, ea.ld = ldo, ea.tiles = tiles, ea.out = out, ea.add = add;
-        CUtensorMap mapX, mapY;
-        if(!encode || !encodeMatrix(encode, &mapX, P, n, T, ldp, 64, xRows, CU_TENSOR_MAP_SWIZZLE_128B)
-           || !encodeMatrix(encode, &mapY, W, D, n, ldw, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B))
-            return cudaErrorNotSupported;
-        const uint32_t block = (uint32_t(xRows) + 256u) * 128u, behind = uint32_t(128 - xRows) * 128u;
-        const int      room  = 226 * 1024 - 1024 - int(behind);
-        parts                = int(std::min<int64_t>(parts, (n + 63) / 64)); // a short last piece: every part has something to add
-        AccArgs a{};
-        a.tilesM     = parts * tiles;
-        a.tilesN     = int((D + 255) / 256);
-        a.kBlocks    = int((n + 63) / 64);
-        a.chunk      = 16;
-        a.sub        = room / int(2 * block) >= 3 ? 2 : 1;
-        a.kParts     = parts;
-        a.kElems     = 64;
-        a.xRows      = xRows;
-        a.ksplit     = 1;
-        a.groupM     = a.tilesM;
-        a.stages     = std::min<int>(kAccMaxStages, room / int(block * a.sub));
-        a.stageBytes = (uint32_t(a.stages * a.sub) * block + behind + 1023) / 1024 * 1024;
-        a.idesc      = (1u << 4) | (type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | (uint32_t(256 >> 3) << 17)
-                  | (uint32_t(128 >> 4) << 24); // Y transposed
-        a.status     = status;
-        a.statusCode = kStatusSoftmax;
-        return launchAccumulate<HiddenEpi, false, 256, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden");
-    }
-
-    cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
-                                     const float* scale, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream)
-    {
-        PFN_encodeTiled encode = tensorMapEncoder();
-        WeightArgs      ea{};
-        ea.rows = n, ea.cols = D, ea.scale = scale;
-        CUtensorMap mapX, mapY;
-        if(!encode || !encodeMatrix(encode, &mapX, P, n, K, ldp, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
-           || !encodeMatrix(encode, &mapY, H, D, K, ldh, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
-           || !encodeMatrix(encode, &ea.mapD, dW, D, n, ldw, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
-            return cudaErrorNotSupported;
-        AccArgs a{};
-        a.tilesM     = int((n + 255) / 256);
-        a.tilesN     = int((D + 255) / 256);
-        a.kBlocks    = int((K + 63) / 64);
-        a.chunk      = 16;
-        a.kElems     = 64;
-        a.xRows      = 128;
-        a.ksplit     = 1;
-        a.groupM     = int(std::max<int64_t>(1, std::min<int64_t>(a.tilesM, (int64_t(32) << 20) / (256 * K * 2))));
-        a.sub        = 2;
-        a.kParts     = 1;
-        a.stages     = int((226 * 1024 - 1024 - WeightEpi<__half>::ROOM) / 65536);
-        a.stageBytes = uint32_t(a.stages) * 65536u;
-        // f32 sums, both operands transposed (contiguous along their rows)
-        a.idesc = (1u << 4) | (type == CUDA_R_16BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | (uint32_t(256 >> 3) << 17)
-                  | (uint32_t(256 >> 4) << 24);
-        a.status     = status;
-        a.statusCode = kStatusSoftmax;
-        return type == CUDA_R_16F ? launchAccumulate<WeightEpi<__half>, true, 256, true, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight")
-                                  : launchAccumulate<WeightEpi<__nv_bfloat16>, true, 256, true, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_weight");
-    }
-
-    // A row of dW is a sum over the tokens of which the class's own ones outweigh the others: over few tokens the rounding of
-    // P does not average out (up to 1.5 times the rounding of dW itself). P is then handed over as two numbers, which
-    // doubles a short sum that is bound by the bytes of dW all the same.
-    bool splitProbabilities(int64_t T)
-    {
-        return T <= 64;
+        // A row of dW is a sum over the tokens of which the class's own ones outweigh the others: over few tokens the rounding
+        // of P does not average out (up to 1.5 times the rounding of dW itself). P is then handed over as two numbers,
+        // which doubles a short sum that is bound by the bytes of dW all the same. f32: three bf16 numbers, as H and W.
+        return type == CUDA_R_32F ? 3 : (T <= 64 ? 2 : 1);
     }
 
     cudaError_t launchHeadLoss(const HeadProduct& h, int64_t v0, const int64_t* targets, float alpha, void* part, float* state, int smCount,
@@ -880,61 +839,111 @@ namespace htb
     cudaError_t launchLossJoin(const void* part, int64_t n, int64_t T, float* state, bool first, bool last, int64_t V, int64_t ignore,
                                const int64_t* targets, float* loss, float* lse, int* status, cudaStream_t stream)
     {
-        const int group = kHeadGroup;
-        join_kernel<<<unsigned((T + 31) / 32), 32 * kJoinWarps, 0, stream>>>(static_cast<const float2*>(part), (n + group - 1) / group, T, state, first,
-                                                                            last, V, ignore, targets, loss, lse, status);
+        join_kernel<<<unsigned((T + 31) / 32), 32 * kJoinWarps, 0, stream>>>(static_cast<const float2*>(part), (n + kHeadGroup - 1) / kHeadGroup, T,
+                                                                            state, first, last, V, ignore, targets, loss, lse, status);
         return noted("cross_entropy_join");
     }
 
     cudaError_t launchHeadGradient(const HeadProduct& h, int64_t v0, int64_t V, int64_t ignore, const int64_t* targets, const float* lse,
-                                   const float* g, float alpha, const float* scale, void* P, int64_t ldp, float* rest, int smCount, int* status,
+                                   const float* g, float alpha, const float* scale, const Probabilities& P, float* rest, int smCount, int* status,
                                    cudaStream_t stream)
     {
         HeadArgs ea{};
         ea.T = h.T, ea.n = h.n, ea.v0 = v0, ea.V = V, ea.ignore = ignore;
         ea.targets = targets, ea.alpha = alpha, ea.lse = lse, ea.g = g, ea.scale = scale, ea.rest = rest;
+        ea.rowsP               = P.rows;
         PFN_encodeTiled encode = tensorMapEncoder();
-        const bool      two    = splitProbabilities(h.T), half = h.type == CUDA_R_16F;
-        if(!encode || !encodeMatrix(encode, &ea.mapP, P, h.n, h.T, ldp, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B)
-           || !encodeMatrix(encode, &ea.mapLow, static_cast<const char*>(P) + (two ? h.T * ldp * 2 : 0), h.n, h.T, ldp, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+        if(!encode || !encodeMatrix(encode, &ea.mapP, P.data, h.n, P.parts * P.rows, P.ld, 64, 32))
             return cudaErrorNotSupported;
-        const char* name = "cross_entropy_head_gradient";
-        if(two)
+        const char *name = "cross_entropy_head_gradient", *pairName = "cross_entropy_head_gradient_pair";
+        const bool  half = h.type == CUDA_R_16F, narrow = narrowHead(h.T);
+        if(P.parts == 3)
+            return narrow ? launchHeadForm<ProbabilityEpi<__nv_bfloat16, 3>, false>(h, ea, smCount, status, stream, name)
+                          : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 3>, true>(h, ea, smCount, status, stream, pairName);
+        if(P.parts == 2) // few tokens
             return half ? launchHeadForm<ProbabilityEpi<__half, 2>, false>(h, ea, smCount, status, stream, name)
                         : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 2>, false>(h, ea, smCount, status, stream, name);
-        if(narrowHead(h.T))
+        if(narrow)
             return half ? launchHeadForm<ProbabilityEpi<__half, 1>, false>(h, ea, smCount, status, stream, name)
                         : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 1>, false>(h, ea, smCount, status, stream, name);
-        return half ? launchHeadForm<ProbabilityEpi<__half, 1>, true>(h, ea, smCount, status, stream, "cross_entropy_head_gradient_pair")
-                    : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 1>, true>(h, ea, smCount, status, stream, "cross_entropy_head_gradient_pair");
+        return half ? launchHeadForm<ProbabilityEpi<__half, 1>, true>(h, ea, smCount, status, stream, pairName)
+                    : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 1>, true>(h, ea, smCount, status, stream, pairName);
     }
 
-    cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t cols, int64_t ld, void* X2,
-                               const int64_t* targets, int64_t ignore, int64_t V, int* status, bool twice, cudaStream_t stream)
+    // How many parts of the classes dH's products run in, side by side: the tiles of [T, D] alone would leave SMs idle when
+    // there are few. About one unit for every CTA (pair), each of at least 1024 classes.
+    int hiddenParts(int64_t T, int64_t D, int64_t piece)
     {
-        const int grid = rowGrid(count);
-        if(type == CUDA_R_32F)
-            pack_rows_kernel<float><<<grid, 256, 0, stream>>>((const float*)X, rows, count, cols, ld, (float*)X2, targets, ignore, V, status, twice);
-        else if(type == CUDA_R_16F)
-            pack_rows_kernel<__half><<<grid, 256, 0, stream>>>((const __half*)X, rows, count, cols, ld, (__half*)X2, targets, ignore, V, status, twice);
+        const int64_t tiles = (D + 255) / 256 * (narrowHead(T) ? 1 : (T + 255) / 256), units = narrowHead(T) ? 148 : 74;
+        return int(std::max<int64_t>(1, std::min<int64_t>((units + tiles / 2) / tiles, piece / 1024)));
+    }
+
+    cudaError_t launchHiddenGradient(const HeadProduct& h, const Probabilities& P, int parts, float* out, int64_t ldo, bool add, int smCount,
+                                     int* status, cudaStream_t stream)
+    {
+        PFN_encodeTiled encode = tensorMapEncoder();
+        const bool      narrow = narrowHead(h.T);
+        const int       xRows = narrow ? rowsLoaded(h.T) : 128, segP = h.segments > 1 ? P.parts : 1; // the second part of few tokens is for dW
+        CUtensorMap     mapX, mapY;
+        if(!encode || !encodeMatrix(encode, &mapX, P.data, h.n, P.parts * P.rows, P.ld, 64, xRows)
+           || !encodeMatrix(encode, &mapY, h.W, h.D, h.segments > 1 ? h.segments * h.segW : h.n, h.ldw, 64, 64))
+            return cudaErrorNotSupported;
+        AccArgs a{};
+        if(narrow)
+            fillCommon<HiddenEpi, false>(a, h.T, h.D, xRows, h.n * 2 * segP, status);
         else
-            pack_rows_kernel<__nv_bfloat16>
-                <<<grid, 256, 0, stream>>>((const __nv_bfloat16*)X, rows, count, cols, ld, (__nv_bfloat16*)X2, targets, ignore, V, status, twice);
+            fillCommon<HiddenEpi, true>(a, h.T, h.D, xRows, h.n * 2 * segP, status);
+        segmentPairs(segP, h.segments, a, int((h.n + 63) / 64));
+        a.xSegR = int(P.rows), a.ySegK = int(h.segW);
+        a.idesc  = instruction(h.type == CUDA_R_16F, !narrow, false, true);
+        a.kParts = std::min(parts, a.kBlocks); // a short last piece: every part has something to add
+        HiddenArgs ea{};
+        ea.T = h.T, ea.ld = ldo, ea.out = out, ea.add = add;
+        ea.rows  = int64_t(a.tilesM) * (narrow ? 128 : 256);
+        a.groupM = a.tilesM *= a.kParts;
+        return narrow ? launchAccumulate<HiddenEpi, false, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden")
+                      : launchAccumulate<HiddenEpi, true, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden_pair");
+    }
+
+    cudaError_t launchWeightGradient(const HeadProduct& h, const Probabilities& P, const float* scale, int typeOut, void* dW, int64_t ldw, int smCount,
+                                     int* status, cudaStream_t stream)
+    {
+        PFN_encodeTiled encode = tensorMapEncoder();
+        const bool      wide   = typeOut == CUDA_R_32F;
+        WeightArgs      ea{};
+        ea.rows = h.n, ea.cols = h.D, ea.scale = scale;
+        CUtensorMap mapX, mapY;
+        // one segment: rows past the tokens are not there (zeros); more: they hold zeros
+        if(!encode || !encodeMatrix(encode, &mapX, P.data, h.n, P.parts > 1 ? P.parts * P.rows : h.T, P.ld, 64, 64)
+           || !encodeMatrix(encode, &mapY, h.H, h.D, h.segments > 1 ? h.segments * h.segH : h.T, h.ldh, 64, 64)
+           || !encodeMatrix(encode, &ea.mapD, dW, h.D, h.n, ldw, wide ? 32 : 64, 32, wide))
+            return cudaErrorNotSupported;
+        AccArgs a{};
+        fillCommon<WeightEpi<float>, true>(a, h.n, h.D, 128, h.T * 2 * P.parts, status);
+        segmentPairs(P.parts, h.segments, a, int((h.T + 63) / 64));
+        a.xSegK = int(P.rows), a.ySegK = int(h.segH);
+        a.idesc = instruction(h.type == CUDA_R_16F, true, true, true);
+        const char* name = "cross_entropy_weight";
+        return wide                    ? launchAccumulate<WeightEpi<float>, true, true, true>(mapX, mapY, a, ea, smCount, stream, name)
+               : typeOut == CUDA_R_16F ? launchAccumulate<WeightEpi<__half>, true, true, true>(mapX, mapY, a, ea, smCount, stream, name)
+                                       : launchAccumulate<WeightEpi<__nv_bfloat16>, true, true, true>(mapX, mapY, a, ea, smCount, stream, name);
+    }
+
+    cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t total, int64_t cols, int64_t ld, void* X2,
+                               const int64_t* targets, int64_t ignore, int64_t V, int* status, cudaStream_t stream)
+    {
+        const RowShape  s   = rowShape(total, ld / 8);
+        unsigned short* out = static_cast<unsigned short*>(X2);
+        if(type == CUDA_R_32F)
+            pack_rows_kernel<float, true><<<s.grid, s.block, 0, stream>>>((const float*)X, rows, count, total, cols, ld, out, targets, ignore, V, status,
+                                                                          rowsAligned(rows, X, 4, 4));
+        else if(type == CUDA_R_16F)
+            pack_rows_kernel<__half, false><<<s.grid, s.block, 0, stream>>>((const __half*)X, rows, count, total, cols, ld, out, targets, ignore, V,
+                                                                            status, rowsAligned(rows, X, 8, 2));
+        else
+            pack_rows_kernel<__nv_bfloat16, false><<<s.grid, s.block, 0, stream>>>((const __nv_bfloat16*)X, rows, count, total, cols, ld, out, targets,
+                                                                                   ignore, V, status, rowsAligned(rows, X, 8, 2));
         return noted("cross_entropy_pack");
-    }
-
-    cudaError_t launchSoftmaxPiece(const float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, const int64_t* targets, float* state,
-                                   cudaStream_t stream)
-    {
-        softmax_piece_kernel<<<rowGrid(T), 256, 0, stream>>>(z, ldz, T, v0, count, targets, state);
-        return noted("cross_entropy_softmax");
-    }
-
-    cudaError_t launchLossFinish(const float* state, int64_t T, int64_t V, int64_t ignore, const int64_t* targets, float* loss, float* lse,
-                                 int* deviceStatus, cudaStream_t stream)
-    {
-        loss_finish_kernel<<<unsigned((T + 255) / 256), 256, 0, stream>>>(state, T, V, ignore, targets, loss, lse, deviceStatus);
-        return noted("cross_entropy_loss");
     }
 
     cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, float* scale, cudaStream_t stream)
@@ -943,23 +952,17 @@ namespace htb
         return noted("cross_entropy_scale");
     }
 
-    cudaError_t launchProbabilities(float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, int64_t V, int64_t ignore,
-                                    const int64_t* targets, const float* lse, const float* g, float alpha, cudaStream_t stream)
-    {
-        probabilities_kernel<<<rowGrid(T), 256, 0, stream>>>(z, ldz, T, v0, count, V, ignore, targets, lse, g, alpha);
-        return noted("cross_entropy_probabilities");
-    }
-
     cudaError_t launchStoreRows(int type, const float* X, int64_t ldx, int64_t count, int64_t cols, const float* scale, void* Y,
                                 const TokenRows& rows, const TargetRest& rest, int parts, cudaStream_t stream)
     {
-        const int grid = rowGrid(count);
+        const RowShape s   = rowShape(count, (cols + 3) / 4);
+        const bool     vec = rowsAligned(rows, Y, 4, type == CUDA_R_32F ? 4 : 2);
         if(type == CUDA_R_32F)
-            store_rows_kernel<float><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (float*)Y, rows, rest, parts);
+            store_rows_kernel<float><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (float*)Y, rows, rest, parts, vec);
         else if(type == CUDA_R_16F)
-            store_rows_kernel<__half><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (__half*)Y, rows, rest, parts);
+            store_rows_kernel<__half><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (__half*)Y, rows, rest, parts, vec);
         else
-            store_rows_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(X, ldx, count, cols, scale, (__nv_bfloat16*)Y, rows, rest, parts);
+            store_rows_kernel<__nv_bfloat16><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (__nv_bfloat16*)Y, rows, rest, parts, vec);
         return noted("cross_entropy_store");
     }
 } // namespace htb

@@ -26,11 +26,14 @@ namespace htb
     // What one call does, piece by piece, and where its scratch lies (byte offsets into the workspace).
     struct CrossEntropyLayout
     {
-        bool     packH, packW; // operands copied into the workspace as packed rows of ld elements
+        bool     packH, packW; // operands copied into the workspace as packed rows of ld 16-bit elements
+        bool     direct; // rows of dW can be written by bulk stores
+        int      segments; // numbers of 16 bits that an element of the copies is a sum of: 3 for f32
+        int64_t  rowsT; // of a segment of H's copy and of P
         int64_t  ld;
         int      parts; // sums of dH that are kept apart
-        int64_t  piece; // classes of a piece (a multiple of kPieceUnit, or all of them)
-        uint64_t hOff, wOff, stateOff, zOff, partOff, pOff, dhOff, dwOff, scaleOff, restOff;
+        int64_t  piece; // classes of a piece, a multiple of 256
+        uint64_t hOff, wOff, stateOff, partOff, pOff, dhOff, dwOff, scaleOff, restOff;
         uint64_t bytes;
     };
 
@@ -45,18 +48,28 @@ namespace htb
         int64_t ext[kMaxGroup], stride[kMaxGroup];
         int64_t elem; // stride along the contracted mode
     };
-    // X2[r, 0 .. ld) = X[row r, 0 .. cols), zeros behind. With targets: rows whose target is `ignore` or no class become zeros,
-    // and the latter raise the status word. twice: the rows again behind the first `count`.
-    cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t cols, int64_t ld, void* X2,
-                               const int64_t* targets, int64_t ignore, int64_t V, int* status, bool twice, cudaStream_t stream);
+    // X2[r, 0 .. ld) = X[row r, 0 .. cols), zeros behind and in rows count .. total - 1; f32 as three segments of `total` rows. With
+    // targets: rows whose target is `ignore` or no class become zeros, and the latter raise the status word.
+    cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t total, int64_t cols, int64_t ld, void* X2,
+                               const int64_t* targets, int64_t ignore, int64_t V, int* status, cudaStream_t stream);
 
-    // f16 / bf16: logits of n classes from v0 on, used where they are made
+    // the logits of n classes, used where they are made: operands in 16 bits, `segments` of segH / segW rows each
     struct HeadProduct
     {
         const void *H, *W; // rows of D elements, ldh / ldw apart, at multiples of 16 bytes
         int64_t     T, n, D, ldh, ldw;
-        int         type;
+        int         type; // CUDA_R_16F or CUDA_R_16BF
+        int         segments;
+        int64_t     segH, segW;
     };
+    // P, [parts][rows][ld] in 16 bits
+    struct Probabilities
+    {
+        void*   data;
+        int     parts;
+        int64_t rows, ld;
+    };
+    int           probabilityParts(int type, int64_t T);
     constexpr int kHeadGroup = 128; // classes that share one partial maximum and sum
     // part: ceil(n / kHeadGroup) x T pairs of floats; the target logits go to state[2T .. 3T)
     cudaError_t launchHeadLoss(const HeadProduct& h, int64_t v0, const int64_t* targets, float alpha, void* part, float* state, int smCount,
@@ -64,30 +77,17 @@ namespace htb
     // joins a piece's partial results with state[0 .. 2T) (maximum, sum in powers of two); after the last piece loss and lse
     cudaError_t launchLossJoin(const void* part, int64_t n, int64_t T, float* state, bool first, bool last, int64_t V, int64_t ignore,
                                const int64_t* targets, float* loss, float* lse, int* status, cudaStream_t stream);
-    // P[t, v] = (exp(z - lse) - [v0 + v == target]) * g * alpha (* scale[0]); rest[t]: what rounding took from the target's entry;
-    // with splitProbabilities(T) what it took from every entry in T more rows
-    bool splitProbabilities(int64_t T);
+    // P[t, v] = (exp(z - lse) - [v0 + v == target]) * g * alpha (* scale[0]); rest[t]: what rounding took from the target's entry
     cudaError_t launchHeadGradient(const HeadProduct& h, int64_t v0, int64_t V, int64_t ignore, const int64_t* targets, const float* lse,
-                                   const float* g, float alpha, const float* scale, void* P, int64_t ldp, float* rest, int smCount, int* status,
+                                   const float* g, float alpha, const float* scale, const Probabilities& P, float* rest, int smCount, int* status,
                                    cudaStream_t stream);
-
     // out[part][t, d] = (add: +=) sum over a part of the classes of P[t, v] W[v, d], `parts` of them side by side
     int         hiddenParts(int64_t T, int64_t D, int64_t piece);
-    cudaError_t launchHiddenGradient(int type, const void* P, int64_t ldp, const void* W, int64_t ldw, int64_t T, int64_t n, int64_t D, int parts,
-                                     float* out, int64_t ldo, bool add, int smCount, int* status, cudaStream_t stream);
-    // dW[v, d] = sum over K rows of P[k, v] H[k, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes
-    cudaError_t launchWeightGradient(int type, const void* P, int64_t ldp, const void* H, int64_t ldh, int64_t K, int64_t n, int64_t D,
-                                     const float* scale, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream);
-
-    // f32: logits of a piece in memory, z[t, v] with rows ldz apart
-    // running maximum / sum / target logit per token: state[0 .. T), [T .. 2T), [2T .. 3T)
-    cudaError_t launchSoftmaxPiece(const float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, const int64_t* targets, float* state,
-                                   cudaStream_t stream);
-    cudaError_t launchLossFinish(const float* state, int64_t T, int64_t V, int64_t ignore, const int64_t* targets, float* loss, float* lse,
-                                 int* deviceStatus, cudaStream_t stream);
-    // z becomes P in place
-    cudaError_t launchProbabilities(float* z, int64_t ldz, int64_t T, int64_t v0, int64_t count, int64_t V, int64_t ignore,
-                                    const int64_t* targets, const float* lse, const float* g, float alpha, cudaStream_t stream);
+    cudaError_t launchHiddenGradient(const HeadProduct& h, const Probabilities& P, int parts, float* out, int64_t ldo, bool add, int smCount,
+                                     int* status, cudaStream_t stream);
+    // dW[v, d] = sum over the tokens of P[t, v] H[t, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes
+    cudaError_t launchWeightGradient(const HeadProduct& h, const Probabilities& P, const float* scale, int typeOut, void* dW, int64_t ldw, int smCount,
+                                     int* status, cudaStream_t stream);
 
     // f16: scale[0] = a power of two that brings max |g * alpha| close to the top of the range, scale[1] = its reciprocal
     cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, float* scale, cudaStream_t stream);

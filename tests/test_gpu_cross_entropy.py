@@ -72,7 +72,8 @@ ALL = [torch.bfloat16, torch.float16, torch.float32]
 @pytest.mark.parametrize("pref", [ht.WORKSPACE_MIN, ht.WORKSPACE_MAX])
 @pytest.mark.parametrize("kind", ALL)
 @pytest.mark.parametrize("t,v,d", [(1, 1, 1), (1, 1000, 64), (2, 257, 8), (17, 1031, 136), (130, 2000, 72), (300, 777, 260),
-                                   (513, 513, 64), (700, 4100, 520), (40, 700, 2100), (300, 600, 4200)])
+                                   (513, 513, 64), (700, 4100, 520), (40, 700, 2100), (300, 600, 4200),
+                                   (129, 3000, 40), (400, 1500, 1100), (65, 9000, 24)])
 def test_sizes(h, t, v, d, kind, pref):
     c = Call(h, *inputs(t, v, d, kind), pref=pref)
     c.forward()
