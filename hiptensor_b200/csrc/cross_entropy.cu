@@ -412,13 +412,23 @@ namespace htb
                 }
                 const float    c  = a.alpha * kLog2e;
                 const uint64_t c2 = pack2(c, c), l2 = pack2(-l, -l);
-                const int64_t  t = live ? target - a.v0 - col : -1;
-                if(t >= 0 && t < COLS)
+                const int      t  = live && target - a.v0 - col >= 0 && target - a.v0 - col < COLS ? int(target - a.v0 - col) : -1;
+                // P takes the sums' place
+#pragma unroll
+                for(int i = 0; i < COLS / 2; i++)
                 {
-                    const float x = unpack2(fma2(pack2(Sums::at(int(t)), 0.f), c2, l2)).x;
-                    const float p = (exp2f(x) - 1.f) * f;
-                    if constexpr(PARTS < 3)
-                        a.rest[row] = p - widen(narrow<TP>(p));
+                    const float2 x  = unpack2(fma2(acc[i], c2, l2));
+                    float        p0 = exp2f(x.x), p1 = exp2f(x.y);
+                    if(t == 2 * i)
+                        p0 -= 1.f;
+                    if(t == 2 * i + 1)
+                        p1 -= 1.f;
+                    acc[i] = live ? pack2(p0 * f, p1 * f) : 0;
+                }
+                if(PARTS < 3 && t >= 0)
+                {
+                    const float p = Sums::at(t);
+                    a.rest[row]   = p - widen(narrow<TP>(p));
                 }
 #pragma unroll 1
                 for(int low = 0; low < PARTS; low++)
@@ -437,22 +447,11 @@ namespace htb
 #pragma unroll
                             for(int j = 0; j < 4; j++)
                             {
-                                const int    k = r + 8 * u + 2 * j;
-                                const float2 x = unpack2(fma2(acc[k / 2], c2, l2));
-                                float        p0 = exp2f(x.x), p1 = exp2f(x.y);
-                                if(t == k)
-                                    p0 -= 1.f;
-                                if(t == k + 1)
-                                    p1 -= 1.f;
-                                p0 = live ? p0 * f : 0.f;
-                                p1 = live ? p1 * f : 0.f;
+                                uint64_t&    pair = acc[(r + 8 * u + 2 * j) / 2];
+                                const float2 x    = unpack2(pair);
+                                const TP     lo = narrow<TP>(x.x), hi = narrow<TP>(x.y);
                                 if constexpr(PARTS > 1)
-                                    for(int i = 0; i < low; i++)
-                                    {
-                                        p0 -= widen(narrow<TP>(p0));
-                                        p1 -= widen(narrow<TP>(p1));
-                                    }
-                                const TP lo = narrow<TP>(p0), hi = narrow<TP>(p1);
+                                    pair = pack2(x.x - widen(lo), x.y - widen(hi)); // for the next part
                                 q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo))
                                        | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
                             }
@@ -489,13 +488,14 @@ namespace htb
             const float* scale;
             CUtensorMap  mapD;
         };
-        template <typename TD>
+        // SLOTS: of 4 KiB for a warp's results. A short sum (few tokens) is bound by its stores and takes two; a long one leaves the
+        // room to the stages.
+        template <typename TD, int SLOTS>
         struct WeightEpi : HeadSums<256>
         {
             using Args                   = WeightArgs;
             static constexpr int  kSide  = 0;
             static constexpr bool kSplit = false;
-            static constexpr int  SLOTS  = 1;
             static constexpr int  ROUND  = 128 / int(sizeof(TD)); // columns of a slot: rows of 128 bytes
             static constexpr int  ROOM   = 8 * SLOTS * 4096;
             const Args&           a;
@@ -715,6 +715,12 @@ namespace htb
             a.kBlocks   = pairs * kBlocksOfOne;
         }
 
+        template <class T>
+        struct Named // a type as an argument
+        {
+            using Type = T;
+        };
+
         // what every launch has in common; xRows: rows of X that a CTA loads
         template <class Epi, bool PAIR>
         void fillCommon(AccArgs& a, int64_t rows, int64_t cols, int xRows, int64_t bytesOfRow, int* status)
@@ -777,12 +783,16 @@ namespace htb
             return e;
         }
 
-        // Up to 128 tokens the classes' rows are the traffic and a tile of 128 tokens is enough: 128 x 256 tiles of one CTA each.
-        // (1 token, 32000 x 4096: 54 us; tiles of 128 classes 60, of 64 94, of 32 146: a K block costs the same however narrow.)
-        // Beyond, 256 x 256 tiles of CTA pairs.
-        bool narrowHead(int64_t T)
+        // 128 x 256 tiles of one CTA each, or 256 x 256 tiles of CTA pairs, which load less. Up to 128 tokens a tile of 128 is
+        // enough and the classes' rows are the traffic (1 token, 32000 x 4096: 54 us; with tiles of 128 classes 60, of 64 94: a
+        // K block costs the same however narrow). Beyond, the form with the shorter sequence of tiles, one of a single CTA
+        // taking about 1.4 times a pair's (it is bound by what it loads).
+        bool singleTiles(int64_t T, int64_t columns, int sms)
         {
-            return T <= 128;
+            if(T <= 128)
+                return true;
+            const int64_t single = ((T + 127) / 128 * columns + sms - 1) / sms, pairs = ((T + 255) / 256 * columns + sms / 2 - 1) / (sms / 2);
+            return 7 * single < 5 * pairs;
         }
         int rowsLoaded(int64_t T) // no more rows than there are tokens
         {
@@ -815,6 +825,14 @@ namespace htb
         }
     } // namespace
 
+    namespace
+    {
+        int smsOf(int smCount)
+        {
+            return smCount > 0 ? smCount : 148;
+        }
+    } // namespace
+
     int probabilityParts(int type, int64_t T)
     {
         // A row of dW is a sum over the tokens of which the class's own ones outweigh the others: over few tokens the rounding
@@ -832,7 +850,7 @@ namespace htb
         ea.alpha       = alpha;
         ea.part        = static_cast<float2*>(part);
         ea.targetLogit = state + 2 * h.T;
-        return narrowHead(h.T) ? launchHeadForm<LossEpi, false>(h, ea, smCount, status, stream, "cross_entropy_head")
+        return singleTiles(h.T, (h.n + 255) / 256, smsOf(smCount)) ? launchHeadForm<LossEpi, false>(h, ea, smCount, status, stream, "cross_entropy_head")
                                : launchHeadForm<LossEpi, true>(h, ea, smCount, status, stream, "cross_entropy_head_pair");
     }
 
@@ -856,11 +874,11 @@ namespace htb
         if(!encode || !encodeMatrix(encode, &ea.mapP, P.data, h.n, P.parts * P.rows, P.ld, 64, 32))
             return cudaErrorNotSupported;
         const char *name = "cross_entropy_head_gradient", *pairName = "cross_entropy_head_gradient_pair";
-        const bool  half = h.type == CUDA_R_16F, narrow = narrowHead(h.T);
+        const bool  half = h.type == CUDA_R_16F, narrow = singleTiles(h.T, (h.n + 255) / 256, smsOf(smCount));
         if(P.parts == 3)
             return narrow ? launchHeadForm<ProbabilityEpi<__nv_bfloat16, 3>, false>(h, ea, smCount, status, stream, name)
                           : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 3>, true>(h, ea, smCount, status, stream, pairName);
-        if(P.parts == 2) // few tokens
+        if(P.parts == 2) // few tokens, single tiles
             return half ? launchHeadForm<ProbabilityEpi<__half, 2>, false>(h, ea, smCount, status, stream, name)
                         : launchHeadForm<ProbabilityEpi<__nv_bfloat16, 2>, false>(h, ea, smCount, status, stream, name);
         if(narrow)
@@ -871,18 +889,32 @@ namespace htb
     }
 
     // How many parts of the classes dH's products run in, side by side: the tiles of [T, D] alone would leave SMs idle when
-    // there are few. About one unit for every CTA (pair), each of at least 1024 classes.
+    // there are few, or in their last round when there are some. A round of tiles over n classes takes about n x 5.9 ns
+    // (measured rate of a pair), a part more T x D x 8 bytes of traffic; a part has at least 1024 classes.
     int hiddenParts(int64_t T, int64_t D, int64_t piece)
     {
-        const int64_t tiles = (D + 255) / 256 * (narrowHead(T) ? 1 : (T + 255) / 256), units = narrowHead(T) ? 148 : 74;
-        return int(std::max<int64_t>(1, std::min<int64_t>((units + tiles / 2) / tiles, piece / 1024)));
+        const bool    single = T <= 128;
+        const int64_t tiles  = (D + 255) / 256 * (single ? 1 : (T + 255) / 256), units = single ? 148 : 74;
+        int           best   = 1;
+        double        least  = 0;
+        for(int parts = 1; parts <= 148 && (parts == 1 || parts * 1024 <= piece); parts++)
+        {
+            const double rounds = double((tiles * parts + units - 1) / units) / parts;
+            const double time   = rounds * double(piece) * 5.9e-9 + parts * double(T) * double(D) * 8 / 6.5e12;
+            if(parts == 1 || time < least)
+            {
+                least = time;
+                best  = parts;
+            }
+        }
+        return best;
     }
 
     cudaError_t launchHiddenGradient(const HeadProduct& h, const Probabilities& P, int parts, float* out, int64_t ldo, bool add, int smCount,
                                      int* status, cudaStream_t stream)
     {
         PFN_encodeTiled encode = tensorMapEncoder();
-        const bool      narrow = narrowHead(h.T);
+        const bool      narrow = h.T <= 128;
         const int       xRows = narrow ? rowsLoaded(h.T) : 128, segP = h.segments > 1 ? P.parts : 1; // the second part of few tokens is for dW
         CUtensorMap     mapX, mapY;
         if(!encode || !encodeMatrix(encode, &mapX, P.data, h.n, P.parts * P.rows, P.ld, 64, xRows)
@@ -918,15 +950,22 @@ namespace htb
            || !encodeMatrix(encode, &mapY, h.H, h.D, h.segments > 1 ? h.segments * h.segH : h.T, h.ldh, 64, 64)
            || !encodeMatrix(encode, &ea.mapD, dW, h.D, h.n, ldw, wide ? 32 : 64, 32, wide))
             return cudaErrorNotSupported;
-        AccArgs a{};
-        fillCommon<WeightEpi<float>, true>(a, h.n, h.D, 128, h.T * 2 * P.parts, status);
-        segmentPairs(P.parts, h.segments, a, int((h.T + 63) / 64));
-        a.xSegK = int(P.rows), a.ySegK = int(h.segH);
-        a.idesc = instruction(h.type == CUDA_R_16F, true, true, true);
+        const bool  few  = h.T * P.parts <= 256;
         const char* name = "cross_entropy_weight";
-        return wide                    ? launchAccumulate<WeightEpi<float>, true, true, true>(mapX, mapY, a, ea, smCount, stream, name)
-               : typeOut == CUDA_R_16F ? launchAccumulate<WeightEpi<__half>, true, true, true>(mapX, mapY, a, ea, smCount, stream, name)
-                                       : launchAccumulate<WeightEpi<__nv_bfloat16>, true, true, true>(mapX, mapY, a, ea, smCount, stream, name);
+        auto        run  = [&](auto epi) {
+            using Epi = decltype(epi);
+            AccArgs a{};
+            fillCommon<typename Epi::Type, true>(a, h.n, h.D, 128, h.T * 2 * P.parts, status);
+            segmentPairs(P.parts, h.segments, a, int((h.T + 63) / 64));
+            a.xSegK = int(P.rows), a.ySegK = int(h.segH);
+            a.idesc = instruction(h.type == CUDA_R_16F, true, true, true);
+            return launchAccumulate<typename Epi::Type, true, true, true>(mapX, mapY, a, ea, smCount, stream, name);
+        };
+        if(wide)
+            return few ? run(Named<WeightEpi<float, 2>>{}) : run(Named<WeightEpi<float, 1>>{});
+        if(typeOut == CUDA_R_16F)
+            return few ? run(Named<WeightEpi<__half, 2>>{}) : run(Named<WeightEpi<__half, 1>>{});
+        return few ? run(Named<WeightEpi<__nv_bfloat16, 2>>{}) : run(Named<WeightEpi<__nv_bfloat16, 1>>{});
     }
 
     cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t total, int64_t cols, int64_t ld, void* X2,
