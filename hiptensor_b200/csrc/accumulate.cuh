@@ -190,6 +190,7 @@ namespace htb
         //   add(taddr, first, release)      reads the chunk's sums from tensor memory, calls release, and adds them
         //   end(row, col)                   the tile's sums are complete
         //   leave()                         no tile follows
+        //   kParted                         whether AccArgs::kParts may be above 1
         //   send(..), endSplit(..)          with kSplit: the exchange of a tile whose K range is cut
         // With Epi::kSide > 0, warp 3 fetches kSide floats for every K block (the scales), a group of kSideGroup blocks at a time,
         // into a ring of kSideSlots groups, ahead of the epilogue and across tiles:
@@ -290,7 +291,7 @@ namespace htb
             int  kbBegin = PAIR ? 0 : int((long long)a.kBlocks * int(rank) / a.ksplit);
             int  kbEnd   = PAIR ? a.kBlocks : int((long long)a.kBlocks * (int(rank) + 1) / a.ksplit);
             auto part    = [&](int& tm) { // kParts: the K range is the tile's
-                if(a.kParts > 1)
+                if(Epi::kParted && a.kParts > 1)
                 {
                     const int tiles = a.tilesM / a.kParts, p = tm / tiles;
                     kbBegin = int((long long)a.kBlocks * p / a.kParts);
@@ -409,9 +410,12 @@ namespace htb
                     bool           ok = true;
                     for(int u = clusterId; ok && u < units; u += numClusters)
                     {
-                        int tm, tn;
-                        tileOf(a, u, tm, tn);
-                        part(tm);
+                        if constexpr(Epi::kParted)
+                        {
+                            int tm, tn;
+                            tileOf(a, u, tm, tn);
+                            part(tm);
+                        }
                         for(int kb = kbBegin; ok && kb < kbEnd; kb += a.chunk, seq++)
                         {
                             const uint32_t buf = seq & 1;

@@ -158,6 +158,7 @@ namespace htb
             static constexpr int kSide = 128 + (VECY ? TN : 4);
             static constexpr int SLOTS = 2; // of 4 KiB, per warp, for the result
             static constexpr bool kSplit = !BULK;
+            static constexpr bool kParted = false;
             static constexpr int BYTES = kSideSlots * kSideGroup * kSide * 4; // of the ring, in front of them
             static constexpr int ROUND = 128 / int(sizeof(TD)); // columns of a slot: rows of 128 bytes
 

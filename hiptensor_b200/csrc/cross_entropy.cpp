@@ -12,7 +12,7 @@ namespace htb
     namespace
     {
         constexpr int64_t  kPieceUnit   = 256; // classes: a tile's columns
-        constexpr uint64_t kRecommended = uint64_t(512) << 20; // bytes of the pieces' buffers under WORKSPACE_RECOMMENDED
+        constexpr uint64_t kRecommended = uint64_t(1) << 30; // bytes of the pieces' buffers under WORKSPACE_RECOMMENDED
 
         int64_t roundUp(int64_t n, int64_t to)
         {
@@ -68,7 +68,7 @@ namespace htb
             l.stateOff       = take(!gradient, T * 12);
             l.scaleOff       = take(gradient, 8);
             l.restOff        = take(gradient, T * 4);
-            l.dhOff          = take(gradient, uint64_t(l.parts) * T * ld * 4);
+            l.dhOff          = take(gradient, uint64_t(l.parts) * uint64_t(hiddenRows(p.T)) * ld * 4);
             l.wOff           = take(l.packW, seg * n * ld * 2);
             l.partOff        = take(!gradient, n / kHeadGroup * T * 8);
             l.pOff           = take(gradient, uint64_t(partsP) * uint64_t(l.rowsT) * n * 2);
@@ -333,7 +333,7 @@ namespace htb
         if(p.T == 0)
         {
             if(dW) // no token, no gradient
-                HTB_TRY(launchStoreRows(p.type, nullptr, 0, p.V, p.D, nullptr, dW, plainRows(p.wV, p.wD, p.V), TargetRest{}, 0, stream));
+                HTB_TRY(launchStoreRows(p.type, nullptr, 0, p.V, p.D, nullptr, dW, plainRows(p.wV, p.wD, p.V), TargetRest{}, 0, 0, stream));
             return HIPTENSOR_STATUS_SUCCESS;
         }
         const CrossEntropyLayout l = layoutIn(p, true, workspace ? workspaceSize : 0);
@@ -385,13 +385,14 @@ namespace htb
                 {
                     // rows of W that no bulk store can write: through f32 in the workspace
                     HTB_TRY(launchWeightGradient(head, P, nullptr, CUDA_R_32F, dw, l.ld, st->smCount, st->deviceStatus, stream));
-                    HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, 1, stream));
+                    HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, 1, 0, stream));
                 }
             }
         }
         if(dH)
             HTB_TRY(launchStoreRows(p.type, dh, l.ld, p.T, p.D, scale, dH, rowsOfH(p),
-                                    P.parts == 3 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, l.parts, stream));
+                                    P.parts == 3 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, l.parts, hiddenRows(p.T),
+                                    stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }
 } // namespace htb

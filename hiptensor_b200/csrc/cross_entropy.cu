@@ -148,7 +148,7 @@ namespace htb
         template <typename T>
         __global__ void store_rows_kernel(const float* __restrict__ X, int64_t ldx, int64_t count, int64_t cols, const float* __restrict__ scale,
                                           T* __restrict__ Y, const __grid_constant__ TokenRows rows, const __grid_constant__ TargetRest rest, int parts,
-                                          bool vec)
+                                          int64_t partRows, bool vec)
         {
             const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 4;
             const float   f = scale ? scale[1] : 1.f;
@@ -159,7 +159,7 @@ namespace htb
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                 for(int i = 0; i < parts; i++)
                 {
-                    const float4 v = *reinterpret_cast<const float4*>(X + (int64_t(i) * count + r) * ldx + c); // ldx is a multiple of eight
+                    const float4 v = *reinterpret_cast<const float4*>(X + (int64_t(i) * partRows + r) * ldx + c); // ldx is a multiple of eight
                     x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
                 }
                 float y[4] = {x.x, x.y, x.z, x.w};
@@ -309,6 +309,7 @@ namespace htb
             using Sums                 = HeadSums<256>;
             static constexpr int kSide = 0;
             static constexpr bool kSplit = false;
+            static constexpr bool kParted = false;
             static constexpr int ROOM  = 0; // shared memory behind the stages
             const Args&          a;
 
@@ -374,6 +375,7 @@ namespace htb
             using Sums                 = HeadSums<256>;
             static constexpr int kSide = 0;
             static constexpr bool kSplit = false;
+            static constexpr bool kParted = false;
             static constexpr int ROUND = 64; // columns of a slot: rows of 128 bytes
             static constexpr int SLOTS = 1;
             static constexpr int ROOM  = 8 * SLOTS * 4096;
@@ -496,6 +498,7 @@ namespace htb
             using Args                   = WeightArgs;
             static constexpr int  kSide  = 0;
             static constexpr bool kSplit = false;
+            static constexpr bool kParted = false;
             static constexpr int  ROUND  = 128 / int(sizeof(TD)); // columns of a slot: rows of 128 bytes
             static constexpr int  ROOM   = 8 * SLOTS * 4096;
             const Args&           a;
@@ -571,24 +574,32 @@ namespace htb
             }
         };
 
-        // dH = P W over parts of the classes: f32 sums of every part, [part][T][ld]
+        // dH = P W over parts of the classes: f32 sums of every part, [part][rows][ld], stored or (later pieces) added by bulk
+        // copies; each element has one writer, so results are the same every time.
         struct HiddenArgs
         {
-            int64_t T, ld;
-            int64_t rows; // of a part, in whole tiles
-            float*  out;
-            int     add; // to what the pieces before left there
+            int64_t     T, ld;
+            int64_t     tileRows; // of a part, in whole tiles
+            int64_t     rows; // of a part in the result: a multiple of 32
+            int         add;
+            CUtensorMap mapOut;
         };
         struct HiddenEpi : HeadSums<256>
         {
-            using Args                   = HiddenArgs;
-            static constexpr int  kSide  = 0;
-            static constexpr bool kSplit = false;
-            static constexpr int  ROOM   = 0;
+            using Args                    = HiddenArgs;
+            static constexpr int  kSide   = 0;
+            static constexpr bool kSplit  = false;
+            static constexpr bool kParted = true;
+            static constexpr int  SLOTS   = 1;
+            static constexpr int  ROOM    = 8 * SLOTS * 4096;
             const Args&           a;
+            const int             lane;
+            const uint32_t        slot;
 
-            __device__ HiddenEpi(const Args& args, int, int, unsigned char*)
+            __device__ HiddenEpi(const Args& args, int w, int l, unsigned char* smem)
                 : a(args)
+                , lane(l)
+                , slot(smemAddr(smem) + uint32_t(w * SLOTS * 4096))
             {
             }
             __device__ __forceinline__ void begin() {}
@@ -599,25 +610,45 @@ namespace htb
             }
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
-                const int64_t part = row / a.rows, t = row - part * a.rows;
-                if(t >= a.T)
-                    return;
-                float* out = a.out + (part * a.T + t) * a.ld + col; // ld is a multiple of eight
+                const int64_t part = row / a.tileRows, t = row - part * a.tileRows;
 #pragma unroll
-                for(int j = 0; j < COLS; j += 4)
-                    if(col + j < a.ld)
+                for(int r = 0; r < COLS; r += 32)
+                {
+                    if(lane == 0)
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); // the slot's last copy has read it
+                    __syncwarp();
+#pragma unroll
+                    for(int u = 0; u < 8; u++)
                     {
-                        const float2 x = unpack2(acc[j / 2]), y = unpack2(acc[j / 2 + 1]);
-                        float4       v = make_float4(x.x, x.y, y.x, y.y);
-                        if(a.add)
-                        {
-                            const float4 o = *reinterpret_cast<const float4*>(out + j);
-                            v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
-                        }
-                        *reinterpret_cast<float4*>(out + j) = v;
+                        const float2 x = unpack2(acc[(r + 4 * u) / 2]), y = unpack2(acc[(r + 4 * u) / 2 + 1]);
+                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(slot + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))),
+                                     "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y)
+                                     : "memory");
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if(lane == 0)
+                    {
+                        if(t < a.T && col + r < a.ld)
+                        {
+                            if(a.add)
+                                asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&a.mapOut),
+                                             "r"(slot), "r"(int(col + r)), "r"(int(part * a.rows + t))
+                                             : "memory");
+                            else
+                                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&a.mapOut), "r"(slot),
+                                             "r"(int(col + r)), "r"(int(part * a.rows + t))
+                                             : "memory");
+                        }
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
             }
-            __device__ __forceinline__ void leave() {}
+            __device__ __forceinline__ void leave()
+            {
+                if(lane == 0)
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
         };
 
         // Joins the partial maxima and sums of a piece, 32 tokens a block, a slice of the classes a warp (in the order of the
@@ -910,6 +941,11 @@ namespace htb
         return best;
     }
 
+    int64_t hiddenRows(int64_t T)
+    {
+        return (T + 31) / 32 * 32;
+    }
+
     cudaError_t launchHiddenGradient(const HeadProduct& h, const Probabilities& P, int parts, float* out, int64_t ldo, bool add, int smCount,
                                      int* status, cudaStream_t stream)
     {
@@ -930,8 +966,11 @@ namespace htb
         a.idesc  = instruction(h.type == CUDA_R_16F, !narrow, false, true);
         a.kParts = std::min(parts, a.kBlocks); // a short last piece: every part has something to add
         HiddenArgs ea{};
-        ea.T = h.T, ea.ld = ldo, ea.out = out, ea.add = add;
-        ea.rows  = int64_t(a.tilesM) * (narrow ? 128 : 256);
+        ea.T = h.T, ea.ld = ldo, ea.add = add;
+        ea.rows     = hiddenRows(h.T);
+        ea.tileRows = int64_t(a.tilesM) * (narrow ? 128 : 256);
+        if(!encodeMatrix(encode, &ea.mapOut, out, ldo, parts * ea.rows, ldo, 32, 32, true))
+            return cudaErrorNotSupported;
         a.groupM = a.tilesM *= a.kParts;
         return narrow ? launchAccumulate<HiddenEpi, false, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden")
                       : launchAccumulate<HiddenEpi, true, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden_pair");
@@ -992,16 +1031,16 @@ namespace htb
     }
 
     cudaError_t launchStoreRows(int type, const float* X, int64_t ldx, int64_t count, int64_t cols, const float* scale, void* Y,
-                                const TokenRows& rows, const TargetRest& rest, int parts, cudaStream_t stream)
+                                const TokenRows& rows, const TargetRest& rest, int parts, int64_t partRows, cudaStream_t stream)
     {
         const RowShape s   = rowShape(count, (cols + 3) / 4);
         const bool     vec = rowsAligned(rows, Y, 4, type == CUDA_R_32F ? 4 : 2);
         if(type == CUDA_R_32F)
-            store_rows_kernel<float><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (float*)Y, rows, rest, parts, vec);
+            store_rows_kernel<float><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (float*)Y, rows, rest, parts, partRows, vec);
         else if(type == CUDA_R_16F)
-            store_rows_kernel<__half><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (__half*)Y, rows, rest, parts, vec);
+            store_rows_kernel<__half><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (__half*)Y, rows, rest, parts, partRows, vec);
         else
-            store_rows_kernel<__nv_bfloat16><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (__nv_bfloat16*)Y, rows, rest, parts, vec);
+            store_rows_kernel<__nv_bfloat16><<<s.grid, s.block, 0, stream>>>(X, ldx, count, cols, scale, (__nv_bfloat16*)Y, rows, rest, parts, partRows, vec);
         return noted("cross_entropy_store");
     }
 } // namespace htb

@@ -82,6 +82,7 @@ namespace htb
                                    const float* g, float alpha, const float* scale, const Probabilities& P, float* rest, int smCount, int* status,
                                    cudaStream_t stream);
     // out[part][t, d] = (add: +=) sum over a part of the classes of P[t, v] W[v, d], `parts` of them side by side
+    int64_t     hiddenRows(int64_t T); // of a part in `out`
     int         hiddenParts(int64_t T, int64_t D, int64_t piece);
     cudaError_t launchHiddenGradient(const HeadProduct& h, const Probabilities& P, int parts, float* out, int64_t ldo, bool add, int smCount,
                                      int* status, cudaStream_t stream);
@@ -91,7 +92,7 @@ namespace htb
 
     // f16: scale[0] = a power of two that brings max |g * alpha| close to the top of the range, scale[1] = its reciprocal
     cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, float* scale, cudaStream_t stream);
-    // Y[row r, c] = (sum of `parts` X[r, c] + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; parts 0: zeros; rest null: none
+    // Y[row r, c] = (sum of `parts` X[r, c], partRows rows apart, + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; parts 0: zeros; rest null: none
     struct TargetRest
     {
         const float*   rest;
@@ -100,7 +101,7 @@ namespace htb
         const void*    W;
     };
     cudaError_t launchStoreRows(int type, const float* X, int64_t ldx, int64_t count, int64_t cols, const float* scale, void* Y,
-                                const TokenRows& rows, const TargetRest& rest, int parts, cudaStream_t stream);
+                                const TokenRows& rows, const TargetRest& rest, int parts, int64_t partRows, cudaStream_t stream);
 
     int crossEntropy(const hiptensorHandle_t* handle, const CrossEntropyPlan* plan, const void* alpha, const void* H, const void* W,
                      const int64_t* targets, float* loss, float* lse, void* workspace, uint64_t workspaceSize, void* stream);
