@@ -1,5 +1,6 @@
 """ctypes loader for libhiptensor_b200.so (the flat C ABI in include/hiptensor_b200.h)."""
 import ctypes
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -82,13 +83,24 @@ def i64(v):
     return (ctypes.c_int64 * len(v))(*[int(x) for x in v])
 
 
+# The library only reads mode and block lists, so the array of a tuple can serve every call that names the same one (a
+# call's marshalling costs as much as a small kernel).
+@functools.lru_cache(maxsize=1024)
+def _array(kind, v):
+    return (kind * len(v))(*[int(x) for x in v])
+
+
 def i32(v):
     if v is None:
         return None
+    if type(v) is tuple:
+        return _array(ctypes.c_int32, v)
     return (ctypes.c_int32 * len(v))(*[int(x) for x in v])
 
 
 def u32(v):
     if v is None:
         return None
+    if type(v) is tuple:
+        return _array(ctypes.c_uint32, v)
     return (ctypes.c_uint32 * len(v))(*[int(x) for x in v])

@@ -16,6 +16,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.hpp"
 #include "scaled.hpp"
@@ -34,18 +35,67 @@ namespace htb
             asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
             return r;
         }
-        __device__ __forceinline__ float widen(float v)
+        // Eight elements as they lie in memory: four words of 16-bit pairs, or eight f32 words.
+        template <typename T>
+        struct Eight
         {
-            return v;
-        }
-        __device__ __forceinline__ float widen(__half v)
+            static constexpr int W = int(sizeof(T)) * 2;
+            uint32_t             w[W];
+
+            __device__ __forceinline__ float2 pair(int j) const // elements 2 j, 2 j + 1
+            {
+                if constexpr(sizeof(T) == 4)
+                    return make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+                else if constexpr(std::is_same<T, __nv_bfloat16>::value)
+                    return make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+                else
+                    return __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            }
+            __device__ __forceinline__ float at(int j) const
+            {
+                const float2 f = pair(j >> 1);
+                return (j & 1) ? f.y : f.x;
+            }
+            // the largest magnitude (NaN if there is one): 16-bit numbers two in an instruction
+            __device__ __forceinline__ float top() const
+            {
+                if constexpr(sizeof(T) == 4)
+                {
+                    float m = fabsf(__uint_as_float(w[0]));
+#pragma unroll
+                    for(int j = 1; j < 8; j++)
+                        m = maxNan(m, fabsf(__uint_as_float(w[j])));
+                    return m;
+                }
+                else
+                {
+                    using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+                    T2 m     = __habs2(*reinterpret_cast<const T2*>(&w[0]));
+#pragma unroll
+                    for(int j = 1; j < 4; j++)
+                        m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2*>(&w[j])));
+                    return maxNan(__low2float(m), __high2float(m));
+                }
+            }
+        };
+        // 16 bytes of elements `stride` apart, zeros from element n on. Out of line: the tiles at the edges take it, and unrolled
+        // into every row of a tile it cost the registers that keep loads in flight.
+        template <typename T>
+        __device__ __noinline__ uint4 gather(const T* src, int n, int64_t stride)
         {
-            return __half2float(v);
+            constexpr int N = 16 / int(sizeof(T));
+            __align__(16) T e[N];
+#pragma unroll
+            for(int j = 0; j < N; j++)
+                e[j] = j < n ? src[j * stride] : T(0.f);
+            return *reinterpret_cast<const uint4*>(e);
         }
-        __device__ __forceinline__ float widen(__nv_bfloat16 v)
+        __device__ __noinline__ void scatter(unsigned char* dst, uint2 w, int n, int64_t stride)
         {
-            return __bfloat162float(v);
+            for(int j = 0; j < n; j++)
+                dst[j * stride] = (unsigned char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
         }
+
         // a * r rounded to odd
         __device__ __forceinline__ float mulOdd(float a, float r)
         {
@@ -62,7 +112,7 @@ namespace htb
         struct QuantArgs
         {
             QuantPlan p;
-            int64_t   tilesR, tilesC, tiles;
+            int64_t   tilesR, tilesC;
             int       vecStore; // the result's runs are aligned: 8- and 16-byte stores
         };
 
@@ -73,49 +123,58 @@ namespace htb
             BLOCK_BOTH = 2 // 128 x 128
         };
 
+        __host__ __device__ constexpr int rowsPerThread(int form, bool trans)
+        {
+            return (form == BLOCK_ROW && !trans) ? 4 : 8;
+        }
+        // resident blocks that the registers are limited for: 32 or 64 of a thread's hold elements (16 or 32: rows in order)
+        __host__ __device__ constexpr int blocksPerSm(int form, bool trans, int size)
+        {
+            return (form == BLOCK_ROW && !trans) ? (size == 2 ? 5 : 4) : (size == 2 ? 3 : 2);
+        }
+
         // One tile of P * 16 rows and 128 columns at a time. Thread (tx, ty) holds columns tx * 8 .. + 7 of rows
-        // ty * P .. + P - 1 in registers, so A is read once; a row's maximum is a shuffle over 16 lanes, a column's goes
+        // ty * P .. + P - 1 in registers, so A is read once (and as it is: 16-bit elements take half the registers, which is
+        // what keeps enough loads in flight); a row's maximum is a shuffle over 16 lanes, a column's goes
         // through shared memory. VEC: rows of A are read as 16-byte words. TRANS: the result is contiguous along A's
         // rows' mode: the bytes pass through shared memory, 8 rows at a time, in units of 8 bytes whose place in a column
         // is XORed with the thread's tx so that the 16 threads of a row write to 16 different pairs of banks.
         template <typename T, int FORM, bool TRANS, bool VEC, bool E5M2>
-        __global__ void __launch_bounds__(kThreads) block_quantize_kernel(const T* __restrict__ A, unsigned char* __restrict__ Q,
-                                                                          float* __restrict__ S, const __grid_constant__ QuantArgs a)
+        __global__ void __launch_bounds__(kThreads, blocksPerSm(FORM, TRANS, sizeof(T)))
+            block_quantize_kernel(const T* __restrict__ A, unsigned char* __restrict__ Q, float* __restrict__ S, const __grid_constant__ QuantArgs a)
         {
-            constexpr int   P    = (FORM == BLOCK_ROW && !TRANS) ? 2 : 8;
+            constexpr int   P    = rowsPerThread(FORM, TRANS);
             constexpr float kMax = E5M2 ? 57344.f : 448.f;
             const QuantPlan& p   = a.p;
             const int        tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
             __shared__ float part[FORM == BLOCK_ROW ? 1 : (FORM == BLOCK_COL ? 16 * kTile : 16)];
             __shared__ __align__(16) unsigned char turn[TRANS ? kTile * kTile : 16];
 
-            for(int64_t t = blockIdx.x; t < a.tiles; t += gridDim.x)
+            // tiles by the grid's three dimensions (decoding a running number takes longer than the rest)
+#pragma unroll 1
+            for(int64_t b = blockIdx.z; b < p.batch; b += gridDim.z)
+#pragma unroll 1
+            for(int64_t tc = blockIdx.y; tc < a.tilesC; tc += gridDim.y)
+#pragma unroll 1
+            for(int64_t tr = blockIdx.x; tr < a.tilesR; tr += gridDim.x)
             {
-                const int64_t tc = t % a.tilesC, rest = t / a.tilesC;
-                const int64_t tr = rest % a.tilesR, b = rest / a.tilesR;
                 const int64_t r0 = tr * (16 * P) + ty * P, c0 = tc * kTile + tx * 8;
                 const int     nr = int(min(int64_t(P), p.rows - r0)), nc = int(min(int64_t(8), p.cols - c0)); // may be negative
                 const T*      src = A + b * p.aB + r0 * p.aR + c0 * p.aC;
-                float         v[P][8];
+                Eight<T>      v[P];
 #pragma unroll
-                for(int i = 0; i < P; i++)
+                for(int i = 0; i < P; i++, src += p.aR)
                 {
-                    if(VEC && i < nr && nc == 8)
+                    constexpr int N = 16 / int(sizeof(T));
+#pragma unroll
+                    for(int w = 0; w < Eight<T>::W / 4; w++) // 16-byte words
                     {
-                        constexpr int kWords = int(sizeof(T)) / 2; // 16-byte words of eight elements
-                        T             e[8];
-#pragma unroll
-                        for(int w = 0; w < kWords; w++)
-                            reinterpret_cast<uint4*>(e)[w] = __ldg(reinterpret_cast<const uint4*>(src + i * p.aR) + w);
-#pragma unroll
-                        for(int j = 0; j < 8; j++)
-                            v[i][j] = widen(e[j]);
-                    }
-                    else
-                    {
-#pragma unroll
-                        for(int j = 0; j < 8; j++)
-                            v[i][j] = (i < nr && j < nc) ? widen(src[i * p.aR + j * p.aC]) : 0.f;
+                        uint4 q = make_uint4(0, 0, 0, 0);
+                        if(VEC && i < nr && nc == 8)
+                            q = __ldg(reinterpret_cast<const uint4*>(src) + w);
+                        else if(i < nr && nc > w * N)
+                            q = gather<T>(src + w * N * p.aC, nc - w * N, p.aC);
+                        v[i].w[4 * w] = q.x, v[i].w[4 * w + 1] = q.y, v[i].w[4 * w + 2] = q.z, v[i].w[4 * w + 3] = q.w;
                     }
                 }
 
@@ -123,20 +182,24 @@ namespace htb
                 float scale[FORM == BLOCK_ROW ? P : (FORM == BLOCK_COL ? 8 : 1)];
                 if constexpr(FORM == BLOCK_ROW)
                 {
+                    // the 16 lanes of a row share its divisions: lane i < P makes the factor of row i, lane P + i its scale
+                    float mine = 0.f;
 #pragma unroll
                     for(int i = 0; i < P; i++)
                     {
-                        float m = kFloor;
-#pragma unroll
-                        for(int j = 0; j < 8; j++)
-                            m = maxNan(m, fabsf(v[i][j]));
+                        float m = maxNan(kFloor, v[i].top());
 #pragma unroll
                         for(int s = 8; s >= 1; s >>= 1)
                             m = maxNan(m, __shfl_xor_sync(0xffffffffu, m, s));
-                        scale[i] = __fdiv_rn(kMax, m);
-                        if(tx == 0 && i < nr)
-                            S[b * p.sB + (r0 + i) * p.sR + tc * p.sC] = __fdiv_rn(m, kMax);
+                        if((tx & (P - 1)) == i)
+                            mine = m;
                     }
+                    const float d = tx < P ? __fdiv_rn(kMax, mine) : __fdiv_rn(mine, kMax);
+#pragma unroll
+                    for(int i = 0; i < P; i++)
+                        scale[i] = __shfl_sync(0xffffffffu, d, int(threadIdx.x & 16) + i);
+                    if(tx >= P && tx < 2 * P && tx - P < nr)
+                        S[b * p.sB + (r0 + tx - P) * p.sR + tc * p.sC] = d;
                 }
                 else if constexpr(FORM == BLOCK_COL)
                 {
@@ -147,7 +210,7 @@ namespace htb
                         m[j] = kFloor;
 #pragma unroll
                         for(int i = 0; i < P; i++)
-                            m[j] = maxNan(m[j], fabsf(v[i][j]));
+                            m[j] = maxNan(m[j], fabsf(v[i].at(j)));
                     }
                     __syncthreads(); // the maxima of the tile before have been read
 #pragma unroll
@@ -175,9 +238,7 @@ namespace htb
                     float m = kFloor;
 #pragma unroll
                     for(int i = 0; i < P; i++)
-#pragma unroll
-                        for(int j = 0; j < 8; j++)
-                            m = maxNan(m, fabsf(v[i][j]));
+                        m = maxNan(m, v[i].top());
 #pragma unroll
                     for(int s = 16; s >= 1; s >>= 1)
                         m = maxNan(m, __shfl_xor_sync(0xffffffffu, m, s));
@@ -198,23 +259,22 @@ namespace htb
                 {
                     unsigned char* dst = Q + b * p.qB + r0 * p.qR + c0 * p.qC;
 #pragma unroll
-                    for(int i = 0; i < P; i++)
+                    for(int i = 0; i < P; i++, dst += p.qR)
                     {
                         if(i >= nr || nc <= 0)
                             continue;
                         uint32_t w[4];
 #pragma unroll
                         for(int j = 0; j < 4; j++)
-                            w[j] = pair8<E5M2>(mulOdd(v[i][2 * j], factor(i, 2 * j)), mulOdd(v[i][2 * j + 1], factor(i, 2 * j + 1)));
-                        if(a.vecStore && nc == 8)
-                            *reinterpret_cast<uint2*>(dst + i * p.qR) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-                        else
                         {
-#pragma unroll
-                            for(int j = 0; j < 8; j++)
-                                if(j < nc)
-                                    dst[i * p.qR + j * p.qC] = (unsigned char)(w[j >> 1] >> (8 * (j & 1)));
+                            const float2 f = v[i].pair(j);
+                            w[j]           = pair8<E5M2>(mulOdd(f.x, factor(i, 2 * j)), mulOdd(f.y, factor(i, 2 * j + 1)));
                         }
+                        const uint2 bytes = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+                        if(a.vecStore && nc == 8)
+                            *reinterpret_cast<uint2*>(dst) = bytes;
+                        else
+                            scatter(dst, bytes, nc, p.qC);
                     }
                 }
                 else
@@ -226,7 +286,7 @@ namespace htb
                         uint32_t w[4];
 #pragma unroll
                         for(int i = 0; i < 4; i++)
-                            w[i] = pair8<E5M2>(mulOdd(v[2 * i][j], factor(2 * i, j)), mulOdd(v[2 * i + 1][j], factor(2 * i + 1, j)));
+                            w[i] = pair8<E5M2>(mulOdd(v[2 * i].at(j), factor(2 * i, j)), mulOdd(v[2 * i + 1].at(j), factor(2 * i + 1, j)));
                         *reinterpret_cast<uint2*>(&turn[(tx * 8 + j) * kTile + ((ty ^ tx) << 3)])
                             = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
                     }
@@ -251,11 +311,8 @@ namespace htb
                             *reinterpret_cast<uint4*>(dst) = w;
                         else
                         {
-                            const uint32_t e[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                            for(int i = 0; i < 16; i++)
-                                if(i < left)
-                                    dst[i * p.qR] = (unsigned char)(e[i >> 2] >> (8 * (i & 3)));
+                            scatter(dst, make_uint2(w.x, w.y), min(left, 8), p.qR);
+                            scatter(dst + 8 * p.qR, make_uint2(w.z, w.w), left - 8, p.qR);
                         }
                     }
                 }
@@ -263,7 +320,7 @@ namespace htb
         }
 
         template <typename T, int FORM, bool TRANS>
-        cudaError_t launchForm(const QuantArgs& a, bool vec, int grid, const void* A, void* Q, float* S, cudaStream_t stream)
+        cudaError_t launchForm(const QuantArgs& a, bool vec, dim3 grid, const void* A, void* Q, float* S, cudaStream_t stream)
         {
             const bool e5m2 = a.p.typeQ == CUDA_R_8F_E5M2;
             auto       kernel = vec ? (e5m2 ? block_quantize_kernel<T, FORM, TRANS, true, true> : block_quantize_kernel<T, FORM, TRANS, true, false>)
@@ -277,7 +334,7 @@ namespace htb
         }
 
         template <typename T>
-        cudaError_t launchTyped(const QuantPlan& p, const void* A, void* Q, float* S, int smCount, cudaStream_t stream)
+        cudaError_t launchTyped(const QuantPlan& p, const void* A, void* Q, float* S, cudaStream_t stream)
         {
             const int  form  = p.blockR > 1 ? (p.blockC > 1 ? BLOCK_BOTH : BLOCK_COL) : BLOCK_ROW;
             const bool trans = p.qR == 1 && p.qC != 1; // else along the columns, or along neither
@@ -287,11 +344,12 @@ namespace htb
             const int64_t unit  = trans ? 16 : 8;
             QuantArgs     a;
             a.p        = p;
-            a.tilesR   = (p.rows + (form == BLOCK_ROW && !trans ? 31 : 127)) / (form == BLOCK_ROW && !trans ? 32 : 128);
-            a.tilesC   = (p.cols + kTile - 1) / kTile;
-            a.tiles    = a.tilesR * a.tilesC * p.batch;
+            const int64_t tileRows = 16 * rowsPerThread(form, trans);
+            a.tilesR               = (p.rows + tileRows - 1) / tileRows;
+            a.tilesC               = (p.cols + kTile - 1) / kTile;
             a.vecStore = (trans ? p.qR : p.qC) == 1 && (trans ? p.qC : p.qR) % unit == 0 && p.qB % unit == 0 && uintptr_t(Q) % unit == 0;
-            const int grid = int(std::min<int64_t>(a.tiles, int64_t(smCount > 0 ? smCount : 148) * 4096));
+            const dim3 grid(unsigned(std::min<int64_t>(a.tilesR, 0x7fffffff)), unsigned(std::min<int64_t>(a.tilesC, 65535)),
+                            unsigned(std::min<int64_t>(p.batch, 65535)));
             if(form == BLOCK_ROW)
                 return trans ? launchForm<T, BLOCK_ROW, true>(a, vec, grid, A, Q, S, stream)
                              : launchForm<T, BLOCK_ROW, false>(a, vec, grid, A, Q, S, stream);
@@ -303,13 +361,13 @@ namespace htb
         }
     } // namespace
 
-    cudaError_t launchQuantize(const QuantPlan& p, const void* A, void* Q, float* S, int smCount, cudaStream_t stream)
+    cudaError_t launchQuantize(const QuantPlan& p, const void* A, void* Q, float* S, cudaStream_t stream)
     {
         switch(p.typeA)
         {
-        case CUDA_R_32F: return launchTyped<float>(p, A, Q, S, smCount, stream);
-        case CUDA_R_16F: return launchTyped<__half>(p, A, Q, S, smCount, stream);
-        case CUDA_R_16BF: return launchTyped<__nv_bfloat16>(p, A, Q, S, smCount, stream);
+        case CUDA_R_32F: return launchTyped<float>(p, A, Q, S, stream);
+        case CUDA_R_16F: return launchTyped<__half>(p, A, Q, S, stream);
+        case CUDA_R_16BF: return launchTyped<__nv_bfloat16>(p, A, Q, S, stream);
         }
         return cudaErrorNotSupported;
     }

@@ -302,7 +302,7 @@ namespace htb
             return HIPTENSOR_STATUS_SUCCESS;
         if(!A || !Q || !S || (uintptr_t(A) % uintptr_t(dtypeSize(p.typeA))) || (uintptr_t(S) & 3))
             return HIPTENSOR_STATUS_INVALID_VALUE;
-        return launchResult(fn, launchQuantize(p, A, Q, S, st->smCount, cudaStream_t(stream)));
+        return launchResult(fn, launchQuantize(p, A, Q, S, cudaStream_t(stream)));
     }
 
     int scaledContraction(const hiptensorHandle_t* handle, const ScaledPlan* plan, const void* alpha, const void* A,

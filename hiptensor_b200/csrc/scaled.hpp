@@ -43,7 +43,7 @@ namespace htb
                    const hiptensorTensorDescriptor_t& scaleB, const uint32_t* blockB, const hiptensorTensorDescriptor_t* C,
                    const hiptensorTensorDescriptor_t& D, const int32_t* modeD, int typeCompute, ScaledPlan* out);
 
-    cudaError_t launchQuantize(const QuantPlan& p, const void* A, void* Q, float* S, int smCount, cudaStream_t stream);
+    cudaError_t launchQuantize(const QuantPlan& p, const void* A, void* Q, float* S, cudaStream_t stream);
     cudaError_t launchScaled(const ScaledPlan& p, float alpha, const void* A, const float* scaleA, const void* B,
                              const float* scaleB, float beta, const void* C, void* D, int smCount, int* deviceStatus,
                              cudaStream_t stream);
