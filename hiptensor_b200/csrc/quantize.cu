@@ -9,8 +9,8 @@
 //
 // ONE rounding. A * R rounded to f32 and then to 8 bits would round twice: an f32 product can land exactly on the border
 // between two 8-bit numbers although the product itself lies beside it. The product is therefore rounded to f32 "to odd":
-// truncated, and its last bit set when the truncation was not exact (the fused multiply-add gives the exact remainder).
-// A number rounded to odd at 24 bits rounds to 4 bits or fewer as the number itself does.
+// truncated, and its last bit set when the truncation was not exact. A number rounded to odd at 24 bits rounds to 4 bits or
+// fewer as the number itself does.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -96,12 +96,22 @@ namespace htb
                 dst[j * stride] = (unsigned char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
         }
 
-        // a * r rounded to odd
-        __device__ __forceinline__ float mulOdd(float a, float r)
+        // a * r rounded to odd. Exact products matter only where they lie on a border between two 8-bit numbers, which has at most
+        // five significant bits: r is then one of at most five bits itself (r = border / a is a 24-bit number only if a's odd
+        // part divides the border's). For a 16-bit a and such an r the product is exact; for any other r the last bit may
+        // always be set. So the bit depends on r alone: bitFor(r). An f32 a takes the remainder.
+        __device__ __forceinline__ uint32_t bitFor(float r)
+        {
+            return (__float_as_uint(r) & 0x7ffffu) ? 1u : 0u;
+        }
+        template <typename T>
+        __device__ __forceinline__ float mulOdd(float a, float r, uint32_t bit)
         {
             const float p = __fmul_rz(a, r);
-            const float e = __fmaf_rn(a, r, -p);
-            return e != 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+            if constexpr(sizeof(T) == 2)
+                return __uint_as_float(__float_as_uint(p) | bit);
+            else
+                return __fmaf_rn(a, r, -p) != 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
         }
         template <bool E5M2>
         __device__ __forceinline__ uint32_t pair8(float lo, float hi)
@@ -123,14 +133,14 @@ namespace htb
             BLOCK_BOTH = 2 // 128 x 128
         };
 
-        __host__ __device__ constexpr int rowsPerThread(int form, bool trans)
+        __host__ __device__ constexpr int rowsPerThread(int form, bool trans, int size)
         {
-            return (form == BLOCK_ROW && !trans) ? 4 : 8;
+            return (form == BLOCK_ROW && !trans && size == 4) ? 4 : 8;
         }
-        // resident blocks that the registers are limited for: 32 or 64 of a thread's hold elements (16 or 32: rows in order)
+        // resident blocks that the registers are limited for: 32 or 64 of a thread's hold elements
         __host__ __device__ constexpr int blocksPerSm(int form, bool trans, int size)
         {
-            return (form == BLOCK_ROW && !trans) ? (size == 2 ? 5 : 4) : (size == 2 ? 3 : 2);
+            return (form == BLOCK_ROW && !trans) ? 4 : (size == 2 ? 3 : 2);
         }
 
         // One tile of P * 16 rows and 128 columns at a time. Thread (tx, ty) holds columns tx * 8 .. + 7 of rows
@@ -143,7 +153,7 @@ namespace htb
         __global__ void __launch_bounds__(kThreads, blocksPerSm(FORM, TRANS, sizeof(T)))
             block_quantize_kernel(const T* __restrict__ A, unsigned char* __restrict__ Q, float* __restrict__ S, const __grid_constant__ QuantArgs a)
         {
-            constexpr int   P    = rowsPerThread(FORM, TRANS);
+            constexpr int   P    = rowsPerThread(FORM, TRANS, sizeof(T));
             constexpr float kMax = E5M2 ? 57344.f : 448.f;
             const QuantPlan& p   = a.p;
             const int        tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -253,7 +263,14 @@ namespace htb
                     if(threadIdx.x == 0)
                         S[b * p.sB + tr * p.sR + tc * p.sC] = __fdiv_rn(m, kMax);
                 }
-                auto factor = [&](int i, int j) { return scale[FORM == BLOCK_ROW ? i : (FORM == BLOCK_COL ? j : 0)]; };
+                auto     factor = [&](int i, int j) { return scale[FORM == BLOCK_ROW ? i : (FORM == BLOCK_COL ? j : 0)]; };
+                uint32_t bits[FORM == BLOCK_ROW ? P : (FORM == BLOCK_COL ? 8 : 1)];
+#pragma unroll
+                for(int k = 0; k < int(sizeof(bits) / 4); k++)
+                    bits[k] = bitFor(scale[k]);
+                auto odd = [&](float x, int i, int j) {
+                    return mulOdd<T>(x, factor(i, j), bits[FORM == BLOCK_ROW ? i : (FORM == BLOCK_COL ? j : 0)]);
+                };
 
                 if constexpr(!TRANS)
                 {
@@ -268,7 +285,7 @@ namespace htb
                         for(int j = 0; j < 4; j++)
                         {
                             const float2 f = v[i].pair(j);
-                            w[j]           = pair8<E5M2>(mulOdd(f.x, factor(i, 2 * j)), mulOdd(f.y, factor(i, 2 * j + 1)));
+                            w[j]           = pair8<E5M2>(odd(f.x, i, 2 * j), odd(f.y, i, 2 * j + 1));
                         }
                         const uint2 bytes = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
                         if(a.vecStore && nc == 8)
@@ -286,7 +303,7 @@ namespace htb
                         uint32_t w[4];
 #pragma unroll
                         for(int i = 0; i < 4; i++)
-                            w[i] = pair8<E5M2>(mulOdd(v[2 * i].at(j), factor(2 * i, j)), mulOdd(v[2 * i + 1].at(j), factor(2 * i + 1, j)));
+                            w[i] = pair8<E5M2>(odd(v[2 * i].at(j), 2 * i, j), odd(v[2 * i + 1].at(j), 2 * i + 1, j));
                         *reinterpret_cast<uint2*>(&turn[(tx * 8 + j) * kTile + ((ty ^ tx) << 3)])
                             = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
                     }
@@ -344,7 +361,7 @@ namespace htb
             const int64_t unit  = trans ? 16 : 8;
             QuantArgs     a;
             a.p        = p;
-            const int64_t tileRows = 16 * rowsPerThread(form, trans);
+            const int64_t tileRows = 16 * rowsPerThread(form, trans, sizeof(T));
             a.tilesR               = (p.rows + tileRows - 1) / tileRows;
             a.tilesC               = (p.cols + kTile - 1) / kTile;
             a.vecStore = (trans ? p.qR : p.qC) == 1 && (trans ? p.qC : p.qR) % unit == 0 && p.qB % unit == 0 && uintptr_t(Q) % unit == 0;
