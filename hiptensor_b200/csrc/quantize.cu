@@ -77,6 +77,36 @@ namespace htb
                     return maxNan(__low2float(m), __high2float(m));
                 }
             }
+            // the same for each of the eight columns over N rows
+            template <int N>
+            static __device__ __forceinline__ void tops(const Eight (&v)[N], float (&m)[8])
+            {
+                if constexpr(sizeof(T) == 4)
+                {
+#pragma unroll
+                    for(int j = 0; j < 8; j++)
+                    {
+                        m[j] = fabsf(v[0].at(j));
+#pragma unroll
+                        for(int i = 1; i < N; i++)
+                            m[j] = maxNan(m[j], fabsf(v[i].at(j)));
+                    }
+                }
+                else
+                {
+                    using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+#pragma unroll
+                    for(int j = 0; j < 4; j++)
+                    {
+                        T2 t = __habs2(*reinterpret_cast<const T2*>(&v[0].w[j]));
+#pragma unroll
+                        for(int i = 1; i < N; i++)
+                            t = __hmax2_nan(t, __habs2(*reinterpret_cast<const T2*>(&v[i].w[j])));
+                        m[2 * j]     = __low2float(t);
+                        m[2 * j + 1] = __high2float(t);
+                    }
+                }
+            }
         };
         // 16 bytes of elements `stride` apart, zeros from element n on. Out of line: the tiles at the edges take it, and unrolled
         // into every row of a tile it cost the registers that keep loads in flight.
@@ -214,14 +244,10 @@ namespace htb
                 else if constexpr(FORM == BLOCK_COL)
                 {
                     float m[8];
+                    Eight<T>::template tops<P>(v, m);
 #pragma unroll
                     for(int j = 0; j < 8; j++)
-                    {
-                        m[j] = kFloor;
-#pragma unroll
-                        for(int i = 0; i < P; i++)
-                            m[j] = maxNan(m[j], fabsf(v[i].at(j)));
-                    }
+                        m[j] = maxNan(m[j], kFloor);
                     __syncthreads(); // the maxima of the tile before have been read
 #pragma unroll
                     for(int j = 0; j < 8; j += 4)
