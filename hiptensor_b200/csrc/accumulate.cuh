@@ -8,7 +8,7 @@
 //     rounding.
 //
 // Roles: warp 0 loads by TMA, one thread of warp 1 (8 bit: of warps 1 and 2) issues the MMAs, warp 3 fetches scales, warps 4 .. 11 are the epilogue. Tensor memory holds two
-// chunks: while one is read, the next is summed. Epilogue warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and half
+// chunks or four: while one is read, the next are summed. Epilogue warp w reads lanes 32 (w % 4) .. + 31 (rows of the tile) and half
 // (w - 4) / 4 of the columns, so a thread owns one row and TN / 2 neighbouring columns of the tile.
 //
 // PAIR: two CTAs work on a 256 x 256 tile (cta_group::2), each with 128 rows of X and half of the 256 rows of Y in shared
@@ -29,8 +29,7 @@ namespace htb
         constexpr int kAccRegs = 168, kAccRegsLoad = 72, kAccRegsEpi = 216;
         static_assert(128 * kAccRegsLoad + 256 * kAccRegsEpi <= kAccThreads * kAccRegs, "the shares exceed what the launch has");
         constexpr int kAccMaxStages = 16;
-        constexpr int kSideSlots    = 2; // groups of kSideGroup K blocks in the side ring
-        constexpr int kSideGroup    = 4;
+        constexpr int kSideSlots    = 2; // groups of Epi::kGroup K blocks in the side ring
 
         struct AccArgs
         {
@@ -192,7 +191,7 @@ namespace htb
         //   leave()                         no tile follows
         //   kParted                         whether AccArgs::kParts may be above 1
         //   send(..), endSplit(..)          with kSplit: the exchange of a tile whose K range is cut
-        // With Epi::kSide > 0, warp 3 fetches kSide floats for every K block (the scales), a group of kSideGroup blocks at a time,
+        // With Epi::kSide > 0, warp 3 fetches kSide floats for every K block (the scales), a group of kGroup blocks at a time,
         // into a ring of kSideSlots groups, ahead of the epilogue and across tiles:
         //   Side(args, lane), begin(first row of this CTA, first column), fetch(slot, first K block, past the last one)
         // Registers that a kernel with wide tiles was built with must be what the shares above add up to: a smaller
@@ -221,11 +220,14 @@ namespace htb
             constexpr uint32_t yOff   = PAIR ? 16384u : uint32_t(TN) * 128u;
             const uint32_t     kBlock = PAIR ? 32768u : yOff + uint32_t(a.xRows) * 128u; // of one K block
             const uint32_t     kStage = kBlock * uint32_t(a.sub);
-            constexpr uint32_t kCols  = 2 * TN < 32 ? 32 : 2 * TN;
+            // accumulators in tensor memory: what the two hand-overs of a chunk take (1000 cycles and more) passes behind the other
+            // ones' sums; narrow tiles have room for more than two
+            constexpr uint32_t NBUF   = (F8 && TN <= 128) ? 4 : 2;
+            constexpr uint32_t kCols  = NBUF * TN;
             extern __shared__ unsigned char smemRaw[];
             unsigned char* tiles = (unsigned char*)((uintptr_t(smemRaw) + 1023) & ~uintptr_t(1023));
             __shared__ __align__(8) unsigned long long fullBar[kAccMaxStages], emptyBar[kAccMaxStages];
-            __shared__ __align__(8) unsigned long long tmemFullBar[2], tmemEmptyBar[2];
+            __shared__ __align__(8) unsigned long long tmemFullBar[2], tmemEmptyBar[4];
             __shared__ uint32_t tmemBase;
             __shared__ int      abortFlag;
             __shared__ __align__(8) unsigned long long sideFullBar[kSideSlots], sideEmptyBar[kSideSlots];
@@ -252,10 +254,9 @@ namespace htb
                     mbarInit(smemAddr(&emptyBar[s]), 1);
                 }
                 for(int i = 0; i < 2; i++)
-                {
                     mbarInit(smemAddr(&tmemFullBar[i]), 1);
+                for(int i = 0; i < int(NBUF); i++)
                     mbarInit(smemAddr(&tmemEmptyBar[i]), (PAIR ? 2 : 1) * (kAccEpi / 32));
-                }
                 for(int i = 0; i < kSideSlots; i++)
                 {
                     mbarInit(smemAddr(&sideFullBar[i]), 32);
@@ -395,9 +396,9 @@ namespace htb
                 // 8 bit: two issuers, warp 1 takes the even chunks (first accumulator), warp 2 the odd ones. An MMA is accepted
                 // only shortly before the one ahead of it is done, so what a thread does between its MMAs (the waits, the
                 // commits: 700 cycles around 512 of MMAs for a chunk of one block) would leave the tensor cores idle. A
-                // barrier tells apart two rounds of the stages only, so neither issuer may look more than a round ahead: a
-                // chunk begins after the one two before it was read, hence (in order) all before that, and with four
-                // stages or more (checked by the launcher) that covers the stage's last use.
+                // barrier tells apart two rounds of the stages only, so no issuer may look more than a round ahead: the number
+                // of stages is even (checked by the launcher), so a stage is always the same issuer's, which waits for its
+                // rounds in order.
                 // Half precision: long chunks, one issuer.
                 constexpr uint32_t ISSUERS = F8 ? 2 : 1;
                 if(lane == 0 && leader && uint32_t(warp) <= ISSUERS)
@@ -406,7 +407,7 @@ namespace htb
                     const uint64_t descX = XMN ? smemDescMn(addrX) : smemDesc(addrX), descY = YMN ? smemDescMn(addrY) : smemDesc(addrY);
                     constexpr int  stepX = XMN ? 128 : 2, stepY = YMN ? 128 : 2; // a K step of 32 bytes (MN: of 16 rows), in 16 bytes
                     const uint32_t self = uint32_t(warp) - 1;
-                    uint32_t       stage = 0, phase = 0, bufPhase = 0, seq = 0;
+                    uint32_t       stage = 0, phase = 0, seq = 0;
                     bool           ok = true;
                     for(int u = clusterId; ok && u < units; u += numClusters)
                     {
@@ -418,8 +419,8 @@ namespace htb
                         }
                         for(int kb = kbBegin; ok && kb < kbEnd; kb += a.chunk, seq++)
                         {
-                            const uint32_t buf = seq & 1;
-                            if(ISSUERS == 2 && buf != self)
+                            const uint32_t buf = seq % NBUF;
+                            if(ISSUERS == 2 && (seq & 1) != self)
                             {
                                 if(++stage == uint32_t(a.stages)) // the other issuer's stage (a chunk is one block)
                                 {
@@ -433,11 +434,9 @@ namespace htb
                             // the first stage before the accumulator: the latter is what comes late, and nothing should
                             // stand between its release and the MMAs
                             ok = mbarWaitTight(fullAddr + 8 * stage, phase, abortP)
-                                 && mbarWaitTight(smemAddr(&tmemEmptyBar[buf]), bufPhase ^ 1, abortP);
+                                 && mbarWaitTight(smemAddr(&tmemEmptyBar[buf]), ((seq / NBUF) & 1) ^ 1, abortP);
                             if(!ok)
                                 break;
-                            if(ISSUERS == 2 || buf == 1)
-                                bufPhase ^= 1;
                             for(int k = kb; k < end; k += a.sub)
                             {
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -500,8 +499,8 @@ namespace htb
                             ok = __all_sync(0xffffffffu, mbarWaitTight(smemAddr(&sideEmptyBar[slot]), phase ^ 1, abortP));
                             if(!ok)
                                 break;
-                            const int end = min((kb / kSideGroup + 1) * kSideGroup, kbEnd);
-                            side.fetch(ring + slot * (Epi::kSide * kSideGroup), kb, end);
+                            const int end = min((kb / Epi::kGroup + 1) * Epi::kGroup, kbEnd);
+                            side.fetch(ring + slot * (Epi::kSide * Epi::kGroup), kb, end);
                             mbarArrive(smemAddr(&sideFullBar[slot]));
                             kb = end;
                             if(++slot == kSideSlots)
@@ -545,11 +544,11 @@ namespace htb
                     {
                         if constexpr(Epi::kSide > 0)
                         {
-                            if(kb == kbBegin || kb % kSideGroup == 0)
+                            if(kb == kbBegin || kb % Epi::kGroup == 0)
                                 ok = __all_sync(0xffffffffu, mbarWaitTight(smemAddr(&sideFullBar[slot]), slotPhase, abortP));
                             if(!ok)
                                 break;
-                            epi.side(ring + (slot * kSideGroup + kb % kSideGroup) * Epi::kSide, row, half);
+                            epi.side(ring + (slot * Epi::kGroup + kb % Epi::kGroup) * Epi::kSide, row, half);
                         }
                         ok = __all_sync(0xffffffffu, F8 ? mbarWaitTight(emptyAddr + 8 * stage, phase, abortP)
                                                         : mbarWaitTight(smemAddr(&tmemFullBar[buf]), bufPhase, abortP));
@@ -574,7 +573,7 @@ namespace htb
                         epi.add(tmem + (uint32_t(quad * 32) << 16) + buf * TN + uint32_t(half * (TN / 2)), kb == kbBegin, release);
                         if constexpr(Epi::kSide > 0)
                         {
-                            if(kb + 1 == kbEnd || (kb + 1) % kSideGroup == 0) // the group's last block
+                            if(kb + 1 == kbEnd || (kb + 1) % Epi::kGroup == 0) // the group's last block
                             {
                                 __syncwarp();
                                 if(lane == 0)
@@ -586,8 +585,11 @@ namespace htb
                                 }
                             }
                         }
-                        buf ^= 1;
-                        bufPhase ^= buf == 0;
+                        if(++buf == NBUF)
+                        {
+                            buf = 0;
+                            bufPhase ^= 1;
+                        }
                         if(++stage == uint32_t(a.stages))
                         {
                             stage = 0;

@@ -156,10 +156,13 @@ namespace htb
             static constexpr int CH    = COLS < 32 ? COLS : 32; // columns per round of stores
             static constexpr int CL    = CH; // columns per load from tensor memory
             static constexpr int kSide = 128 + (VECY ? TN : 4);
+            // K blocks whose scales are fetched together: a fetch takes a trip to memory, and narrow tiles need a block's every
+            // few hundred cycles
+            static constexpr int kGroup = TN <= 64 ? 16 : (VECY ? 8 : 4);
             static constexpr int SLOTS = 2; // of 4 KiB, per warp, for the result
             static constexpr bool kSplit = !BULK;
             static constexpr bool kParted = false;
-            static constexpr int BYTES = kSideSlots * kSideGroup * kSide * 4; // of the ring, in front of them
+            static constexpr int BYTES = kSideSlots * kGroup * kSide * 4; // of the ring, in front of them
             static constexpr int ROUND = 128 / int(sizeof(TD)); // columns of a slot: rows of 128 bytes
 
             // Scales along k are mostly contiguous (sxK == 1): four blocks come as one 16-byte load, one value at a time would
@@ -186,29 +189,33 @@ namespace htb
                 __device__ __forceinline__ void batch(float* ring, int at, const float* src, int64_t first, int64_t limit, int block, int64_t sRow,
                                                       int64_t sK, bool quad, int kb, int end, bool mine)
                 {
-                    float v[N][kSideGroup];
+                    float v[N][kGroup];
 #pragma unroll
                     for(int i = 0; i < N; i++)
                     {
                         const int64_t r = first + i * 32;
                         const float*  p = src + (block > 1 ? r / kScaleBlock : r) * sRow + kb * sK;
 #pragma unroll
-                        for(int j = 0; j < kSideGroup; j++)
-                            v[i][j] = 0.f; // rows and columns past the result
-                        if(mine && r < limit)
+                        for(int j = 0; j < kGroup; j += 4)
                         {
-                            if(quad && end - kb == kSideGroup)
+                            float4 q = make_float4(0.f, 0.f, 0.f, 0.f); // rows and columns past the result
+                            if(mine && r < limit && kb + j < end)
                             {
-                                const float4 q = __ldg(reinterpret_cast<const float4*>(p));
-                                v[i][0] = q.x, v[i][1] = q.y, v[i][2] = q.z, v[i][3] = q.w;
+                                // (a group begins at a multiple of four blocks unless a K split cuts it)
+                                if(quad && kb + j + 4 <= end && (kb & 3) == 0)
+                                    q = __ldg(reinterpret_cast<const float4*>(p + j));
+                                else
+                                {
+                                    q.x = __ldg(p + j * sK);
+                                    if(kb + j + 1 < end)
+                                        q.y = __ldg(p + (j + 1) * sK);
+                                    if(kb + j + 2 < end)
+                                        q.z = __ldg(p + (j + 2) * sK);
+                                    if(kb + j + 3 < end)
+                                        q.w = __ldg(p + (j + 3) * sK);
+                                }
                             }
-                            else
-                            {
-#pragma unroll
-                                for(int j = 0; j < kSideGroup; j++)
-                                    if(kb + j < end)
-                                        v[i][j] = __ldg(p + j * sK);
-                            }
+                            v[i][j] = q.x, v[i][j + 1] = q.y, v[i][j + 2] = q.z, v[i][j + 3] = q.w;
                         }
                     }
                     if(!mine)
@@ -216,9 +223,9 @@ namespace htb
 #pragma unroll
                     for(int i = 0; i < N; i++)
 #pragma unroll
-                        for(int j = 0; j < kSideGroup; j++)
+                        for(int j = 0; j < kGroup; j++)
                             if(kb + j < end)
-                                ring[(kb % kSideGroup + j) * kSide + at + i * 32 + lane] = v[i][j];
+                                ring[(kb % kGroup + j) * kSide + at + i * 32 + lane] = v[i][j];
                 }
                 __device__ __forceinline__ void fetch(float* ring, int kb, int end)
                 {
@@ -444,49 +451,77 @@ namespace htb
                 if(BULK && lane == 0)
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             }
-            // exchange zone in the stages of CTA q: [sending rank][column of q's slice][128 rows]
-            __device__ __forceinline__ void send(uint32_t zone, uint32_t rank, int ksplit, int row, int half)
+            // K split over KS = 2 or 4 CTAs: CTA q finishes columns q TN / KS .. of the tile. A thread's columns are KS / 2 slices,
+            // each of one CTA. Exchange zone in the stages of CTA q: [sending rank][four columns][128 rows] of 16 bytes.
+            template <int KS>
+            __device__ __forceinline__ void sendTo(uint32_t zone, uint32_t rank, int row, int half)
             {
-                const int wide = TN / ksplit;
+                constexpr int WIDE = TN / KS, SLICES = KS / 2;
 #pragma unroll
-                for(int j = 0; j < COLS; j++)
+                for(int s = 0; s < SLICES; s++)
                 {
-                    const int      col = half * COLS + j;
-                    const uint32_t q   = uint32_t(col / wide);
-                    if(q != rank)
+                    const uint32_t q = uint32_t(half * SLICES + s);
+                    if(q == rank)
+                        continue;
+                    const uint32_t dst = mapToRank(zone + rank * uint32_t(WIDE * 512) + uint32_t(row) * 16u, q);
+#pragma unroll
+                    for(int j = 0; j < WIDE; j += 4)
                     {
-                        const uint32_t dst = mapToRank(zone + uint32_t(((int(rank) * wide + col - int(q) * wide) * 128 + row) * 4), q);
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(sum(j)) : "memory");
+                        const float2 x = unpack2(acc[(s * WIDE + j) / 2]), y = unpack2(acc[(s * WIDE + j) / 2 + 1]);
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + uint32_t(j / 4) * 2048u), "f"(x.x), "f"(x.y),
+                                     "f"(y.x), "f"(y.y)
+                                     : "memory");
                     }
                 }
             }
+            template <int KS>
+            __device__ __forceinline__ void finishSplit(uint32_t zone, uint32_t rank, int row, int half, int64_t r, int64_t col0)
+            {
+                constexpr int WIDE = TN / KS, SLICES = KS / 2, W = WIDE < 32 ? WIDE : 32;
+#pragma unroll
+                for(int s = 0; s < SLICES; s++)
+                {
+                    if(uint32_t(half * SLICES + s) != rank)
+                        continue;
+#pragma unroll
+                    for(int c = 0; c < WIDE; c += W)
+                    {
+                        float w[W];
+#pragma unroll
+                        for(int j = 0; j < W; j += 4)
+                        {
+                            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                            for(int q = 0; q < KS; q++) // in the order of the ranks
+                            {
+                                const float2 x = unpack2(acc[(s * WIDE + c + j) / 2]), y = unpack2(acc[(s * WIDE + c + j) / 2 + 1]);
+                                float4       v = make_float4(x.x, x.y, y.x, y.y);
+                                if(uint32_t(q) != rank)
+                                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                                                 : "r"(zone + uint32_t(q * WIDE * 512) + uint32_t((c + j) / 4) * 2048u + uint32_t(row) * 16u)
+                                                 : "memory");
+                                t = make_float4(t.x + v.x, t.y + v.y, t.z + v.z, t.w + v.w);
+                            }
+                            w[j] = t.x, w[j + 1] = t.y, w[j + 2] = t.z, w[j + 3] = t.w;
+                        }
+                        store<W>(a, slot, lane, w, r, col0 + half * COLS + s * WIDE + c);
+                    }
+                }
+            }
+            __device__ __forceinline__ void send(uint32_t zone, uint32_t rank, int ksplit, int row, int half)
+            {
+                if(ksplit == 2)
+                    sendTo<2>(zone, rank, row, half);
+                else
+                    sendTo<4>(zone, rank, row, half);
+            }
             __device__ __forceinline__ void endSplit(uint32_t zone, uint32_t rank, int ksplit, int row, int half, int64_t r, int64_t col0)
             {
-                const int wide = TN / ksplit, first = int(rank) * wide; // this CTA's columns of the tile
-#pragma unroll
-                for(int c = 0; c < COLS; c += 8)
-                {
-                    const int at = half * COLS + c - first; // a slice is a multiple of eight columns
-                    if(at < 0 || at >= wide)
-                        continue;
-                    float w[8];
-#pragma unroll
-                    for(int j = 0; j < 8; j++)
-                        w[j] = 0.f;
-                    for(int q = 0; q < ksplit; q++)
-#pragma unroll
-                        for(int j = 0; j < 8; j++)
-                        {
-                            float v = sum(c + j);
-                            if(q != int(rank))
-                                asm volatile("ld.shared.f32 %0, [%1];"
-                                             : "=f"(v)
-                                             : "r"(zone + uint32_t(((q * wide + at + j) * 128 + row) * 4))
-                                             : "memory");
-                            w[j] += v;
-                        }
-                    store<8>(a, slot, lane, w, r, col0 + half * COLS + c);
-                }
+                if(ksplit == 2)
+                    finishSplit<2>(zone, rank, row, half, r, col0);
+                else
+                    finishSplit<4>(zone, rank, row, half, r, col0);
             }
         };
 
@@ -554,12 +589,11 @@ namespace htb
         {
             using Epi               = ScaledEpi<TD, TN, VECY, BULK>;
             auto           kernel   = accumulate_kernel<Epi, PAIR, TN, true>;
-            const uint32_t stage    = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
+            constexpr uint32_t stage = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
             // the ring of scales, two slots of 4 KiB per warp for the result, and room to align the stages
             constexpr uint32_t room = (Epi::BYTES + 1023) / 1024 * 1024 + 8 * Epi::SLOTS * 4096 + 1024;
-            a.stages                = std::min<int>(kAccMaxStages, int((226 * 1024 - room) / stage));
-            static_assert((226 * 1024 - ((Epi::BYTES + 1023) / 1024 * 1024 + 8 * Epi::SLOTS * 4096 + 1024)) / (16384 + (PAIR ? 128 : TN) * 128) >= 4,
-                          "two issuers need four stages");
+            a.stages                = std::min<int>(kAccMaxStages, int((226 * 1024 - room) / stage)) & ~1; // even: see the issuers
+            static_assert((226 * 1024 - room) / stage >= 4, "as many stages as accumulators");
             const size_t smem       = size_t(a.stages) * stage + room;
             static const cudaError_t regs = accCheckRegs((const void*)kernel, TN);
             if(regs != cudaSuccess)
