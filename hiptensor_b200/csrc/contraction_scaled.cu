@@ -318,27 +318,24 @@ namespace htb
                 v *= a.alpha;
                 return narrow<TD>(a.C ? fmaf(a.beta, widen(static_cast<const TD*>(a.C)[at]), v) : v);
             }
-            // Columns col0 .. col0 + W - 1 of row `row` from w: through shared memory when the columns are contiguous, so that
-            // lanes that follow each other write (and read C) along a row; else as they are. Kept out of line where the
-            // columns' indexes allow it: unrolled over a tile it was 64 KiB of code, fetched anew for every tile.
+            // Columns col0 .. col0 + W - 1 of row `row` as they are: neighbouring lanes write neighbouring rows
+            template <int W>
+            __device__ __forceinline__ void storeDirect(const float (&w)[W], int64_t row, int64_t col0)
+            {
+                if(row >= a.rows)
+                    return;
+                int64_t at = row * a.dRow + col0 * a.dCol;
+#pragma unroll
+                for(int j = 0; j < W; j++, at += a.dCol)
+                    if(col0 + j < a.cols)
+                        static_cast<TD*>(a.D)[at] = finish(a, w[j], at);
+            }
+            // The same through shared memory when the columns are contiguous, so that lanes that follow each other write (and
+            // read C) along a row. Out of line: unrolled over a tile it was 64 KiB of code, fetched anew for every tile.
             template <int W>
             static __device__ __noinline__ void store(const Args& a, float* slot, int lane, const float (&w)[W], int64_t row, int64_t col0)
             {
                 TD* D = static_cast<TD*>(a.D);
-                if(!a.vec)
-                {
-                    if(row < a.rows)
-                    {
-#pragma unroll
-                        for(int j = 0; j < W; j++)
-                            if(col0 + j < a.cols)
-                            {
-                                const int64_t at = row * a.dRow + (col0 + j) * a.dCol;
-                                D[at]            = finish(a, w[j], at);
-                            }
-                    }
-                    return;
-                }
                 constexpr int U = W / 4; // 16-byte units of a row, XORed with the row against bank conflicts
                 __syncwarp(); // the round before has been read
 #pragma unroll
@@ -441,15 +438,51 @@ namespace htb
 #pragma unroll
                         for(int j = 0; j < CH; j++)
                             w[j] = sum(c + j);
-                        store<CH>(a, slot, lane, w, row, col + c);
+                        if(!a.vec)
+                            storeDirect<CH>(w, row, col + c);
+                        else
+                            store<CH>(a, slot, lane, w, row, col + c);
                     }
                 }
             }
             // before the block ends: the bulk stores have read their slots
             __device__ __forceinline__ void leave()
             {
-                if(BULK && lane == 0)
+                if(lane == 0) // (nothing to wait for where none was issued)
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+            // 32 rows of W columns by one bulk store, rows packed in a slot (a K split's results: the map's box is W wide)
+            template <int W>
+            __device__ __forceinline__ void bulkBlock(const float (&w)[W], int64_t row, int64_t col)
+            {
+                const uint32_t at = smemAddr(slot) + uint32_t((stores % SLOTS) * 4096);
+                if(lane == 0)
+                    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(SLOTS - 1) : "memory");
+                __syncwarp();
+                stores++;
+                constexpr int PER = 16 / int(sizeof(TD)); // columns of a 16-byte word
+#pragma unroll
+                for(int u = 0; u < W / PER; u++)
+                {
+                    TD e[PER];
+#pragma unroll
+                    for(int j = 0; j < PER; j++)
+                        e[j] = narrow<TD>(w[u * PER + j] * a.alpha);
+                    const uint32_t* q = reinterpret_cast<const uint32_t*>(e);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * (W * int(sizeof(TD))) + u * 16)), "r"(q[0]),
+                                 "r"(q[1]), "r"(q[2]), "r"(q[3])
+                                 : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if(lane == 0)
+                {
+                    if(row < a.rows && col < a.cols)
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&a.mapD), "r"(at),
+                                     "r"(int(col)), "r"(int(row))
+                                     : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
             }
             // K split over KS = 2 or 4 CTAs: CTA q finishes columns q TN / KS .. of the tile. A thread's columns are KS / 2 slices,
             // each of one CTA. Exchange zone in the stages of CTA q: [sending rank][four columns][128 rows] of 16 bytes.
@@ -505,7 +538,13 @@ namespace htb
                             }
                             w[j] = t.x, w[j + 1] = t.y, w[j + 2] = t.z, w[j + 3] = t.w;
                         }
-                        store<W>(a, slot, lane, w, r, col0 + half * COLS + s * WIDE + c);
+                        const int64_t col = col0 + half * COLS + s * WIDE + c;
+                        if(!a.vec)
+                            storeDirect<W>(w, r, col);
+                        else if(a.tma)
+                            bulkBlock<W>(w, r, col);
+                        else
+                            store<W>(a, slot, lane, w, r, col);
                     }
                 }
             }
@@ -534,13 +573,14 @@ namespace htb
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
                    == CUDA_SUCCESS;
         }
-        bool encodeResult(PFN_encodeTiled encode, CUtensorMap* map, int type, void* base, int64_t cols, int64_t rows, int64_t strideBytes)
+        // box: 32 rows of `boxCols` columns, or (0) of 128 bytes in the swizzled layout
+        bool encodeResult(PFN_encodeTiled encode, CUtensorMap* map, int type, void* base, int64_t cols, int64_t rows, int64_t strideBytes, int boxCols)
         {
             const bool wide    = type == CUDA_R_32F;
             cuuint64_t gdim[2] = {cuuint64_t(cols), cuuint64_t(rows)}, gstr[1] = {cuuint64_t(strideBytes)};
-            cuuint32_t bx[2] = {wide ? 32u : 64u, 32}, estr[2] = {1, 1};
+            cuuint32_t bx[2] = {boxCols ? cuuint32_t(boxCols) : (wide ? 32u : 64u), 32}, estr[2] = {1, 1};
             return encode(map, wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, gdim, gstr, bx, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, boxCols ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
                    == CUDA_SUCCESS;
         }
@@ -633,7 +673,7 @@ namespace htb
                 return ea.tma ? launchTensor<TD, true, 256, VECY, true>(mapX, mapY, a, ea, smCount, stream)
                               : launchTensor<TD, true, 256, VECY, false>(mapX, mapY, a, ea, smCount, stream);
             if(f.tn == 128)
-                return ea.tma ? launchTensor<TD, false, 128, VECY, true>(mapX, mapY, a, ea, smCount, stream)
+                return ea.tma && f.ksplit == 1 ? launchTensor<TD, false, 128, VECY, true>(mapX, mapY, a, ea, smCount, stream)
                               : launchTensor<TD, false, 128, VECY, false>(mapX, mapY, a, ea, smCount, stream);
             if(f.tn == 64)
                 return launchTensor<TD, false, 64, VECY, false>(mapX, mapY, a, ea, smCount, stream);
@@ -686,10 +726,11 @@ namespace htb
                     ea.alpha = alpha, ea.beta = beta;
                     const uintptr_t four = 4 * sizeof(TD);
                     ea.vec = (ea.dCol == 1 || cols == 1) && (rows == 1 || ea.dRow % 4 == 0) && uintptr_t(D) % four == 0 && uintptr_t(C) % four == 0;
-                    // bulk stores: the wide forms (a slot's row is 128 bytes of the result) without C and without a K split
+                    // bulk stores: the wide forms (a slot's row is 128 bytes of the result) and K splits, without C
                     const int64_t size = int64_t(sizeof(TD)), ld = rows > 1 ? ea.dRow : (cols + 15) / 16 * 16;
-                    ea.tma = f.tn >= 128 && f.ksplit == 1 && !C && (ea.dCol == 1 || cols == 1) && ld * size % 16 == 0 && ld >= cols
-                             && ld < (int64_t(1) << 36) && (uintptr_t(D) & 15) == 0 && encodeResult(encode, &ea.mapD, p.typeD, D, cols, rows, ld * size);
+                    const int boxCols = f.ksplit > 1 ? std::min(f.tn / f.ksplit, 32) : 0;
+                    ea.tma = (f.tn >= 128 || f.ksplit > 1) && !C && (ea.dCol == 1 || cols == 1) && ld * size % 16 == 0 && ld >= cols
+                             && ld < (int64_t(1) << 36) && (uintptr_t(D) & 15) == 0 && encodeResult(encode, &ea.mapD, p.typeD, D, cols, rows, ld * size, boxCols);
                     if(!ea.tma)
                         ea.mapD = mapX; // a valid map, not used
                     return ea.blockY > 1 ? launchForm<TD, false>(f, mapX, mapY, a, ea, sms, stream)
