@@ -46,7 +46,7 @@ namespace htb
             int      segBlocks;
             uint32_t segX, segY;
             int      xSegR, xSegK, ySegR, ySegK;
-            int      xRows; // not PAIR: rows of X that are loaded, a multiple of 8
+            int      xRows, yRows; // not PAIR: rows of X and Y that are loaded, multiples of 8
             int      ksplit; // CTAs of a cluster that share a tile (not PAIR)
             int      stages;
             uint32_t stageBytes; // of all stages, and what the MMAs may read behind them: a multiple of 1024
@@ -183,7 +183,7 @@ namespace htb
         }
 
         // Epi: the epilogue, one object per epilogue thread:
-        //   Epi(args, warp 0 .. 7, lane, shared memory behind the stages)
+        //   Epi(args, warp 0 .. 7, lane, shared memory behind the stages, flag of waits that ran out)
         //   begin()                         a tile begins
         //   side(values, row in the tile, half of the columns)  with kSide: this K block's side values
         //   add(taddr, first, release)      reads the chunk's sums from tensor memory, calls release, and adds them
@@ -216,7 +216,8 @@ namespace htb
         {
             constexpr int      ROWS   = PAIR ? 256 : 128;
             // A K block: PAIR 128 rows of X, then this CTA's 128 rows of Y; else TN rows of Y, then the rows of X that there are
-            // (a.xRows: a few tokens need not fill 128 rows, the MMAs read what lies behind and nobody looks at those rows)
+            // (a.xRows, a.yRows: a few tokens need not fill a tile's rows, the MMAs read what lies there and nobody looks at
+            // those rows of the sums)
             constexpr uint32_t yOff   = PAIR ? 16384u : uint32_t(TN) * 128u;
             const uint32_t     kBlock = PAIR ? 32768u : yOff + uint32_t(a.xRows) * 128u; // of one K block
             const uint32_t     kStage = kBlock * uint32_t(a.sub);
@@ -329,7 +330,7 @@ namespace htb
                             const uint32_t bar = leaderFull + 8 * stage;
                             const int      blocks = min(a.sub, kbEnd - kb);
                             if(leader)
-                                mbarArriveExpectTx(fullAddr + 8 * stage, (PAIR ? 2 : 1) * kBlock * uint32_t(blocks));
+                                mbarArriveExpectTx(fullAddr + 8 * stage, (PAIR ? 2 * 32768u : uint32_t(a.xRows + a.yRows) * 128u) * uint32_t(blocks));
                             for(int i = 0; i < blocks; i++)
                             {
                                 const uint32_t dst = tilesAddr + stage * kStage + i * kBlock;
@@ -524,7 +525,7 @@ namespace htb
                 if constexpr(kMoreRegs)
                     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAccRegsEpi));
                 const int quad = warp & 3, half = (warp - 4) >> 2;
-                Epi       epi(ea, warp - 4, lane, tiles + a.stageBytes);
+                Epi       epi(ea, warp - 4, lane, tiles + a.stageBytes, abortP);
                 uint32_t  buf = 0, bufPhase = 0, stage = 0, phase = 0; // stage and phase: F8, a chunk is one stage
                 uint32_t  slot = 0, slotPhase = 0;
                 const float* ring = reinterpret_cast<const float*>(tiles + a.stageBytes);

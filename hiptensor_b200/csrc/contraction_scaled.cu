@@ -140,21 +140,21 @@ namespace htb
             float        alpha, beta;
             int          vec; // columns contiguous, groups of four aligned
             int          tma; // the result goes out as bulk tensor stores (no C; rows at multiples of 16 bytes)
-            CUtensorMap  mapD;
+            CUtensorMap  mapD, mapC;
         };
 
         // Epilogue of accumulate_kernel: a chunk is one block of 128 along k. A thread multiplies the block's sums of its row by
         // scaleX (one per row and block) and scaleY (VECY: one per column and block; else one for 128 columns) and adds
         // them to its running sums, two columns per instruction. Both come through the side ring: 128 rows, then TN
         // columns (VECY) or the two halves of the columns.
-        // BULK: the result goes out as bulk tensor stores.
-        template <typename TD, int TN, bool VECY, bool BULK>
+        // BULK: the result goes out as bulk tensor stores; WITHC: C comes in by bulk loads, too.
+        template <typename TD, int TN, bool VECY, bool BULK, bool WITHC>
         struct ScaledEpi
         {
             using Args                 = ScaledArgs;
             static constexpr int COLS  = TN / 2;
             static constexpr int CH    = COLS < 32 ? COLS : 32; // columns per round of stores
-            static constexpr int CL    = CH; // columns per load from tensor memory
+            static constexpr int CL    = (VECY && COLS == 128) ? 16 : CH; // columns per load from tensor memory, as registers allow
             static constexpr int kSide = 128 + (VECY ? TN : 4);
             // K blocks whose scales are fetched together: a fetch takes a trip to memory, and narrow tiles need a block's every
             // few hundred cycles
@@ -246,16 +246,32 @@ namespace htb
             const int    lane;
             float*       slot;
             int          stores; // bulk stores of this warp so far, they take the slots in turn
+            volatile int* abort;
+            uint32_t     bar;
             const float* ys;
             uint64_t     s;
             uint64_t     acc[COLS / 2];
 
-            __device__ ScaledEpi(const Args& args, int w, int l, unsigned char* smem)
+            __device__ ScaledEpi(const Args& args, int w, int l, unsigned char* smem, volatile int* abortFlag)
                 : a(args)
                 , lane(l)
                 , slot(reinterpret_cast<float*>(smem + (BYTES + 1023) / 1024 * 1024 + w * (SLOTS * 4096)))
                 , stores(0)
+                , abort(abortFlag)
             {
+                if constexpr(WITHC)
+                {
+                    // one barrier for each slot: C's blocks on their way into it
+                    __shared__ __align__(8) unsigned long long bars[8 * SLOTS];
+                    bar = smemAddr(&bars[w * SLOTS]);
+                    if(l == 0)
+                    {
+                        for(int i = 0; i < SLOTS; i++)
+                            mbarInit(bar + 8 * i, 1);
+                        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+                    }
+                    __syncwarp();
+                }
             }
             __device__ __forceinline__ void begin()
             {
@@ -381,33 +397,56 @@ namespace htb
                     }
                 }
             }
+            // lane 0: fetches C's block of columns col .. of the warp's rows into the slot of bulk store number n
+            __device__ __forceinline__ void fetchC(int n, int64_t row, int64_t col)
+            {
+                const uint32_t b = bar + uint32_t(n % SLOTS) * 8u;
+                if(row < a.rows && col < a.cols)
+                {
+                    mbarArriveExpectTx(b, 4096);
+                    const int c[2] = {int(col), int(row)};
+                    tmaLoad<2>(smemAddr(slot) + uint32_t((n % SLOTS) * 4096), &a.mapC, b, c);
+                }
+                else
+                    mbarArrive(b);
+            }
             // A slot of 32 rows x 128 bytes, 16-byte units permuted as the tensor map's 128-byte swizzle has them, and one
-            // bulk store of it: the tile leaves while the next one is summed.
+            // bulk store of it: the tile leaves while the next one is summed. With C (mapC), the slot holds C's block first.
             __device__ __forceinline__ void bulkStore(int c, int64_t row, int64_t col)
             {
-                const uint32_t at = smemAddr(slot) + uint32_t((stores % SLOTS) * 4096);
-                if(lane == 0)
-                    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(SLOTS - 1) : "memory"); // the slot's last store has read it
+                const uint32_t at = smemAddr(slot) + uint32_t((stores % SLOTS) * 4096), line = at + uint32_t(lane * 128);
+                if constexpr(WITHC)
+                    mbarWaitTight(bar + uint32_t(stores % SLOTS) * 8u, uint32_t(stores / SLOTS) & 1u, abort);
+                else
+                {
+                    if(lane == 0)
+                        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(SLOTS - 1) : "memory"); // the slot's last store has read it
+                }
                 __syncwarp();
                 stores++;
 #pragma unroll
                 for(int u = 0; u < 8; u++)
                 {
-                    uint32_t q[4];
-#pragma unroll
-                    for(int j = 0; j < 4; j++)
+                    constexpr int  PER  = 16 / int(sizeof(TD)); // columns of a unit
+                    const uint32_t unit = line + uint32_t((u ^ (lane & 7)) << 4);
+                    __align__(16) TD e[PER];
+                    if constexpr(WITHC)
                     {
-                        if constexpr(sizeof(TD) == 4)
-                            q[j] = __float_as_uint(sum(c + 4 * u + j) * a.alpha);
-                        else
-                        {
-                            const TD lo = narrow<TD>(sum(c + 8 * u + 2 * j) * a.alpha), hi = narrow<TD>(sum(c + 8 * u + 2 * j + 1) * a.alpha);
-                            q[j] = uint32_t(reinterpret_cast<const unsigned short&>(lo)) | (uint32_t(reinterpret_cast<const unsigned short&>(hi)) << 16);
-                        }
+                        uint32_t q[4];
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(unit) : "memory");
+                        const TD* in = reinterpret_cast<const TD*>(q);
+#pragma unroll
+                        for(int j = 0; j < PER; j++)
+                            e[j] = narrow<TD>(fmaf(a.beta, widen(in[j]), sum(c + PER * u + j) * a.alpha));
                     }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + uint32_t(lane * 128 + ((u ^ (lane & 7)) << 4))),
-                                 "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
-                                 : "memory");
+                    else
+                    {
+#pragma unroll
+                        for(int j = 0; j < PER; j++)
+                            e[j] = narrow<TD>(sum(c + PER * u + j) * a.alpha);
+                    }
+                    const uint32_t* q = reinterpret_cast<const uint32_t*>(e);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(unit), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -419,12 +458,24 @@ namespace htb
                                      "r"(int(col + c)), "r"(int(row))
                                      : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    if(WITHC && c + SLOTS * ROUND < COLS)
+                    {
+                        // the block after the next one, into this slot
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        fetchC(stores + SLOTS - 1, row, col + c + SLOTS * ROUND);
+                    }
                 }
             }
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
                 if constexpr(BULK)
                 {
+                    if(WITHC && lane == 0)
+                    {
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); // the slots are free
+                        for(int i = 0; i < SLOTS && i * ROUND < COLS; i++)
+                            fetchC(stores + i, row, col + i * ROUND);
+                    }
 #pragma unroll
                     for(int c = 0; c < COLS; c += ROUND)
                         bulkStore(c, row, col);
@@ -623,11 +674,11 @@ namespace htb
             return f;
         }
 
-        template <typename TD, bool PAIR, int TN, bool VECY, bool BULK>
+        template <typename TD, bool PAIR, int TN, bool VECY, bool BULK, bool WITHC = false>
         cudaError_t launchTensor(const CUtensorMap& mapX, const CUtensorMap& mapY, AccArgs a, const ScaledArgs& ea, int smCount,
                                  cudaStream_t stream)
         {
-            using Epi               = ScaledEpi<TD, TN, VECY, BULK>;
+            using Epi               = ScaledEpi<TD, TN, VECY, BULK, WITHC>;
             auto           kernel   = accumulate_kernel<Epi, PAIR, TN, true>;
             constexpr uint32_t stage = 16384u + (PAIR ? 128u : uint32_t(TN)) * 128u;
             // the ring of scales, two slots of 4 KiB per warp for the result, and room to align the stages
@@ -641,6 +692,7 @@ namespace htb
             if(cudaError_t e = ensureDynamicSmem((const void*)kernel, int(smem)))
                 return e;
             a.xRows                   = 128;
+            a.yRows                   = PAIR ? 128 : std::min(TN, (int(std::min<int64_t>(ea.cols, TN)) + 7) / 8 * 8); // no more than there are
             a.stageBytes              = uint32_t(a.stages) * stage;
             const int           csize = PAIR ? 2 : a.ksplit;
             cudaLaunchConfig_t  cfg{};
@@ -670,11 +722,13 @@ namespace htb
                                const ScaledArgs& ea, int smCount, cudaStream_t stream)
         {
             if(f.pair)
-                return ea.tma ? launchTensor<TD, true, 256, VECY, true>(mapX, mapY, a, ea, smCount, stream)
-                              : launchTensor<TD, true, 256, VECY, false>(mapX, mapY, a, ea, smCount, stream);
+                return !ea.tma ? launchTensor<TD, true, 256, VECY, false>(mapX, mapY, a, ea, smCount, stream)
+                       : ea.C  ? launchTensor<TD, true, 256, VECY, true, true>(mapX, mapY, a, ea, smCount, stream)
+                               : launchTensor<TD, true, 256, VECY, true>(mapX, mapY, a, ea, smCount, stream);
             if(f.tn == 128)
-                return ea.tma && f.ksplit == 1 ? launchTensor<TD, false, 128, VECY, true>(mapX, mapY, a, ea, smCount, stream)
-                              : launchTensor<TD, false, 128, VECY, false>(mapX, mapY, a, ea, smCount, stream);
+                return !ea.tma || f.ksplit > 1 ? launchTensor<TD, false, 128, VECY, false>(mapX, mapY, a, ea, smCount, stream)
+                       : ea.C                  ? launchTensor<TD, false, 128, VECY, true, true>(mapX, mapY, a, ea, smCount, stream)
+                                               : launchTensor<TD, false, 128, VECY, true>(mapX, mapY, a, ea, smCount, stream);
             if(f.tn == 64)
                 return launchTensor<TD, false, 64, VECY, false>(mapX, mapY, a, ea, smCount, stream);
             return launchTensor<TD, false, 32, VECY, false>(mapX, mapY, a, ea, smCount, stream);
@@ -690,10 +744,10 @@ namespace htb
             {
                 const ScaledForm f = formOf(p, sms);
                 CUtensorMap      mapX, mapY;
-                const int        rowsX = 128, rowsY = f.pair ? 128 : f.tn;
+                const int64_t    rows = f.swap ? p.N : p.M, cols = f.swap ? p.M : p.N, tileRows = f.pair ? 256 : 128;
+                const int        rowsX = 128, rowsY = f.pair ? 128 : std::min(f.tn, (int(std::min<int64_t>(cols, f.tn)) + 7) / 8 * 8);
                 const bool       ok = f.swap ? (encodeRows(encode, &mapX, B, p.K, p.N, p.bN, rowsX) && encodeRows(encode, &mapY, A, p.K, p.M, p.aM, rowsY))
                                              : (encodeRows(encode, &mapX, A, p.K, p.M, p.aM, rowsX) && encodeRows(encode, &mapY, B, p.K, p.N, p.bN, rowsY));
-                const int64_t    rows = f.swap ? p.N : p.M, cols = f.swap ? p.M : p.N, tileRows = f.pair ? 256 : 128;
                 const int64_t    tilesM = (rows + tileRows - 1) / tileRows, tilesN = (cols + f.tn - 1) / f.tn;
                 if(ok && tilesM * tilesN < (int64_t(1) << 30))
                 {
@@ -726,13 +780,12 @@ namespace htb
                     ea.alpha = alpha, ea.beta = beta;
                     const uintptr_t four = 4 * sizeof(TD);
                     ea.vec = (ea.dCol == 1 || cols == 1) && (rows == 1 || ea.dRow % 4 == 0) && uintptr_t(D) % four == 0 && uintptr_t(C) % four == 0;
-                    // bulk stores: the wide forms (a slot's row is 128 bytes of the result) and K splits, without C
+                    // bulk stores: the wide forms (a slot's row is 128 bytes of the result) and, without C, K splits
                     const int64_t size = int64_t(sizeof(TD)), ld = rows > 1 ? ea.dRow : (cols + 15) / 16 * 16;
                     const int boxCols = f.ksplit > 1 ? std::min(f.tn / f.ksplit, 32) : 0;
-                    ea.tma = (f.tn >= 128 || f.ksplit > 1) && !C && (ea.dCol == 1 || cols == 1) && ld * size % 16 == 0 && ld >= cols
-                             && ld < (int64_t(1) << 36) && (uintptr_t(D) & 15) == 0 && encodeResult(encode, &ea.mapD, p.typeD, D, cols, rows, ld * size, boxCols);
-                    if(!ea.tma)
-                        ea.mapD = mapX; // a valid map, not used
+                    ea.tma = (f.tn >= 128 || f.ksplit > 1) && (!C || f.ksplit == 1) && (ea.dCol == 1 || cols == 1) && ld * size % 16 == 0 && ld >= cols
+                             && ld < (int64_t(1) << 36) && ((uintptr_t(D) | uintptr_t(C)) & 15) == 0 && encodeResult(encode, &ea.mapD, p.typeD, D, cols, rows, ld * size, boxCols)
+                             && (!C || encodeResult(encode, &ea.mapC, p.typeD, const_cast<void*>(C), cols, rows, ld * size, 0));
                     return ea.blockY > 1 ? launchForm<TD, false>(f, mapX, mapY, a, ea, sms, stream)
                                          : launchForm<TD, true>(f, mapX, mapY, a, ea, sms, stream);
                 }

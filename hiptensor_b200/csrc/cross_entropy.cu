@@ -313,7 +313,7 @@ namespace htb
             static constexpr int ROOM  = 0; // shared memory behind the stages
             const Args&          a;
 
-            __device__ LossEpi(const Args& args, int, int, unsigned char*)
+            __device__ LossEpi(const Args& args, int, int, unsigned char*, volatile int*)
                 : a(args)
             {
             }
@@ -384,7 +384,7 @@ namespace htb
             const uint32_t       slot;
             int                  stores;
 
-            __device__ ProbabilityEpi(const Args& args, int w, int l, unsigned char* smem)
+            __device__ ProbabilityEpi(const Args& args, int w, int l, unsigned char* smem, volatile int*)
                 : a(args)
                 , lane(l)
                 , slot(smemAddr(smem) + uint32_t(w * SLOTS * 4096))
@@ -506,7 +506,7 @@ namespace htb
             const uint32_t        slot;
             int                   stores;
 
-            __device__ WeightEpi(const Args& args, int w, int l, unsigned char* smem)
+            __device__ WeightEpi(const Args& args, int w, int l, unsigned char* smem, volatile int*)
                 : a(args)
                 , lane(l)
                 , slot(smemAddr(smem) + uint32_t(w * SLOTS * 4096))
@@ -596,7 +596,7 @@ namespace htb
             const int             lane;
             const uint32_t        slot;
 
-            __device__ HiddenEpi(const Args& args, int w, int l, unsigned char* smem)
+            __device__ HiddenEpi(const Args& args, int w, int l, unsigned char* smem, volatile int*)
                 : a(args)
                 , lane(l)
                 , slot(smemAddr(smem) + uint32_t(w * SLOTS * 4096))
@@ -765,6 +765,7 @@ namespace htb
             a.chunk      = 16;
             a.kElems     = 64;
             a.xRows      = xRows;
+            a.yRows      = 256;
             a.ksplit     = 1;
             a.kParts     = 1;
             // Waits and commits between MMAs cost the issuing thread several hundred cycles: two K blocks a stage (1024 cycles

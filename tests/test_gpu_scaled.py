@@ -175,9 +175,10 @@ def test_scaled_blocks_and_orders_of_the_result(h, m, n, k, rowA, rowB, colD):
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("m,n,k", [(7, 260, 520), (520, 777, 300), (40, 50, 0)])
-def test_scaled_alpha_beta(h, m, n, k, out):
-    run_scaled(h, m, n, k, out=out, alpha=-0.75, beta=1.5)
+@pytest.mark.parametrize("m,n,k", [(7, 260, 520), (520, 777, 300), (40, 50, 0), (700, 768, 130), (100, 200, 2048), (2100, 2056, 400)])
+@pytest.mark.parametrize("rowB", [False, True])
+def test_scaled_alpha_beta(h, m, n, k, out, rowB):
+    run_scaled(h, m, n, k, out=out, alpha=-0.75, beta=1.5, rowB=rowB)
 
 
 @pytest.mark.parametrize("layoutA,layoutB", [("odd", "k"), ("k", "odd"), ("m", "k"), ("k", "m"), ("m", "m"), ("odd", "odd")])
@@ -186,10 +187,11 @@ def test_scaled_layouts(h, m, n, k, layoutA, layoutB):
     run_scaled(h, m, n, k, layoutA=layoutA, layoutB=layoutB, rowB=True, out=torch.float32)
 
 
-def test_scaled_in_place_accumulation_and_repeat(h):
-    A, B = operand(300, 1024, torch.float8_e5m2, 1), operand(400, 1024, torch.float8_e4m3fn, 2)
-    sA, sB = torch.rand(300, 8, device="cuda"), torch.rand(400, 8, device="cuda")
-    D = torch.randn(300, 400, device="cuda")
+@pytest.mark.parametrize("m,n", [(300, 400), (2304, 2300)])
+def test_scaled_in_place_accumulation_and_repeat(h, m, n):
+    A, B = operand(m, 1024, torch.float8_e5m2, 1), operand(n, 1024, torch.float8_e4m3fn, 2)
+    sA, sB = torch.rand(m, 8, device="cuda"), torch.rand(n, 8, device="cuda")
+    D = torch.randn(m, n, device="cuda")
     C, dD = D.clone(), desc(h, D)
     plan = h.scaled_contraction_plan(desc(h, A), (0, 2), desc(h, sA), (1, 128), desc(h, B), (1, 2), desc(h, sB), (1, 128), dD, dD, (0, 1))
     h.scaled_contraction(plan, 0.5, A, sA, B, sB, 1.0, D, D)  # C is D
