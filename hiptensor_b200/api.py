@@ -73,6 +73,15 @@ def _ptr(x):
     return ctypes.c_void_p(int(x.data_ptr()))
 
 
+def _addr(x):
+    # as _ptr, for the argument types that take a plain number (a call of a few microseconds notices the difference)
+    return x if x is None or isinstance(x, int) else x.data_ptr()
+
+
+def _stream_addr(stream):
+    return stream if stream is None or isinstance(stream, int) else stream.cuda_stream
+
+
 def _f32_to_bf16_bits(v):
     u = struct.unpack("<I", struct.pack("<f", float(v)))[0]
     return ((u + 0x7FFF + ((u >> 16) & 1)) >> 16) & 0xFFFF
@@ -272,8 +281,8 @@ class Handle:
         """htBlockQuantize: Q[modeQ] (e4m3 / e5m2) and the f32 scales S of A[modeA]; blockA: 1 or 128 for each mode of A. S
         has A's modes with extents ceil(extent / block)."""
         self._same_rank("htBlockQuantize", (descA, modeA, blockA), (descQ, modeQ), (descS, modeA))
-        _check(self._L.htBlockQuantize(self._h, _ptr(A), descA._p, _lib.i32(modeA), _lib.u32(blockA), _ptr(Q), descQ._p,
-                                       _lib.i32(modeQ), _ptr(S), descS._p, _stream_ptr(stream)), "htBlockQuantize")
+        _check(self._L.htBlockQuantize(self._h, _addr(A), descA._p, _lib.i32(modeA), _lib.u32(blockA), _addr(Q), descQ._p,
+                                       _lib.i32(modeQ), _addr(S), descS._p, _stream_addr(stream)), "htBlockQuantize")
 
     def scaled_contraction_plan(self, descA, modeA, descScaleA, blockA, descB, modeB, descScaleB, blockB, descC, descD, modeD,
                                 type_compute=COMPUTE_32F):
@@ -289,9 +298,9 @@ class Handle:
 
     def scaled_contraction(self, plan, alpha, A, scaleA, B, scaleB, beta, C, D, stream=None):
         """htScaledContraction: D = alpha * (A scaleA) (B scaleB) + beta * C."""
-        _check(self._L.htScaledContraction(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _ptr(A), _ptr(scaleA), _ptr(B),
-                                           _ptr(scaleB), ctypes.byref(ctypes.c_float(beta)), _ptr(C), _ptr(D),
-                                           _stream_ptr(stream)), "htScaledContraction")
+        _check(self._L.htScaledContraction(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _addr(A), _addr(scaleA), _addr(B),
+                                           _addr(scaleB), ctypes.byref(ctypes.c_float(beta)), _addr(C), _addr(D),
+                                           _stream_addr(stream)), "htScaledContraction")
 
     # ---- softmax cross entropy of a linear head, logits not kept ----
 
@@ -311,22 +320,24 @@ class Handle:
 
     def cross_entropy(self, plan, alpha, H, W, targets, loss, lse, workspace, workspace_size, stream=None):
         """htCrossEntropy: loss (0 for ignored tokens) and lse, f32, one for each token; targets int64."""
-        _check(self._L.htCrossEntropy(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _ptr(H), _ptr(W), _ptr(targets),
-                                      _ptr(loss), _ptr(lse), _ptr(workspace), int(workspace_size), _stream_ptr(stream)),
+        _check(self._L.htCrossEntropy(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _addr(H), _addr(W), _addr(targets),
+                                      _addr(loss), _addr(lse), _addr(workspace), int(workspace_size), _stream_addr(stream)),
                "htCrossEntropy")
 
     def cross_entropy_gradient(self, plan, alpha, H, W, targets, lse, grad_loss, dH, dW, workspace, workspace_size, stream=None):
         """htCrossEntropyGradient: dH (like H) and dW (like W), either may be None; lse from cross_entropy."""
-        _check(self._L.htCrossEntropyGradient(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _ptr(H), _ptr(W),
-                                              _ptr(targets), _ptr(lse), _ptr(grad_loss), _ptr(dH), _ptr(dW), _ptr(workspace),
-                                              int(workspace_size), _stream_ptr(stream)), "htCrossEntropyGradient")
+        _check(self._L.htCrossEntropyGradient(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _addr(H), _addr(W),
+                                              _addr(targets), _addr(lse), _addr(grad_loss), _addr(dH), _addr(dW), _addr(workspace),
+                                              int(workspace_size), _stream_addr(stream)), "htCrossEntropyGradient")
 
     @staticmethod
     def _same_rank(where, *groups):
         # the library reads one mode (and one block) for each mode of the descriptor
         for desc, *lists in groups:
-            if any(len(x) != len(desc.lens) for x in lists):
-                raise HiptensorError(STATUS_INVALID_VALUE, where)
+            rank = len(desc.lens)
+            for x in lists:
+                if len(x) != rank:
+                    raise HiptensorError(STATUS_INVALID_VALUE, where)
 
 
 def last_kernel_name():

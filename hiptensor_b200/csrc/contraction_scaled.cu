@@ -62,67 +62,67 @@ namespace htb
             const int64_t    m0 = int64_t(blockIdx.x) * 64;
             for(int64_t n0 = int64_t(blockIdx.y) * 64; n0 < p.N; n0 += int64_t(gridDim.y) * 64)
             {
-            float            sum[4][4] = {};
-            for(int64_t k0 = 0; k0 < p.K; k0 += kScaleBlock)
-            {
-                float part[4][4] = {};
-                for(int64_t k1 = k0; k1 < min(k0 + kScaleBlock, p.K); k1 += kStep)
+                float            sum[4][4] = {};
+                for(int64_t k0 = 0; k0 < p.K; k0 += kScaleBlock)
                 {
-                    for(int i = threadIdx.x; i < 64 * kStep; i += 256)
+                    float part[4][4] = {};
+                    for(int64_t k1 = k0; k1 < min(k0 + kScaleBlock, p.K); k1 += kStep)
                     {
-                        // neighbouring threads along the contiguous mode
-                        const int     ra = p.aK == 1 ? i / kStep : i % 64, ka = p.aK == 1 ? i % kStep : i / 64;
-                        const int     rb = p.bK == 1 ? i / kStep : i % 64, kb = p.bK == 1 ? i % kStep : i / 64;
-                        const int64_t m = m0 + ra, n = n0 + rb;
-                        a[ka][ra] = (m < p.M && k1 + ka < p.K) ? widen8(A[m * p.aM + (k1 + ka) * p.aK], aWide) : 0.f;
-                        b[kb][rb] = (n < p.N && k1 + kb < p.K) ? widen8(B[n * p.bN + (k1 + kb) * p.bK], bWide) : 0.f;
-                    }
-                    __syncthreads();
-#pragma unroll 8
-                    for(int k = 0; k < kStep; k++)
-                    {
-                        float x[4], y[4];
-#pragma unroll
-                        for(int i = 0; i < 4; i++)
+                        for(int i = threadIdx.x; i < 64 * kStep; i += 256)
                         {
-                            x[i] = a[k][ty + 16 * i];
-                            y[i] = b[k][tx + 16 * i];
+                            // neighbouring threads along the contiguous mode
+                            const int     ra = p.aK == 1 ? i / kStep : i % 64, ka = p.aK == 1 ? i % kStep : i / 64;
+                            const int     rb = p.bK == 1 ? i / kStep : i % 64, kb = p.bK == 1 ? i % kStep : i / 64;
+                            const int64_t m = m0 + ra, n = n0 + rb;
+                            a[ka][ra] = (m < p.M && k1 + ka < p.K) ? widen8(A[m * p.aM + (k1 + ka) * p.aK], aWide) : 0.f;
+                            b[kb][rb] = (n < p.N && k1 + kb < p.K) ? widen8(B[n * p.bN + (k1 + kb) * p.bK], bWide) : 0.f;
                         }
+                        __syncthreads();
+#pragma unroll 8
+                        for(int k = 0; k < kStep; k++)
+                        {
+                            float x[4], y[4];
 #pragma unroll
-                        for(int i = 0; i < 4; i++)
+                            for(int i = 0; i < 4; i++)
+                            {
+                                x[i] = a[k][ty + 16 * i];
+                                y[i] = b[k][tx + 16 * i];
+                            }
 #pragma unroll
-                            for(int j = 0; j < 4; j++)
-                                part[i][j] = fmaf(x[i], y[j], part[i][j]);
+                            for(int i = 0; i < 4; i++)
+#pragma unroll
+                                for(int j = 0; j < 4; j++)
+                                    part[i][j] = fmaf(x[i], y[j], part[i][j]);
+                        }
+                        __syncthreads();
                     }
-                    __syncthreads();
-                }
-                const int64_t kb = k0 / kScaleBlock;
-                float         x[4], y[4];
+                    const int64_t kb = k0 / kScaleBlock;
+                    float         x[4], y[4];
 #pragma unroll
-                for(int i = 0; i < 4; i++)
-                {
-                    const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * i;
-                    x[i] = m < p.M ? sA[(m / p.blockM) * p.saM + kb * p.saK] : 0.f;
-                    y[i] = n < p.N ? sB[(n / p.blockN) * p.sbN + kb * p.sbK] : 0.f;
+                    for(int i = 0; i < 4; i++)
+                    {
+                        const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * i;
+                        x[i] = m < p.M ? sA[(m / p.blockM) * p.saM + kb * p.saK] : 0.f;
+                        y[i] = n < p.N ? sB[(n / p.blockN) * p.sbN + kb * p.sbK] : 0.f;
+                    }
+#pragma unroll
+                    for(int i = 0; i < 4; i++)
+#pragma unroll
+                        for(int j = 0; j < 4; j++)
+                            sum[i][j] = fmaf(part[i][j], x[i] * y[j], sum[i][j]);
                 }
 #pragma unroll
                 for(int i = 0; i < 4; i++)
 #pragma unroll
                     for(int j = 0; j < 4; j++)
-                        sum[i][j] = fmaf(part[i][j] * x[i], y[j], sum[i][j]);
-            }
-#pragma unroll
-            for(int i = 0; i < 4; i++)
-#pragma unroll
-                for(int j = 0; j < 4; j++)
-                {
-                    const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-                    if(m >= p.M || n >= p.N)
-                        continue;
-                    const int64_t at = m * p.dM + n * p.dN;
-                    const float   v  = alpha * sum[i][j];
-                    D[at]            = narrow<TD>(C ? fmaf(beta, widen(C[at]), v) : v);
-                }
+                    {
+                        const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
+                        if(m >= p.M || n >= p.N)
+                            continue;
+                        const int64_t at = m * p.dM + n * p.dN;
+                        const float   v  = alpha * sum[i][j];
+                        D[at]            = narrow<TD>(C ? fmaf(beta, widen(C[at]), v) : v);
+                    }
             }
         }
 

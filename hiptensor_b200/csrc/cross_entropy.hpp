@@ -20,6 +20,7 @@ namespace htb
         int     nt;
         int64_t tExt[kMaxGroup], tStride[kMaxGroup];
         int64_t hD, wV, wD; // strides in elements
+        int     parts; // of dH's products (hiddenParts for the whole vocabulary)
         int64_t ignore;
     };
 

@@ -147,8 +147,8 @@ int htBlockQuantize(const htHandle* handle, const void* A, const htTensorDescrip
 /* D[modeD] = alpha * sum over the contracted mode of (A * scaleA) (B * scaleB), + beta * C. A and B are e4m3 or e5m2 (each
  * its own), D is f32, f16 or bf16, C (descC == NULL: none) is described as D is. descScaleA / blockA and descScaleB /
  * blockB are those of htBlockQuantize for A's and B's modes. One mode is contracted, with block 128 in both operands; the
- * free modes of an operand fold into one mode, of block 1 or 128. Each block's products are summed in f32, multiplied by the two
- * scales (one after the other, so that only the result has to be in f32's range), and summed in f32 over the blocks.
+ * free modes of an operand fold into one mode, of block 1 or 128. Each block's products are summed in f32, multiplied by the
+ * product of the two scales (an f32 number, which has to be in range), and summed in f32 over the blocks.
  * typeCompute: 4 (f32); alpha and beta point to floats. A mode in A, B and D is not supported (15), as in htContraction. No
  * workspace is needed, and a plan may be used by several calls and streams at once. Operands that are contiguous along the
  * contracted mode, with rows at multiples of 16 bytes, run on the tensor cores; any other strides on FMA. */
@@ -174,7 +174,9 @@ int htScaledContraction(const htHandle* handle, const htScaledContractionPlan* p
  * htCrossEntropyGradient takes lse as htCrossEntropy wrote it; dH or dW may be NULL (not wanted). Rows of H whose target is
  * ignored take no part in the gradient, whatever they hold. A target that is neither a class nor ignoreIndex reads
  * nothing out of range: its loss is NaN, its row of P zero, and the next call on the handle returns 13
- * (EXECUTION_FAILED) once. P is rounded to the type of H (f16: scaled by a power of two for max |gradLoss * alpha|), sums are f32.
+ * (EXECUTION_FAILED) once. P is rounded to the type of H (f16: scaled by a power of two for max |gradLoss * alpha|; up to 64
+ * tokens it is a sum of two such numbers), sums are f32. f32 tensors are multiplied as sums of three bf16 numbers, which is
+ * f32's own accuracy; an infinity among them makes NaN of the logits it takes part in.
  *
  * The workspace holds the pieces: any size from htCrossEntropyGetWorkspaceSize's MIN on (19 below it); with more, pieces
  * are larger and fewer. gradient: 0 for htCrossEntropy, 1 for htCrossEntropyGradient. Two calls that run at the same time (two
