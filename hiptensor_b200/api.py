@@ -7,6 +7,7 @@ Every non-zero status raises HiptensorError.
 """
 import ctypes
 import struct
+import sys
 
 from . import _lib
 
@@ -71,11 +72,6 @@ def _ptr(x):
     if isinstance(x, int):
         return ctypes.c_void_p(x)
     return ctypes.c_void_p(int(x.data_ptr()))
-
-
-def _addr(x):
-    # as _ptr, for the argument types that take a plain number (a call of a few microseconds notices the difference)
-    return x if x is None or isinstance(x, int) else x.data_ptr()
 
 
 def _stream_addr(stream):
@@ -146,11 +142,16 @@ class _Owned:
 class Handle:
     """hiptensorHandle_t bound to the CUDA device current at construction (hiptensorCreate)."""
 
+    _device = None  # of the handle, where torch is there to tell
+
     def __init__(self):
         self._L = _lib.lib()
         h = ctypes.c_void_p(0)
         _check(self._L.htCreate(ctypes.byref(h)), "hiptensorCreate")
         self._h = h
+        torch = sys.modules.get("torch")
+        if torch is not None:
+            self._device = torch.cuda.current_device()
 
     def destroy(self):
         if self._h:
@@ -281,8 +282,8 @@ class Handle:
         """htBlockQuantize: Q[modeQ] (e4m3 / e5m2) and the f32 scales S of A[modeA]; blockA: 1 or 128 for each mode of A. S
         has A's modes with extents ceil(extent / block)."""
         self._same_rank("htBlockQuantize", (descA, modeA, blockA), (descQ, modeQ), (descS, modeA))
-        _check(self._L.htBlockQuantize(self._h, _addr(A), descA._p, _lib.i32(modeA), _lib.u32(blockA), _addr(Q), descQ._p,
-                                       _lib.i32(modeQ), _addr(S), descS._p, _stream_addr(stream)), "htBlockQuantize")
+        _check(self._L.htBlockQuantize(self._h, self._addr(A), descA._p, _lib.i32(modeA), _lib.u32(blockA), self._addr(Q), descQ._p,
+                                       _lib.i32(modeQ), self._addr(S), descS._p, _stream_addr(stream)), "htBlockQuantize")
 
     def scaled_contraction_plan(self, descA, modeA, descScaleA, blockA, descB, modeB, descScaleB, blockB, descC, descD, modeD,
                                 type_compute=COMPUTE_32F):
@@ -298,8 +299,8 @@ class Handle:
 
     def scaled_contraction(self, plan, alpha, A, scaleA, B, scaleB, beta, C, D, stream=None):
         """htScaledContraction: D = alpha * (A scaleA) (B scaleB) + beta * C."""
-        _check(self._L.htScaledContraction(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _addr(A), _addr(scaleA), _addr(B),
-                                           _addr(scaleB), ctypes.byref(ctypes.c_float(beta)), _addr(C), _addr(D),
+        _check(self._L.htScaledContraction(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), self._addr(A), self._addr(scaleA), self._addr(B),
+                                           self._addr(scaleB), ctypes.byref(ctypes.c_float(beta)), self._addr(C), self._addr(D),
                                            _stream_addr(stream)), "htScaledContraction")
 
     # ---- softmax cross entropy of a linear head, logits not kept ----
@@ -320,15 +321,23 @@ class Handle:
 
     def cross_entropy(self, plan, alpha, H, W, targets, loss, lse, workspace, workspace_size, stream=None):
         """htCrossEntropy: loss (0 for ignored tokens) and lse, f32, one for each token; targets int64."""
-        _check(self._L.htCrossEntropy(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _addr(H), _addr(W), _addr(targets),
-                                      _addr(loss), _addr(lse), _addr(workspace), int(workspace_size), _stream_addr(stream)),
+        _check(self._L.htCrossEntropy(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), self._addr(H), self._addr(W), self._addr(targets),
+                                      self._addr(loss), self._addr(lse), self._addr(workspace), int(workspace_size), _stream_addr(stream)),
                "htCrossEntropy")
 
     def cross_entropy_gradient(self, plan, alpha, H, W, targets, lse, grad_loss, dH, dW, workspace, workspace_size, stream=None):
         """htCrossEntropyGradient: dH (like H) and dW (like W), either may be None; lse from cross_entropy."""
-        _check(self._L.htCrossEntropyGradient(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), _addr(H), _addr(W),
-                                              _addr(targets), _addr(lse), _addr(grad_loss), _addr(dH), _addr(dW), _addr(workspace),
+        _check(self._L.htCrossEntropyGradient(self._h, plan._p, ctypes.byref(ctypes.c_float(alpha)), self._addr(H), self._addr(W),
+                                              self._addr(targets), self._addr(lse), self._addr(grad_loss), self._addr(dH), self._addr(dW), self._addr(workspace),
                                               int(workspace_size), _stream_addr(stream)), "htCrossEntropyGradient")
+
+    def _addr(self, x):
+        """A tensor's (or a plain) address; a tensor that is not on the handle's device is refused."""
+        if x is None or isinstance(x, int):
+            return x
+        if x.get_device() != self._device and (self._device is not None or x.get_device() < 0):
+            raise HiptensorError(STATUS_ARCH_MISMATCH, "a tensor on another device than the handle's")
+        return x.data_ptr()
 
     @staticmethod
     def _same_rank(where, *groups):

@@ -740,7 +740,9 @@ namespace htb
         {
             const int sms = smCount > 0 ? smCount : 148;
             PFN_encodeTiled encode = tensorMapEncoder();
-            if(encode && p.K > 0 && rowsForTma(A, p.K, p.M, p.aK, p.aM) && rowsForTma(B, p.K, p.N, p.bK, p.bN))
+            // (a fold of modes may have more rows than a tensor map's coordinates reach)
+            const int64_t most = (int64_t(1) << 31) - 512;
+            if(encode && p.K > 0 && p.M < most && p.N < most && rowsForTma(A, p.K, p.M, p.aK, p.aM) && rowsForTma(B, p.K, p.N, p.bK, p.bN))
             {
                 const ScaledForm f = formOf(p, sms);
                 CUtensorMap      mapX, mapY;

@@ -400,7 +400,7 @@ namespace htb
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
                 int64_t target = -1;
-                float   l = 0.f, f = 0.f;
+                float   lse = 0.f, f = 0.f;
                 bool    live = false;
                 if(row < a.T)
                 {
@@ -408,19 +408,32 @@ namespace htb
                     live   = counts(target, a.ignore, a.V);
                     if(live)
                     {
-                        l = a.lse[row] * kLog2e;
+                        lse = a.lse[row];
                         f = a.g[row] * a.alpha * (a.scale ? a.scale[0] : 1.f);
                     }
                 }
                 const float    c  = a.alpha * kLog2e;
+                const float    l  = lse * kLog2e;
                 const uint64_t c2 = pack2(c, c), l2 = pack2(-l, -l);
                 const int      t  = live && target - a.v0 - col >= 0 && target - a.v0 - col < COLS ? int(target - a.v0 - col) : -1;
                 // P takes the sums' place
 #pragma unroll
                 for(int i = 0; i < COLS / 2; i++)
                 {
-                    const float2 x  = unpack2(fma2(acc[i], c2, l2));
-                    float        p0 = exp2f(x.x), p1 = exp2f(x.y);
+                    float p0, p1;
+                    if constexpr(PARTS == 3)
+                    {
+                        // f32: an exponent of 15 in powers of two is rounded by 2^-20, which would be P's largest error
+                        const float2 z = unpack2(acc[i]);
+                        p0 = expf(fmaf(z.x, a.alpha, -lse));
+                        p1 = expf(fmaf(z.y, a.alpha, -lse));
+                    }
+                    else
+                    {
+                        const float2 x = unpack2(fma2(acc[i], c2, l2));
+                        p0 = exp2f(x.x);
+                        p1 = exp2f(x.y);
+                    }
                     if(t == 2 * i)
                         p0 -= 1.f;
                     if(t == 2 * i + 1)
@@ -742,6 +755,8 @@ namespace htb
                     a.segY |= uint32_t(y) << (4 * pairs);
                     pairs++;
                 }
+            if(nx > 1 && ny > 1)
+                a.chunk = 4; // f32's accuracy: shorter truncated sums
             a.segBlocks = kBlocksOfOne;
             a.kBlocks   = pairs * kBlocksOfOne;
         }

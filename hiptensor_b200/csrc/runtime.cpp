@@ -181,7 +181,7 @@ namespace htb
             int         bytes[kMaxDevices];
         };
         static std::mutex mutex;
-        static Entry      table[64];
+        static Entry      table[256];
         static int        used = 0;
         int               dev  = 0;
         if(cudaGetDevice(&dev) != cudaSuccess)
@@ -191,7 +191,7 @@ namespace htb
         for(int i = 0; i < used && !e; i++)
             if(table[i].fn == kernel)
                 e = &table[i];
-        if(!e && used < 64)
+        if(!e && used < 256)
         {
             e     = &table[used++];
             e->fn = kernel;

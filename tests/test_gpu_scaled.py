@@ -269,3 +269,6 @@ def test_a_wrong_pointer_is_refused(h):
         with pytest.raises(ht.HiptensorError) as e:
             h.scaled_contraction(plan, 1.0, *args)
         assert e.value.status == ht.STATUS_INVALID_VALUE
+    with pytest.raises(ht.HiptensorError) as e:
+        h.scaled_contraction(plan, 1.0, A.cpu(), s, B, s, 1.0, D, D)
+    assert e.value.status == ht.STATUS_ARCH_MISMATCH
