@@ -55,7 +55,8 @@ namespace htb
             const int partsP = gradient ? probabilityParts(p.type, p.T) : 1;
             // segments of tokens are contracted in blocks of 64: zeros up to there
             l.rowsT = l.segments > 1 || partsP > 1 ? roundUp(p.T, 64) : p.T;
-            l.parts = gradient ? int(std::max<int64_t>(1, std::min<int64_t>(p.parts, piece / 1024))) : 1;
+            const int pairs = f32 ? 6 : 1;
+            l.parts         = gradient ? int(std::max<int64_t>(1, std::min<int64_t>(p.parts, piece * pairs / 1024))) : 1;
             uint64_t at   = 0;
             auto     take = [&](bool wanted, uint64_t bytes) {
                 const uint64_t here = at;
@@ -222,7 +223,7 @@ namespace htb
             p.T = 0;
         if(p.V >= (int64_t(1) << 31) - 512 || p.T >= (int64_t(1) << 31) - 512 || p.D > (int64_t(1) << 26))
             return HIPTENSOR_STATUS_NOT_SUPPORTED;
-        p.parts = p.T > 0 ? hiddenParts(p.T, p.D, p.V) : 1;
+        p.parts = p.T > 0 ? hiddenParts(p.T, p.D, p.V * (type == CUDA_R_32F ? 6 : 1)) : 1;
         *out    = p;
         return HIPTENSOR_STATUS_SUCCESS;
     }

@@ -937,7 +937,8 @@ namespace htb
 
     // How many parts of the classes dH's products run in, side by side: the tiles of [T, D] alone would leave SMs idle when
     // there are few, or in their last round when there are some. A round of tiles over n classes takes about n x 5.9 ns
-    // (measured rate of a pair), a part more T x D x 8 bytes of traffic; a part has at least 1024 classes.
+    // (measured rate of a pair), a part more T x D x 8 bytes of traffic; a part's sums have at least 1024 terms. `piece`: classes
+    // times the products that an element's product is made of.
     int hiddenParts(int64_t T, int64_t D, int64_t piece)
     {
         const bool    single = T <= 128;
