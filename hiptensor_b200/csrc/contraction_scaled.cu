@@ -147,7 +147,7 @@ namespace htb
             void*        D;
             int64_t      dRow, dCol;
             float        alpha, beta;
-            int          vec; // columns contiguous, groups of four aligned
+            int          vec; // columns contiguous
             int          tma; // the result goes out as bulk tensor stores (no C; rows at multiples of 16 bytes)
             CUtensorMap  mapD, mapC;
         };
@@ -355,54 +355,48 @@ namespace htb
                     if(col0 + j < a.cols)
                         static_cast<TD*>(a.D)[at] = finish(a, w[j], at);
             }
-            // The same through shared memory when the columns are contiguous, so that lanes that follow each other write (and
-            // read C) along a row. Out of line: unrolled over a tile it was 64 KiB of code, fetched anew for every tile.
+            // The same through shared memory when the columns are contiguous: lanes that follow each other write (and read C)
+            // along a row, one element each, so that any row stride and start will do (rows of odd length: 4096 x 4097 x 4096
+            // in bf16 takes 119 us, 260 with every lane on a row of its own; 85 by bulk stores
+            // when N is 4096). Eight rows' worth of C is read ahead of their stores.
             template <int W>
-            static __device__ __noinline__ void store(const Args& a, float* slot, int lane, const float (&w)[W], int64_t row, int64_t col0)
+            __device__ __forceinline__ void store(const float (&w)[W], int64_t row, int64_t col0)
             {
-                TD* D = static_cast<TD*>(a.D);
-                constexpr int U = W / 4; // 16-byte units of a row, XORed with the row against bank conflicts
+                constexpr int U = W / 4, STEP = 32 / W; // 16-byte units of a row, XORed with the row against bank conflicts; rows at a time
                 __syncwarp(); // the round before has been read
 #pragma unroll
                 for(int u = 0; u < U; u++)
                     *reinterpret_cast<float4*>(slot + lane * W + ((u ^ (lane & (U - 1))) << 2))
                         = make_float4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
                 __syncwarp();
-                const int64_t row0 = row - lane;
-                const int     u = lane % U;
-                const int64_t c = col0 + 4 * u;
+                const int     j = lane % W, first = lane / W;
+                const int64_t row0 = row - lane, c = col0 + j;
+                const int     rows = int(min(int64_t(32), a.rows - row0)); // may be negative
+                if(c >= a.cols)
+                    return;
+                int64_t at = (row0 + first) * a.dRow + c;
+                TD*     D  = static_cast<TD*>(a.D);
 #pragma unroll 1
-                for(int i = 0; i < U; i++)
+                for(int r = first; r < rows; r += 8 * STEP)
                 {
-                    const int     rr = i * (32 / U) + lane / U;
-                    const float4  q  = *reinterpret_cast<const float4*>(slot + rr * W + ((u ^ (rr & (U - 1))) << 2));
-                    const int64_t at = (row0 + rr) * a.dRow + c;
-                    if(row0 + rr >= a.rows || c >= a.cols)
-                        continue;
-                    const float f[4] = {q.x, q.y, q.z, q.w};
-                    if(c + 4 <= a.cols)
+                    TD in[8];
+                    if(a.C)
                     {
-                        struct alignas(4 * sizeof(TD)) Four
-                        {
-                            TD e[4];
-                        };
-                        Four o, in;
-                        if(a.C)
-                            in = *reinterpret_cast<const Four*>(static_cast<const TD*>(a.C) + at);
 #pragma unroll
-                        for(int j = 0; j < 4; j++)
-                        {
-                            const float v = f[j] * a.alpha;
-                            o.e[j]        = narrow<TD>(a.C ? fmaf(a.beta, widen(in.e[j]), v) : v);
-                        }
-                        *reinterpret_cast<Four*>(D + at) = o;
+                        for(int i = 0; i < 8; i++)
+                            if(r + i * STEP < rows)
+                                in[i] = static_cast<const TD*>(a.C)[at + i * STEP * a.dRow];
                     }
-                    else
-                    {
 #pragma unroll
-                        for(int j = 0; j < 4; j++)
-                            if(c + j < a.cols)
-                                D[at + j] = finish(a, f[j], at + j);
+                    for(int i = 0; i < 8; i++)
+                    {
+                        const int rr = r + i * STEP;
+                        if(rr < rows)
+                        {
+                            const float v = slot[rr * W + ((((j >> 2) ^ (rr & (U - 1))) << 2) | (j & 3))] * a.alpha;
+                            D[at]         = narrow<TD>(a.C ? fmaf(a.beta, widen(in[i]), v) : v);
+                        }
+                        at += STEP * a.dRow;
                     }
                 }
             }
@@ -501,7 +495,7 @@ namespace htb
                         if(!a.vec)
                             storeDirect<CH>(w, row, col + c);
                         else
-                            store<CH>(a, slot, lane, w, row, col + c);
+                            store<CH>(w, row, col + c);
                     }
                 }
             }
@@ -604,7 +598,7 @@ namespace htb
                         else if(a.tma)
                             bulkBlock<W>(w, r, col);
                         else
-                            store<W>(a, slot, lane, w, r, col);
+                            store<W>(w, r, col);
                     }
                 }
             }
@@ -789,8 +783,7 @@ namespace htb
                     ea.C = C, ea.D = D;
                     ea.dRow = f.swap ? p.dN : p.dM, ea.dCol = f.swap ? p.dM : p.dN;
                     ea.alpha = alpha, ea.beta = beta;
-                    const uintptr_t four = 4 * sizeof(TD);
-                    ea.vec = (ea.dCol == 1 || cols == 1) && (rows == 1 || ea.dRow % 4 == 0) && uintptr_t(D) % four == 0 && uintptr_t(C) % four == 0;
+                    ea.vec = ea.dCol == 1 || cols == 1;
                     // bulk stores: the wide forms (a slot's row is 128 bytes of the result) and, without C, K splits
                     const int64_t size = int64_t(sizeof(TD)), ld = rows > 1 ? ea.dRow : (cols + 15) / 16 * 16;
                     const int boxCols = f.ksplit > 1 ? std::min(f.tn / f.ksplit, 32) : 0;
