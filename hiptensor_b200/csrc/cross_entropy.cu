@@ -682,7 +682,8 @@ namespace htb
             float             m = -INFINITY, s = 0.f;
             auto              join = [](float& m, float& s, float m2, float s2) {
                 const float top = maxNan(m, m2), ref = reference(top);
-                s = s * exp2f(reference(m) - ref) + s2 * exp2f(reference(m2) - ref);
+                // nothing yet, or nothing above -infinity: not 0 * exp2(0 - ref), which is NaN below ref = -128
+                s = (m == -INFINITY ? 0.f : s * exp2f(reference(m) - ref)) + (m2 == -INFINITY ? 0.f : s2 * exp2f(reference(m2) - ref));
                 m = top;
             };
             if(t < T)

@@ -176,6 +176,19 @@ def test_alpha_and_large_logits(h, kind, alpha):
     c.check_gradient()
 
 
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("t,v", [(1, 40), (3, 700), (40, 700), (300, 9000)])
+def test_every_logit_far_from_zero(h, t, v, sign, kind):
+    """Logits of about 130 to 2000, all of one sign: nothing is taken relative to zero."""
+    H, W, y, gl = inputs(t, v, 64, kind)
+    c = Call(h, (H.abs() + 1) * sign, W.abs() * 8 + 2, y, gl)
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+
+
 def test_infinite_logits(h):
     H, W, y, gl = inputs(40, 600, 64, torch.bfloat16, ignored=0)
     H[:], y[:] = H.abs() + 0.1, 5

@@ -96,7 +96,9 @@ def gradient(h, w, targets, lse, g, alpha, ignore):
     eP = f.abs() * p * (dz + 2.0 ** -21 + 2.0 ** -22 * x.abs()) + P.abs() * (round_p + 2.0 ** -22)
     if kind == torch.float16:
         eP = eP + f.abs().max() * 2.0 ** -38
-    elif kind == torch.bfloat16:
+    else:
+        # the smallest step of a bf16 number is 2^-133: a P rounded to one is off by at most half of it, an f32 P as a sum of
+        # bf16 numbers by at most half of it in its last one, and another half where the product reads them
         eP = eP + 2.0 ** -133
 
     def product(P, eP, y, n):
