@@ -785,9 +785,10 @@ namespace htb
                     ea.alpha = alpha, ea.beta = beta;
                     ea.vec = ea.dCol == 1 || cols == 1;
                     // bulk stores: the wide forms (a slot's row is 128 bytes of the result) and, without C, K splits
+                    // (not where a row ends inside 16 bytes: a bulk store writes all of them, into what lies behind the row)
                     const int64_t size = int64_t(sizeof(TD)), ld = rows > 1 ? ea.dRow : (cols + 15) / 16 * 16;
                     const int boxCols = f.ksplit > 1 ? std::min(f.tn / f.ksplit, 32) : 0;
-                    ea.tma = (f.tn >= 128 || f.ksplit > 1) && (!C || f.ksplit == 1) && (ea.dCol == 1 || cols == 1) && ld * size % 16 == 0 && ld >= cols
+                    ea.tma = (f.tn >= 128 || f.ksplit > 1) && (!C || f.ksplit == 1) && (ea.dCol == 1 || cols == 1) && ld * size % 16 == 0 && cols * size % 16 == 0 && ld >= cols
                              && ld < (int64_t(1) << 36) && ((uintptr_t(D) | uintptr_t(C)) & 15) == 0 && encodeResult(encode, &ea.mapD, p.typeD, D, cols, rows, ld * size, boxCols)
                              && (!C || encodeResult(encode, &ea.mapC, p.typeD, const_cast<void*>(C), cols, rows, ld * size, 0));
                     return ea.blockY > 1 ? launchForm<TD, false>(f, mapX, mapY, a, ea, sms, stream)

@@ -48,7 +48,7 @@ namespace htb
             // reach dW through 0 * NaN
             l.packH    = gradient || f32 || !wordsH;
             l.packW    = f32 || !wordsW;
-            l.direct   = wordsW;
+            l.direct   = wordsW && p.D % unit == 0; // a bulk store writes whole words of 16 bytes, behind a row's end too
             l.segments = f32 ? 3 : 1;
             l.ld       = roundUp(p.D, 8);
             l.piece    = piece;

@@ -111,6 +111,18 @@ def test_tokens_in_several_modes_and_weights_the_other_way_round(h, kind):
 
 
 @pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t,v,d,ldpad", [(20, 40, 4100, 4), (300, 700, 101, 3), (150, 900, 1026, 2), (130, 300, 60, 68)])
+def test_what_lies_between_the_rows_of_dw_stays(h, t, v, d, ldpad, kind):
+    c = Call(h, *inputs(t, v, d, kind, ldpad=ldpad))
+    wide = torch.full((v, d + ldpad), 7.0, device="cuda", dtype=kind)
+    c.dW = wide[:, :d]
+    c.forward()
+    c.backward()
+    c.check_gradient()
+    assert bool((wide[:, d:] == 7).all())
+
+
+@pytest.mark.parametrize("kind", ALL)
 def test_what_ignored_tokens_hold_counts_for_nothing(h, kind):
     H, W, y, gl = inputs(200, 900, 128, kind)
     H[y == IGNORE] = float("nan")

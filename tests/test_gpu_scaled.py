@@ -181,10 +181,11 @@ def test_scaled_alpha_beta(h, m, n, k, out, rowB):
     run_scaled(h, m, n, k, out=out, alpha=-0.75, beta=1.5, rowB=rowB)
 
 
-@pytest.mark.parametrize("start,pad", [(0, 0), (1, 2), (3, 1)])
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("start,pad", [(0, 0), (1, 2), (3, 1), (0, 3), (0, 7), (8, 11)])
 @pytest.mark.parametrize("out", [torch.float32, torch.float16])
-@pytest.mark.parametrize("m,n,k,rowB", [(3, 131, 2100, False), (130, 301, 1000, True), (2307, 2049, 256, False)])
-def test_scaled_results_at_any_start_and_row_stride(h, m, n, k, rowB, out, start, pad):
+@pytest.mark.parametrize("m,n,k,rowB", [(1, 4097, 1100, False), (3, 133, 2100, False), (130, 301, 1000, True), (2307, 2049, 256, False)])
+def test_scaled_results_at_any_start_and_row_stride(h, m, n, k, rowB, out, start, pad, add):
     """The result and C are columns start .. start + n of a wider matrix; what lies beside them stays."""
     A, B = operand(m, k, torch.float8_e4m3fn, 1), operand(n, k, torch.float8_e4m3fn, 2)
     bA, bB = (1, 128), (1 if rowB else 128, 128)
@@ -193,10 +194,10 @@ def test_scaled_results_at_any_start_and_row_stride(h, m, n, k, rowB, out, start
     wide = torch.randn(m, start + n + pad, device="cuda").to(out)
     before, D = wide.clone(), wide[:, start : start + n]
     C = before[:, start : start + n]
-    dD = desc(h, D)
-    plan = h.scaled_contraction_plan(desc(h, A), (0, 2), desc(h, sA), bA, desc(h, B), (1, 2), desc(h, sB), bB, dD, dD, (0, 1))
-    h.scaled_contraction(plan, 0.5, A, sA, B, sB, 2.0, C, D)
-    want, bound = ref.scaled(A, sA, bA, B, sB, bB, 0.5, 2.0, C)
+    dD, C = desc(h, D), C if add else None
+    plan = h.scaled_contraction_plan(desc(h, A), (0, 2), desc(h, sA), bA, desc(h, B), (1, 2), desc(h, sB), bB, dD if add else None, dD, (0, 1))
+    h.scaled_contraction(plan, 0.5, A, sA, B, sB, 2.0 if add else 0.0, C, D)
+    want, bound = ref.scaled(A, sA, bA, B, sB, bB, 0.5, 2.0 if add else None, C)
     bound = bound + (ref.half_step(out) * 1.01 if out != torch.float32 else 2.0 ** -23) * want.abs() + 2.0 ** -25 * (out == torch.float16)
     assert bool(((D.double() - want).abs() <= bound).all())
     assert torch.equal(wide[:, :start], before[:, :start]) and torch.equal(wide[:, start + n :], before[:, start + n :])
