@@ -36,6 +36,39 @@ namespace htb
             return true;
         }
 
+        // Whether and how a call runs in one pass over W (few tokens; this and the tensor cores in us): gradients of 8 tokens of f32
+        // (x 32000 x 1024: 98 and 247) and of rows that no TMA load can read (f16, x 30011 x 1001: 154 and 207), of 4 tokens of
+        // others (bf16, x 11722 x 2064: 56 and 73; 8 tokens x 32000 x 4096: 376 and 184); losses of 8 tokens of f32 (x 32000 x 1024:
+        // 62 and 126) and of 4 of rows that no TMA load can read (bf16, x 30011 x 1001: 48 and 72, 8 tokens 73 and 71).
+        FewShape fewShape(const CrossEntropyPlan& p, bool gradient)
+        {
+            FewShape      f{};
+            const int64_t size = dtypeSize(p.type), unit = 16 / size;
+            f.tokens = 1;
+            while(f.tokens < p.T && f.tokens < 8)
+                f.tokens *= 2;
+            const int64_t smem = f.tokens * p.D * (size + (gradient ? 4 : 0)) + 16;
+            const bool    words = (p.wD == 1 || p.D == 1) && p.D % unit == 0 && (p.V == 1 || p.wV % unit == 0);
+            const int     most  = size == 4 ? 8 : (gradient ? (words ? 4 : 8) : (words ? 0 : 4));
+            if(p.T < 1 || p.T > most || (p.wD != 1 && p.D > 1) || smem > 200 * 1024)
+                return f;
+            f.use     = true;
+            f.unit    = words ? int(unit) : (p.D % 2 == 0 && (p.V == 1 || p.wV % 2 == 0) ? 2 : 1);
+            f.units   = p.D / f.unit;
+            f.ldh     = roundUp(p.D, 4);
+            f.smem    = int(smem);
+            // equal rounds over a row's units; 512 threads per SM (their registers) as far as shared memory allows. Fewer threads
+            // per block, and more blocks, are slower: one token x 32000 x 1024 f32 47 us in one round, 69 in four.
+            const int64_t rounds = (f.units + 255) / 256;
+            f.threads            = int(roundUp((f.units + rounds - 1) / rounds, 32));
+            const int64_t each   = std::max<int64_t>(1, std::min<int64_t>(512 / f.threads, (227 << 10) / (smem + 5120)));
+            int64_t       n      = std::min(148 * each, (p.V + 3) / 4);
+            if(gradient)
+                n = std::min(n, std::max<int64_t>(1, p.V * size / (4 * p.T)));
+            f.blocks = int(n);
+            return f;
+        }
+
         // The layout for pieces of `piece` classes. Every buffer starts at a multiple of 256 bytes.
         CrossEntropyLayout layoutFor(const CrossEntropyPlan& p, bool gradient, int64_t piece)
         {
@@ -75,6 +108,16 @@ namespace htb
             l.pOff           = take(gradient, uint64_t(partsP) * uint64_t(l.rowsT) * n * 2);
             l.dwOff          = take(gradient && !l.direct, n * ld * 4);
             l.bytes          = at + 256; // room to align the caller's pointer
+            return l;
+        }
+        // of a call in one pass
+        CrossEntropyLayout layoutFew(const CrossEntropyPlan& p, const FewShape& f, bool gradient)
+        {
+            CrossEntropyLayout l{};
+            const uint64_t     T = uint64_t(p.T), n = uint64_t(f.blocks);
+            l.stateOff = l.dhOff = 0;
+            l.partOff            = (T * 12 + 255) / 256 * 256;
+            l.bytes              = 256 + (gradient ? n * T * uint64_t(f.ldh) * 4 : l.partOff + n * T * 8);
             return l;
         }
         // the largest pieces that fit into `bytes`; piece = 0 when not even the smallest do
@@ -232,6 +275,8 @@ namespace htb
     {
         if(p.T == 0)
             return 0;
+        if(const FewShape f = fewShape(p, gradient); f.use)
+            return layoutFew(p, f, gradient).bytes;
         const uint64_t least = layoutFor(p, gradient, kPieceUnit).bytes, most = layoutFor(p, gradient, roundUp(p.V, kPieceUnit)).bytes;
         if(pref == HIPTENSOR_WORKSPACE_MIN)
             return least;
@@ -264,8 +309,10 @@ namespace htb
                           hiptensorGetErrorString(HIPTENSOR_STATUS_INVALID_VALUE));
             return HIPTENSOR_STATUS_INVALID_VALUE;
         }
-        const CrossEntropyLayout l = layoutIn(p, false, workspace ? workspaceSize : 0);
-        if(l.piece == 0)
+        const FewShape           f    = fewShape(p, false);
+        const uint64_t           room = workspace ? workspaceSize : 0;
+        const CrossEntropyLayout l    = f.use ? layoutFew(p, f, false) : layoutIn(p, false, room);
+        if(f.use ? l.bytes > room : l.piece == 0)
         {
             HTB_LOG_ERROR(fn, "Insufficient workspace: req: %llu alloc: %llu (%s)",
                           (unsigned long long)crossEntropyWorkspace(p, false, HIPTENSOR_WORKSPACE_MIN), (unsigned long long)workspaceSize,
@@ -278,6 +325,13 @@ namespace htb
         const int64_t      size   = dtypeSize(p.type);
         const int          type16 = p.type == CUDA_R_16F ? CUDA_R_16F : CUDA_R_16BF;
         float*             state  = reinterpret_cast<float*>(ws + l.stateOff);
+        if(f.use)
+        {
+            HTB_TRY(launchFewLoss(p, f, H, rowsOfH(p), W, targets, a, ws + l.partOff, state, st->deviceStatus, stream));
+            HTB_TRY(launchLossJoin(ws + l.partOff, int64_t(f.blocks) * kHeadGroup, p.T, state, true, true, p.V, p.ignore, targets, loss, lse,
+                                   st->deviceStatus, stream));
+            return HIPTENSOR_STATUS_SUCCESS;
+        }
         const void*        h      = H;
         int64_t            ldh    = rowStride(p, l);
         if(l.packH)
@@ -338,8 +392,10 @@ namespace htb
                 HTB_TRY(launchStoreRows(p.type, nullptr, 0, p.V, p.D, nullptr, dW, plainRows(p.wV, p.wD, p.V), TargetRest{}, 0, 0, stream));
             return HIPTENSOR_STATUS_SUCCESS;
         }
-        const CrossEntropyLayout l = layoutIn(p, true, workspace ? workspaceSize : 0);
-        if(l.piece == 0)
+        const FewShape           f    = fewShape(p, true);
+        const uint64_t           room = workspace ? workspaceSize : 0;
+        const CrossEntropyLayout l    = f.use ? layoutFew(p, f, true) : layoutIn(p, true, room);
+        if(f.use ? l.bytes > room : l.piece == 0)
         {
             HTB_LOG_ERROR(fn, "Insufficient workspace: req: %llu alloc: %llu (%s)",
                           (unsigned long long)crossEntropyWorkspace(p, true, HIPTENSOR_WORKSPACE_MIN), (unsigned long long)workspaceSize,
@@ -348,6 +404,12 @@ namespace htb
         }
         unsigned char* ws     = reinterpret_cast<unsigned char*>((uintptr_t(workspace) + 255) & ~uintptr_t(255));
         const float    a      = *(const float*)alpha;
+        if(f.use)
+        {
+            HTB_TRY(launchFewGradient(p, f, H, rowsOfH(p), W, targets, lse, gradLoss, a, reinterpret_cast<float*>(ws + l.dhOff), dH, dW,
+                                      st->deviceStatus, stream));
+            return HIPTENSOR_STATUS_SUCCESS;
+        }
         const int      type16 = p.type == CUDA_R_16F ? CUDA_R_16F : CUDA_R_16BF;
         float*         scale  = nullptr;
         if(p.type == CUDA_R_16F)

@@ -5,67 +5,20 @@
 //
 // Many tokens are bound by the tensor cores under the power limit: 8192 tokens x 128000 classes x 4096 bf16, loss 6.0 to 6.8 ms
 // (1.26 to 1.43 PFLOP/s; a plain library product of that size runs at 1.39 sustained), 4096 tokens' gradient 10.0 to 10.7 ms
-// (1.20 to 1.28). Few tokens are bound by the bytes of W: 1 token x 32000 x 4096, loss 54 us (4.9 TB/s), gradient 183 us.
+// (1.20 to 1.28). Few tokens are bound by the bytes of W: 1 token x 32000 x 4096, loss 54 us (4.9 TB/s); 8 tokens' gradient
+// 184 us. Gradients of fewer tokens run in one pass over W (cross_entropy_few.cu).
 // f32: 1024 x 32000 x 1024, loss 350 us, gradient 1.08 ms (190 TFLOP/s, 0.7 of a sixth of bf16's rate).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
 #include "accumulate.cuh"
 #include "cross_entropy.hpp"
+#include "cross_entropy_device.cuh"
 #include "kernels.hpp"
 
 namespace htb
 {
     namespace
     {
-        __device__ __forceinline__ float widen(float v)
-        {
-            return v;
-        }
-        __device__ __forceinline__ float widen(__half v)
-        {
-            return __half2float(v);
-        }
-        __device__ __forceinline__ float widen(__nv_bfloat16 v)
-        {
-            return __bfloat162float(v);
-        }
-        template <typename T>
-        __device__ __forceinline__ T narrow(float v);
-        template <>
-        __device__ __forceinline__ float narrow<float>(float v)
-        {
-            return v;
-        }
-        template <>
-        __device__ __forceinline__ __half narrow<__half>(float v)
-        {
-            return __float2half_rn(v);
-        }
-        template <>
-        __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v)
-        {
-            return __float2bfloat16_rn(v);
-        }
-
-        __device__ __forceinline__ int64_t rowOffset(const TokenRows& r, int64_t row)
-        {
-            int64_t off = 0;
-            for(int i = r.nt - 1; i >= 0; i--)
-            {
-                const int64_t q = i ? row / r.ext[i] : 0;
-                off += (row - q * r.ext[i]) * r.stride[i];
-                row = q;
-            }
-            return off;
-        }
-        __device__ __forceinline__ bool counts(int64_t target, int64_t ignore, int64_t V)
-        {
-            return target != ignore && target >= 0 && target < V;
-        }
-
         // Rows of a strided tensor as packed rows of ld 16-bit elements, eight elements a thread. SPLIT: f32 numbers as three bf16
         // ones, x = h + m + l up to 2^-27 of x, [3][rows][ld] (an infinity or NaN stays in h).
         template <typename T, bool SPLIT>
@@ -226,20 +179,6 @@ namespace htb
         }
 
         // ------------------------------------------------------------------ logits that stay on the chip
-        constexpr float kLog2e = 1.4426950408889634f;
-
-        __device__ __forceinline__ float maxNan(float a, float b)
-        {
-            float r;
-            asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-            return r;
-        }
-        // the value that exponents are taken relative to: 0 where a maximum is infinite
-        __device__ __forceinline__ float reference(float m)
-        {
-            return fabsf(m) == INFINITY ? 0.f : m;
-        }
-
         struct HeadArgs
         {
             int64_t        T, n, v0, V; // tokens; classes of this piece, its first class, all classes
@@ -680,12 +619,6 @@ namespace htb
             const int         lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
             const int64_t     t = int64_t(blockIdx.x) * 32 + lane;
             float             m = -INFINITY, s = 0.f;
-            auto              join = [](float& m, float& s, float m2, float s2) {
-                const float top = maxNan(m, m2), ref = reference(top);
-                // nothing yet, or nothing above -infinity: not 0 * exp2(0 - ref), which is NaN below ref = -128
-                s = (m == -INFINITY ? 0.f : s * exp2f(reference(m) - ref)) + (m2 == -INFINITY ? 0.f : s2 * exp2f(reference(m2) - ref));
-                m = top;
-            };
             if(t < T)
             {
                 int64_t i = warp;
@@ -697,12 +630,12 @@ namespace htb
                         p[j] = part[(i + j * kJoinWarps) * T + t];
 #pragma unroll
                     for(int j = 0; j < 4; j++)
-                        join(m, s, p[j].x, p[j].y);
+                        joinSums(m, s, p[j].x, p[j].y);
                 }
                 for(; i < groups; i += kJoinWarps)
                 {
                     const float2 p = part[i * T + t];
-                    join(m, s, p.x, p.y);
+                    joinSums(m, s, p.x, p.y);
                 }
             }
             mine[warp][lane] = make_float2(m, s);
@@ -710,9 +643,9 @@ namespace htb
             if(warp != 0 || t >= T)
                 return;
             for(int w = 1; w < kJoinWarps; w++)
-                join(m, s, mine[w][lane].x, mine[w][lane].y);
+                joinSums(m, s, mine[w][lane].x, mine[w][lane].y);
             if(!first)
-                join(m, s, state[t], state[T + t]);
+                joinSums(m, s, state[t], state[T + t]);
             if(!last)
             {
                 state[t]     = m;

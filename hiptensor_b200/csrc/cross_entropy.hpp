@@ -104,6 +104,23 @@ namespace htb
     cudaError_t launchStoreRows(int type, const float* X, int64_t ldx, int64_t count, int64_t cols, const float* scale, void* Y,
                                 const TokenRows& rows, const TargetRest& rest, int parts, int64_t partRows, cudaStream_t stream);
 
+    // A few tokens, in one pass over W (cross_entropy_few.cu)
+    struct FewShape
+    {
+        bool    use;
+        int     unit; // elements of a row that are read at a time: 16 bytes, two elements or one
+        int     tokens; // rounded up to a power of two
+        int     threads, smem, blocks;
+        int64_t units, ldh;
+    };
+    // part: `blocks` x T pairs of floats, as launchLossJoin reads them; the target logits go to state[2T .. 3T)
+    cudaError_t launchFewLoss(const CrossEntropyPlan& p, const FewShape& f, const void* H, const TokenRows& rows, const void* W, const int64_t* targets,
+                              float alpha, void* part, float* state, int* status, cudaStream_t stream);
+    // part: [blocks][T][ldh] floats; dH or dW may be null
+    cudaError_t launchFewGradient(const CrossEntropyPlan& p, const FewShape& f, const void* H, const TokenRows& rows, const void* W,
+                                  const int64_t* targets, const float* lse, const float* g, float alpha, float* part, void* dH, void* dW, int* status,
+                                  cudaStream_t stream);
+
     int crossEntropy(const hiptensorHandle_t* handle, const CrossEntropyPlan* plan, const void* alpha, const void* H, const void* W,
                      const int64_t* targets, float* loss, float* lse, void* workspace, uint64_t workspaceSize, void* stream);
     int crossEntropyGradient(const hiptensorHandle_t* handle, const CrossEntropyPlan* plan, const void* alpha, const void* H,

@@ -1,0 +1,81 @@
+// What the kernels of the linear cross entropy share: conversions, rows of a strided tensor, joining of partial softmax sums.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "cross_entropy.hpp"
+
+namespace htb
+{
+    namespace
+    {
+        __device__ __forceinline__ float widen(float v)
+        {
+            return v;
+        }
+        __device__ __forceinline__ float widen(__half v)
+        {
+            return __half2float(v);
+        }
+        __device__ __forceinline__ float widen(__nv_bfloat16 v)
+        {
+            return __bfloat162float(v);
+        }
+        template <typename T>
+        __device__ __forceinline__ T narrow(float v);
+        template <>
+        __device__ __forceinline__ float narrow<float>(float v)
+        {
+            return v;
+        }
+        template <>
+        __device__ __forceinline__ __half narrow<__half>(float v)
+        {
+            return __float2half_rn(v);
+        }
+        template <>
+        __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v)
+        {
+            return __float2bfloat16_rn(v);
+        }
+
+        __device__ __forceinline__ int64_t rowOffset(const TokenRows& r, int64_t row)
+        {
+            int64_t off = 0;
+            for(int i = r.nt - 1; i >= 0; i--)
+            {
+                const int64_t q = i ? row / r.ext[i] : 0;
+                off += (row - q * r.ext[i]) * r.stride[i];
+                row = q;
+            }
+            return off;
+        }
+        __device__ __forceinline__ bool counts(int64_t target, int64_t ignore, int64_t V)
+        {
+            return target != ignore && target >= 0 && target < V;
+        }
+
+        constexpr float kLog2e = 1.4426950408889634f;
+
+        __device__ __forceinline__ float maxNan(float a, float b)
+        {
+            float r;
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+            return r;
+        }
+        // the value that exponents are taken relative to: 0 where a maximum is infinite
+        __device__ __forceinline__ float reference(float m)
+        {
+            return fabsf(m) == INFINITY ? 0.f : m;
+        }
+        // (m, s): a maximum and a sum of powers of two relative to it; takes (m2, s2) in
+        __device__ __forceinline__ void joinSums(float& m, float& s, float m2, float s2)
+        {
+            const float top = maxNan(m, m2), ref = reference(top);
+            // nothing yet, or nothing above -infinity: not 0 * exp2(0 - ref), which is NaN below ref = -128
+            s = (m == -INFINITY ? 0.f : s * exp2f(reference(m) - ref)) + (m2 == -INFINITY ? 0.f : s2 * exp2f(reference(m2) - ref));
+            m = top;
+        }
+    } // namespace
+} // namespace htb

@@ -149,6 +149,82 @@ def test_every_token_ignored(h, kind):
     assert bool((c.loss == 0).all()) and bool((c.dH == 0).all()) and bool((c.dW == 0).all())
 
 
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("v,d,ldpad", [(1, 8, 0), (3, 4100, 4), (1201, 98, 0), (1500, 33, 3), (4001, 1026, 2), (700, 2048, 8), (2, 8200, 0)])
+def test_few_tokens(h, v, d, ldpad, t, kind):
+    c = Call(h, *inputs(t, v, d, kind, ldpad=ldpad))
+    wide = torch.full((v, d + ldpad), 7.0, device="cuda", dtype=kind)
+    c.dW = wide[:, :d]
+    c.forward()
+    c.check()
+    c.backward()
+    c.check_gradient()
+    assert bool((wide[:, d:] == 7).all())
+    both = c.dH.clone(), c.dW.clone()
+    for want in ((True, False), (False, True)):
+        c.dH.fill_(5), c.dW.fill_(5)
+        c.backward(want=want)
+        for got, before, wanted in zip((c.dH, c.dW), both, want):
+            assert torch.equal(got, before) if wanted else bool((got == 5).all())
+    assert h.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t", [1, 3, 4, 8])
+def test_few_tokens_some_of_which_count_for_nothing(h, t, kind):
+    H, W, y, gl = inputs(t, 900, 130, kind, ignored=0)
+    if t > 3:
+        H = H.view(2, t // 2, 130).transpose(0, 1)  # tokens in two modes that do not fold: the second token is row t / 2
+    y[0], gl[0] = IGNORE, float("nan")
+    if t > 3:
+        H[0, 0], H[0, 1] = float("nan"), float("inf")
+    else:
+        H[0], H[1:2] = float("nan"), float("inf")
+    if t > 1:
+        y[1] = 900
+    c = Call(h, H, W, y, gl, modes=((0, 5, 2), (1, 2)) if t > 3 else ((0, 2), (1, 2)))
+    c.forward()
+    torch.cuda.synchronize()
+    rows = c.H.reshape(t, 130)
+    bad = y == 900
+    assert float(c.loss[0]) == 0 and torch.equal(c.loss.isnan(), bad)
+    keep = (y >= 0) & ~bad
+    if bool(bad.any()):
+        assert h.device_status() == 7
+        with pytest.raises(ht.HiptensorError):
+            c.backward()
+    lse = torch.where(keep, c.lse, torch.full_like(c.lse, float("nan")))
+    c.lse = lse
+    c.backward()
+    torch.cuda.synchronize()
+    if bool(bad.any()):
+        assert h.device_status() == 7
+        with pytest.raises(ht.HiptensorError):
+            c.forward()
+    dH = c.dH.reshape(t, 130)
+    assert bool((dH[~keep] == 0).all())
+    a, b, ea, eb = ref.gradient(rows, W, y, lse, gl, 1.0, IGNORE)
+    within(a, b, ea, eb, dH, c.dW)
+
+
+def test_few_tokens_and_infinite_weights(h):
+    H, W, y, gl = inputs(3, 600, 64, torch.float32, ignored=0)
+    H[:], y[:] = H.abs() + 0.1, 5
+    W[17], W[400] = -float("inf"), -float("inf")
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    keep = [i for i in range(600) if i not in (17, 400)]
+    lse = torch.logsumexp(H.double() @ W[keep].double().T, 1)
+    assert bool(((c.lse.double() - lse).abs() < 2.0 ** -17 * (1 + lse.abs())).all())
+    W[17] = float("inf")
+    c.forward()
+    assert bool((c.lse == float("inf")).all())
+    W[17] = float("nan")
+    c.forward()
+    assert bool(c.lse.isnan().all()) and bool(c.loss.isnan().all())
+
+
 def test_an_ignored_index_inside_the_vocabulary(h):
     H, W, y, gl = inputs(100, 300, 64, torch.bfloat16, ignored=0)
     y[::3] = 0
