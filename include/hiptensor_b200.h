@@ -175,8 +175,9 @@ int htScaledContraction(const htHandle* handle, const htScaledContractionPlan* p
  * ignored take no part in the gradient, whatever they hold. A target that is neither a class nor ignoreIndex reads
  * nothing out of range: its loss is NaN, its row of P zero, and the next call on the handle returns 13
  * (EXECUTION_FAILED) once. P is rounded to the type of H (f16: scaled by a power of two for max |gradLoss * alpha|; up to 64
- * tokens it is a sum of two such numbers), sums are f32. f32 tensors are multiplied as sums of three bf16 numbers, which is
- * f32's own accuracy; an infinity among them makes NaN of the logits it takes part in.
+ * tokens it is a sum of two such numbers, of a few tokens it stays f32), sums are f32. f32 tensors of more than a few tokens
+ * are multiplied as sums of three bf16 numbers, which is f32's own accuracy; an infinity among them makes NaN of the logits
+ * it takes part in.
  *
  * The workspace holds the pieces: any size from htCrossEntropyGetWorkspaceSize's MIN on (19 below it); with more, pieces
  * are larger and fewer. gradient: 0 for htCrossEntropy, 1 for htCrossEntropyGradient. Two calls that run at the same time (two
