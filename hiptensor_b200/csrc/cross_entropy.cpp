@@ -415,7 +415,7 @@ namespace htb
         if(p.type == CUDA_R_16F)
         {
             scale = reinterpret_cast<float*>(ws + l.scaleOff);
-            HTB_TRY(launchGradientScale(gradLoss, a, p.T, scale, stream));
+            HTB_TRY(launchGradientScale(gradLoss, a, p.T, targets, p.ignore, p.V, scale, stream));
         }
         void* h = ws + l.hOff;
         HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, l.rowsT, p.D, l.ld, h, targets, p.ignore, p.V, st->deviceStatus, stream));

@@ -78,12 +78,19 @@ namespace htb
             }
         }
 
-        __global__ void __launch_bounds__(1024) gradient_scale_kernel(const float* __restrict__ g, float alpha, int64_t T, float* scale)
+        // Only tokens whose row of P is not zero have a say, and of these only finite factors: one that is not makes its own row
+        // (and dW) what it is, and the others' rows need their power of two all the same.
+        __global__ void __launch_bounds__(1024) gradient_scale_kernel(const float* __restrict__ g, float alpha, int64_t T,
+                                                                      const int64_t* __restrict__ targets, int64_t ignore, int64_t V, float* scale)
         {
             __shared__ float part[32];
             float            m = 0.f;
             for(int64_t t = threadIdx.x; t < T; t += 1024)
-                m = fmaxf(m, fabsf(g[t] * alpha));
+            {
+                const float f = fabsf(g[t] * alpha);
+                if(f < INFINITY && counts(targets[t], ignore, V))
+                    m = fmaxf(m, f);
+            }
             for(int s = 16; s; s >>= 1)
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
             if((threadIdx.x & 31) == 0)
@@ -94,7 +101,7 @@ namespace htb
                 for(int i = 0; i < 32; i++)
                     m = fmaxf(m, part[i]);
                 int e = 15; // m < 2^e: the factor 2^(15 - e) keeps |P| below 2^15
-                if(m > 0.f && m < INFINITY)
+                if(m > 0.f)
                     frexpf(m, &e);
                 e        = max(e, -100);
                 scale[0] = ldexpf(1.f, 15 - e);
@@ -980,9 +987,10 @@ namespace htb
         return noted("cross_entropy_pack");
     }
 
-    cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, float* scale, cudaStream_t stream)
+    cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, const int64_t* targets, int64_t ignore, int64_t V, float* scale,
+                                    cudaStream_t stream)
     {
-        gradient_scale_kernel<<<1, 1024, 0, stream>>>(g, alpha, T, scale);
+        gradient_scale_kernel<<<1, 1024, 0, stream>>>(g, alpha, T, targets, ignore, V, scale);
         return noted("cross_entropy_scale");
     }
 

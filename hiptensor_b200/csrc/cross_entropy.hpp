@@ -91,8 +91,10 @@ namespace htb
     cudaError_t launchWeightGradient(const HeadProduct& h, const Probabilities& P, const float* scale, int typeOut, void* dW, int64_t ldw, int smCount,
                                      int* status, cudaStream_t stream);
 
-    // f16: scale[0] = a power of two that brings max |g * alpha| close to the top of the range, scale[1] = its reciprocal
-    cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, float* scale, cudaStream_t stream);
+    // f16: scale[0] = a power of two that brings max |g * alpha| over the tokens that count (finite ones) close to the top of the range,
+    // scale[1] = its reciprocal
+    cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, const int64_t* targets, int64_t ignore, int64_t V, float* scale,
+                                    cudaStream_t stream);
     // Y[row r, c] = (sum of `parts` X[r, c], partRows rows apart, + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; parts 0: zeros; rest null: none
     struct TargetRest
     {

@@ -140,6 +140,43 @@ def test_what_ignored_tokens_hold_counts_for_nothing(h, kind):
 
 
 @pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t", [9, 40, 200])
+@pytest.mark.parametrize("poison", [1e30, float("inf"), float("nan")])
+def test_what_the_losses_gradients_of_tokens_that_do_not_count_hold(h, t, poison, kind):
+    """Probabilities of about 1e-5 times a factor next to factors of ignored and out-of-range tokens that dwarf it. Logits are
+    made by alpha = 1 / 64, so that small entries of P make gradients of ordinary size."""
+    H, W, y, _ = inputs(t, 900, 128, kind)
+    y[0], y[1], y[2:4] = IGNORE, 900, y[2:4].clamp(min=0)
+    gl = torch.full((t,), 2.0 ** -6, device="cuda") * (1 + torch.arange(t, device="cuda") % 3)
+    keep = (y >= 0) & (y < 900)
+    gl[~keep] = poison
+    c = Call(h, H * 64, W, y, gl, alpha=1 / 64)
+    c.forward()
+    torch.cuda.synchronize()
+    with pytest.raises(ht.HiptensorError):  # the forward pass met the target that is no class
+        c.backward()
+    c.backward()
+    torch.cuda.synchronize()
+    with pytest.raises(ht.HiptensorError):
+        c.forward()
+    assert bool((c.dH[~keep] == 0).all())
+    c.check_gradient()
+
+
+@pytest.mark.parametrize("t", [9, 40, 200])
+def test_one_infinite_loss_gradient_leaves_the_other_tokens_theirs(h, t):
+    H, W, y, _ = inputs(t, 900, 128, torch.float16, ignored=0)
+    gl = torch.full((t,), 2.0 ** -6, device="cuda")
+    gl[t // 2] = float("inf")
+    c = Call(h, H * 64, W, y, gl, alpha=1 / 64)
+    c.forward()
+    c.backward()
+    rows = torch.arange(t, device="cuda") != t // 2
+    want, _, bound, _ = ref.gradient(c.H[rows], W, y[rows], c.lse[rows], gl[rows], 1 / 64, IGNORE)
+    assert bool(((c.dH[rows].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("kind", ALL)
 def test_every_token_ignored(h, kind):
     H, W, y, gl = inputs(70, 300, 64, kind)
     y[:] = IGNORE
