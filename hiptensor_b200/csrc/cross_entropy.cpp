@@ -455,7 +455,7 @@ namespace htb
         }
         if(dH)
             HTB_TRY(launchStoreRows(p.type, dh, l.ld, p.T, p.D, scale, dH, rowsOfH(p),
-                                    P.parts == 3 ? TargetRest{} : TargetRest{rest, targets, p.ignore, p.V, p.wV, p.wD, W}, l.parts, hiddenRows(p.T),
+                                    TargetRest{P.parts == 3 ? nullptr : rest, targets, p.ignore, p.V, p.wV, p.wD, W}, l.parts, hiddenRows(p.T),
                                     stream));
         return HIPTENSOR_STATUS_SUCCESS;
     }

@@ -109,7 +109,8 @@ namespace htb
             }
         }
 
-        // Y[row r, c] = (sum of the parts' X[r, c] + rest[r] * W[target of r, c]) * scale[1]; four columns a thread
+        // Y[row r, c] = (sum of the parts' X[r, c] + rest[r] * W[target of r, c]) * scale[1]; four columns a thread. A token that does
+        // not count gets zeros, whatever W holds: its row of P is 0, but 0 times an infinity in W is NaN.
         template <typename T>
         __global__ void store_rows_kernel(const float* __restrict__ X, int64_t ldx, int64_t count, int64_t cols, const float* __restrict__ scale,
                                           T* __restrict__ Y, const __grid_constant__ TokenRows rows, const __grid_constant__ TargetRest rest, int parts,
@@ -121,25 +122,23 @@ namespace htb
             {
                 if(c >= cols)
                     continue;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                for(int i = 0; i < parts; i++)
+                const int64_t target = rest.targets ? rest.targets[r] : 0;
+                const bool    live   = !rest.targets || counts(target, rest.ignore, rest.V);
+                float4        x      = make_float4(0.f, 0.f, 0.f, 0.f);
+                for(int i = 0; live && i < parts; i++)
                 {
                     const float4 v = *reinterpret_cast<const float4*>(X + (int64_t(i) * partRows + r) * ldx + c); // ldx is a multiple of eight
                     x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
                 }
                 float y[4] = {x.x, x.y, x.z, x.w};
-                if(rest.rest)
+                if(rest.rest && live)
                 {
-                    const int64_t target = rest.targets[r];
-                    if(counts(target, rest.ignore, rest.V))
-                    {
-                        const T*    w = static_cast<const T*>(rest.W) + target * rest.wV + c * rest.wD;
-                        const float e = rest.rest[r];
+                    const T*    w = static_cast<const T*>(rest.W) + target * rest.wV + c * rest.wD;
+                    const float e = rest.rest[r];
 #pragma unroll
-                        for(int j = 0; j < 4; j++)
-                            if(c + j < cols)
-                                y[j] = fmaf(e, widen(w[j * rest.wD]), y[j]);
-                    }
+                    for(int j = 0; j < 4; j++)
+                        if(c + j < cols)
+                            y[j] = fmaf(e, widen(w[j * rest.wD]), y[j]);
                 }
                 T* dst = Y + rowOffset(rows, r) + c * rows.elem;
                 if(vec && c + 4 <= cols)

@@ -95,7 +95,8 @@ namespace htb
     // scale[1] = its reciprocal
     cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, const int64_t* targets, int64_t ignore, int64_t V, float* scale,
                                     cudaStream_t stream);
-    // Y[row r, c] = (sum of `parts` X[r, c], partRows rows apart, + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; parts 0: zeros; rest null: none
+    // Y[row r, c] = (sum of `parts` X[r, c], partRows rows apart, + rest[r] * W[target of r, c]) (* scale[1]) rounded to `type`; parts 0: zeros; rest null:
+    // none. With targets: 0 in the rows of tokens that do not count.
     struct TargetRest
     {
         const float*   rest;

@@ -172,7 +172,7 @@ int htScaledContraction(const htHandle* handle, const htScaledContractionPlan* p
  *     P = (exp(z - lse) - [class == target]) * gradLoss * alpha, 0 where target == ignoreIndex
  *     dH = P contracted with W (laid out like H),   dW = P contracted with H (laid out like W)
  * htCrossEntropyGradient takes lse as htCrossEntropy wrote it; dH or dW may be NULL (not wanted). Rows of H whose target is
- * ignored take no part in the gradient, whatever they hold. A target that is neither a class nor ignoreIndex reads
+ * ignored take no part in the gradient, whatever they hold, and their rows of dH are 0, whatever W holds. A target that is neither a class nor ignoreIndex reads
  * nothing out of range: its loss is NaN, its row of P zero, and the next call on the handle returns 13
  * (EXECUTION_FAILED) once. P is rounded to the type of H (f16: scaled by a power of two for the largest finite |gradLoss * alpha|
  * of the tokens that count; up to 64 tokens it is a sum of two such numbers, of a few tokens it stays f32), sums are f32. f32 tensors of more than a few tokens

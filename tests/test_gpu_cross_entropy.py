@@ -177,6 +177,23 @@ def test_one_infinite_loss_gradient_leaves_the_other_tokens_theirs(h, t):
 
 
 @pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t", [3, 8, 9, 40, 200])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_tokens_that_do_not_count_get_zeros_whatever_the_weights_hold(h, t, value, kind):
+    H, W, y, gl = inputs(t, 600, 64, kind, ignored=0)
+    W[17], W[400, 3] = value, value
+    y[0], y[t // 2] = IGNORE, 600
+    c = Call(h, H, W, y, gl)
+    c.lse.fill_(1.0)
+    c.backward()
+    torch.cuda.synchronize()
+    with pytest.raises(ht.HiptensorError):
+        c.forward()
+    dead = (y < 0) | (y >= 600)
+    assert bool((c.dH[dead] == 0).all()) and bool(c.dH[~dead].isnan().any())
+
+
+@pytest.mark.parametrize("kind", ALL)
 def test_every_token_ignored(h, kind):
     H, W, y, gl = inputs(70, 300, 64, kind)
     y[:] = IGNORE
