@@ -191,7 +191,7 @@ namespace htb
             int64_t        ignore;
             const int64_t* targets;
             float          alpha;
-            // loss: partial (maximum, sum) of 128 classes each, [classes][T], in powers of two; target logits
+            // loss: partial (maximum, sum of exponentials relative to it) of 128 classes each, [classes][T]; target logits
             float2* part;
             float*  targetLogit;
             // gradient
@@ -251,7 +251,7 @@ namespace htb
             }
         };
 
-        // Loss: one pass over a tile's logits in registers, maximum then sum of powers of two; what leaves the SM are two
+        // Loss: one pass over a tile's logits in registers, maximum then sum of exponentials; what leaves the SM are two
         // floats for 128 logits.
         struct LossEpi : HeadSums<256>
         {
@@ -280,14 +280,13 @@ namespace htb
                 const int64_t t = a.targets[row] - a.v0 - col;
                 if(t >= 0 && t < COLS && col + t < a.n)
                     a.targetLogit[row] = Sums::at(int(t)) * a.alpha;
-                const float    c  = a.alpha * kLog2e;
-                const uint64_t c2 = pack2(c, c);
+                const uint64_t alpha2 = pack2(a.alpha, a.alpha), log2e2 = pack2(kLog2e, kLog2e);
                 float          m  = -INFINITY;
                 const int      n  = int(min(int64_t(COLS), a.n - col));
 #pragma unroll
                 for(int i = 0; i < COLS / 2; i++)
                 {
-                    acc[i]         = mul2(acc[i], c2);
+                    acc[i]         = mul2(acc[i], alpha2);
                     const float2 f = unpack2(acc[i]);
                     if(n == COLS)
                         m = maxNan(maxNan(f.x, f.y), m);
@@ -304,7 +303,7 @@ namespace htb
 #pragma unroll
                 for(int i = 0; i < COLS / 2; i++)
                 {
-                    const float2 f = unpack2(add2(acc[i], less));
+                    const float2 f = unpack2(mul2(add2(acc[i], less), log2e2));
                     sum[i & 3]     = add2(sum[i & 3], pack2(exp2f(f.x), exp2f(f.y)));
                 }
                 const float2 s = unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
@@ -362,9 +361,7 @@ namespace htb
                         f = a.g[row] * a.alpha * (a.scale ? a.scale[0] : 1.f);
                     }
                 }
-                const float    c  = a.alpha * kLog2e;
-                const float    l  = lse * kLog2e;
-                const uint64_t c2 = pack2(c, c), l2 = pack2(-l, -l);
+                const uint64_t alpha2 = pack2(a.alpha, a.alpha), lse2 = pack2(-lse, -lse), log2e2 = pack2(kLog2e, kLog2e);
                 const int      t  = live && target - a.v0 - col >= 0 && target - a.v0 - col < COLS ? int(target - a.v0 - col) : -1;
                 // P takes the sums' place
 #pragma unroll
@@ -380,7 +377,7 @@ namespace htb
                     }
                     else
                     {
-                        const float2 x = unpack2(fma2(acc[i], c2, l2));
+                        const float2 x = unpack2(mul2(fma2(acc[i], alpha2, lse2), log2e2));
                         p0 = exp2f(x.x);
                         p1 = exp2f(x.y);
                     }
@@ -658,9 +655,9 @@ namespace htb
                 state[T + t] = s;
                 return;
             }
-            const float   l = (reference(m) + log2f(s)) * 0.6931471805599453f;
+            const float   ref = reference(m), l = logf(s);
             const int64_t target = targets[t];
-            lse[t] = l;
+            lse[t] = ref + l;
             if(target == ignore)
                 loss[t] = 0.f;
             else if(target < 0 || target >= V)
@@ -669,7 +666,7 @@ namespace htb
                 atomicExch_system(status, kStatusBadTarget);
             }
             else
-                loss[t] = l - state[2 * T + t];
+                loss[t] = (ref - state[2 * T + t]) + l; // at least 0, and 0 where nothing but the target has a share
         }
 
         bool encodeMatrix(PFN_encodeTiled encode, CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int boxCols, int boxRows,

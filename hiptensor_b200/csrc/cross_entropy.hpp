@@ -75,7 +75,7 @@ namespace htb
     // part: ceil(n / kHeadGroup) x T pairs of floats; the target logits go to state[2T .. 3T)
     cudaError_t launchHeadLoss(const HeadProduct& h, int64_t v0, const int64_t* targets, float alpha, void* part, float* state, int smCount,
                                int* status, cudaStream_t stream);
-    // joins a piece's partial results with state[0 .. 2T) (maximum, sum in powers of two); after the last piece loss and lse
+    // joins a piece's partial results with state[0 .. 2T) (maximum, sum of exponentials); after the last piece loss and lse
     cudaError_t launchLossJoin(const void* part, int64_t n, int64_t T, float* state, bool first, bool last, int64_t V, int64_t ignore,
                                const int64_t* targets, float* loss, float* lse, int* status, cudaStream_t stream);
     // P[t, v] = (exp(z - lse) - [v0 + v == target]) * g * alpha (* scale[0]); rest[t]: what rounding took from the target's entry

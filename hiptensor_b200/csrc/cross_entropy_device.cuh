@@ -69,12 +69,14 @@ namespace htb
         {
             return fabsf(m) == INFINITY ? 0.f : m;
         }
-        // (m, s): a maximum and a sum of powers of two relative to it; takes (m2, s2) in
+        // (m, s): a maximum and a sum of exponentials relative to it; takes (m2, s2) in. Logits stay in natural units until the maximum
+        // is taken away from them: a product with log2(e) before that would overflow for a mask of the type's lowest value, and round
+        // the target's logit otherwise than the maximum (losses below 0).
         __device__ __forceinline__ void joinSums(float& m, float& s, float m2, float s2)
         {
             const float top = maxNan(m, m2), ref = reference(top);
-            // nothing yet, or nothing above -infinity: not 0 * exp2(0 - ref), which is NaN below ref = -128
-            s = (m == -INFINITY ? 0.f : s * exp2f(reference(m) - ref)) + (m2 == -INFINITY ? 0.f : s2 * exp2f(reference(m2) - ref));
+            // nothing yet, or nothing above -infinity: not 0 * exp2(0 - ref), which is NaN far below 0
+            s = (m == -INFINITY ? 0.f : s * exp2f((reference(m) - ref) * kLog2e)) + (m2 == -INFINITY ? 0.f : s2 * exp2f((reference(m2) - ref) * kLog2e));
             m = top;
         }
     } // namespace

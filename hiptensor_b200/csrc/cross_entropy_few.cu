@@ -30,7 +30,7 @@ namespace htb
             int64_t        ignore;
             float          alpha;
             int*           status;
-            // loss: (maximum, sum) of a block's classes in powers of two, [block][T]; target logits
+            // loss: (maximum, sum of exponentials) of a block's classes, [block][T]; target logits
             float2* part;
             float*  targetLogit;
             // gradient
@@ -168,8 +168,8 @@ namespace htb
                 {
                     if(warp == 0 && v < a.V) // the other warps go on to the next classes
                     {
-                        const float x = logit(), x2 = x * kLog2e;
-                        joinSums(m, s, x2, exp2f(x2 - reference(x2))); // 1, or what an infinity stands for
+                        const float x = logit();
+                        joinSums(m, s, x, exp2f(x - reference(x))); // 1, or what an infinity stands for
                         if(v == y && live)
                             a.targetLogit[t] = x;
                     }

@@ -194,6 +194,62 @@ def test_tokens_that_do_not_count_get_zeros_whatever_the_weights_hold(h, t, valu
 
 
 @pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t", [1, 4, 9, 40, 300])
+def test_the_loss_of_the_only_class_is_nothing(h, t, kind):
+    H, W, _, gl = inputs(t, 1, 64, kind)
+    H = H.abs() * (1 + 5 * torch.rand(t, 1, device="cuda")).to(kind)
+    c = Call(h, H, W.abs() + 1, torch.zeros(t, device="cuda", dtype=torch.int64), gl, alpha=0.37)
+    c.forward()
+    assert bool((c.loss == 0).all()) and bool((c.lse > 1).all())
+
+
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("t,v", [(1, 300), (4, 700), (9, 300), (40, 700), (300, 4100)])
+def test_no_loss_is_below_nothing(h, t, v, kind):
+    """Every target is the class of the largest logit, about 100 to 1500, by margins from none to much."""
+    H, W, y, gl = inputs(t, v, 64, kind, ignored=0)
+    H, W = H.abs() + 1, W.abs() * 4 + 1
+    W[v // 2] = W.amax(0) + (torch.arange(64, device="cuda") % 3).to(kind)
+    y[:] = v // 2
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    assert bool((c.loss >= 0).all())
+    c.check()
+
+
+@pytest.mark.parametrize("kind,t", [(torch.bfloat16, 1), (torch.bfloat16, 40), (torch.bfloat16, 300), (torch.float16, 40), (torch.float32, 5)])
+def test_classes_masked_by_the_lowest_value(h, kind, t):
+    """The last column of W is the lowest value of the type for masked classes and H's is 1: they take no part."""
+    H, W, y, gl = inputs(t, 600, 64, kind, ignored=0)
+    low, open_ = torch.finfo(kind).min, 450
+    H[:, 63], W[:, 63], W[open_:, 63], y[:] = 1, 0, low, y % open_
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    within(*ref.loss(H, W[:open_], y, 1.0, IGNORE), c.loss, c.lse)
+    c.backward()
+    a, b, ea, eb = ref.gradient(H, W[:open_], y, c.lse, gl, 1.0, IGNORE)
+    within(a, b, ea, eb, c.dH, c.dW[:open_])
+    assert bool((c.dW[open_:] == 0).all())
+    y[0] = open_ + 7  # a target that is masked: as far away as the mask is
+    c.forward()
+    assert abs(float(c.loss[0]) / -low - 1) < 2.0 ** -10
+
+
+@pytest.mark.parametrize("kind,t", [(torch.bfloat16, 1), (torch.bfloat16, 40), (torch.bfloat16, 300), (torch.float16, 40), (torch.float32, 5)])
+def test_a_token_whose_every_class_is_masked_by_the_lowest_value(h, kind, t):
+    H, W, y, gl = inputs(t, 600, 64, kind, ignored=0)
+    low = torch.finfo(kind).min
+    H[:, 63], W[:, 63], H[t // 2, 63] = 0, low, 1
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    others = torch.arange(t, device="cuda") != t // 2
+    near = abs(low) * 2.0 ** -20  # the other terms of the sum (60 at most) are lost next to the mask
+    assert abs(float(c.lse[t // 2]) - low) <= near + 60 and abs(float(c.loss[t // 2])) <= near + 60
+    a, b, ea, eb = ref.loss(H[others], W, y[others], 1.0, IGNORE)
+    within(a, b, ea, eb, c.loss[others], c.lse[others])
+
+
+@pytest.mark.parametrize("kind", ALL)
 def test_every_token_ignored(h, kind):
     H, W, y, gl = inputs(70, 300, 64, kind)
     y[:] = IGNORE
