@@ -20,7 +20,8 @@ namespace htb
     namespace
     {
         // Rows of a strided tensor as packed rows of ld 16-bit elements, eight elements a thread. SPLIT: f32 numbers as three bf16
-        // ones, x = h + m + l up to 2^-27 of x, [3][rows][ld] (an infinity or NaN stays in h).
+        // ones, x = h + m + l up to 2^-27 of x, [3][rows][ld] (an infinity or NaN stays in h; a number that would round to an infinity,
+        // as f32's lowest value would, is truncated in h).
         template <typename T, bool SPLIT>
         __global__ void pack_rows_kernel(const T* __restrict__ X, const __grid_constant__ TokenRows rows, int64_t count, int64_t total, int64_t cols,
                                          int64_t ld, unsigned short* __restrict__ X2, const int64_t* __restrict__ targets, int64_t ignore,
@@ -62,13 +63,15 @@ namespace htb
 #pragma unroll
                     for(int j = 0; j < 8; j++)
                     {
-                        float       left = x[j];
-                        const float whole = widen(narrow<__nv_bfloat16>(left));
+                        const bool finite = fabsf(x[j]) < INFINITY;
+                        float      left   = x[j];
 #pragma unroll
                         for(int k = 0; k < 3; k++)
                         {
                             part[k][j] = narrow<__nv_bfloat16>(left);
-                            left       = fabsf(whole) < INFINITY ? left - widen(part[k][j]) : 0.f;
+                            if(k == 0 && finite && fabsf(widen(part[0][j])) == INFINITY)
+                                part[0][j] = __float2bfloat16_rz(left);
+                            left = finite ? left - widen(part[k][j]) : 0.f;
                         }
                     }
 #pragma unroll

@@ -217,7 +217,8 @@ def test_no_loss_is_below_nothing(h, t, v, kind):
     c.check()
 
 
-@pytest.mark.parametrize("kind,t", [(torch.bfloat16, 1), (torch.bfloat16, 40), (torch.bfloat16, 300), (torch.float16, 40), (torch.float32, 5)])
+@pytest.mark.parametrize("kind,t", [(torch.bfloat16, 1), (torch.bfloat16, 40), (torch.bfloat16, 300), (torch.float16, 40), (torch.float32, 5),
+                                    (torch.float32, 9), (torch.float32, 40), (torch.float32, 300)])
 def test_classes_masked_by_the_lowest_value(h, kind, t):
     """The last column of W is the lowest value of the type for masked classes and H's is 1: they take no part."""
     H, W, y, gl = inputs(t, 600, 64, kind, ignored=0)
@@ -235,7 +236,8 @@ def test_classes_masked_by_the_lowest_value(h, kind, t):
     assert abs(float(c.loss[0]) / -low - 1) < 2.0 ** -10
 
 
-@pytest.mark.parametrize("kind,t", [(torch.bfloat16, 1), (torch.bfloat16, 40), (torch.bfloat16, 300), (torch.float16, 40), (torch.float32, 5)])
+@pytest.mark.parametrize("kind,t", [(torch.bfloat16, 1), (torch.bfloat16, 40), (torch.bfloat16, 300), (torch.float16, 40), (torch.float32, 5),
+                                    (torch.float32, 9), (torch.float32, 40), (torch.float32, 300)])
 def test_a_token_whose_every_class_is_masked_by_the_lowest_value(h, kind, t):
     H, W, y, gl = inputs(t, 600, 64, kind, ignored=0)
     low = torch.finfo(kind).min
