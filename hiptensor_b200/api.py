@@ -7,7 +7,6 @@ Every non-zero status raises HiptensorError.
 """
 import ctypes
 import struct
-import sys
 
 from . import _lib
 
@@ -142,16 +141,14 @@ class _Owned:
 class Handle:
     """hiptensorHandle_t bound to the CUDA device current at construction (hiptensorCreate)."""
 
-    _device = None  # of the handle, where torch is there to tell
-
     def __init__(self):
         self._L = _lib.lib()
         h = ctypes.c_void_p(0)
         _check(self._L.htCreate(ctypes.byref(h)), "hiptensorCreate")
         self._h = h
-        torch = sys.modules.get("torch")
-        if torch is not None:
-            self._device = torch.cuda.current_device()
+        device = ctypes.c_int32(-1)
+        _check(self._L.htGetDevice(self._h, ctypes.byref(device)), "htGetDevice")
+        self._device = device.value
 
     def destroy(self):
         if self._h:
@@ -335,7 +332,7 @@ class Handle:
         """A tensor's (or a plain) address; a tensor that is not on the handle's device is refused."""
         if x is None or isinstance(x, int):
             return x
-        if x.get_device() != self._device and (self._device is not None or x.get_device() < 0):
+        if x.get_device() != self._device:
             raise HiptensorError(STATUS_ARCH_MISMATCH, "a tensor on another device than the handle's")
         return x.data_ptr()
 

@@ -308,6 +308,17 @@ int htGetDeviceStatus(const htHandle* handle, int32_t* status)
     return HIPTENSOR_STATUS_SUCCESS;
 }
 
+int htGetDevice(const htHandle* handle, int32_t* device)
+{
+    if(!handle || !device)
+        return HIPTENSOR_STATUS_NOT_INITIALIZED;
+    const htb::HandleState* st = htb::stateOf(H(handle));
+    if(!st)
+        return HIPTENSOR_STATUS_NOT_INITIALIZED;
+    *device = st->device;
+    return HIPTENSOR_STATUS_SUCCESS;
+}
+
 int htInjectDeviceStatus(const htHandle* handle, int32_t code)
 {
     if(!handle)

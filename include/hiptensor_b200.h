@@ -225,6 +225,8 @@ const char* htLastKernelName(void);
  * clear it; the next operation on the handle reports HIPTENSOR_STATUS_EXECUTION_FAILED once and clears it. No
  * reference counterpart: the reference's kernels have no device-side waits. */
 int htGetDeviceStatus(const htHandle* handle, int32_t* status);
+/* The CUDA device that the handle is bound to (the current one when it was made). No reference counterpart. */
+int htGetDevice(const htHandle* handle, int32_t* device);
 /* Test aid (host-side fault injection): writes the status word as a timed-out kernel would, so that the error
  * path of the next operation can be exercised without making a kernel wait. */
 int htInjectDeviceStatus(const htHandle* handle, int32_t code);
