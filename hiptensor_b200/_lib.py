@@ -85,17 +85,24 @@ def i64(v):
 
 
 # The library only reads mode and block lists, so the array of a tuple can serve every call that names the same one (a
-# call's marshalling costs as much as a small kernel).
+# call's marshalling costs as much as a small kernel). Only of plain integers: other objects may not be hashable, or stand for
+# another number next time.
 @functools.lru_cache(maxsize=1024)
 def _array(kind, v):
-    return (kind * len(v))(*[int(x) for x in v])
+    for x in v:
+        if type(x) is not int:
+            raise TypeError
+    return (kind * len(v))(*v)
 
 
 def i32(v):
     if v is None:
         return None
     if type(v) is tuple:
-        return _array(ctypes.c_int32, v)
+        try:
+            return _array(ctypes.c_int32, v)
+        except TypeError:
+            pass
     return (ctypes.c_int32 * len(v))(*[int(x) for x in v])
 
 
@@ -103,5 +110,8 @@ def u32(v):
     if v is None:
         return None
     if type(v) is tuple:
-        return _array(ctypes.c_uint32, v)
+        try:
+            return _array(ctypes.c_uint32, v)
+        except TypeError:
+            pass
     return (ctypes.c_uint32 * len(v))(*[int(x) for x in v])
