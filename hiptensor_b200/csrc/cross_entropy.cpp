@@ -12,6 +12,7 @@ namespace htb
     namespace
     {
         constexpr int64_t  kPieceUnit   = 256; // classes: a tile's columns
+        constexpr int64_t  kIndexRange  = (int64_t(1) << 31) - 512; // of a load's coordinate, and a tile behind it
         constexpr uint64_t kRecommended = uint64_t(1) << 30; // bytes of the pieces' buffers under WORKSPACE_RECOMMENDED
 
         int64_t roundUp(int64_t n, int64_t to)
@@ -120,10 +121,17 @@ namespace htb
             l.bytes              = 256 + (gradient ? n * T * uint64_t(f.ldh) * 4 : l.partOff + n * T * 8);
             return l;
         }
+        // Units of the largest piece there may be. Coordinates of loads are 32-bit numbers: the three parts of an f32 piece lie behind
+        // each other (3 n rows), and the classes that dH's product contracts are counted through all six products (6 n).
+        int64_t mostUnits(const CrossEntropyPlan& p, bool gradient)
+        {
+            const int64_t all = roundUp(p.V, kPieceUnit) / kPieceUnit;
+            return p.type == CUDA_R_32F ? std::min(all, kIndexRange / ((gradient ? 6 : 3) * kPieceUnit)) : all;
+        }
         // the largest pieces that fit into `bytes`; piece = 0 when not even the smallest do
         CrossEntropyLayout layoutIn(const CrossEntropyPlan& p, bool gradient, uint64_t bytes)
         {
-            int64_t lo = 0, hi = roundUp(p.V, kPieceUnit) / kPieceUnit; // pieces of lo units fit
+            int64_t lo = 0, hi = mostUnits(p, gradient); // pieces of lo units fit
             while(lo < hi)
             {
                 const int64_t mid = (lo + hi + 1) / 2;
@@ -264,7 +272,8 @@ namespace htb
             return HIPTENSOR_STATUS_INVALID_VALUE;
         if(empty)
             p.T = 0;
-        if(p.V >= (int64_t(1) << 31) - 512 || p.T >= (int64_t(1) << 31) - 512 || p.D > (int64_t(1) << 26))
+        // (f32: the tokens' three parts lie behind each other, in rows of a multiple of 64)
+        if(p.V >= kIndexRange || p.T >= kIndexRange || (type == CUDA_R_32F && 3 * roundUp(p.T, 64) >= kIndexRange) || p.D > (int64_t(1) << 26))
             return HIPTENSOR_STATUS_NOT_SUPPORTED;
         p.parts = p.T > 0 ? hiddenParts(p.T, p.D, p.V * (type == CUDA_R_32F ? 6 : 1)) : 1;
         *out    = p;
@@ -277,7 +286,7 @@ namespace htb
             return 0;
         if(const FewShape f = fewShape(p, gradient); f.use)
             return layoutFew(p, f, gradient).bytes;
-        const uint64_t least = layoutFor(p, gradient, kPieceUnit).bytes, most = layoutFor(p, gradient, roundUp(p.V, kPieceUnit)).bytes;
+        const uint64_t least = layoutFor(p, gradient, kPieceUnit).bytes, most = layoutFor(p, gradient, mostUnits(p, gradient) * kPieceUnit).bytes;
         if(pref == HIPTENSOR_WORKSPACE_MIN)
             return least;
         if(pref == HIPTENSOR_WORKSPACE_MAX)

@@ -140,6 +140,24 @@ def test_cross_entropy_workspace(h):
     assert h.cross_entropy_workspace_size(none, True) == 0
 
 
+@pytest.mark.parametrize("t,status", [((1 << 31) // 3 - 300, 0), ((1 << 31) // 3 - 100, UNSUPPORTED), (1 << 30, UNSUPPORTED)])
+def test_cross_entropy_of_more_f32_tokens_than_three_parts_can_be_counted(h, t, status):
+    """Coordinates of loads are 32-bit numbers, and the three parts of f32 tokens follow each other."""
+    assert ce_status(h, lensH=(t, 1), lensW=(1000, 1), t=F32) == status
+    assert ce_status(h, lensH=(t, 1), lensW=(1000, 1), t=BF) == 0
+
+
+@pytest.mark.parametrize("gradient,times", [(False, 3), (True, 6)])
+def test_cross_entropy_pieces_of_f32_stay_countable(h, gradient, times):
+    """The largest workspace holds the parts of a piece of at most 2^31 / 3 (gradient: / 6) classes, 8 elements a row here."""
+    v = (1 << 30) + 12345
+    plan = h.cross_entropy_plan(desc(h, (20, 8), F32), (0, 2), desc(h, (v, 8), F32), (1, 2))
+    most = h.cross_entropy_workspace_size(plan, gradient, ht.WORKSPACE_MAX)
+    per_class = 3 * 8 * 2 + (3 * 64 * 2 if gradient else 20 * 8 / 128)
+    assert most >= (1 << 31) / times * 0.99 * per_class
+    assert most <= (1 << 31) / times * per_class + (1 << 20)
+
+
 def test_null_arguments(h):
     L = _lib.lib()
     p = ctypes.c_void_p(0)
