@@ -27,11 +27,9 @@ namespace htb
                                          int64_t ld, unsigned short* __restrict__ X2, const int64_t* __restrict__ targets, int64_t ignore,
                                          int64_t V, int* status, bool vec)
         {
-            const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
+            for(int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8; c < ld; c += int64_t(gridDim.y) * blockDim.x * 8)
             for(int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; r < total; r += int64_t(gridDim.x) * blockDim.y)
             {
-                if(c >= ld)
-                    continue;
                 bool live = r < count;
                 if(live && targets)
                 {
@@ -119,12 +117,10 @@ namespace htb
                                           T* __restrict__ Y, const __grid_constant__ TokenRows rows, const __grid_constant__ TargetRest rest, int parts,
                                           int64_t partRows, bool vec)
         {
-            const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 4;
-            const float   f = scale ? scale[1] : 1.f;
+            const float f = scale ? scale[1] : 1.f;
+            for(int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 4; c < cols; c += int64_t(gridDim.y) * blockDim.x * 4)
             for(int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; r < count; r += int64_t(gridDim.x) * blockDim.y)
             {
-                if(c >= cols)
-                    continue;
                 const int64_t target = rest.targets ? rest.targets[r] : 0;
                 const bool    live   = !rest.targets || counts(target, rest.ignore, rest.V);
                 float4        x      = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -176,7 +172,8 @@ namespace htb
             while(tx < 256 && tx < units)
                 tx *= 2;
             const unsigned ty = 256 / tx;
-            return RowShape{dim3(unsigned(std::min<int64_t>((rows + ty - 1) / ty, 1 << 20)), unsigned((units + tx - 1) / tx)), dim3(tx, ty)};
+            return RowShape{dim3(unsigned(std::min<int64_t>((rows + ty - 1) / ty, 1 << 20)), unsigned(std::min<int64_t>((units + tx - 1) / tx, 65535))),
+                            dim3(tx, ty)};
         }
         // every row of a strided tensor starts at a multiple of `unit` elements
         bool rowsAligned(const TokenRows& rows, const void* base, int64_t unit, int64_t size)

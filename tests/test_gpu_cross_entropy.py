@@ -251,6 +251,23 @@ def test_a_token_whose_every_class_is_masked_by_the_lowest_value(h, kind, t):
     within(a, b, ea, eb, c.loss[others], c.lse[others])
 
 
+def test_the_longest_rows(h):
+    """2^26 columns: more of them than a grid has blocks in its second dimension. All but a few columns are zeros."""
+    d = 1 << 26
+    H, W = torch.zeros(9, d, device="cuda", dtype=torch.bfloat16), torch.zeros(5, d, device="cuda", dtype=torch.bfloat16)
+    some = torch.tensor([0, 1, 8191, d // 3, d - 1000, d - 2, d - 1], device="cuda")
+    h0, w0, y, gl = inputs(9, 5, 7, torch.bfloat16, ignored=0)
+    H[:, some], W[:, some] = h0, w0
+    c = Call(h, H, W, y, gl, pref=ht.WORKSPACE_MIN)
+    c.forward()
+    c.backward()
+    within(*ref.loss(h0, w0, y, 1.0, IGNORE), c.loss, c.lse)
+    a, b, ea, eb = ref.gradient(h0, w0, y, c.lse, gl, 1.0, IGNORE)
+    within(a, b, ea, eb, c.dH[:, some], c.dW[:, some])
+    c.dH[:, some], c.dW[:, some] = 0, 0
+    assert not bool(c.dH.any()) and not bool(c.dW.any())
+
+
 @pytest.mark.parametrize("kind", ALL)
 def test_every_token_ignored(h, kind):
     H, W, y, gl = inputs(70, 300, 64, kind)
