@@ -1,6 +1,6 @@
 // Kernels of the linear cross entropy and its gradient. All products run on the shared pipeline of accumulate.cuh; logits and
 // probabilities are made in the epilogue of the product that needs them. f32 operands are sums of three bf16 numbers each, of
-// whose nine products the six that matter are added (2^-26 of the whole is left out): the rate is a sixth of bf16's, as with the
+// whose nine products the six that matter are added (at most 2^-24 of a product is left out, 2^-27 in the mean): the rate is a sixth of bf16's, as with the
 // TF32 split of the f32 contraction, and everything else is shared.
 //
 // Many tokens are bound by the tensor cores under the power limit: 8192 tokens x 128000 classes x 4096 bf16, loss 6.0 to 6.8 ms
@@ -20,7 +20,7 @@ namespace htb
     namespace
     {
         // Rows of a strided tensor as packed rows of ld 16-bit elements, eight elements a thread. SPLIT: f32 numbers as three bf16
-        // ones, x = h + m + l up to 2^-27 of x, [3][rows][ld] (an infinity or NaN stays in h; a number that would round to an infinity,
+        // ones, x = h + m + l, [3][rows][ld] (an infinity or NaN stays in h; a number that would round to an infinity,
         // as f32's lowest value would, is truncated in h).
         template <typename T, bool SPLIT>
         __global__ void pack_rows_kernel(const T* __restrict__ X, const __grid_constant__ TokenRows rows, int64_t count, int64_t total, int64_t cols,
@@ -370,7 +370,7 @@ namespace htb
                     float p0, p1;
                     if constexpr(PARTS == 3)
                     {
-                        // f32: an exponent of 15 in powers of two is rounded by 2^-20, which would be P's largest error
+                        // f32: an exponent of 15 as one of powers of two is rounded by 2^-20, which would be P's largest error
                         const float2 z = unpack2(acc[i]);
                         p0 = expf(fmaf(z.x, a.alpha, -lse));
                         p1 = expf(fmaf(z.y, a.alpha, -lse));
@@ -682,7 +682,7 @@ namespace htb
         }
 
         // The pairs of segments that are multiplied when X is a sum of nx numbers and Y of ny: the products that are left out
-        // are below 2^-26 of the whole.
+        // are at most 2^-24 of the whole, 2^-27 in the mean.
         void segmentPairs(int nx, int ny, AccArgs& a, int kBlocksOfOne)
         {
             int pairs = 0;

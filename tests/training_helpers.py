@@ -57,8 +57,8 @@ def scaled(a, sa, blockA, b, sb, blockB, alpha, beta, c):
 
 
 def logits(h, w, alpha):
-    """(z, bound of |error of z|): f32 sums of at most D exact products (f32 operands are split in two 11-bit parts: what is
-    left out is below 2^-20 of a product)."""
+    """(z, bound of |error of z|): f32 sums of at most D exact products (f32 operands are sums of three bf16 numbers: what is left
+    out is at most 2^-24 of a product, for which the bound has room)."""
     z = alpha * (h.double() @ w.double().T)
     mag = abs(alpha) * (h.double().abs() @ w.double().abs().T)
     per = (h.shape[1] + 4) * 2.0 ** -23 + (2.0 ** -20 if h.dtype == torch.float32 else 0)
