@@ -182,18 +182,6 @@ namespace htb
             tm            = g * a.groupM + in - tn * gm;
         }
 
-        // Epi: the epilogue, one object per epilogue thread:
-        //   Epi(args, warp 0 .. 7, lane, shared memory behind the stages, flag of waits that ran out)
-        //   begin()                         a tile begins
-        //   side(values, row in the tile, half of the columns)  with kSide: this K block's side values
-        //   add(taddr, first, release)      reads the chunk's sums from tensor memory, calls release, and adds them
-        //   end(row, col)                   the tile's sums are complete
-        //   leave()                         no tile follows
-        //   kParted                         whether AccArgs::kParts may be above 1
-        //   send(..), endSplit(..)          with kSplit: the exchange of a tile whose K range is cut
-        // With Epi::kSide > 0, warp 3 fetches kSide floats for every K block (the scales), a group of kGroup blocks at a time,
-        // into a ring of kSideSlots groups, ahead of the epilogue and across tiles:
-        //   Side(args, lane), begin(first row of this CTA, first column), fetch(slot, first K block, past the last one)
         // Registers that a kernel with wide tiles was built with must be what the shares above add up to: a smaller
         // launch would make the epilogue wait for registers that are not there.
         inline cudaError_t accCheckRegs(const void* kernel, int tn)
@@ -207,6 +195,18 @@ namespace htb
             return at.numRegs >= kAccRegs ? cudaSuccess : cudaErrorInvalidKernelImage;
         }
 
+        // Epi: the epilogue, one object per epilogue thread:
+        //   Epi(args, warp 0 .. 7, lane, shared memory behind the stages, flag of waits that ran out)
+        //   begin()                         a tile begins
+        //   side(values, row in the tile, half of the columns)  with kSide: this K block's side values
+        //   add(taddr, first, release)      reads the chunk's sums from tensor memory, calls release, and adds them
+        //   end(row, col)                   the tile's sums are complete
+        //   leave()                         no tile follows
+        //   kParted                         whether AccArgs::kParts may be above 1
+        //   send(..), endSplit(..)          with kSplit: the exchange of a tile whose K range is cut
+        // With Epi::kSide > 0, warp 3 fetches kSide floats for every K block (the scales), a group of kGroup blocks at a time,
+        // into a ring of kSideSlots groups, ahead of the epilogue and across tiles:
+        //   Side(args, lane), begin(first row of this CTA, first column), fetch(slot, first K block, past the last one)
         // XMN, YMN: the operand is contiguous along its rows (a matrix with one row per k; half precision): 64-row chunks of
         // [64 k][128 bytes] instead of rows of 128 bytes along k, transposed descriptors.
         template <class Epi, bool PAIR, int TN, bool F8, bool XMN = false, bool YMN = false>

@@ -655,7 +655,7 @@ namespace htb
         ScaledForm formOf(const ScaledPlan& p, int sms)
         {
             ScaledForm    f{};
-            const int64_t kb = (p.K + 127) / 128, small = std::min(p.M, p.N), large = std::max(p.M, p.N);
+            const int64_t kb = (p.K + 127) / 128, small = std::min(p.M, p.N);
             // few rows on one side (a token, a few of them): that side becomes the columns of narrow tiles, the other
             // one, the weights, fills the 128 rows
             if(small <= 64)
@@ -673,7 +673,6 @@ namespace htb
             const int64_t tiles = f.pair ? 0 : ((f.swap ? p.N : p.M) + 127) / 128 * (((f.swap ? p.M : p.N) + f.tn - 1) / f.tn);
             while(!f.pair && f.ksplit < 4 && tiles * f.ksplit * 2 <= sms && kb >= f.ksplit * 4)
                 f.ksplit *= 2;
-            (void)large;
             return f;
         }
 

@@ -24,7 +24,7 @@ namespace htb
             const void*    H;
             const void*    W;
             TokenRows      rows; // of H
-            int64_t        T, V, D, wV;
+            int64_t        T, V, wV;
             int64_t        units; // of a row: 16 bytes, two elements or one
             const int64_t* targets;
             int64_t        ignore;
@@ -319,7 +319,7 @@ namespace htb
         {
             FewArgs a{};
             a.H = H, a.W = W, a.rows = rows;
-            a.T = p.T, a.V = p.V, a.D = p.D, a.wV = p.wV;
+            a.T = p.T, a.V = p.V, a.wV = p.wV;
             a.units   = f.units;
             a.targets = targets, a.ignore = p.ignore, a.alpha = alpha, a.status = status;
             return a;
