@@ -58,18 +58,32 @@ namespace htb
                 else
                 {
                     __nv_bfloat16 part[3][8];
+                    bool          odd = false;
 #pragma unroll
                     for(int j = 0; j < 8; j++)
                     {
-                        const bool finite = fabsf(x[j]) < INFINITY;
-                        float      left   = x[j];
+                        float left = x[j];
 #pragma unroll
                         for(int k = 0; k < 3; k++)
                         {
                             part[k][j] = narrow<__nv_bfloat16>(left);
-                            if(k == 0 && finite && fabsf(widen(part[0][j])) == INFINITY)
-                                part[0][j] = __float2bfloat16_rz(left);
-                            left = finite ? left - widen(part[k][j]) : 0.f;
+                            left -= widen(part[k][j]);
+                        }
+                        odd = odd || !(fabsf(widen(part[0][j])) < INFINITY);
+                    }
+                    if(odd)
+                    {
+#pragma unroll
+                        for(int j = 0; j < 8; j++)
+                        {
+                            if(fabsf(widen(part[0][j])) < INFINITY)
+                                continue;
+                            const bool finite = fabsf(x[j]) < INFINITY;
+                            if(finite)
+                                part[0][j] = __float2bfloat16_rz(x[j]);
+                            const float left = finite ? x[j] - widen(part[0][j]) : 0.f;
+                            part[1][j] = narrow<__nv_bfloat16>(left);
+                            part[2][j] = narrow<__nv_bfloat16>(left - widen(part[1][j]));
                         }
                     }
 #pragma unroll
@@ -124,12 +138,12 @@ namespace htb
                 const int64_t target = rest.targets ? rest.targets[r] : 0;
                 const bool    live   = !rest.targets || counts(target, rest.ignore, rest.V);
                 float4        x      = make_float4(0.f, 0.f, 0.f, 0.f);
-                for(int i = 0; live && i < parts; i++)
+                for(int i = 0; i < parts; i++)
                 {
                     const float4 v = *reinterpret_cast<const float4*>(X + (int64_t(i) * partRows + r) * ldx + c); // ldx is a multiple of eight
                     x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
                 }
-                float y[4] = {x.x, x.y, x.z, x.w};
+                float y[4] = {live ? x.x : 0.f, live ? x.y : 0.f, live ? x.z : 0.f, live ? x.w : 0.f};
                 if(rest.rest && live)
                 {
                     const T*    w = static_cast<const T*>(rest.W) + target * rest.wV + c * rest.wD;
