@@ -197,7 +197,7 @@ namespace htb
 
         // Epi: the epilogue, one object per epilogue thread:
         //   Epi(args, warp 0 .. 7, lane, shared memory behind the stages, flag of waits that ran out)
-        //   begin()                         a tile begins
+        //   begin(row)                      a tile begins, row is this thread's
         //   side(values, row in the tile, half of the columns)  with kSide: this K block's side values
         //   add(taddr, first, release)      reads the chunk's sums from tensor memory, calls release, and adds them
         //   end(row, col)                   the tile's sums are complete
@@ -540,7 +540,7 @@ namespace htb
                     part(tm);
                     const int     row = quad * 32 + lane;
                     const int64_t r = int64_t(tile) * ROWS + (PAIR ? int(rank) * 128 : 0) + row, c = int64_t(tn) * TN + half * (TN / 2);
-                    epi.begin();
+                    epi.begin(r);
                     for(int kb = kbBegin; kb < kbEnd; kb += a.chunk)
                     {
                         if constexpr(Epi::kSide > 0)

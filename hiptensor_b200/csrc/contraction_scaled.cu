@@ -282,7 +282,7 @@ namespace htb
                     __syncwarp();
                 }
             }
-            __device__ __forceinline__ void begin()
+            __device__ __forceinline__ void begin(int64_t)
             {
 #pragma unroll
                 for(int j = 0; j < COLS / 2; j++)

@@ -103,6 +103,8 @@ namespace htb
             l.stateOff       = take(!gradient, T * 12);
             l.scaleOff       = take(gradient, 8);
             l.restOff        = take(gradient, T * 4);
+            l.lists          = gradient && partsP == 1;
+            l.listOff        = take(l.lists, uint64_t(2 * roundUp(p.T, 64) + p.V) * 4);
             l.dhOff          = take(gradient, uint64_t(l.parts) * uint64_t(hiddenRows(p.T)) * ld * 4);
             l.wOff           = take(l.packW, seg * n * ld * 2);
             l.partOff        = take(!gradient, n / kHeadGroup * T * 8);
@@ -345,7 +347,7 @@ namespace htb
         int64_t            ldh    = rowStride(p, l);
         if(l.packH)
         {
-            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, l.rowsT, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, nullptr, stream));
+            HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, l.rowsT, p.D, l.ld, ws + l.hOff, nullptr, 0, 0, TokenLists{}, nullptr, stream));
             h   = ws + l.hOff;
             ldh = l.ld;
         }
@@ -356,7 +358,7 @@ namespace htb
             int64_t       ldw = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, n, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, TokenLists{}, nullptr, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
@@ -426,8 +428,17 @@ namespace htb
             scale = reinterpret_cast<float*>(ws + l.scaleOff);
             HTB_TRY(launchGradientScale(gradLoss, a, p.T, targets, p.ignore, p.V, scale, stream));
         }
-        void* h = ws + l.hOff;
-        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, l.rowsT, p.D, l.ld, h, targets, p.ignore, p.V, st->deviceStatus, stream));
+        void* h       = ws + l.hOff;
+        TokenLists lists{};
+        if(l.lists)
+        {
+            lists.classes = reinterpret_cast<int*>(ws + l.listOff); // (read in whole words of 16 bytes)
+            lists.next    = lists.classes + roundUp(p.T, 64);
+            lists.first   = lists.next + roundUp(p.T, 64);
+        }
+        HTB_TRY(launchPackRows(p.type, H, rowsOfH(p), p.T, l.rowsT, p.D, l.ld, h, targets, p.ignore, p.V, lists, st->deviceStatus, stream));
+        if(l.lists && dW)
+            HTB_TRY(launchTokenLists(lists, p.T, p.V, stream));
         float*              dh   = reinterpret_cast<float*>(ws + l.dhOff);
         float*              dw   = reinterpret_cast<float*>(ws + l.dwOff);
         float*              rest = reinterpret_cast<float*>(ws + l.restOff);
@@ -441,7 +452,7 @@ namespace htb
             int64_t       ldw   = p.wV;
             if(l.packW)
             {
-                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, rowsW, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, nullptr, stream));
+                HTB_TRY(launchPackRows(p.type, w, plainRows(p.wV, p.wD, n), n, rowsW, p.D, l.ld, ws + l.wOff, nullptr, 0, 0, TokenLists{}, nullptr, stream));
                 w   = ws + l.wOff;
                 ldw = l.ld;
             }
@@ -453,11 +464,11 @@ namespace htb
             {
                 unsigned char* out = static_cast<unsigned char*>(dW) + v0 * p.wV * size;
                 if(l.direct)
-                    HTB_TRY(launchWeightGradient(head, P, scale, p.type, out, p.wV, st->smCount, st->deviceStatus, stream));
+                    HTB_TRY(launchWeightGradient(head, P, v0, lists, rest, scale, p.type, out, p.wV, st->smCount, st->deviceStatus, stream));
                 else
                 {
                     // rows of W that no bulk store can write: through f32 in the workspace
-                    HTB_TRY(launchWeightGradient(head, P, nullptr, CUDA_R_32F, dw, l.ld, st->smCount, st->deviceStatus, stream));
+                    HTB_TRY(launchWeightGradient(head, P, v0, lists, rest, nullptr, CUDA_R_32F, dw, l.ld, st->smCount, st->deviceStatus, stream));
                     HTB_TRY(launchStoreRows(p.type, dw, l.ld, n, p.D, scale, out, plainRows(p.wV, p.wD, n), TargetRest{}, 1, 0, stream));
                 }
             }

@@ -25,7 +25,7 @@ namespace htb
         template <typename T, bool SPLIT>
         __global__ void pack_rows_kernel(const T* __restrict__ X, const __grid_constant__ TokenRows rows, int64_t count, int64_t total, int64_t cols,
                                          int64_t ld, unsigned short* __restrict__ X2, const int64_t* __restrict__ targets, int64_t ignore,
-                                         int64_t V, int* status, bool vec)
+                                         int64_t V, int* __restrict__ classes, int* status, bool vec)
         {
             for(int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8; c < ld; c += int64_t(gridDim.y) * blockDim.x * 8)
             for(int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; r < total; r += int64_t(gridDim.x) * blockDim.y)
@@ -37,6 +37,8 @@ namespace htb
                     live                 = counts(target, ignore, V);
                     if(!live && target != ignore && c == 0)
                         atomicExch_system(status, kStatusBadTarget);
+                    if(classes && c == 0)
+                        classes[r] = live ? int(target) : -1;
                 }
                 T x[8];
                 if(live && vec && c + 8 <= cols)
@@ -91,6 +93,84 @@ namespace htb
                         *reinterpret_cast<uint4*>(X2 + (k * total + r) * ld + c) = *reinterpret_cast<const uint4*>(part[k]);
                 }
             }
+        }
+
+        // The lists of tokens of 32 classes a block: each of its warps searches an eighth of the tokens, 16 a lane and round, in an
+        // order that is always the same, and the warps' lists are linked in the order of the warps. Classes whose list is full
+        // are no longer looked for, so that a frequent one (a token's turn takes about 50 instructions) does not outlast the products.
+        // 4 bytes a token for 32 classes, out of L2: 1024 tokens x 32000 classes 5 us, 65536 x 8000 22 us.
+        constexpr int kListWarps = 8;
+        __global__ void __launch_bounds__(32 * kListWarps) token_lists_kernel(const __grid_constant__ TokenLists lists, int64_t T, int64_t V)
+        {
+            __shared__ int firsts[kListWarps][32], lasts[kListWarps][32], counts[kListWarps][32];
+            const int      lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            const int64_t  v0   = int64_t(blockIdx.x) * 32, share = ((T + kListWarps - 1) / kListWarps + 511) / 512 * 512;
+            const int64_t  begin = warp * share, end = min(begin + share, T);
+            const int      base  = int(v0);
+            int            first = -1, last = -1, count = 0;
+            uint32_t       open  = v0 + 32 <= V ? 0xffffffffu : (1u << (V - v0)) - 1;
+            int4           next[4];
+            auto           load = [&](int64_t t0) {
+#pragma unroll
+                for(int j = 0; j < 4; j++)
+                {
+                    const int64_t t = t0 + j * 128 + lane * 4; // (the buffer is of whole words)
+                    next[j]         = t < end ? *reinterpret_cast<const int4*>(lists.classes + t) : make_int4(-1, -1, -1, -1);
+                }
+            };
+            load(begin);
+            for(int64_t t0 = begin; t0 < end && open; t0 += 512)
+            {
+                int      c[16];
+                uint32_t hits = 0; // token t0 + 128 j + 4 lane + k is number 4 j + k
+#pragma unroll
+                for(int j = 0; j < 16; j++)
+                {
+                    const int4& q = next[j / 4];
+                    c[j]          = (j % 4 == 0 ? q.x : (j % 4 == 1 ? q.y : (j % 4 == 2 ? q.z : q.w))) - base;
+                    if(uint32_t(c[j]) < 32u && (open >> c[j] & 1) && t0 + j / 4 * 128 + lane * 4 + j % 4 < end)
+                        hits |= 1u << j;
+                }
+                load(t0 + 512);
+                for(uint32_t lanes; (lanes = __ballot_sync(0xffffffffu, hits != 0)) != 0;)
+                {
+                    // the first lane's first token and its class
+                    const int bit = __ffs(int(hits)) - 1, from = __ffs(int(lanes)) - 1;
+                    int       its = c[0];
+#pragma unroll
+                    for(int j = 1; j < 16; j++)
+                        its = bit == j ? c[j] : its;
+                    const int number = __shfl_sync(0xffffffffu, bit, from), token = int(t0) + number / 4 * 128 + from * 4 + number % 4;
+                    if(lane == from)
+                        hits &= hits - 1;
+                    if(__shfl_sync(0xffffffffu, its, from) == lane && count < kListed)
+                    {
+                        if(count++ == 0)
+                            first = token;
+                        else
+                            lists.next[last] = token;
+                        last = token;
+                    }
+                }
+                open &= __ballot_sync(0xffffffffu, count < kListed);
+            }
+            firsts[warp][lane] = first, lasts[warp][lane] = last, counts[warp][lane] = count;
+            __syncthreads();
+            if(warp != 0 || v0 + lane >= V)
+                return;
+            for(int w = 1; w < kListWarps && count < kListed; w++)
+                if(counts[w][lane])
+                {
+                    if(count)
+                        lists.next[last] = firsts[w][lane];
+                    else
+                        first = firsts[w][lane];
+                    last = lasts[w][lane];
+                    count += counts[w][lane];
+                }
+            if(count)
+                lists.next[last] = -1;
+            lists.first[v0 + lane] = first;
         }
 
         // Only tokens whose row of P is not zero have a say, and of these only finite factors: one that is not makes its own row
@@ -281,7 +361,7 @@ namespace htb
                 : a(args)
             {
             }
-            __device__ __forceinline__ void begin() {}
+            __device__ __forceinline__ void begin(int64_t) {}
             template <class Release>
             __device__ __forceinline__ void add(uint32_t taddr, bool first, Release release)
             {
@@ -327,9 +407,10 @@ namespace htb
         };
 
         // Gradient: P = (exp(z - lse) - [class is the target]) * g * alpha, rounded to the operands' type for the two products
-        // that follow (the products' sums are f32; a rounding of 2^-9 or 2^-12 of each entry is about what the rounding of
-        // the results to the same type costs). The target's entry outweighs the others: what its rounding takes is kept and
-        // added to dH in f32. PARTS > 1: P as a sum of that many numbers, each what rounding took from the ones before, in
+        // that follow (the products' sums are f32). The target's entry outweighs the others: what its rounding takes is kept and
+        // added to dH and dW in f32, which leaves both with the error of their own rounding (512 x 20000 x 4096: 1.66e-3 in bf16, as
+        // with P in 64 bits; dW without it 2.2e-3). The others' rounding, at most 2^-8 (f16: 2^-11) of each, is a twentieth of that
+        // there. PARTS > 1: P as a sum of that many numbers, each what rounding took from the ones before, in
         // segments of rowsP rows (a multiple of 32; rows past the tokens hold zeros there).
         template <typename TP, int PARTS>
         struct ProbabilityEpi : HeadSums<256>
@@ -354,7 +435,7 @@ namespace htb
                 , stores(0)
             {
             }
-            __device__ __forceinline__ void begin() {}
+            __device__ __forceinline__ void begin(int64_t) {}
             template <class Release>
             __device__ __forceinline__ void add(uint32_t taddr, bool first, Release release)
             {
@@ -462,7 +543,13 @@ namespace htb
         {
             int64_t      rows, cols;
             const float* scale;
-            CUtensorMap  mapD;
+            // what rounding took from the targets' entries of P (no lists: nothing is added), and H, rows of 16-bit elements ldh apart
+            TokenLists            lists;
+            const float*          rest;
+            const unsigned short* H;
+            int64_t               ldh, T, v0;
+            int                   half; // H is f16, else bf16
+            CUtensorMap           mapD;
         };
         // SLOTS: of 4 KiB for a warp's results. A short sum (few tokens) is bound by its stores and takes two; a long one leaves the
         // room to the stages.
@@ -478,23 +565,68 @@ namespace htb
             const Args&           a;
             const int             lane;
             const uint32_t        slot;
-            int                   stores;
+            int                   stores, mine;
 
             __device__ WeightEpi(const Args& args, int w, int l, unsigned char* smem, volatile int*)
                 : a(args)
                 , lane(l)
                 , slot(smemAddr(smem) + uint32_t(w * SLOTS * 4096))
                 , stores(0)
+                , mine(-1)
             {
             }
-            __device__ __forceinline__ void begin() {}
+            // (asked for here, so that it is there when the sums are)
+            __device__ __forceinline__ void begin(int64_t row)
+            {
+                mine = a.lists.first && row < a.rows ? a.lists.first[a.v0 + row] : -1;
+            }
             template <class Release>
             __device__ __forceinline__ void add(uint32_t taddr, bool first, Release release)
             {
                 addSums(taddr, first, release);
             }
+            // sums += rest[token] * H[token, col ..] for this thread's class
+            __device__ __forceinline__ void addToken(int token, int64_t col)
+            {
+                constexpr int         LOADS = 8;
+                const float           e   = a.rest[token];
+                const uint64_t        e2  = pack2(e, e);
+                const unsigned short* src = a.H + token * a.ldh + col;
+#pragma unroll
+                for(int c = 0; c < COLS; c += 8 * LOADS)
+                {
+                    uint4 q[LOADS]; // on their way together
+#pragma unroll
+                    for(int l = 0; l < LOADS; l++)
+                        q[l] = col + c + 8 * l < a.ldh ? *reinterpret_cast<const uint4*>(src + c + 8 * l) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for(int j = 0; j < 4 * LOADS; j++)
+                    {
+                        const uint4&   v = q[j / 4];
+                        const uint32_t w = j % 4 == 0 ? v.x : (j % 4 == 1 ? v.y : (j % 4 == 2 ? v.z : v.w));
+                        const float2   f = a.half ? __half22float2(reinterpret_cast<const __half2&>(w))
+                                                  : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+                        acc[c / 2 + j] = fma2(pack2(f.x, f.y), e2, acc[c / 2 + j]);
+                    }
+                }
+            }
+            // The targets' entries outweigh the others in a class's row: what rounding took from them is added here, token by token, behind
+            // the next tile's MMAs. With the lists it takes, of a gradient: nothing of 4096 x 128000 x 4096 (10.0 ms), 7 of 210 us of
+            // 1024 x 32000 x 1024, 17 of 190 of 128 x 32000 x 4096 (a tile's sum is short there), 20 of 95 of 4096 x 1000 x 1024 (the lists'
+            // 16 tokens for most classes); twice the products' terms, P as two numbers, would take a third of each.
+            __device__ __forceinline__ void addRests(int64_t col)
+            {
+                while(__any_sync(0xffffffffu, mine >= 0))
+                    if(mine >= 0)
+                    {
+                        const int token = mine;
+                        mine            = a.lists.next[token];
+                        addToken(token, col);
+                    }
+            }
             __device__ __forceinline__ void end(int64_t row, int64_t col)
             {
+                addRests(col);
                 const float    f  = a.scale ? a.scale[1] : 1.f;
                 const uint64_t f2 = pack2(f, f);
 #pragma unroll
@@ -576,7 +708,7 @@ namespace htb
                 , slot(smemAddr(smem) + uint32_t(w * SLOTS * 4096))
             {
             }
-            __device__ __forceinline__ void begin() {}
+            __device__ __forceinline__ void begin(int64_t) {}
             template <class Release>
             __device__ __forceinline__ void add(uint32_t taddr, bool first, Release release)
             {
@@ -949,13 +1081,16 @@ namespace htb
                       : launchAccumulate<HiddenEpi, true, false, true>(mapX, mapY, a, ea, smCount, stream, "cross_entropy_hidden_pair");
     }
 
-    cudaError_t launchWeightGradient(const HeadProduct& h, const Probabilities& P, const float* scale, int typeOut, void* dW, int64_t ldw, int smCount,
-                                     int* status, cudaStream_t stream)
+    cudaError_t launchWeightGradient(const HeadProduct& h, const Probabilities& P, int64_t v0, const TokenLists& lists, const float* rest, const float* scale,
+                                     int typeOut, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream)
     {
         PFN_encodeTiled encode = tensorMapEncoder();
         const bool      wide   = typeOut == CUDA_R_32F;
         WeightArgs      ea{};
         ea.rows = h.n, ea.cols = h.D, ea.scale = scale;
+        ea.lists = lists;
+        ea.rest = rest, ea.H = static_cast<const unsigned short*>(h.H), ea.ldh = h.ldh, ea.T = h.T, ea.v0 = v0;
+        ea.half = h.type == CUDA_R_16F;
         CUtensorMap mapX, mapY;
         // one segment: rows past the tokens are not there (zeros); more: they hold zeros
         if(!encode || !encodeMatrix(encode, &mapX, P.data, h.n, P.parts > 1 ? P.parts * P.rows : h.T, P.ld, 64, 64)
@@ -981,20 +1116,26 @@ namespace htb
     }
 
     cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t total, int64_t cols, int64_t ld, void* X2,
-                               const int64_t* targets, int64_t ignore, int64_t V, int* status, cudaStream_t stream)
+                               const int64_t* targets, int64_t ignore, int64_t V, const TokenLists& lists, int* status, cudaStream_t stream)
     {
         const RowShape  s   = rowShape(total, ld / 8);
         unsigned short* out = static_cast<unsigned short*>(X2);
         if(type == CUDA_R_32F)
-            pack_rows_kernel<float, true><<<s.grid, s.block, 0, stream>>>((const float*)X, rows, count, total, cols, ld, out, targets, ignore, V, status,
+            pack_rows_kernel<float, true><<<s.grid, s.block, 0, stream>>>((const float*)X, rows, count, total, cols, ld, out, targets, ignore, V, lists.classes, status,
                                                                           rowsAligned(rows, X, 4, 4));
         else if(type == CUDA_R_16F)
-            pack_rows_kernel<__half, false><<<s.grid, s.block, 0, stream>>>((const __half*)X, rows, count, total, cols, ld, out, targets, ignore, V,
+            pack_rows_kernel<__half, false><<<s.grid, s.block, 0, stream>>>((const __half*)X, rows, count, total, cols, ld, out, targets, ignore, V, lists.classes,
                                                                             status, rowsAligned(rows, X, 8, 2));
         else
             pack_rows_kernel<__nv_bfloat16, false><<<s.grid, s.block, 0, stream>>>((const __nv_bfloat16*)X, rows, count, total, cols, ld, out, targets,
-                                                                                   ignore, V, status, rowsAligned(rows, X, 8, 2));
+                                                                                   ignore, V, lists.classes, status, rowsAligned(rows, X, 8, 2));
         return noted("cross_entropy_pack");
+    }
+
+    cudaError_t launchTokenLists(const TokenLists& lists, int64_t T, int64_t V, cudaStream_t stream)
+    {
+        token_lists_kernel<<<unsigned((V + 31) / 32), 32 * kListWarps, 0, stream>>>(lists, T, V);
+        return noted("cross_entropy_lists");
     }
 
     cudaError_t launchGradientScale(const float* g, float alpha, int64_t T, const int64_t* targets, int64_t ignore, int64_t V, float* scale,

@@ -34,13 +34,23 @@ namespace htb
         int64_t  ld;
         int      parts; // sums of dH that are kept apart
         int64_t  piece; // classes of a piece, a multiple of 256
-        uint64_t hOff, wOff, stateOff, partOff, pOff, dhOff, dwOff, scaleOff, restOff;
+        bool     lists; // of the tokens of each class
+        uint64_t hOff, wOff, stateOff, partOff, pOff, dhOff, dwOff, scaleOff, restOff, listOff;
         uint64_t bytes;
     };
 
     int planCrossEntropy(const hiptensorTensorDescriptor_t& H, const int32_t* modeH, const hiptensorTensorDescriptor_t& W,
                          const int32_t* modeW, int64_t ignoreIndex, int typeCompute, CrossEntropyPlan* out);
     uint64_t crossEntropyWorkspace(const CrossEntropyPlan& p, bool gradient, int pref);
+
+    // The tokens of every class (null: not wanted): `first` has a class's first token, `next` a token's follower, -1 where there is none.
+    // A list ends after kListed tokens (it may go on for as many). `classes`: every token's class (-1: does not count).
+    constexpr int kListed = 16;
+    struct TokenLists
+    {
+        int *classes, *next, *first;
+    };
+    cudaError_t launchTokenLists(const TokenLists& lists, int64_t T, int64_t V, cudaStream_t stream);
 
     // token rows of a strided tensor
     struct TokenRows
@@ -50,9 +60,10 @@ namespace htb
         int64_t elem; // stride along the contracted mode
     };
     // X2[r, 0 .. ld) = X[row r, 0 .. cols), zeros behind and in rows count .. total - 1; f32 as three segments of `total` rows. With
-    // targets: rows whose target is `ignore` or no class become zeros, and the latter raise the status word.
+    // targets: rows whose target is `ignore` or no class become zeros, and the latter raise the status word. lists: `classes` is
+    // written.
     cudaError_t launchPackRows(int type, const void* X, const TokenRows& rows, int64_t count, int64_t total, int64_t cols, int64_t ld, void* X2,
-                               const int64_t* targets, int64_t ignore, int64_t V, int* status, cudaStream_t stream);
+                               const int64_t* targets, int64_t ignore, int64_t V, const TokenLists& lists, int* status, cudaStream_t stream);
 
     // the logits of n classes, used where they are made: operands in 16 bits, `segments` of segH / segW rows each
     struct HeadProduct
@@ -87,9 +98,10 @@ namespace htb
     int         hiddenParts(int64_t T, int64_t D, int64_t piece);
     cudaError_t launchHiddenGradient(const HeadProduct& h, const Probabilities& P, int parts, float* out, int64_t ldo, bool add, int smCount,
                                      int* status, cudaStream_t stream);
-    // dW[v, d] = sum over the tokens of P[t, v] H[t, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes
-    cudaError_t launchWeightGradient(const HeadProduct& h, const Probabilities& P, const float* scale, int typeOut, void* dW, int64_t ldw, int smCount,
-                                     int* status, cudaStream_t stream);
+    // dW[v, d] = sum over the tokens of P[t, v] H[t, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes. With
+    // lists, rest[t] H[t, d] is added for the listed tokens t of class v.
+    cudaError_t launchWeightGradient(const HeadProduct& h, const Probabilities& P, int64_t v0, const TokenLists& lists, const float* rest, const float* scale,
+                                     int typeOut, void* dW, int64_t ldw, int smCount, int* status, cudaStream_t stream);
 
     // f16: scale[0] = a power of two that brings max |g * alpha| over the tokens that count (finite ones) close to the top of the range,
     // scale[1] = its reciprocal

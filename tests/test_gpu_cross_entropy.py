@@ -268,6 +268,44 @@ def test_the_longest_rows(h):
     assert not bool(c.dH.any()) and not bool(c.dW.any())
 
 
+@pytest.mark.parametrize("pref", [ht.WORKSPACE_MIN, ht.WORKSPACE_MAX])
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("times", [1, 3, 16])
+@pytest.mark.parametrize("t,v,d", [(40, 300, 64), (65, 300, 64), (130, 2000, 72), (300, 1031, 101), (700, 4100, 260), (1500, 9000, 24)])
+def test_the_targets_entries_are_not_rounded(h, t, v, d, times, kind, pref):
+    """An lse far above every logit leaves -gradLoss alone in each row of P; `times` tokens have the same class (of up to 16 the
+    entries are kept whole). dW and dH are then off by their own rounding alone, and dW by that of its f32 sum."""
+    H, W, y, gl = inputs(t, v, d, kind, ignored=0)
+    y[:] = torch.arange(t, device="cuda") % -(-t // times) * 11 % v  # (no v is a multiple of 11)
+    y[t // 2] = IGNORE
+    gl[:] = (1 + torch.rand(t, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")) * (1 - 2 * (torch.arange(t, device="cuda") % 2))
+    c = Call(h, H, W, y, gl, pref=pref)
+    c.lse.fill_(1e4)
+    c.backward()
+    P = torch.zeros(t, v, device="cuda", dtype=torch.float64)
+    keep = y >= 0
+    P[torch.arange(t, device="cuda")[keep], y[keep]] = -gl[keep].double()
+    step = ref.half_step(kind) if kind != torch.float32 else 2.0 ** -22  # (f32: products of three-part sums, one more rounding)
+    for got, p, x in ((c.dH, P, W.double()), (c.dW, P.T, H.double())):
+        want, mag = p @ x, p.abs() @ x.abs()
+        assert bool(((got.double() - want).abs() <= 1.01 * step * want.abs() + (times + 8) * 2.0 ** -23 * mag + 2.0 ** -25).all())
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+def test_a_class_of_very_many_tokens(h, kind):
+    H, W, y, gl = inputs(900, 700, 136, kind, ignored=0.1)
+    y[y >= 0] = torch.where(torch.arange(900, device="cuda") % 5 < 4, 333, y)[y >= 0]
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    c.backward()
+    c.check_gradient()
+    first = c.dW.clone()
+    for _ in range(3):
+        c.dW.fill_(9)
+        c.backward()
+        assert torch.equal(c.dW, first)
+
+
 @pytest.mark.parametrize("kind", ALL)
 def test_every_token_ignored(h, kind):
     H, W, y, gl = inputs(70, 300, 64, kind)
