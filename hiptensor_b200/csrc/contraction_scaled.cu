@@ -4,11 +4,13 @@
 // The scales forbid to sum over blocks in tensor memory: each block's sums are taken from there, scaled and added in registers
 // (accumulate.cuh). What bounds the large products is that hand-over: with two accumulators of 256 columns (all of tensor
 // memory), a block costs the start and end of its MMAs (1000 cycles, 512 of them MMAs), the reads with the additions in
-// between (540) and the way back to the issuer (350), over two blocks in flight: about 950 cycles. 8192^3 to bf16: 595 to 720 us
-// by the power the data cost, 1.5 to 1.85 PFLOP/s; the same pipeline without the additions takes 400. A scale per column as
-// well (weight gradients) doubles the additions, which then bound it: 1.0 to 1.25 PFLOP/s. Narrow tiles are bound by what an
+// between (540) and the way back to the issuer (350), over two blocks in flight: about 950 cycles. 8192^3 to bf16: 720 us
+// one after the other (1.52 PFLOP/s, the card at its power limit), 610 after a pause; the same pipeline without the additions
+// takes 400. A scale per column as well (weight gradients) doubles the additions, which then bound it: 8192^3 820 to 850 us,
+// 4096 x 4096 x 8192 added to f32 280 (1.0 PFLOP/s). Narrow tiles are bound by what an
 // SM loads (about 39 bytes a cycle): few tokens are cut along K over clusters to load with more SMs (4096 x 4096: 1 token
-// 10.4 us, 128 tokens 12.4).
+// 10.7 us, 128 tokens 12.6). Operands that no such load can read take the FMA kernel: 4096^3 8.1 ms, 777 x 2057 x 1001 262 us
+// (18 in rows of whole 16-byte words).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -357,7 +359,7 @@ namespace htb
             }
             // The same through shared memory when the columns are contiguous: lanes that follow each other write (and read C)
             // along a row, one element each, so that any row stride and start will do (rows of odd length: 4096 x 4097 x 4096
-            // in bf16 takes 119 us, 260 with every lane on a row of its own; 85 by bulk stores
+            // in bf16 takes 120 us, 260 with every lane on a row of its own; 87 by bulk stores
             // when N is 4096). Eight rows' worth of C is read ahead of their stores.
             template <int W>
             __device__ __forceinline__ void store(const float (&w)[W], int64_t row, int64_t col0)

@@ -38,9 +38,9 @@ namespace htb
         }
 
         // Whether and how a call runs in one pass over W (few tokens; this and the tensor cores in us): gradients of 8 tokens of f32
-        // (x 32000 x 1024: 98 and 247) and of rows that no TMA load can read (f16, x 30011 x 1001: 154 and 207), of 4 tokens of
-        // others (bf16, x 11722 x 2064: 56 and 73; 8 tokens x 32000 x 4096: 376 and 184); losses of 8 tokens of f32 (x 32000 x 1024:
-        // 62 and 126) and of 4 of rows that no TMA load can read (bf16, x 30011 x 1001: 48 and 72, 8 tokens 73 and 71).
+        // (x 32000 x 1024: 103 and 247) and of rows that no TMA load can read (f16, x 30011 x 1001: 154 and 207), of 4 tokens of
+        // others (bf16, x 11722 x 2064: 56 and 73; 8 tokens x 32000 x 4096: 376 and 230); losses of 8 tokens of f32 (x 32000 x 1024:
+        // 64 and 126) and of 4 of rows that no TMA load can read (bf16, x 30011 x 1001: 48 and 72, 8 tokens 73 and 71).
         FewShape fewShape(const CrossEntropyPlan& p, bool gradient)
         {
             FewShape      f{};

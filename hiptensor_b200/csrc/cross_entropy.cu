@@ -3,11 +3,13 @@
 // whose nine products the six that matter are added (at most 2^-24 of a product is left out, 2^-27 in the mean): the rate is a sixth of bf16's, as with the
 // TF32 split of the f32 contraction, and everything else is shared.
 //
-// Many tokens are bound by the tensor cores under the power limit: 8192 tokens x 128000 classes x 4096 bf16, loss 6.0 to 6.8 ms
-// (1.26 to 1.43 PFLOP/s; a plain library product of that size runs at 1.39 sustained), 4096 tokens' gradient 10.0 to 10.7 ms
-// (1.20 to 1.28). Few tokens are bound by the bytes of W: 1 token x 32000 x 4096, loss 54 us (4.9 TB/s); 8 tokens' gradient
-// 184 us. Gradients of fewer tokens run in one pass over W (cross_entropy_few.cu).
-// f32: 1024 x 32000 x 1024, loss 350 us, gradient 1.08 ms (190 TFLOP/s, 0.7 of a sixth of bf16's rate).
+// Many tokens are bound by the tensor cores under the power limit: 8192 tokens x 128000 classes x 4096 bf16, loss 6.6 to 6.8 ms
+// (1.26 to 1.30 PFLOP/s; a plain library product of that size runs at 1.39 sustained; 5.7 after a pause), 4096 tokens' gradient 10.3
+// to 10.9 ms (1.18 to 1.25). Few tokens are bound by the bytes of W: 1 token x 32000 x 4096, loss 56 us (4.7 TB/s); 8 tokens'
+// gradient 230 us (W read twice, dW written). Gradients of fewer tokens run in one pass over W (cross_entropy_few.cu).
+// f32: 1024 x 32000 x 1024, loss 370 to 480 us (by where the copies lie in memory), gradient 1.1 ms (185 TFLOP/s, 0.7 of a sixth
+// of bf16's rate). A W whose classes are contiguous ([d, v]) is copied and its gradient stored element by element: 1024 x 32000 x
+// 1024 bf16 takes 196 us for the loss and 673 for the gradient, 73 and 201 as [v, d].
 #include <algorithm>
 
 #include "accumulate.cuh"
@@ -613,7 +615,7 @@ namespace htb
             // The targets' entries outweigh the others in a class's row: what rounding took from them is added here, token by token, behind
             // the next tile's MMAs. With the lists it takes, of a gradient: nothing of 4096 x 128000 x 4096 (10.0 ms), 7 of 210 us of
             // 1024 x 32000 x 1024, 17 of 190 of 128 x 32000 x 4096 (a tile's sum is short there), 20 of 95 of 4096 x 1000 x 1024 (the lists'
-            // 16 tokens for most classes); twice the products' terms, P as two numbers, would take a third of each.
+            // 16 tokens for most classes); P as two numbers instead would add a third to the gradient's operations.
             __device__ __forceinline__ void addRests(int64_t col)
             {
                 while(__any_sync(0xffffffffu, mine >= 0))

@@ -5,8 +5,8 @@
 // are still in the first-level cache: a class's row of dW is written once, and dH's sums over the block's classes stay in
 // shared memory until the end, when a second kernel adds the blocks up in a fixed order. All sums and P are f32.
 //
-// One token x 32000 x 1024 f32: gradient 47 us (5.6 TB/s; by the tensor cores 242), loss 30 (123); 8 tokens 98 (247) and 62
-// (126): instructions, no longer bytes. 2 tokens x 128000 x 4096 bf16: gradient 422 us (5.0 TB/s; 664).
+// One token x 32000 x 1024 f32: gradient 51 us (5.2 TB/s; by the tensor cores 242), loss 33 (123); 8 tokens 103 (247) and 64
+// (126): instructions, no longer bytes. 2 tokens x 128000 x 4096 bf16: gradient 433 us (4.8 TB/s; 664).
 #include <algorithm>
 
 #include "common.hpp"

@@ -12,9 +12,10 @@
 // truncated, and its last bit set when the truncation was not exact. A number rounded to odd at 24 bits rounds to 4 bits or
 // fewer as the number itself does.
 //
-// Bound by memory: each element is read once and written once. Rows of 16-bit elements run at 5.1 to 5.8 TB/s (16384 x 8192
-// bf16: 71 us back to back; at the copy rate it would be 62), other blocks and orders at 4.0 to 4.7 (about ten
-// instructions an element), f32 at 4.8 to 5.1; one token of 4096 takes 2.5 us.
+// Bound by memory: each element is read once and written once. 16384 x 8192 bf16 in blocks along rows takes 76 to 80 us (5.1 to 5.4
+// TB/s; at the copy rate it would be 62), other blocks and orders of that size 85 to 101 (4.0 to 4.8: about ten instructions
+// an element), f32 137 (4.9); 8192 x 4096 f32 in other blocks and orders 36 to 37 (4.5 to 4.7). Smaller tensors have fewer
+// tiles in flight: 5001 x 4104 bf16 in blocks along columns, turned, 19 us (3.2 TB/s). One token of 4096 takes 2.7 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

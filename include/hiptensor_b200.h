@@ -176,9 +176,12 @@ int htScaledContraction(const htHandle* handle, const htScaledContractionPlan* p
  * nothing out of range: its loss is NaN, its row of P zero, and the next call on the handle returns 13
  * (EXECUTION_FAILED) once. Sums are f32, softmax statistics too. Of a few tokens P stays f32; else it is rounded to the type of H
  * (f16: scaled by a power of two for the largest finite |gradLoss * alpha| of the tokens that count) but for the targets' entries,
- * which outweigh the others: what rounding takes from them is added in f32 (dW: of at least the first 16 tokens of a class). For dW
- * of up to 64 tokens P is a sum of two such numbers. f32 tensors of more than a few tokens are multiplied as sums of three bf16
+ * which outweigh the others: what rounding takes from them is added in f32 (dW: of at least 16 of a class's tokens). For dW of
+ * up to 64 tokens P is a sum of two such numbers. f32 tensors of more than a few tokens are multiplied as sums of three bf16
  * numbers, which is f32's own accuracy; an infinity among them makes NaN of the logits it takes part in.
+ *
+ * Fastest are H and W contiguous along the contracted mode, in rows at multiples of 16 bytes; W contiguous along the classes takes
+ * two to three and a half times as long. dH and dW need a place for every element, and neither they nor the workspace overlap an operand.
  *
  * The workspace holds the pieces: any size from htCrossEntropyGetWorkspaceSize's MIN on (19 below it); with more, pieces
  * are larger and fewer. gradient: 0 for htCrossEntropy, 1 for htCrossEntropyGradient. Two calls that run at the same time (two
