@@ -292,6 +292,27 @@ def test_the_targets_entries_are_not_rounded(h, t, v, d, times, kind, pref):
 
 
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,v,d", [(3, 20000, 512), (40, 9000, 256), (300, 20000, 256), (1000, 9000, 520)])
+def test_gradients_are_off_by_their_own_rounding_in_the_mean(h, t, v, d, kind):
+    """A bound for each element has room for the worst of thousands of classes; the norm of the whole error has not. A rounding is
+    off by a step over the root of 12 in the mean, relative to a number at least step / (2 half_step): at most 2 / sqrt(12) half
+    steps. The entries of P that are not targets' are rounded once more. f32 sums: 2^-18 is far above their error."""
+    H, W, y, gl = inputs(t, v, d, kind)
+    c = Call(h, H, W, y, gl)
+    c.forward()
+    c.backward()
+    keep = y >= 0
+    P = torch.exp(H.double() @ W.double().T - c.lse.double()[:, None]) * torch.where(keep, gl, torch.zeros_like(gl)).double()[:, None]
+    full = P.clone()
+    full[torch.arange(t, device="cuda")[keep], y[keep]] -= gl[keep].double()
+    P[torch.arange(t, device="cuda")[keep], y[keep]] = 0
+    for got, whole, others in ((c.dH, full @ W.double(), P @ W.double()), (c.dW, full.T @ H.double(), P.T @ H.double())):
+        share = float(others.norm() / whole.norm())
+        off = float((got.double() - whole).norm() / whole.norm())
+        assert off <= 2 / 12 ** 0.5 * ref.half_step(kind) * (1 + share) + 2.0 ** -18, off / ref.half_step(kind)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
 def test_a_class_of_very_many_tokens(h, kind):
     H, W, y, gl = inputs(900, 700, 136, kind, ignored=0.1)
     y[y >= 0] = torch.where(torch.arange(900, device="cuda") % 5 < 4, 333, y)[y >= 0]
