@@ -11,13 +11,12 @@
 // SM loads (about 39 bytes a cycle): few tokens are cut along K over clusters to load with more SMs (4096 x 4096: 1 token
 // 10.7 us, 128 tokens 12.6). Operands that no such load can read take the FMA kernel: 4096^3 8.1 ms, 777 x 2057 x 1001 262 us
 // (18 in rows of whole 16-byte words).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
 
 #include "accumulate.cuh"
+#include "convert.cuh"
 #include "kernels.hpp"
 #include "scaled.hpp"
 
@@ -29,36 +28,6 @@ namespace htb
         {
             return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, e5m2 ? __NV_E5M2 : __NV_E4M3)));
         }
-        template <typename TD>
-        __device__ __forceinline__ TD narrow(float v);
-        template <>
-        __device__ __forceinline__ float narrow<float>(float v)
-        {
-            return v;
-        }
-        template <>
-        __device__ __forceinline__ __half narrow<__half>(float v)
-        {
-            return __float2half_rn(v);
-        }
-        template <>
-        __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v)
-        {
-            return __float2bfloat16_rn(v);
-        }
-        __device__ __forceinline__ float widen(float v)
-        {
-            return v;
-        }
-        __device__ __forceinline__ float widen(__half v)
-        {
-            return __half2float(v);
-        }
-        __device__ __forceinline__ float widen(__nv_bfloat16 v)
-        {
-            return __bfloat162float(v);
-        }
-
         // Any strides and extents: 64 x 64 tiles, 16 x 16 threads with 4 x 4 results each, byte loads into shared memory as
         // f32, FMA. A block's products are summed by themselves and scaled once.
         template <typename TD>

@@ -1,45 +1,13 @@
-// What the kernels of the linear cross entropy share: conversions, rows of a strided tensor, joining of partial softmax sums.
+// What the kernels of the linear cross entropy share: rows of a strided tensor, joining of partial softmax sums.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+#include "convert.cuh"
 #include "cross_entropy.hpp"
 
 namespace htb
 {
     namespace
     {
-        __device__ __forceinline__ float widen(float v)
-        {
-            return v;
-        }
-        __device__ __forceinline__ float widen(__half v)
-        {
-            return __half2float(v);
-        }
-        __device__ __forceinline__ float widen(__nv_bfloat16 v)
-        {
-            return __bfloat162float(v);
-        }
-        template <typename T>
-        __device__ __forceinline__ T narrow(float v);
-        template <>
-        __device__ __forceinline__ float narrow<float>(float v)
-        {
-            return v;
-        }
-        template <>
-        __device__ __forceinline__ __half narrow<__half>(float v)
-        {
-            return __float2half_rn(v);
-        }
-        template <>
-        __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v)
-        {
-            return __float2bfloat16_rn(v);
-        }
-
         __device__ __forceinline__ int64_t rowOffset(const TokenRows& r, int64_t row)
         {
             int64_t off = 0;
