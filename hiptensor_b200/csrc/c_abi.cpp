@@ -391,8 +391,9 @@ int htCreateCrossEntropyPlan(const htHandle* handle, htCrossEntropyPlan** plan, 
     *plan = nullptr;
     if(!handle || !descH || !modeH || !descW || !modeW)
         return HIPTENSOR_STATUS_NOT_INITIALIZED;
-    htb::CrossEntropyPlan p;
-    const int rc = htb::planCrossEntropy(descH->d, modeH, descW->d, modeW, ignoreIndex, typeCompute, &p);
+    htb::CrossEntropyPlan   p;
+    const htb::HandleState* st = htb::stateOf(H(handle));
+    const int               rc = htb::planCrossEntropy(descH->d, modeH, descW->d, modeW, ignoreIndex, typeCompute, st ? st->smCount : 0, &p);
     if(rc != HIPTENSOR_STATUS_SUCCESS)
     {
         HTB_LOG_ERROR("htCreateCrossEntropyPlan", "no cross entropy over these tensors (%s)", hiptensorGetErrorString(hiptensorStatus_t(rc)));

@@ -63,7 +63,7 @@ namespace htb
             const int64_t rounds = (f.units + 255) / 256;
             f.threads            = int(roundUp((f.units + rounds - 1) / rounds, 32));
             const int64_t each   = std::max<int64_t>(1, std::min<int64_t>(512 / f.threads, (227 << 10) / (smem + 5120)));
-            int64_t       n      = std::min(148 * each, (p.V + 3) / 4);
+            int64_t       n      = std::min(p.sms * each, (p.V + 3) / 4);
             if(gradient)
                 n = std::min(n, std::max<int64_t>(1, p.V * size / (4 * p.T)));
             f.blocks = int(n);
@@ -188,7 +188,7 @@ namespace htb
     } // namespace
 
     int planCrossEntropy(const hiptensorTensorDescriptor_t& H, const int32_t* modeH, const hiptensorTensorDescriptor_t& W,
-                         const int32_t* modeW, int64_t ignoreIndex, int typeCompute, CrossEntropyPlan* out)
+                         const int32_t* modeW, int64_t ignoreIndex, int typeCompute, int smCount, CrossEntropyPlan* out)
     {
         const int type = H.mType;
         if((type != CUDA_R_16F && type != CUDA_R_16BF && type != CUDA_R_32F) || W.mType != type || typeCompute != HIPTENSOR_COMPUTE_32F
@@ -203,6 +203,7 @@ namespace htb
         CrossEntropyPlan p{};
         p.type   = type;
         p.ignore = ignoreIndex;
+        p.sms    = smCount > 0 ? smCount : 148;
         p.T = p.V = p.D = 1;
         p.hD = p.wD = 1;
         p.wV        = 1;
@@ -277,7 +278,7 @@ namespace htb
         // (f32: the tokens' three parts lie behind each other, in rows of a multiple of 64)
         if(p.V >= kIndexRange || p.T >= kIndexRange || (type == CUDA_R_32F && 3 * roundUp(p.T, 64) >= kIndexRange) || p.D > (int64_t(1) << 26))
             return HIPTENSOR_STATUS_NOT_SUPPORTED;
-        p.parts = p.T > 0 ? hiddenParts(p.T, p.D, p.V * (type == CUDA_R_32F ? 6 : 1)) : 1;
+        p.parts = p.T > 0 ? hiddenParts(p.T, p.D, p.V * (type == CUDA_R_32F ? 6 : 1), p.sms) : 1;
         *out    = p;
         return HIPTENSOR_STATUS_SUCCESS;
     }

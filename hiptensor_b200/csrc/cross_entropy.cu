@@ -1029,13 +1029,13 @@ namespace htb
     // there are few, or in their last round when there are some. A round of tiles over n classes takes about n x 5.9 ns
     // (measured rate of a pair), a part more T x D x 8 bytes of traffic; a part's sums have at least 1024 terms. `piece`: classes
     // times the products that an element's product is made of.
-    int hiddenParts(int64_t T, int64_t D, int64_t piece)
+    int hiddenParts(int64_t T, int64_t D, int64_t piece, int sms)
     {
         const bool    single = T <= 128;
-        const int64_t tiles  = (D + 255) / 256 * (single ? 1 : (T + 255) / 256), units = single ? 148 : 74;
+        const int64_t tiles  = (D + 255) / 256 * (single ? 1 : (T + 255) / 256), units = single ? sms : sms / 2;
         int           best   = 1;
         double        least  = 0;
-        for(int parts = 1; parts <= 148 && (parts == 1 || parts * 1024 <= piece); parts++)
+        for(int parts = 1; parts <= sms && (parts == 1 || parts * 1024 <= piece); parts++)
         {
             const double rounds = double((tiles * parts + units - 1) / units) / parts;
             const double time   = rounds * double(piece) * 5.9e-9 + parts * double(T) * double(D) * 8 / 6.5e12;

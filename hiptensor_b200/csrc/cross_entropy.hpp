@@ -20,6 +20,7 @@ namespace htb
         int     nt;
         int64_t tExt[kMaxGroup], tStride[kMaxGroup];
         int64_t hD, wV, wD; // strides in elements
+        int     sms; // of the handle's device
         int     parts; // of dH's products (hiddenParts for the whole vocabulary)
         int64_t ignore;
     };
@@ -40,7 +41,7 @@ namespace htb
     };
 
     int planCrossEntropy(const hiptensorTensorDescriptor_t& H, const int32_t* modeH, const hiptensorTensorDescriptor_t& W,
-                         const int32_t* modeW, int64_t ignoreIndex, int typeCompute, CrossEntropyPlan* out);
+                         const int32_t* modeW, int64_t ignoreIndex, int typeCompute, int smCount, CrossEntropyPlan* out);
     uint64_t crossEntropyWorkspace(const CrossEntropyPlan& p, bool gradient, int pref);
 
     // The tokens of every class (null: not wanted): `first` has a class's first token, `next` a token's follower, -1 where there is none.
@@ -95,7 +96,7 @@ namespace htb
                                    cudaStream_t stream);
     // out[part][t, d] = (add: +=) sum over a part of the classes of P[t, v] W[v, d], `parts` of them side by side
     int64_t     hiddenRows(int64_t T); // of a part in `out`
-    int         hiddenParts(int64_t T, int64_t D, int64_t piece);
+    int         hiddenParts(int64_t T, int64_t D, int64_t piece, int sms);
     cudaError_t launchHiddenGradient(const HeadProduct& h, const Probabilities& P, int parts, float* out, int64_t ldo, bool add, int smCount,
                                      int* status, cudaStream_t stream);
     // dW[v, d] = sum over the tokens of P[t, v] H[t, d] (* scale[1]); rows of dW ldw apart, at multiples of 16 bytes. With
